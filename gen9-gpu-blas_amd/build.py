@@ -1,4 +1,5 @@
-"""Builds libgen9blas.so (HIP, gfx950) and libgen9blas_blas.so (CBLAS/BLAS shim) in this directory.
+"""Builds libgen9blas.so (HIP, gfx950), libgen9blas_llm.so (MX4 and mixture-of-experts operators, HIP) and
+libgen9blas_blas.so (CBLAS/BLAS shim) in this directory.
 
     python gen9-gpu-blas_amd/build.py            # rebuild what changed
     python gen9-gpu-blas_amd/build.py --force    # rebuild everything
@@ -21,6 +22,7 @@ INCLUDE = os.path.join(ROOT, "include")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 LIB = os.path.join(HERE, "libgen9blas.so")
 BLAS_LIB = os.path.join(HERE, "libgen9blas_blas.so")
+LLM_LIB = os.path.join(HERE, "libgen9blas_llm.so")
 CALIB_LIB = os.path.join(HERE, "libgen9blas_calib.so")   # bench.py's calibration kernels, not part of the library
 
 HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++20", "-fPIC", "-fvisibility=hidden", "-I" + INCLUDE, "-I" + CSRC,
@@ -29,6 +31,7 @@ HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++20", "-fPIC", "-fvisibilit
              "-Wall", "-Wno-unused-function"]
 HIP_SOURCES = ["runtime.hip", "gemm.hip", "gemm_kernels.hip", "skinny.hip", "level12.hip", "level12_kernels.hip",
                "packed.hip", "level3.hip", "level2.hip", "noalloc.hip"]
+LLM_SOURCES = ["llm_runtime.hip", "mx4.hip", "mx4_gemm.hip", "moe.hip"]
 # every header of csrc/ counts as a dependency of every object: a new header cannot be left out
 HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith(".h"))
 
@@ -50,9 +53,9 @@ def _stale(target, deps):
 
 def build(force=False, jobs=None, verbose=True):
     os.makedirs(BUILD, exist_ok=True)
-    hdr = [os.path.join(CSRC, h) for h in HEADERS] + [os.path.join(INCLUDE, h) for h in ("gen9blas.h", "gen9blas_hip.h", "gen9blas_ml.h")]
+    hdr = [os.path.join(CSRC, h) for h in HEADERS] + [os.path.join(INCLUDE, h) for h in ("gen9blas.h", "gen9blas_hip.h", "gen9blas_ml.h", "gen9blas_llm.h")]
     objs, todo = [], []
-    for s in HIP_SOURCES:
+    for s in HIP_SOURCES + LLM_SOURCES:
         src, obj = os.path.join(CSRC, s), os.path.join(BUILD, s.replace(".hip", ".o"))
         objs.append(obj)
         if force or _stale(obj, [src] + hdr):
@@ -62,10 +65,16 @@ def build(force=False, jobs=None, verbose=True):
         for out in ex.map(_run, todo):
             if out.strip() and verbose:
                 print(out, file=sys.stderr)
-    if force or todo or _stale(LIB, objs + [os.path.join(CSRC, "exports.map")]):
+    lib_objs, llm_objs = objs[:len(HIP_SOURCES)], objs[len(HIP_SOURCES):]
+    if force or _stale(LIB, lib_objs + [os.path.join(CSRC, "exports.map")]):
         _run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-Wl,-soname,libgen9blas.so",
-              "-Wl,--version-script=" + os.path.join(CSRC, "exports.map"), "-o", LIB + ".tmp"] + objs)
+              "-Wl,--version-script=" + os.path.join(CSRC, "exports.map"), "-o", LIB + ".tmp"] + lib_objs)
         os.replace(LIB + ".tmp", LIB)
+    if force or _stale(LLM_LIB, llm_objs + [LIB, os.path.join(CSRC, "exports.map")]):
+        _run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-Wl,-soname,libgen9blas_llm.so",
+              "-Wl,--version-script=" + os.path.join(CSRC, "exports.map"), "-o", LLM_LIB + ".tmp"] + llm_objs +
+             ["-L" + HERE, "-lgen9blas", "-Wl,-rpath,$ORIGIN"])
+        os.replace(LLM_LIB + ".tmp", LLM_LIB)
     _build_blas(force)
     _build_calib(force)
     return LIB

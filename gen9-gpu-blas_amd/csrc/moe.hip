@@ -1,0 +1,295 @@
+// Mixture of experts: the router (gen9blas_moe_route) and the products of each token's experts (gen9blas_moe_gemm).
+#include "mx4_gemm_kernel.h"
+
+namespace g9llm {
+
+constexpr int MAX_EXPERTS = 1024, MAX_K = 64;
+
+struct RouteArgs {
+    const void *logits;
+    long long ldl;
+    const float *bias;
+    int T, E, sigmoid, groups, top_groups, k, renorm;
+    float scale;
+    int *ids;
+    float *weights;
+};
+
+// An order on floats (no NaN) as unsigned numbers; −0 and +0 are equal after adding +0.
+__device__ __forceinline__ unsigned ordered(float x) {
+    const unsigned u = __builtin_bit_cast(unsigned, x + 0.f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+    return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    return v;
+}
+
+// A wave routes a token: lane l holds the experts l, l + 64, ... The choice of the k experts is k rounds of a wave's
+// maximum over (choice, lowest index).
+template <class T, int NL>
+__global__ void __launch_bounds__(256) moe_route_kernel(RouteArgs a) {
+    const float ninf = -__builtin_inff();
+    extern __shared__ float lds[];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const long long t = (long long)blockIdx.x * 4 + wv;
+    if (t >= a.T) return;   // whole waves: nothing below waits for another wave
+    const T *row = (const T *)a.logits + t * a.ldl;
+    float score[NL], choice[NL];
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < NL; i++) {
+        const int e = i * 64 + lane;
+        score[i] = e < a.E ? (float)row[e] : ninf;
+        nan |= score[i] != score[i];
+    }
+    nan = __ballot(nan) != 0;
+    if (a.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const bool out = !(score[i] > ninf);
+            score[i] = 1.f / (1.f + expf(-score[i]));
+            choice[i] = out ? ninf : score[i];
+        }
+    } else {
+        float m = ninf, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < NL; i++) m = fmaxf(m, score[i]);
+        m = wave_max(m);
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            choice[i] = score[i] > ninf ? score[i] : ninf;
+            score[i] = m > ninf ? expf(score[i] - m) : 0.f;
+            sum += score[i];
+        }
+        sum = wave_sum(sum);
+#pragma unroll
+        for (int i = 0; i < NL; i++) score[i] /= sum;
+        if (a.bias)
+#pragma unroll
+            for (int i = 0; i < NL; i++)
+                if (choice[i] > ninf) choice[i] = score[i];
+    }
+    if (a.bias)
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const int e = i * 64 + lane;
+            if (e < a.E && choice[i] > ninf) choice[i] += a.bias[e];
+            if (choice[i] != choice[i]) choice[i] = ninf, nan = true;
+        }
+    nan = __ballot(nan) != 0;
+    if (a.groups > 1) {
+        float *mine = lds + wv * a.E;
+        const int size = a.E / a.groups;
+#pragma unroll
+        for (int i = 0; i < NL; i++)
+            if (i * 64 + lane < a.E) mine[i * 64 + lane] = choice[i];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // other lanes read what these wrote
+        __builtin_amdgcn_wave_barrier();
+        float best = ninf, second = ninf;
+        if (lane < a.groups)
+            for (int i = 0; i < size; i++) {
+                const float c = mine[lane * size + i];
+                second = fmaxf(second, fminf(best, c));
+                best = fmaxf(best, c);
+            }
+        // a group with one expert left counts as that one; one with none is never chosen
+        const unsigned key = ordered(a.sigmoid && second > ninf ? best + second : best);
+        int rank = 0;
+        for (int j = 0; j < a.groups; j++) {
+            const unsigned other = __shfl(key, j);
+            rank += other > key || (other == key && j < lane);
+        }
+        const unsigned long long keep = __ballot(lane < a.groups && rank < a.top_groups);
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const int e = i * 64 + lane;
+            if (e < a.E && !(keep >> (e / size) & 1)) choice[i] = ninf;
+        }
+    }
+    int id = -1;      // lane j: the j-th choice
+    float w = 0.f;
+    for (int j = 0; j < a.k; j++) {
+        unsigned long long best = 0;   // (choice, lowest index first); 0: none left
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const unsigned long long key = (unsigned long long)ordered(choice[i]) << 32 | (0xffffffffu - (i * 64 + lane));
+            if (choice[i] > ninf && key > best) best = key;
+        }
+#pragma unroll
+        for (int d = 32; d; d >>= 1) {
+            const unsigned long long other = __shfl_xor(best, d);
+            best = other > best ? other : best;
+        }
+        if (!best) break;
+        const int e = (int)(0xffffffffu - (unsigned)best);
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NL; i++)
+            if (i == e / 64) {
+                s = score[i];
+                if (lane == e % 64) choice[i] = ninf;
+            }
+        s = __shfl(s, e % 64);
+        if (lane == j) id = e, w = s;
+    }
+    if (a.renorm) {
+        const float sum = wave_sum(w);
+        w = sum == 0.f ? 0.f : w / sum;
+    }
+    w *= a.scale;
+    if (nan) w = __builtin_nanf("");
+    if (lane < a.k) {
+        a.ids[t * a.k + lane] = id;
+        a.weights[t * a.k + lane] = w;
+    }
+}
+
+// The plan of a grouped product: slots by expert (order; places whose id is no expert come last, as expert E), off[e] where
+// expert e's begin, and the tiles of `rows` slots: (expert, first place), (−1, 0) past the last. One workgroup. The order of
+// a group's slots varies from call to call; no result depends on it.
+__global__ void __launch_bounds__(1024) moe_plan_kernel(const int *__restrict__ ids, long long n, int E, int rows, int *order, int *off,
+                                                        int *tiles, int most) {
+    __shared__ int count[MAX_EXPERTS + 1], base[MAX_EXPERTS + 2], tile0[MAX_EXPERTS + 2];
+    for (int i = threadIdx.x; i <= E; i += 1024) count[i] = 0;
+    __syncthreads();
+    for (long long i = threadIdx.x; i < n; i += 1024) {
+        const unsigned e = (unsigned)ids[i];
+        atomicAdd(&count[e < (unsigned)E ? e : E], 1);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int b = 0, t = 0;
+        for (int e = 0; e <= E; e++) {
+            base[e] = b, tile0[e] = t;
+            b += count[e], t += (count[e] + rows - 1) / rows;
+        }
+        base[E + 1] = b, tile0[E + 1] = t;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e <= E + 1; e += 1024) {
+        off[e] = base[e];
+        if (e <= E)
+            for (int t = tile0[e]; t < tile0[e + 1]; t++) tiles[2 * t] = e, tiles[2 * t + 1] = base[e] + (t - tile0[e]) * rows;
+    }
+    for (int t = tile0[E + 1] + threadIdx.x; t < most; t += 1024) tiles[2 * t] = -1, tiles[2 * t + 1] = 0;
+    __syncthreads();
+    for (long long i = threadIdx.x; i < n; i += 1024) {
+        const unsigned e = (unsigned)ids[i];
+        order[atomicAdd(&base[e < (unsigned)E ? e : E], 1)] = (int)i;
+    }
+}
+
+// C(t) = Σ_s weights(t, s) · y(t, s), in the order of s; places that are no expert's are left out.
+template <class T>
+__global__ void __launch_bounds__(256) moe_join_kernel(const float *__restrict__ y, const int *__restrict__ ids, const float *__restrict__ weights,
+                                                       int S, int E, int N, T *__restrict__ C, long long ldct) {
+    const long long t = blockIdx.y;
+    const int n = blockIdx.x * 256 + threadIdx.x;
+    if (n >= N) return;
+    float sum = 0.f;
+    for (int s = 0; s < S; s++)
+        if ((unsigned)ids[t * S + s] < (unsigned)E) sum += weights[t * S + s] * y[(t * S + s) * N + n];
+    C[t * ldct + n] = (T)sum;
+}
+
+template <class T> static int launch_route(const RouteArgs &a) {
+    const dim3 grid((unsigned)cdiv(a.T, 4)), block(256);
+    const size_t lds = a.groups > 1 ? (size_t)a.E * 16 : 0;
+    if (a.E <= 64) hipLaunchKernelGGL((moe_route_kernel<T, 1>), grid, block, lds, stream, a);
+    else if (a.E <= 128) hipLaunchKernelGGL((moe_route_kernel<T, 2>), grid, block, lds, stream, a);
+    else if (a.E <= 256) hipLaunchKernelGGL((moe_route_kernel<T, 4>), grid, block, lds, stream, a);
+    else if (a.E <= 512) hipLaunchKernelGGL((moe_route_kernel<T, 8>), grid, block, lds, stream, a);
+    else hipLaunchKernelGGL((moe_route_kernel<T, 16>), grid, block, lds, stream, a);
+    G9_HIP(hipGetLastError());
+    return 0;
+}
+
+template <class T, class O, bool GATED> static int launch_grouped(const Rows &R, const Mx4View &W, const Mx4View &G, int E, int most) {
+    hipLaunchKernelGGL((mx4_gemm_any_kernel<T, O, 2, true, GATED>), dim3((unsigned)((long long)most * W.rt)), dim3(256), 0, stream, R, W, G, E);
+    G9_HIP(hipGetLastError());
+    return 0;
+}
+
+template <class T>
+static int experts(int Tn, int S, const int *ids, const void *X, int64_t ldt, int64_t lds, const gen9blas_mx4 *W, const gen9blas_mx4 *gate,
+                   const float *weights, void *C, int64_t ldct, int64_t ldcs) {
+    const long long n = (long long)Tn * S;
+    const int E = W->count, N = W->rows, rows = 32;
+    const long long most = cdiv(n, rows) + E + 1;
+    if (most * W->rt > 0xffffff || n > 0x7fffffff)
+        G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "moe_gemm: more tiles than one launch can index");
+    void *plan = nullptr, *slots = nullptr;
+    G9_TRY(scratch(SLOT_PLAN, (size_t)(n + E + 2 + 2 * most) * 4, &plan));
+    if (weights) G9_TRY(scratch(SLOT_SLOTS, (size_t)n * N * 4, &slots));
+    int *order = (int *)plan, *off = order + n, *tiles = off + E + 2;
+    hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(1024), 0, stream, ids, n, E, rows, order, off, tiles, (int)most);
+    G9_HIP(hipGetLastError());
+    Rows R = {X, C, ldt, lds, ldct, ldcs, 0, S, tiles, order, off};
+    const Mx4View w = view(W), g = gate ? view(gate) : w;
+    if (!weights)
+        return gate ? launch_grouped<T, T, true>(R, w, g, E, (int)most) : launch_grouped<T, T, false>(R, w, g, E, (int)most);
+    R.C = slots, R.ldct = (long long)S * N, R.ldcs = N;
+    G9_TRY((gate ? launch_grouped<T, float, true>(R, w, g, E, (int)most) : launch_grouped<T, float, false>(R, w, g, E, (int)most)));
+    for (int t0 = 0; t0 < Tn; t0 += 65535) {   // the grid's y limit
+        const int rowsy = min(Tn - t0, 65535);
+        hipLaunchKernelGGL((moe_join_kernel<T>), dim3((unsigned)cdiv(N, 256), (unsigned)rowsy), dim3(256), 0, stream,
+                           (const float *)slots + (long long)t0 * S * N, ids + (long long)t0 * S, weights + (long long)t0 * S, S, E, N,
+                           (T *)C + t0 * ldct, (long long)ldct);
+    }
+    G9_HIP(hipGetLastError());
+    return 0;
+}
+
+}  // namespace g9llm
+
+using namespace g9llm;
+
+extern "C" {
+
+int gen9blas_moe_route(int type, int T, int E, const void *logits, int ldl, const float *bias, int score, int groups, int top_groups, int k,
+                       int renorm, float scale, int *ids, float *weights) {
+    G9_TRY(begin());
+    if (type != GEN9BLAS_H && type != GEN9BLAS_S) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "moe_route: type %d unavailable", type);
+    if (score != GEN9BLAS_SOFTMAX && score != GEN9BLAS_SIGMOID) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "moe_route: score %d unavailable", score);
+    if (E < 1 || E > MAX_EXPERTS || k < 1 || k > MAX_K || k > E || ldl < E)
+        G9_FAIL(GEN9BLAS_ERR_INVALID_ARG, "moe_route: E = %d (1..%d), k = %d (1..min(E, %d)), ldl = %d", E, MAX_EXPERTS, k, MAX_K, ldl);
+    if (groups < 1 || groups > 64 || E % groups || top_groups < 1 || top_groups > groups)
+        G9_FAIL(GEN9BLAS_ERR_INVALID_ARG, "moe_route: groups = %d (1..64, a divisor of E = %d), top_groups = %d", groups, E, top_groups);
+    if (T <= 0) return 0;
+    G9_TRY(need_device(logits, ((size_t)(T - 1) * ldl + E) * elem_size(type), "moe_route: logits"));
+    if (bias) G9_TRY(need_device(bias, (size_t)E * 4, "moe_route: bias"));
+    G9_TRY(need_device(ids, (size_t)T * k * 4, "moe_route: ids"));
+    G9_TRY(need_device(weights, (size_t)T * k * 4, "moe_route: weights"));
+    const RouteArgs a = {logits, ldl, bias, T, E, score == GEN9BLAS_SIGMOID, groups, top_groups, k, renorm, scale, ids, weights};
+    return type == GEN9BLAS_H ? launch_route<_Float16>(a) : launch_route<float>(a);
+}
+
+int gen9blas_moe_gemm(int type, int T, int S, const int *ids, const void *X, int64_t ldt, int64_t lds, const gen9blas_mx4 *W,
+                      const gen9blas_mx4 *gate, const float *weights, void *C, int64_t ldct, int64_t ldcs) {
+    G9_TRY(begin());
+    if (type != GEN9BLAS_H && type != GEN9BLAS_S) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "moe_gemm: type %d unavailable", type);
+    if (!W || W->count > MAX_EXPERTS) G9_FAIL(GEN9BLAS_ERR_INVALID_ARG, "moe_gemm: %s", W ? "more than 1024 experts" : "no W");
+    if (gate && (gate->count != W->count || gate->rows != W->rows || gate->K != W->K))
+        G9_FAIL(GEN9BLAS_ERR_INVALID_ARG, "moe_gemm: the gate's shape is not W's");
+    if (T <= 0 || S <= 0) return 0;
+    const int K = W->K, N = W->rows, es = elem_size(type);
+    if (lds < 0 || (lds > 0 && lds < K) || ldt < (lds ? (S - 1) * lds + K : K))
+        G9_FAIL(GEN9BLAS_ERR_INVALID_ARG, "moe_gemm: rows of X overlap (ldt %lld, lds %lld, K %d)", (long long)ldt, (long long)lds, K);
+    if (weights ? ldct < N : (ldcs < N || ldct < (S - 1) * ldcs + N))
+        G9_FAIL(GEN9BLAS_ERR_INVALID_ARG, "moe_gemm: rows of C overlap (ldct %lld, ldcs %lld, N %d)", (long long)ldct, (long long)ldcs, N);
+    G9_TRY(need_device(ids, (size_t)T * S * 4, "moe_gemm: ids"));
+    G9_TRY(need_device(X, ((size_t)(T - 1) * ldt + (size_t)(S - 1) * lds + K) * es, "moe_gemm: X"));
+    G9_TRY(need_device(C, ((size_t)(T - 1) * ldct + (weights ? 0 : (size_t)(S - 1) * ldcs) + N) * es, "moe_gemm: C"));
+    if (weights) G9_TRY(need_device(weights, (size_t)T * S * 4, "moe_gemm: weights"));
+    return type == GEN9BLAS_H ? experts<_Float16>(T, S, ids, X, ldt, lds, W, gate, weights, C, ldct, ldcs)
+                              : experts<float>(T, S, ids, X, ldt, lds, W, gate, weights, C, ldct, ldcs);
+}
+
+}  // extern "C"

@@ -1,0 +1,112 @@
+// gen9blas_mx4_gemm and gen9blas_mx4_gemm_q: products of FP16, FP32 or MX4 rows with MX4 weights.
+#include "mx4_gemm_kernel.h"
+
+namespace g9llm {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// Both operands MX4, any shape: a workgroup makes 64 rows × 16 columns, its 4 waves every fourth group of 512 k.
+template <class O>
+__global__ void __launch_bounds__(256) mx4_gemm_q_any_kernel(Mx4View A, Mx4View W, O *__restrict__ C, long long ldc) {
+    constexpr int MT = 4;
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    const int nt = blockIdx.x % W.rt, mt = blockIdx.x / W.rt * MT;
+    f32x4 acc[MT];
+#pragma unroll
+    for (int m = 0; m < MT; m++) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const u32x4 *wc = reinterpret_cast<const u32x4 *>(W.codes) + (long long)nt * W.kc * 64 + lane;
+    const int *ws = reinterpret_cast<const int *>(W.scales) + (long long)nt * W.kg * 64 + lane;
+    for (int grp = wv; grp < W.kg; grp += 4) {
+        const int sw = ws[grp * 64];
+        int sa[MT];
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+            sa[m] = reinterpret_cast<const int *>(A.scales)[((long long)min(mt + m, A.rt - 1) * A.kg + grp) * 64 + lane];
+        auto step = [&](auto J) {
+            constexpr int j = decltype(J)::value;
+            const int c = grp * 4 + j;
+            if (c >= W.kc) return;
+            const u32x4 w = wc[(long long)c * 64];
+            const i32x8 wf = {(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                const u32x4 a = reinterpret_cast<const u32x4 *>(A.codes)[((long long)min(mt + m, A.rt - 1) * A.kc + c) * 64 + lane];
+                const i32x8 af = {(int)a[0], (int)a[1], (int)a[2], (int)a[3]};
+                acc[m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, af, acc[m], 4, 4, j, sw, j, sa[m]);
+            }
+        };
+        step(std::integral_constant<int, 0>());
+        step(std::integral_constant<int, 1>());
+        step(std::integral_constant<int, 2>());
+        step(std::integral_constant<int, 3>());
+    }
+    __shared__ f32x4 part[3][MT][64];
+    if (wv) {
+#pragma unroll
+        for (int m = 0; m < MT; m++) part[wv - 1][m][lane] = acc[m];
+    }
+    __syncthreads();
+    if (wv) return;
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+        f32x4 v = acc[m];
+#pragma unroll
+        for (int w = 0; w < 3; w++) v += part[w][m][lane];
+        const int row = (mt + m) * 16 + r;
+        if (row >= A.rows) continue;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int n = nt * 16 + 4 * g + j;
+            if (n < W.rows) C[row * ldc + n] = (O)v[j];
+        }
+    }
+}
+
+template <class T> static int launch_dense(const Rows &R, const Mx4View &W) {
+    const long long wgs = cdiv(R.M, 32) * W.rt;
+    if (wgs > 0xffffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm: more tiles than one launch can index");
+    if (R.M <= 16)
+        hipLaunchKernelGGL((mx4_gemm_any_kernel<T, T, 1, false, false>), dim3((unsigned)(cdiv(R.M, 16) * W.rt)), dim3(256), 0, stream, R, W, W, 1);
+    else
+        hipLaunchKernelGGL((mx4_gemm_any_kernel<T, T, 2, false, false>), dim3((unsigned)wgs), dim3(256), 0, stream, R, W, W, 1);
+    G9_HIP(hipGetLastError());
+    return 0;
+}
+
+}  // namespace g9llm
+
+using namespace g9llm;
+
+extern "C" {
+
+int gen9blas_mx4_gemm(int type, int M, const void *A, int lda, const gen9blas_mx4 *W, void *C, int ldc) {
+    G9_TRY(begin());
+    if (type != GEN9BLAS_H && type != GEN9BLAS_S) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm: type %d unavailable", type);
+    if (!W || W->count != 1) G9_FAIL(GEN9BLAS_ERR_INVALID_ARG, "mx4_gemm: %s", W ? "W holds several matrices" : "no W");
+    if (M <= 0) return 0;
+    if (lda < W->K || ldc < W->rows) G9_FAIL(GEN9BLAS_ERR_INVALID_ARG, "mx4_gemm: lda %d < K %d or ldc %d < N %d", lda, W->K, ldc, W->rows);
+    const int es = elem_size(type);
+    G9_TRY(need_device(A, ((size_t)(M - 1) * lda + W->K) * es, "mx4_gemm: A"));
+    G9_TRY(need_device(C, ((size_t)(M - 1) * ldc + W->rows) * es, "mx4_gemm: C"));
+    const Rows R = {A, C, lda, 0, ldc, 0, M, 1, nullptr, nullptr, nullptr};
+    return type == GEN9BLAS_H ? launch_dense<_Float16>(R, view(W)) : launch_dense<float>(R, view(W));
+}
+
+int gen9blas_mx4_gemm_q(int type, const gen9blas_mx4 *A, const gen9blas_mx4 *W, void *C, int ldc) {
+    G9_TRY(begin());
+    if (type != GEN9BLAS_H && type != GEN9BLAS_S) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm_q: type %d unavailable", type);
+    if (!A || !W || A->count != 1 || W->count != 1) G9_FAIL(GEN9BLAS_ERR_INVALID_ARG, "mx4_gemm_q: %s", A && W ? "an operand holds several matrices" : "no A or no W");
+    if (A->K != W->K || ldc < W->rows) G9_FAIL(GEN9BLAS_ERR_INVALID_ARG, "mx4_gemm_q: K %d and %d, ldc %d, N %d", A->K, W->K, ldc, W->rows);
+    G9_TRY(need_device(C, ((size_t)(A->rows - 1) * ldc + W->rows) * elem_size(type), "mx4_gemm_q: C"));
+    const long long wgs = cdiv(A->rt, 4) * W->rt;
+    if (wgs > 0xffffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm_q: more tiles than one launch can index");
+    const dim3 grid((unsigned)wgs), block(256);
+    if (type == GEN9BLAS_H)
+        hipLaunchKernelGGL((mx4_gemm_q_any_kernel<_Float16>), grid, block, 0, stream, view(A), view(W), (_Float16 *)C, (long long)ldc);
+    else
+        hipLaunchKernelGGL((mx4_gemm_q_any_kernel<float>), grid, block, 0, stream, view(A), view(W), (float *)C, (long long)ldc);
+    G9_HIP(hipGetLastError());
+    return 0;
+}
+
+}  // extern "C"

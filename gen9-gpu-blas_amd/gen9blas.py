@@ -5,6 +5,10 @@
     C = gen9blas.sgemm(A.T, B, alpha=2.0)     # a transposed view travels as a transpose flag, not as a copy
     C = gen9blas.gemm_batched(A3, B3)         # (count, M, K) · (count, K, N) in one launch
     y = gen9blas.gemv(A, x); d = gen9blas.dot(x, y); gen9blas.axpy(0.5, x, y)
+    W = gen9blas.mx4_quantize(Wf)             # 4-bit weights (MX4); C = A·Wᵀ with them:
+    C = gen9blas.mx4_gemm(A, W)               # A float16, float32 or MX4
+    ids, w = gen9blas.moe_route(logits, 8)    # a mixture of experts: its router, and
+    y = gen9blas.moe_gemm(x, ids, We, weights=w)   # its experts' products on MX4 weights
 
 API contract (reference lib/gen9blas.py:96-610): the same public names, positional arguments and defaults.
 - The compute type follows the data: float16, float64, and float32 for every other element type.
@@ -134,8 +138,13 @@ def hip_stream():
     return _lib.gen9blas_hip_stream()
 
 
+_nowait = False
+
+
 def set_nowait(on):
     """No-wait mode: calls whose operands are all in device memory return once queued; flush() waits for them."""
+    global _nowait
+    _nowait = bool(on)
     _lib.gen9blas_set_nowait(1 if on else 0)
 
 
@@ -885,3 +894,224 @@ def spr2(alpha, x, y, Ap, uplo="L"):
     ap = _packed(Ap, t, vx.n, out=True)
     _call("spr2", _TYPE_CODE[t], _UPLO_CODE[uplo], vx.n, alpha, vx.ptr, vx.inc, vy.ptr, vy.inc, ap.ptr)
     return Ap
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# 4-bit weights (MX4) and mixtures of experts: libgen9blas_llm.so
+# ------------------------------------------------------------------------------------------------------------------
+# These operators work on GPU memory: torch GPU tensors in place, and NumPy arrays (or CPU tensors) through a copy to
+# the GPU and back. float16 computes from float16 and gives float16; every other type is converted to float32.
+_LLM_SIGNATURES = """
+    llm_error=s:  llm_last_status=i:  mx4_create=p:iii  mx4_free=v:p  mx4_quantize=i:ipilp  mx4_load=i:pipip
+    mx4_dequantize=i:ppil  mx4_gemm=i:iipippi  mx4_gemm_q=i:ipppi  moe_route=i:iiipipiiiiifpp
+    moe_gemm=i:iiippllppppll
+"""
+_llm = None
+
+
+def _llm_library():
+    """libgen9blas_llm.so, loaded at first use from the directory of libgen9blas.so."""
+    global _llm
+    if _llm is None:
+        _torch_module()
+        _init()
+        lib = ctypes.CDLL(os.path.join(os.path.dirname(_library_path()), "libgen9blas_llm.so"))
+        for item in _LLM_SIGNATURES.split():
+            name, sig = item.split("=")
+            result, args = sig.split(":")
+            fn = getattr(lib, "gen9blas_" + name)
+            fn.restype = _CTYPE[result]
+            fn.argtypes = [_CTYPE[c] for c in args]
+        _llm = lib
+    return _llm
+
+
+def _llm_call(fn, *args):
+    """fn(*args) on the library's stream, in order with torch's current one (its default stream orders itself), then a wait
+    unless in no-wait mode."""
+    current = _torch.cuda.current_stream()
+    side = current.cuda_stream != 0
+    if side:
+        ours = _torch.cuda.ExternalStream(hip_stream())
+        ours.wait_stream(current)
+    if fn(*args) != 0:
+        raise RuntimeError(_llm.gen9blas_llm_error().decode())
+    if side:
+        current.wait_stream(ours)
+    if not _nowait:
+        flush()
+
+
+def _device_rows(X, dims):
+    """X as a GPU tensor of float16 or float32 whose rows are contiguous, of one of the numbers of dimensions in `dims`."""
+    torch = _torch
+    if not (_is_tensor(X) and X.is_cuda):
+        X = torch.as_tensor(X).cuda()
+    if X.dim() not in dims:
+        raise ValueError(f"expected {' or '.join(map(str, dims))} dimensions, got {X.dim()}")
+    if X.dtype != torch.float16 and X.dtype != torch.float32:
+        X = X.float()
+    return X if X.stride(-1) == 1 or X.shape[-1] <= 1 else X.contiguous()
+
+
+def _host_like(X, result):
+    """`result` where X lives: a GPU tensor, or for host operands a NumPy array."""
+    if (_is_tensor(X) and X.is_cuda) or hasattr(X, "__cuda_array_interface__") or isinstance(X, MX4):
+        return result
+    return result.cpu().numpy()
+
+
+def _llm_out(C, shape, dtype, what="C"):
+    """The given result, or a new one: a GPU tensor of this shape and type with contiguous rows."""
+    if C is None:
+        return _torch.empty(shape, dtype=dtype, device="cuda")
+    if not (_is_tensor(C) and C.is_cuda and C.shape == tuple(shape) and C.dtype == dtype and (C.stride(-1) == 1 or shape[-1] <= 1)):
+        raise ValueError(f"{what} must be a GPU tensor of shape {tuple(shape)} and type {dtype} with contiguous rows")
+    return C
+
+
+def _row_step(X, dim=-2):
+    """Stride between rows, at least the row's length (a dimension of one has any stride)."""
+    return X.stride(dim) if X.shape[dim] > 1 else max(X.shape[-1], 1)
+
+
+class MX4:
+    """A matrix (rows, K), or a stack of them (count, rows, K), in microscaled 4-bit floating point on the GPU: E2M1 values,
+    one power-of-two scale for each 32 consecutive values of a row. Zeros until it is filled by mx4_quantize or mx4_load."""
+
+    def __init__(self, *shape):
+        lib = _llm_library()
+        self._handle = None
+        self.shape = tuple(int(n) for n in shape)
+        if len(self.shape) not in (2, 3):
+            raise ValueError("MX4 matrices have a shape (rows, K) or (count, rows, K)")
+        self.count = self.shape[0] if len(self.shape) == 3 else 1
+        self._handle = lib.gen9blas_mx4_create(self.count, *self.shape[-2:])
+        if not self._handle:
+            raise RuntimeError(lib.gen9blas_llm_error().decode())
+
+    def __del__(self):
+        if getattr(self, "_handle", None) and not _exiting:
+            _llm.gen9blas_mx4_free(self._handle)
+            self._handle = None
+
+
+def mx4_quantize(X, out=None):
+    """X, (rows, K) or (count, rows, K), rounded to MX4 (a new one, or `out` of the same shape). A block's scale is
+    2^(floor(log2 max|x|) - 2); values round to the nearest, ties to even codes, beyond 6 scales to 6."""
+    lib = _llm_library()
+    X = _device_rows(X, (2, 3))
+    if out is None:
+        out = MX4(*X.shape)
+    elif out.shape != tuple(X.shape):
+        raise ValueError(f"X has shape {tuple(X.shape)}, the MX4 matrix {out.shape}")
+    _llm_call(lib.gen9blas_mx4_quantize, 1 if X.dtype == _torch.float32 else 0, X.data_ptr(), _row_step(X),
+              X.stride(0) if X.dim() == 3 else 0, out._handle)
+    return out
+
+
+def mx4_load(codes, scales, K=None):
+    """An MX4 matrix, or a stack of them, from a checkpoint's uint8 rows: codes (..., rows, K/2), two to a byte, the even one
+    in the low half; scales (..., rows, K/32), the exponent + 127. K defaults to twice the width of codes."""
+    lib = _llm_library()
+    torch = _torch
+    c, s = (x if _is_tensor(x) and x.is_cuda else torch.as_tensor(x).cuda() for x in (codes, scales))
+    if c.dtype != torch.uint8 or s.dtype != torch.uint8:
+        raise TypeError("codes and scales are uint8")
+    K = 2 * c.shape[-1] if K is None else int(K)
+    want = (*c.shape[:-1], -(-K // 32))
+    if c.dim() not in (2, 3) or c.shape[-1] != -(-K // 2) or tuple(s.shape) != want:
+        raise ValueError(f"codes {tuple(c.shape)} and scales {tuple(s.shape)} do not belong to rows of {K} values")
+    q = MX4(*c.shape[:-1], K)
+    c, s = c.contiguous(), s.contiguous()
+    _llm_call(lib.gen9blas_mx4_load, c.data_ptr(), c.shape[-1], s.data_ptr(), s.shape[-1], q._handle)
+    return q
+
+
+def mx4_dequantize(Q, out=None):
+    """The values of an MX4 matrix in float32."""
+    lib = _llm_library()
+    X = _llm_out(out, Q.shape, _torch.float32, "out")
+    _llm_call(lib.gen9blas_mx4_dequantize, Q._handle, X.data_ptr(), _row_step(X), X.stride(0) if X.dim() == 3 else 0)
+    return X
+
+
+def mx4_gemm(A, W, C=None, dtype=None):
+    """C = A·Wᵀ, W an MX4 matrix (N, K). A (M, K): float16 or float32, and C in the same type; or MX4, and C in `dtype`
+    (np.float16 by default, or the type of a given C)."""
+    lib = _llm_library()
+    torch = _torch
+    if isinstance(A, MX4):
+        if len(A.shape) != 2 or len(W.shape) != 2 or A.shape[1] != W.shape[1]:
+            raise ValueError(f"incompatible dimensions: {A.shape} · {W.shape}ᵀ")
+        if C is not None:
+            t = C.dtype
+        else:
+            t = _torch_dtype(np.dtype(np.float16 if dtype is None else dtype))
+        if t != torch.float16 and t != torch.float32:
+            raise TypeError("C must be float16 or float32")
+        C = _llm_out(C, (A.shape[0], W.shape[0]), t)
+        _llm_call(lib.gen9blas_mx4_gemm_q, 1 if t == torch.float32 else 0, A._handle, W._handle, C.data_ptr(), _row_step(C))
+        return C
+    a = _device_rows(A, (2,))
+    if len(W.shape) != 2 or a.shape[1] != W.shape[1]:
+        raise ValueError(f"incompatible dimensions: {tuple(a.shape)} · {W.shape}ᵀ")
+    out = _llm_out(C, (a.shape[0], W.shape[0]), a.dtype)
+    _llm_call(lib.gen9blas_mx4_gemm, 1 if a.dtype == torch.float32 else 0, a.shape[0], a.data_ptr(), _row_step(a), W._handle,
+              out.data_ptr(), _row_step(out))
+    return _host_like(A, out) if C is None else out
+
+
+_SCORE_CODE = {"softmax": 0, "sigmoid": 1}
+
+
+def moe_route(logits, k, bias=None, score="softmax", groups=1, top_groups=1, renorm=True, scale=1.0, out=None):
+    """The k experts of each token, from a router's logits (T, experts): (ids, weights), int32 and float32 of shape (T, k), by
+    falling choice. choice: the score ("softmax" or "sigmoid") plus bias; groups > 1: only from the top_groups best groups.
+    weights: the scores without bias, divided by their sum if renorm, times scale. Masked experts (logit -inf) are never
+    chosen; places left over get id -1 and weight 0. `out`: (ids, weights) to write into."""
+    lib = _llm_library()
+    torch = _torch
+    x = _device_rows(logits, (2,))
+    T, E = x.shape
+    if bias is not None:
+        bias = _device_rows(bias, (1,)).float().contiguous()
+        if bias.shape[0] != E:
+            raise ValueError(f"bias has {bias.shape[0]} elements for {E} experts")
+    ids = _llm_out(out[0] if out else None, (T, k), torch.int32, "ids")
+    w = _llm_out(out[1] if out else None, (T, k), torch.float32, "weights")
+    if not (ids.is_contiguous() and w.is_contiguous()):
+        raise ValueError("ids and weights must be contiguous")
+    _llm_call(lib.gen9blas_moe_route, 1 if x.dtype == torch.float32 else 0, T, E, x.data_ptr(), _row_step(x),
+              None if bias is None else bias.data_ptr(), _SCORE_CODE[score], groups, top_groups, k, bool(renorm), scale,
+              ids.data_ptr(), w.data_ptr())
+    return (ids, w) if out else (_host_like(logits, ids), _host_like(logits, w))
+
+
+def moe_gemm(X, ids, W, gate=None, weights=None, C=None):
+    """The products of each token's rows with its experts' weights: W an MX4 stack (experts, N, K), ids (T, S) int32.
+    X (T, K): one row for all places of a token, or (T, S, K). y[t, s] = X[t(, s)]·W[ids[t, s]]ᵀ, and with `gate` (as W)
+    silu(X[t(, s)]·gate[ids[t, s]]ᵀ)·y[t, s]. The result is y (T, S, N), or with weights (T, S) float32 the sum over s of
+    weights[t, s]·y[t, s] (T, N). An id that is no expert's (-1) is an empty place, its y is zero."""
+    lib = _llm_library()
+    torch = _torch
+    x = _device_rows(X, (2, 3))
+    i = ids if _is_tensor(ids) and ids.is_cuda else torch.as_tensor(ids).cuda()
+    i = i.to(torch.int32).contiguous()
+    if i.dim() != 2 or len(W.shape) != 3 or x.shape[-1] != W.shape[2] or x.shape[0] != i.shape[0] or \
+            (x.dim() == 3 and x.shape[1] != i.shape[1]) or (gate is not None and gate.shape != W.shape):
+        raise ValueError(f"incompatible shapes: X {tuple(x.shape)}, ids {tuple(i.shape)}, W {W.shape}"
+                         + (f", gate {gate.shape}" if gate is not None else ""))
+    (T, S), N = i.shape, W.shape[1]
+    if weights is not None:
+        weights = _device_rows(weights, (2,)).float().contiguous()
+        if weights.shape != i.shape:
+            raise ValueError(f"weights {tuple(weights.shape)} for ids {tuple(i.shape)}")
+    out = _llm_out(C, (T, N) if weights is not None else (T, S, N), x.dtype)
+    lds = 0 if x.dim() == 2 else _row_step(x, 1)
+    ldt = x.stride(0) if T > 1 else max(lds * S, x.shape[-1])
+    ldcs = N if weights is not None else _row_step(out, 1)
+    ldct = out.stride(0) if T > 1 else ldcs * max(S, 1)
+    _llm_call(lib.gen9blas_moe_gemm, 1 if x.dtype == torch.float32 else 0, T, S, i.data_ptr(), x.data_ptr(), ldt, lds, W._handle,
+              None if gate is None else gate._handle, None if weights is None else weights.data_ptr(), out.data_ptr(), ldct, ldcs)
+    return _host_like(X, out) if C is None else out
