@@ -1,5 +1,5 @@
 // Mixture of experts: the router (gen9blas_moe_route) and the products of each token's experts (gen9blas_moe_gemm).
-#include "mx4_gemm_kernel.h"
+#include "mx4_tile_kernel.h"
 
 namespace g9llm {
 
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(256) moe_route_kernel(RouteArgs a) {
 }
 
 // The plan of a grouped product: slots by expert (order; places whose id is no expert come last, as expert E), off[e] where
-// expert e's begin, and the tiles of `rows` slots: (expert, first place), (−1, 0) past the last. One workgroup. The order of
+// expert e's begin, and the tiles of `rows` slots: (expert, first place), (−1, 0) past the last, their number in front. One workgroup. The order of
 // a group's slots varies from call to call; no result depends on it.
 __global__ void __launch_bounds__(1024) moe_plan_kernel(const int *__restrict__ ids, long long n, int E, int rows, int *order, int *off,
                                                         int *tiles, int most) {
@@ -171,6 +171,7 @@ __global__ void __launch_bounds__(1024) moe_plan_kernel(const int *__restrict__ 
             b += count[e], t += (count[e] + rows - 1) / rows;
         }
         base[E + 1] = b, tile0[E + 1] = t;
+        tiles[-1] = t;
     }
     __syncthreads();
     for (int e = threadIdx.x; e <= E + 1; e += 1024) {
@@ -211,7 +212,17 @@ template <class T> static int launch_route(const RouteArgs &a) {
     return 0;
 }
 
-template <class T, class O, bool GATED> static int launch_grouped(const Rows &R, const Mx4View &W, const Mx4View &G, int E, int most) {
+template <class T, class O, bool GATED> static int launch_grouped(const Rows &R, const Mx4View &W, const Mx4View &G, int E, int most, int rows, int Tn) {
+    if (rows > 32) {
+        Planes A;
+        G9_TRY(stage_planes<T>(R, Tn, W.K, W.kc, &A));
+        const int ntiles = (int)cdiv(W.rt, GATED ? 8 : 16);
+        const dim3 grid((unsigned)(cdiv((long long)most * ntiles, 8) * 8)), block(256);
+        if (rows == 64) hipLaunchKernelGGL((mx4_gemm_tile_kernel<T, O, 4, true, GATED>), grid, block, 0, stream, A, R, W, G, E, 0, ntiles);
+        else hipLaunchKernelGGL((mx4_gemm_tile_kernel<T, O, 8, true, GATED>), grid, block, 0, stream, A, R, W, G, E, 0, ntiles);
+        G9_HIP(hipGetLastError());
+        return 0;
+    }
     hipLaunchKernelGGL((mx4_gemm_any_kernel<T, O, 2, true, GATED>), dim3((unsigned)((long long)most * W.rt)), dim3(256), 0, stream, R, W, G, E);
     G9_HIP(hipGetLastError());
     return 0;
@@ -221,22 +232,22 @@ template <class T>
 static int experts(int Tn, int S, const int *ids, const void *X, int64_t ldt, int64_t lds, const gen9blas_mx4 *W, const gen9blas_mx4 *gate,
                    const float *weights, void *C, int64_t ldct, int64_t ldcs) {
     const long long n = (long long)Tn * S;
-    const int E = W->count, N = W->rows, rows = 32;
+    const int E = W->count, N = W->rows, rows = n > 64LL * E ? 128 : n > 16LL * E ? 64 : 32;
     const long long most = cdiv(n, rows) + E + 1;
     if (most * W->rt > 0xffffff || n > 0x7fffffff)
         G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "moe_gemm: more tiles than one launch can index");
     void *plan = nullptr, *slots = nullptr;
-    G9_TRY(scratch(SLOT_PLAN, (size_t)(n + E + 2 + 2 * most) * 4, &plan));
+    G9_TRY(scratch(SLOT_PLAN, (size_t)(n + E + 3 + 2 * most) * 4, &plan));
     if (weights) G9_TRY(scratch(SLOT_SLOTS, (size_t)n * N * 4, &slots));
-    int *order = (int *)plan, *off = order + n, *tiles = off + E + 2;
+    int *order = (int *)plan, *off = order + n, *tiles = off + E + 3;
     hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(1024), 0, stream, ids, n, E, rows, order, off, tiles, (int)most);
     G9_HIP(hipGetLastError());
     Rows R = {X, C, ldt, lds, ldct, ldcs, 0, S, tiles, order, off};
     const Mx4View w = view(W), g = gate ? view(gate) : w;
     if (!weights)
-        return gate ? launch_grouped<T, T, true>(R, w, g, E, (int)most) : launch_grouped<T, T, false>(R, w, g, E, (int)most);
+        return gate ? launch_grouped<T, T, true>(R, w, g, E, (int)most, rows, Tn) : launch_grouped<T, T, false>(R, w, g, E, (int)most, rows, Tn);
     R.C = slots, R.ldct = (long long)S * N, R.ldcs = N;
-    G9_TRY((gate ? launch_grouped<T, float, true>(R, w, g, E, (int)most) : launch_grouped<T, float, false>(R, w, g, E, (int)most)));
+    G9_TRY((gate ? launch_grouped<T, float, true>(R, w, g, E, (int)most, rows, Tn) : launch_grouped<T, float, false>(R, w, g, E, (int)most, rows, Tn)));
     for (int t0 = 0; t0 < Tn; t0 += 65535) {   // the grid's y limit
         const int rowsy = min(Tn - t0, 65535);
         hipLaunchKernelGGL((moe_join_kernel<T>), dim3((unsigned)cdiv(N, 256), (unsigned)rowsy), dim3(256), 0, stream,

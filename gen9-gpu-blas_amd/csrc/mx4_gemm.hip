@@ -1,5 +1,5 @@
 // gen9blas_mx4_gemm and gen9blas_mx4_gemm_q: products of FP16, FP32 or MX4 rows with MX4 weights.
-#include "mx4_gemm_kernel.h"
+#include "mx4_tile_kernel.h"
 
 namespace g9llm {
 
@@ -62,7 +62,18 @@ __global__ void __launch_bounds__(256) mx4_gemm_q_any_kernel(Mx4View A, Mx4View 
     }
 }
 
+template <class T, int MT> static int launch_tiles(const Rows &R, const Mx4View &W) {
+    Planes A;
+    G9_TRY(stage_planes<T>(R, R.M, W.K, W.kc, &A));
+    const long long mtiles = cdiv(R.M, MT * 16), ntiles = cdiv(W.rt, 16), wgs = cdiv(mtiles * ntiles, 8) * 8;
+    if (wgs > 0xffffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm: more tiles than one launch can index");
+    hipLaunchKernelGGL((mx4_gemm_tile_kernel<T, T, MT, false, false>), dim3((unsigned)wgs), dim3(256), 0, stream, A, R, W, W, 1, (int)mtiles, (int)ntiles);
+    G9_HIP(hipGetLastError());
+    return 0;
+}
+
 template <class T> static int launch_dense(const Rows &R, const Mx4View &W) {
+    if (R.M > 64) return R.M > 192 ? launch_tiles<T, 8>(R, W) : launch_tiles<T, 4>(R, W);
     const long long wgs = cdiv(R.M, 32) * W.rt;
     if (wgs > 0xffffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm: more tiles than one launch can index");
     if (R.M <= 16)
