@@ -1,9 +1,8 @@
 // gen9blas_mx4_gemm and gen9blas_mx4_gemm_q: products of FP16, FP32 or MX4 rows with MX4 weights.
 #include "mx4_tile_kernel.h"
+#include "mx4_q_kernel.h"
 
 namespace g9llm {
-
-typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 // Both operands MX4, any shape: a workgroup makes 64 rows × 16 columns, its 4 waves every fourth group of 512 k.
 template <class O>
@@ -62,6 +61,26 @@ __global__ void __launch_bounds__(256) mx4_gemm_q_any_kernel(Mx4View A, Mx4View 
     }
 }
 
+template <class O, int T> static int launch_q_tiles(const Mx4View &A, const Mx4View &W, O *C, long long ldc) {
+    constexpr int LDS = 4 * 4 * T * 1024 + 2 * 4 * T * 256;
+    static hipError_t allowed = hipFuncSetAttribute((const void *)mx4_gemm_q_tile_kernel<O, T>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    G9_HIP(allowed);
+    const long long mtiles = cdiv(A.rt, 2 * T), ntiles = cdiv(W.rt, 2 * T), wgs = cdiv(mtiles * ntiles, 8) * 8;
+    if (wgs > 0xffffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm_q: more tiles than one launch can index");
+    hipLaunchKernelGGL((mx4_gemm_q_tile_kernel<O, T>), dim3((unsigned)wgs), dim3(256), LDS, stream, A, W, C, ldc, (int)mtiles, (int)ntiles);
+    G9_HIP(hipGetLastError());
+    return 0;
+}
+
+template <class O> static int launch_q(const Mx4View &A, const Mx4View &W, O *C, long long ldc) {
+    if (A.rt > 4) return cdiv(A.rt, 16) * cdiv(W.rt, 16) >= num_cus ? launch_q_tiles<O, 8>(A, W, C, ldc) : launch_q_tiles<O, 4>(A, W, C, ldc);
+    const long long wgs = cdiv(A.rt, 4) * W.rt;
+    if (wgs > 0xffffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm_q: more tiles than one launch can index");
+    hipLaunchKernelGGL((mx4_gemm_q_any_kernel<O>), dim3((unsigned)wgs), dim3(256), 0, stream, A, W, C, ldc);
+    G9_HIP(hipGetLastError());
+    return 0;
+}
+
 template <class T, int MT> static int launch_tiles(const Rows &R, const Mx4View &W) {
     Planes A;
     G9_TRY(stage_planes<T>(R, R.M, W.K, W.kc, &A));
@@ -109,15 +128,7 @@ int gen9blas_mx4_gemm_q(int type, const gen9blas_mx4 *A, const gen9blas_mx4 *W, 
     if (!A || !W || A->count != 1 || W->count != 1) G9_FAIL(GEN9BLAS_ERR_INVALID_ARG, "mx4_gemm_q: %s", A && W ? "an operand holds several matrices" : "no A or no W");
     if (A->K != W->K || ldc < W->rows) G9_FAIL(GEN9BLAS_ERR_INVALID_ARG, "mx4_gemm_q: K %d and %d, ldc %d, N %d", A->K, W->K, ldc, W->rows);
     G9_TRY(need_device(C, ((size_t)(A->rows - 1) * ldc + W->rows) * elem_size(type), "mx4_gemm_q: C"));
-    const long long wgs = cdiv(A->rt, 4) * W->rt;
-    if (wgs > 0xffffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm_q: more tiles than one launch can index");
-    const dim3 grid((unsigned)wgs), block(256);
-    if (type == GEN9BLAS_H)
-        hipLaunchKernelGGL((mx4_gemm_q_any_kernel<_Float16>), grid, block, 0, stream, view(A), view(W), (_Float16 *)C, (long long)ldc);
-    else
-        hipLaunchKernelGGL((mx4_gemm_q_any_kernel<float>), grid, block, 0, stream, view(A), view(W), (float *)C, (long long)ldc);
-    G9_HIP(hipGetLastError());
-    return 0;
+    return type == GEN9BLAS_H ? launch_q<_Float16>(view(A), view(W), (_Float16 *)C, ldc) : launch_q<float>(view(A), view(W), (float *)C, ldc);
 }
 
 }  // extern "C"
