@@ -22,7 +22,7 @@
 
 struct gen9blas_mx4 {
     int count, rows, K;
-    int rt, kc, kg, kt;        // row tiles, tiles and groups along k, bytes of `top` a row (kg rounded up to 4)
+    int rt, kc, kg, kt;        // row tiles, tiles and groups along k, bytes of `top` a row (kg rounded up to 16)
     uint8_t *codes;            // [count][rt][kc][64][16]
     uint8_t *scales;           // [count][rt][kg][64][4]
     uint8_t *top;              // [count][rt][16][kt]
@@ -55,6 +55,14 @@ struct Mx4View {
     int rows, K, rt, kc, kg, kt;
 };
 inline Mx4View view(const gen9blas_mx4 *q) { return {q->codes, q->scales, q->top, q->rows, q->K, q->rt, q->kc, q->kg, q->kt}; }
+
+// A product whose k is split among `parts` workgroups: each leaves its FP32 sums in a plane of rows × ld (gated: two, W's and
+// the gate's), and a second kernel adds the planes in their order.
+struct Split {
+    int parts;
+    float *sums;
+    long long rows, ld;
+};
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));

@@ -1,5 +1,7 @@
 // Mixture of experts: the router (gen9blas_moe_route) and the products of each token's experts (gen9blas_moe_gemm).
 #include "mx4_tile_kernel.h"
+#include "mx4_rows_kernel.h"
+#include <algorithm>
 
 namespace g9llm {
 
@@ -152,39 +154,57 @@ __global__ void __launch_bounds__(256) moe_route_kernel(RouteArgs a) {
 }
 
 // The plan of a grouped product: slots by expert (order; places whose id is no expert come last, as expert E), off[e] where
-// expert e's begin, and the tiles of `rows` slots: (expert, first place), (−1, 0) past the last, their number in front. One workgroup. The order of
-// a group's slots varies from call to call; no result depends on it.
-__global__ void __launch_bounds__(1024) moe_plan_kernel(const int *__restrict__ ids, long long n, int E, int rows, int *order, int *off,
-                                                        int *tiles, int most) {
-    __shared__ int count[MAX_EXPERTS + 1], base[MAX_EXPERTS + 2], tile0[MAX_EXPERTS + 2];
-    for (int i = threadIdx.x; i <= E; i += 1024) count[i] = 0;
-    __syncthreads();
-    for (long long i = threadIdx.x; i < n; i += 1024) {
-        const unsigned e = (unsigned)ids[i];
-        atomicAdd(&count[e < (unsigned)E ? e : E], 1);
+// expert e's begin, and the tiles of `rows` slots: (expert, first place), (−1, 0) past the last, their number in front. One
+// workgroup: the ids are counted in LDS, a scan gives each expert's place, and the ids are read again to be placed. The order
+// of a group's slots varies from call to call; no result depends on it.
+__device__ __forceinline__ int2 scan_pair(int2 v, int lane) {   // sums over the lanes up to this one
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int x = __shfl_up(v.x, d), y = __shfl_up(v.y, d);
+        if (lane >= d) v.x += x, v.y += y;
     }
+    return v;
+}
+__global__ void __launch_bounds__(1024) moe_plan_kernel(const int *__restrict__ ids, int n, int E, int rows, int *order, int *off, int *tiles, int most) {
+    __shared__ int count[MAX_EXPERTS + 1], base[MAX_EXPERTS + 1];
+    __shared__ int2 waves[16];
+    const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+    for (int i = t; i <= E; i += 1024) count[i] = 0;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        int b = 0, t = 0;
-        for (int e = 0; e <= E; e++) {
-            base[e] = b, tile0[e] = t;
-            b += count[e], t += (count[e] + rows - 1) / rows;
+    // eight ids of a thread are on their way at a time
+    auto each = [&](auto use) {
+        for (long long i0 = t; i0 < n; i0 += 8 * 1024) {
+            int id[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) id[j] = i0 + j * 1024 < n ? ids[i0 + j * 1024] : 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (i0 + j * 1024 < n) use((unsigned)id[j] < (unsigned)E ? id[j] : E, (int)(i0 + j * 1024));
         }
-        base[E + 1] = b, tile0[E + 1] = t;
-        tiles[-1] = t;
-    }
+    };
+    each([&](int e, int) { atomicAdd(&count[e], 1); });
     __syncthreads();
-    for (int e = threadIdx.x; e <= E + 1; e += 1024) {
-        off[e] = base[e];
-        if (e <= E)
-            for (int t = tile0[e]; t < tile0[e + 1]; t++) tiles[2 * t] = e, tiles[2 * t + 1] = base[e] + (t - tile0[e]) * rows;
-    }
-    for (int t = tile0[E + 1] + threadIdx.x; t < most; t += 1024) tiles[2 * t] = -1, tiles[2 * t + 1] = 0;
+    const int mine = t < E ? count[t] : 0, own = (mine + rows - 1) / rows;
+    const int2 s = scan_pair({mine, own}, lane);
+    if (lane == 63) waves[wv] = s;
     __syncthreads();
-    for (long long i = threadIdx.x; i < n; i += 1024) {
-        const unsigned e = (unsigned)ids[i];
-        order[atomicAdd(&base[e < (unsigned)E ? e : E], 1)] = (int)i;
+    int2 before = {s.x - mine, s.y - own};
+    for (int w = 0; w < wv; w++) before.x += waves[w].x, before.y += waves[w].y;
+    auto put = [&](int e, int first, int tile, int c) {
+        base[e] = first, off[e] = first;
+        for (int i = 0; i * rows < c; i++) tiles[2 * (tile + i)] = e, tiles[2 * (tile + i) + 1] = first + i * rows;
+    };
+    if (t < E) put(t, before.x, before.y, mine);
+    int2 all = {0, 0};
+    for (int w = 0; w < 16; w++) all.x += waves[w].x, all.y += waves[w].y;
+    const int last = all.y + (count[E] + rows - 1) / rows;
+    if (t == 0) {
+        put(E, all.x, all.y, count[E]);
+        off[E + 1] = n, tiles[-1] = last;
     }
+    for (int i = last + t; i < most; i += 1024) tiles[2 * i] = -1, tiles[2 * i + 1] = 0;
+    __syncthreads();
+    each([&](int e, int i) { order[atomicAdd(&base[e], 1)] = i; });
 }
 
 // C(t) = Σ_s weights(t, s) · y(t, s), in the order of s; places that are no expert's are left out.
@@ -212,7 +232,7 @@ template <class T> static int launch_route(const RouteArgs &a) {
     return 0;
 }
 
-template <class T, class O, bool GATED> static int launch_grouped(const Rows &R, const Mx4View &W, const Mx4View &G, int E, int most, int rows, int Tn) {
+template <class T, class O, bool GATED> static int launch_grouped(const Rows &R, const Mx4View &W, const Mx4View &G, int E, int most, int rows, int Tn, long long n) {
     if (rows > 32) {
         Planes A;
         G9_TRY(stage_planes<T>(R, Tn, W.K, W.kc, &A));
@@ -223,7 +243,23 @@ template <class T, class O, bool GATED> static int launch_grouped(const Rows &R,
         G9_HIP(hipGetLastError());
         return 0;
     }
-    hipLaunchKernelGGL((mx4_gemm_any_kernel<T, O, 2, true, GATED>), dim3((unsigned)((long long)most * W.rt)), dim3(256), 0, stream, R, W, G, E);
+    const Split whole = {1, nullptr, 0, 0};
+    // few: 8 waves share the rows of a chunk, 128·NT columns a workgroup; rows: each wave has its own, 16·NT columns
+    auto few = [&](auto kernel, int cols) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(most * cdiv(W.rt, cols))), dim3(512), 0, stream, R, W, G, E, (int)cdiv(W.rt, cols), whole);
+    };
+    if (rows == 32)
+        // gated, FP16 44 × 4 places of 16 experts, 832 × 1664, and FP32 21 × 8, 768 × 4096: 16.6 and 49.5 µs; two column tiles a
+        // wave 24.3 and 75.3, the rows kernel 17.1 and 55.4
+        few(mx4_gemm_few_kernel<T, O, 2, 1, 4, true, GATED>, 8);
+    else if (sizeof(T) == 2)
+        // gated, 8 places, 1536 × 4096: 15.3 µs; few kernel 20.6 and more
+        hipLaunchKernelGGL((mx4_gemm_rows_kernel<T, O, 1, 1, 1, 2, true, GATED>), dim3((unsigned)((long long)most * W.rt)), dim3(256), 0, stream, R, W, G, E, W.rt, whole);
+    else if (std::min<long long>(n, E) * cdiv(W.rt, 16) >= 2LL * num_cus)
+        // 24 × 4 places of 64 experts, 4096 × 1536: 35.6 µs; one column tile a wave 41.3, the rows kernel 63
+        few(mx4_gemm_few_kernel<T, O, 1, 2, 4, true, GATED>, 16);
+    else
+        few(mx4_gemm_few_kernel<T, O, 1, 1, 4, true, GATED>, 8);
     G9_HIP(hipGetLastError());
     return 0;
 }
@@ -232,7 +268,7 @@ template <class T>
 static int experts(int Tn, int S, const int *ids, const void *X, int64_t ldt, int64_t lds, const gen9blas_mx4 *W, const gen9blas_mx4 *gate,
                    const float *weights, void *C, int64_t ldct, int64_t ldcs) {
     const long long n = (long long)Tn * S;
-    const int E = W->count, N = W->rows, rows = n > 64LL * E ? 128 : n > 16LL * E ? 64 : 32;
+    const int E = W->count, N = W->rows, rows = n > 64LL * E ? 128 : n > 16LL * E ? 64 : n > 8LL * E ? 32 : 16;
     const long long most = cdiv(n, rows) + E + 1;
     if (most * W->rt > 0xffffff || n > 0x7fffffff)
         G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "moe_gemm: more tiles than one launch can index");
@@ -240,14 +276,14 @@ static int experts(int Tn, int S, const int *ids, const void *X, int64_t ldt, in
     G9_TRY(scratch(SLOT_PLAN, (size_t)(n + E + 3 + 2 * most) * 4, &plan));
     if (weights) G9_TRY(scratch(SLOT_SLOTS, (size_t)n * N * 4, &slots));
     int *order = (int *)plan, *off = order + n, *tiles = off + E + 3;
-    hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(1024), 0, stream, ids, n, E, rows, order, off, tiles, (int)most);
+    hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(1024), 0, stream, ids, (int)n, E, rows, order, off, tiles, (int)most);
     G9_HIP(hipGetLastError());
     Rows R = {X, C, ldt, lds, ldct, ldcs, 0, S, tiles, order, off};
     const Mx4View w = view(W), g = gate ? view(gate) : w;
     if (!weights)
-        return gate ? launch_grouped<T, T, true>(R, w, g, E, (int)most, rows, Tn) : launch_grouped<T, T, false>(R, w, g, E, (int)most, rows, Tn);
+        return gate ? launch_grouped<T, T, true>(R, w, g, E, (int)most, rows, Tn, n) : launch_grouped<T, T, false>(R, w, g, E, (int)most, rows, Tn, n);
     R.C = slots, R.ldct = (long long)S * N, R.ldcs = N;
-    G9_TRY((gate ? launch_grouped<T, float, true>(R, w, g, E, (int)most, rows, Tn) : launch_grouped<T, float, false>(R, w, g, E, (int)most, rows, Tn)));
+    G9_TRY((gate ? launch_grouped<T, float, true>(R, w, g, E, (int)most, rows, Tn, n) : launch_grouped<T, float, false>(R, w, g, E, (int)most, rows, Tn, n)));
     for (int t0 = 0; t0 < Tn; t0 += 65535) {   // the grid's y limit
         const int rowsy = min(Tn - t0, 65535);
         hipLaunchKernelGGL((moe_join_kernel<T>), dim3((unsigned)cdiv(N, 256), (unsigned)rowsy), dim3(256), 0, stream,

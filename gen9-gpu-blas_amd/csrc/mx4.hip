@@ -170,7 +170,7 @@ gen9blas_mx4 *gen9blas_mx4_create(int count, int rows, int K) {
     }
     gen9blas_mx4 q;
     q.count = count, q.rows = rows, q.K = K;
-    q.rt = (int)cdiv(rows, 16), q.kc = (int)cdiv(K, 128), q.kg = (int)cdiv(q.kc, 4), q.kt = (int)cdiv(q.kg, 4) * 4;
+    q.rt = (int)cdiv(rows, 16), q.kc = (int)cdiv(K, 128), q.kg = (int)cdiv(q.kc, 4), q.kt = (int)cdiv(q.kg, 16) * 16;
     const long long tiles = (long long)count * q.rt;
     if (tiles * q.kg > 0xffffffLL) {
         fail(GEN9BLAS_ERR_UNSUPPORTED, "mx4_create: %d × %d × %d is more than one launch can index", count, rows, K);

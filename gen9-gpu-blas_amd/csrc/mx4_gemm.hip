@@ -1,6 +1,7 @@
 // gen9blas_mx4_gemm and gen9blas_mx4_gemm_q: products of FP16, FP32 or MX4 rows with MX4 weights.
 #include "mx4_tile_kernel.h"
 #include "mx4_q_kernel.h"
+#include "mx4_rows_kernel.h"
 
 namespace g9llm {
 
@@ -91,16 +92,61 @@ template <class T, int MT> static int launch_tiles(const Rows &R, const Mx4View 
     return 0;
 }
 
-template <class T> static int launch_dense(const Rows &R, const Mx4View &W) {
-    if (R.M > 64) return R.M > 192 ? launch_tiles<T, 8>(R, W) : launch_tiles<T, 4>(R, W);
-    const long long wgs = cdiv(R.M, 32) * W.rt;
-    if (wgs > 0xffffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm: more tiles than one launch can index");
-    if (R.M <= 16)
-        hipLaunchKernelGGL((mx4_gemm_any_kernel<T, T, 1, false, false>), dim3((unsigned)(cdiv(R.M, 16) * W.rt)), dim3(256), 0, stream, R, W, W, 1);
-    else
-        hipLaunchKernelGGL((mx4_gemm_any_kernel<T, T, 2, false, false>), dim3((unsigned)wgs), dim3(256), 0, stream, R, W, W, 1);
+static int split_space(const Rows &R, const Mx4View &W, Split *s) {
+    s->rows = R.M, s->ld = (long long)W.rt * 16;
+    return scratch(SLOT_PART, (size_t)s->parts * s->rows * s->ld * 4, (void **)&s->sums);
+}
+template <class O> static int sum_parts(const Rows &R, const Mx4View &W, const Split &split) {
+    if (split.parts > 1)
+        hipLaunchKernelGGL((mx4_sum_parts_kernel<O>), dim3((unsigned)cdiv(split.rows * split.ld, 256)), dim3(256), 0, stream, R, split, W.rows);
     G9_HIP(hipGetLastError());
     return 0;
+}
+
+// Tiles of MT·16 rows × WN·NT·16 columns; k is split until there is about a workgroup a CU.
+template <class T, int MT, int NT, int WN, int D> static int launch_rows(const Rows &R, const Mx4View &W, int mtiles) {
+    const int ntiles = (int)cdiv(W.rt, NT * WN);
+    const long long tiles = (long long)mtiles * ntiles;
+    Split split = {1, nullptr, 0, 0};
+    const int ways = (int)(num_cus / tiles), most = W.kc / (4 / WN * 2);
+    if (ways > 1 && most > 1) {
+        split.parts = ways < most ? ways : most;
+        G9_TRY(split_space(R, W, &split));
+    }
+    if (tiles * split.parts > 0xffffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm: more tiles than one launch can index");
+    hipLaunchKernelGGL((mx4_gemm_rows_kernel<T, T, MT, NT, WN, D, false, false>), dim3((unsigned)(tiles * split.parts)), dim3(256), 0, stream, R, W, W, 1, ntiles, split);
+    G9_HIP(hipGetLastError());
+    return sum_parts<T>(R, W, split);
+}
+
+// Tiles of MT·16 rows × 128·NT columns; k is split until there is about a workgroup a CU.
+template <class T, int MT, int NT, int D> static int launch_few(const Rows &R, const Mx4View &W) {
+    const int ntiles = (int)cdiv(W.rt, NT * 8);
+    const long long tiles = cdiv(R.M, MT * 16) * ntiles;
+    Split split = {1, nullptr, 0, 0};
+    const int ways = (int)(num_cus / tiles), most = W.kc / 2;
+    if (ways > 1 && most > 1) {
+        split.parts = ways < most ? ways : most;
+        G9_TRY(split_space(R, W, &split));
+    }
+    if (tiles * split.parts > 0x7fffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm: more tiles than one launch can index");
+    hipLaunchKernelGGL((mx4_gemm_few_kernel<T, T, MT, NT, D, false, false>), dim3((unsigned)(tiles * split.parts)), dim3(512), 0, stream, R, W, W, 1, ntiles, split);
+    G9_HIP(hipGetLastError());
+    return sum_parts<T>(R, W, split);
+}
+
+template <class T> static int launch_dense(const Rows &R, const Mx4View &W) {
+    if (R.M > 64) return R.M > 192 ? launch_tiles<T, 8>(R, W) : launch_tiles<T, 4>(R, W);
+    constexpr bool F = sizeof(T) == 4;
+    // µs of the product alone, FP16 1 × 11008 × 4096 and FP32 8 × 4096 × 11008: rows kernel 9.4 and 13.2, few kernel 8.8 to
+    // 9.5 and 10.7: FP32 rows are taken apart once a workgroup there, and once a wave in the rows kernel.
+    if (R.M <= 16) {
+        if (F) return launch_few<T, 1, 2, 4>(R, W);
+        else return launch_rows<T, 1, 1, 1, 4>(R, W, 1);
+    }
+    // 24 × 4096 × 11008: 128 columns a workgroup 10.4 FP16 and 17.3 FP32, 256 columns 13.0 and 16.7
+    if (R.M <= 32) return launch_few<T, 2, F ? 2 : 1, 4>(R, W);
+    return launch_few<T, 4, 1, 2>(R, W);
 }
 
 }  // namespace g9llm

@@ -907,14 +907,18 @@ _LLM_SIGNATURES = """
     moe_gemm=i:iiippllppppll
 """
 _llm = None
+_llm_device = 0        # torch's index of the library's device
+_raw_stream = None     # torch's current stream on it as an int: the public torch.cuda.current_stream() takes 2.7 us
 
 
 def _llm_library():
     """libgen9blas_llm.so, loaded at first use from the directory of libgen9blas.so."""
-    global _llm
+    global _llm, _llm_device, _raw_stream
     if _llm is None:
-        _torch_module()
+        torch = _torch_module()
         _init()
+        _llm_device = torch.cuda.current_device()
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
         lib = ctypes.CDLL(os.path.join(os.path.dirname(_library_path()), "libgen9blas_llm.so"))
         for item in _LLM_SIGNATURES.split():
             name, sig = item.split("=")
@@ -929,15 +933,16 @@ def _llm_library():
 def _llm_call(fn, *args):
     """fn(*args) on the library's stream, in order with torch's current one (its default stream orders itself), then a wait
     unless in no-wait mode."""
-    current = _torch.cuda.current_stream()
-    side = current.cuda_stream != 0
-    if side:
-        ours = _torch.cuda.ExternalStream(hip_stream())
+    if _raw_stream(_llm_device) == 0:
+        if fn(*args) != 0:
+            raise RuntimeError(_llm.gen9blas_llm_error().decode())
+    else:
+        current, ours = _torch.cuda.current_stream(), _torch.cuda.ExternalStream(hip_stream())
         ours.wait_stream(current)
-    if fn(*args) != 0:
-        raise RuntimeError(_llm.gen9blas_llm_error().decode())
-    if side:
+        rc = fn(*args)
         current.wait_stream(ours)
+        if rc != 0:
+            raise RuntimeError(_llm.gen9blas_llm_error().decode())
     if not _nowait:
         flush()
 
@@ -945,18 +950,18 @@ def _llm_call(fn, *args):
 def _device_rows(X, dims):
     """X as a GPU tensor of float16 or float32 whose rows are contiguous, of one of the numbers of dimensions in `dims`."""
     torch = _torch
-    if not (_is_tensor(X) and X.is_cuda):
+    if not (isinstance(X, torch.Tensor) and X.is_cuda):
         X = torch.as_tensor(X).cuda()
     if X.dim() not in dims:
         raise ValueError(f"expected {' or '.join(map(str, dims))} dimensions, got {X.dim()}")
-    if X.dtype != torch.float16 and X.dtype != torch.float32:
+    if X.dtype is not torch.float16 and X.dtype is not torch.float32:
         X = X.float()
     return X if X.stride(-1) == 1 or X.shape[-1] <= 1 else X.contiguous()
 
 
 def _host_like(X, result):
     """`result` where X lives: a GPU tensor, or for host operands a NumPy array."""
-    if (_is_tensor(X) and X.is_cuda) or hasattr(X, "__cuda_array_interface__") or isinstance(X, MX4):
+    if (isinstance(X, _torch.Tensor) and X.is_cuda) or hasattr(X, "__cuda_array_interface__") or isinstance(X, MX4):
         return result
     return result.cpu().numpy()
 
@@ -965,7 +970,7 @@ def _llm_out(C, shape, dtype, what="C"):
     """The given result, or a new one: a GPU tensor of this shape and type with contiguous rows."""
     if C is None:
         return _torch.empty(shape, dtype=dtype, device="cuda")
-    if not (_is_tensor(C) and C.is_cuda and C.shape == tuple(shape) and C.dtype == dtype and (C.stride(-1) == 1 or shape[-1] <= 1)):
+    if not (isinstance(C, _torch.Tensor) and C.is_cuda and C.shape == shape and C.dtype is dtype and (C.stride(-1) == 1 or shape[-1] <= 1)):
         raise ValueError(f"{what} must be a GPU tensor of shape {tuple(shape)} and type {dtype} with contiguous rows")
     return C
 
@@ -991,7 +996,7 @@ class MX4:
             raise RuntimeError(lib.gen9blas_llm_error().decode())
 
     def __del__(self):
-        if getattr(self, "_handle", None) and not _exiting:
+        if getattr(self, "_handle", None) and _exiting is False:   # None: the module is being torn down
             _llm.gen9blas_mx4_free(self._handle)
             self._handle = None
 
@@ -1096,8 +1101,9 @@ def moe_gemm(X, ids, W, gate=None, weights=None, C=None):
     lib = _llm_library()
     torch = _torch
     x = _device_rows(X, (2, 3))
-    i = ids if _is_tensor(ids) and ids.is_cuda else torch.as_tensor(ids).cuda()
-    i = i.to(torch.int32).contiguous()
+    i = ids if isinstance(ids, torch.Tensor) and ids.is_cuda else torch.as_tensor(ids).cuda()
+    if i.dtype is not torch.int32 or not i.is_contiguous():
+        i = i.to(torch.int32).contiguous()
     if i.dim() != 2 or len(W.shape) != 3 or x.shape[-1] != W.shape[2] or x.shape[0] != i.shape[0] or \
             (x.dim() == 3 and x.shape[1] != i.shape[1]) or (gate is not None and gate.shape != W.shape):
         raise ValueError(f"incompatible shapes: X {tuple(x.shape)}, ids {tuple(i.shape)}, W {W.shape}"
