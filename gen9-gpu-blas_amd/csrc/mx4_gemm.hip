@@ -82,16 +82,6 @@ template <class O> static int launch_q(const Mx4View &A, const Mx4View &W, O *C,
     return 0;
 }
 
-template <class T, int MT> static int launch_tiles(const Rows &R, const Mx4View &W) {
-    Planes A;
-    G9_TRY(stage_planes<T>(R, R.M, W.K, W.kc, &A));
-    const long long mtiles = cdiv(R.M, MT * 16), ntiles = cdiv(W.rt, 16), wgs = cdiv(mtiles * ntiles, 8) * 8;
-    if (wgs > 0xffffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm: more tiles than one launch can index");
-    hipLaunchKernelGGL((mx4_gemm_tile_kernel<T, T, MT, false, false>), dim3((unsigned)wgs), dim3(256), 0, stream, A, R, W, W, 1, (int)mtiles, (int)ntiles);
-    G9_HIP(hipGetLastError());
-    return 0;
-}
-
 static int split_space(const Rows &R, const Mx4View &W, Split *s) {
     s->rows = R.M, s->ld = (long long)W.rt * 16;
     return scratch(SLOT_PART, (size_t)s->parts * s->rows * s->ld * 4, (void **)&s->sums);
@@ -119,34 +109,53 @@ template <class T, int MT, int NT, int WN, int D> static int launch_rows(const R
     return sum_parts<T>(R, W, split);
 }
 
-// Tiles of MT·16 rows × 128·NT columns; k is split until there is about a workgroup a CU.
-template <class T, int MT, int NT, int D> static int launch_few(const Rows &R, const Mx4View &W) {
-    const int ntiles = (int)cdiv(W.rt, NT * 8);
-    const long long tiles = cdiv(R.M, MT * 16) * ntiles;
+// Tiles of MT·16 rows × 16·NT·NV columns; k is split until there is about a workgroup a CU.
+template <class T, int MT, int NT, int NV, int D> static int launch_few(const Rows &R, const Mx4View &W) {
+    const int ntiles = (int)cdiv(W.rt, NT * NV), mtiles = (int)cdiv(R.M, MT * 16);
+    const long long tiles = (long long)mtiles * ntiles;
     Split split = {1, nullptr, 0, 0};
-    const int ways = (int)(num_cus / tiles), most = W.kc / 2;
+    const int ways = (int)(num_cus / tiles), most = W.kc / 4;
     if (ways > 1 && most > 1) {
         split.parts = ways < most ? ways : most;
         G9_TRY(split_space(R, W, &split));
     }
     if (tiles * split.parts > 0x7fffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm: more tiles than one launch can index");
-    hipLaunchKernelGGL((mx4_gemm_few_kernel<T, T, MT, NT, D, false, false>), dim3((unsigned)(tiles * split.parts)), dim3(512), 0, stream, R, W, W, 1, ntiles, split);
+    hipLaunchKernelGGL((mx4_gemm_few_kernel<T, T, MT, NT, NV, D, false, false>), dim3((unsigned)(cdiv(tiles * split.parts, 8) * 8)), dim3(NV * 64), 0, stream, R, W, W, 1, mtiles, ntiles, split);
+    G9_HIP(hipGetLastError());
+    return sum_parts<T>(R, W, split);
+}
+
+// Tiles of 64 rows × 256 columns; k is split until there is about a workgroup a CU.
+template <class T> static int launch_tiles(const Rows &R, const Mx4View &W) {
+    Planes A;
+    G9_TRY(stage_planes<T>(R, R.M, W.K, W.kc, &A));
+    const int mtiles = (int)cdiv(R.M, 64), ntiles = (int)cdiv(W.rt, 16);
+    const long long tiles = (long long)mtiles * ntiles;
+    Split split = {1, nullptr, 0, 0};
+    const int ways = (int)(num_cus / tiles), most = W.kc / 4;
+    if (ways > 1 && most > 1) {
+        split.parts = ways < most ? ways : most;
+        G9_TRY(split_space(R, W, &split));
+    }
+    if (tiles * split.parts > 0xffffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm: more tiles than one launch can index");
+    hipLaunchKernelGGL((mx4_gemm_tile_kernel<T, T, false, false>), dim3((unsigned)(cdiv(tiles * split.parts, 8) * 8)), dim3(256), 0, stream, A, R, W, W, 1, mtiles,
+                       ntiles, split);
     G9_HIP(hipGetLastError());
     return sum_parts<T>(R, W, split);
 }
 
 template <class T> static int launch_dense(const Rows &R, const Mx4View &W) {
-    if (R.M > 64) return R.M > 192 ? launch_tiles<T, 8>(R, W) : launch_tiles<T, 4>(R, W);
+    if (R.M > 64) return launch_tiles<T>(R, W);
     constexpr bool F = sizeof(T) == 4;
     // µs of the product alone, FP16 1 × 11008 × 4096 and FP32 8 × 4096 × 11008: rows kernel 9.4 and 13.2, few kernel 8.8 to
     // 9.5 and 10.7: FP32 rows are taken apart once a workgroup there, and once a wave in the rows kernel.
     if (R.M <= 16) {
-        if (F) return launch_few<T, 1, 2, 4>(R, W);
+        if (F) return launch_few<T, 1, 2, 8, 4>(R, W);
         else return launch_rows<T, 1, 1, 1, 4>(R, W, 1);
     }
     // 24 × 4096 × 11008: 128 columns a workgroup 10.4 FP16 and 17.3 FP32, 256 columns 13.0 and 16.7
-    if (R.M <= 32) return launch_few<T, 2, F ? 2 : 1, 4>(R, W);
-    return launch_few<T, 4, 1, 2>(R, W);
+    if (R.M <= 32) return launch_few<T, 2, F ? 2 : 1, 8, 4>(R, W);
+    return launch_few<T, 4, 1, 8, 2>(R, W);
 }
 
 }  // namespace g9llm

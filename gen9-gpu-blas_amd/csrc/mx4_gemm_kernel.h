@@ -2,6 +2,7 @@
 #pragma once
 #include "llm.h"
 #include "lds_dma.h"
+#include <type_traits>
 
 namespace g9llm {
 
@@ -25,7 +26,9 @@ template <> struct Act<_Float16> {
         return Frag{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
     }
     static __device__ __forceinline__ void split(const _Float16 *v, Frag *f) { __builtin_memcpy(f, v, 16); }
-    template <class V4> static __device__ __forceinline__ void split4(V4 v, unsigned long long *h) { __builtin_memcpy(h, &v, 8); }
+    // U elements of a row, as each plane has them
+    template <int U> using Piece = typename std::conditional<U == 8, u32x4, unsigned long long>::type;
+    template <int U, class V> static __device__ __forceinline__ void split_unit(V v, Piece<U> *h) { __builtin_memcpy(h, &v, U * 2); }
     static __device__ __forceinline__ f32x4 mfma(Frag w, Frag a, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(w, a, c, 0, 0, 0); }
     static __device__ __forceinline__ float finish(float v, int e) { return ldexpf(v, e - 140); }
 };
@@ -66,7 +69,9 @@ template <> struct Act<float> {
 #pragma unroll
         for (int q = 0; q < 3; q++) f[q] = __builtin_bit_cast(Frag, o[q]);
     }
-    template <class V4> static __device__ __forceinline__ void split4(V4 v, unsigned long long *h) {
+    template <int U> using Piece = unsigned long long;
+    template <int U, class V> static __device__ __forceinline__ void split_unit(V v, unsigned long long *h) {
+        static_assert(U == 4, "one 16-byte load");
         unsigned a[3], b[3];
         split2(v[0], v[1], a);
         split2(v[2], v[3], b);
@@ -77,17 +82,31 @@ template <> struct Act<float> {
     static __device__ __forceinline__ float finish(float v, int) { return v; }
 };
 
-// The largest scale byte of a row of W (kt: a multiple of 16).
-__device__ __forceinline__ int row_top(const uint8_t *top, int kt) {
-    unsigned m = 0;
-#pragma unroll 2
-    for (int i = 0; i < kt; i += 16) {
-        const u32x4 v = *reinterpret_cast<const u32x4 *>(top + i);
+// The largest scale bytes of N rows of W, top[n] .. top[n] + kt − 1 (kt: a multiple of 16): the loads of all rows together.
+template <int N> __device__ __forceinline__ void row_tops(const uint8_t *const *top, int kt, int *out) {
+    u32x4 v[N];
 #pragma unroll
-        for (int j = 0; j < 4; j++) m = max(max(m, max(v[j] & 255u, v[j] >> 8 & 255u)), max(v[j] >> 16 & 255u, v[j] >> 24));
+    for (int n = 0; n < N; n++) v[n] = *reinterpret_cast<const u32x4 *>(top[n]), out[n] = 0;
+    for (int i = 0; i < kt; i += 16) {
+        u32x4 next[N];
+#pragma unroll
+        for (int n = 0; n < N; n++) next[n] = *reinterpret_cast<const u32x4 *>(top[n] + min(i + 16, kt - 16));
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            unsigned m = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) m = max(max(m, max(v[n][j] & 255u, v[n][j] >> 8 & 255u)), max(v[n][j] >> 16 & 255u, v[n][j] >> 24));
+            out[n] = max(out[n], (int)m);
+            v[n] = next[n];
+        }
     }
-    return (int)m;
 }
+
+// Rows of 128 k in LDS (256 bytes of FP16 or BF16): 16-byte piece q of row m lies at q ^ swizzle(m). ds_read_b128 takes lanes
+// 0-3, 12-15 and 20-27 together (and 4-11, 16-19 and 28-31): rows of two pieces that differ in bit 2. With the rows 0-3 and
+// 12-15 at 0..7 and the others at 8..15 these sixteen lie in different banks; q ^ (m & 15) had them in pairs (half of the LDS
+// cycles of 1000 × 11008 × 4096).
+__device__ __forceinline__ int swizzle(int m) { return (m & 3) | (m >> 1 & 4) | ((m >> 3 ^ m >> 2) & 1) << 3; }
 
 // 8 consecutive elements of a row, zeros past K.
 template <class T> __device__ __forceinline__ void load8(const T *row, int k, int K, T *v) {

@@ -98,9 +98,17 @@ __device__ __forceinline__ void finish4(const Rows &R, const Mx4View &W, const S
         c = (O *)R.C + slot / R.S * R.ldct + slot % R.S * R.ldcs;
     } else
         c = (O *)R.C + (long long)(first + i) * R.ldct;
+    if (GATED)
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-        if (col + j < W.rows) c[col + j] = (O)(GATED ? y[j] * silu(z[j]) : y[j]);
+        for (int j = 0; j < 4; j++) y[j] *= silu(z[j]);
+    if (col + 4 <= W.rows) {
+        typedef O O4 __attribute__((ext_vector_type(4), aligned(sizeof(O))));
+        *reinterpret_cast<O4 *>(c + col) = O4{(O)y[0], (O)y[1], (O)y[2], (O)y[3]};
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (col + j < W.rows) c[col + j] = (O)y[j];
+    }
 }
 
 // C from the parts' sums, the parts in their order: a thread for each element, so that few rows still fill the GPU, sixteen
@@ -176,7 +184,7 @@ __global__ void __launch_bounds__(256) mx4_gemm_rows_kernel(Rows R, Mx4View W, M
             row[m] = (const T *)R.A + at + g * 32;
         }
         const u32x4 *wc[NW][NT];
-        const uint8_t *ws[NW][NT];
+        const uint8_t *ws[NW][NT], *tops[NW * NT];
 #pragma unroll
         for (int q = 0; q < NW; q++)
 #pragma unroll
@@ -185,8 +193,9 @@ __global__ void __launch_bounds__(256) mx4_gemm_rows_kernel(Rows R, Mx4View W, M
                 const long long t = (long long)e * W.rt + min(col0 + n, W.rt - 1);
                 wc[q][n] = reinterpret_cast<const u32x4 *>(V.codes) + t * W.kc * 64 + lane;
                 ws[q][n] = V.scales + t * W.kg * 256 + lane * 4;
-                if (X::P == 1) top[q][n] = row_top(V.top + (t * 16 + r) * W.kt, W.kt);
+                tops[q * NT + n] = V.top + (t * 16 + r) * W.kt;
             }
+        if (X::P == 1) row_tops<NW * NT>(tops, W.kt, &top[0][0]);
         const int ways = split.parts * WK, way = part * WK + wv / WN, whole = W.K / 128;
         const int c1 = (int)((long long)whole * way / ways), end = (int)((long long)whole * (way + 1) / ways);
         u32x4 w[D][NW][NT];
@@ -288,28 +297,34 @@ __device__ __forceinline__ void lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// 8 waves side by side in n, each 16·NT columns (gated: of W and of the gate) of MT·16 rows. The rows of each 128 k are taken
-// apart once for the whole workgroup, into FP16 or BF16 planes in LDS (two buffers; 16-byte piece q of row m at q ^ (m & 15)):
-// thread t loads four k at a time, 32 threads to a row. Weights and rows of the next D chunks are on their way in registers;
-// both, as loads return in order and the wait for the nearest rows would be a wait for all older weights too.
-template <class T, class O, int MT, int NT, int D, bool GROUPED, bool GATED>
-__global__ void __launch_bounds__(512) mx4_gemm_few_kernel(Rows R, Mx4View W, Mx4View G, int experts, int ntiles, Split split) {
+// NV waves side by side in n, each 16·NT columns (gated: of W and of the gate) of MT·16 rows. The rows of each 128 k are taken
+// apart once for the whole workgroup, into FP16 or BF16 planes in LDS (two buffers). A thread loads U elements at a time. Weights and rows of the next D
+// chunks are on their way in registers; both, as loads return in order and the wait for the nearest rows would be a wait for
+// all older weights too.
+template <class T, class O, int MT, int NT, int NV, int D, bool GROUPED, bool GATED>
+__global__ void __launch_bounds__(NV * 64, 2) mx4_gemm_few_kernel(Rows R, Mx4View W, Mx4View G, int experts, int mtiles, int ntiles, Split split) {
     typedef Act<T> X;
     typedef typename X::Frag Frag;
-    typedef T T4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-    constexpr int NW = GATED ? 2 : 1, P = X::P, PLANE = MT * 4096;
+    constexpr int NW = GATED ? 2 : 1, P = X::P, PLANE = MT * 4096, NTH = NV * 64;
+    constexpr int U = MT * 2048 / NTH < (int)(16 / sizeof(T)) ? MT * 2048 / NTH : 16 / sizeof(T);   // elements a load
+    constexpr int PR = 128 / U, NL = MT * 16 * PR / NTH;                                            // threads a row, loads a thread
+    typedef T TU __attribute__((ext_vector_type(U), aligned(sizeof(T))));
     __shared__ __attribute__((aligned(16))) unsigned char smem[2 * P * PLANE];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-    const int part = blockIdx.x % split.parts, tile = blockIdx.x / split.parts;
-    const int mt0 = tile / ntiles, nt0 = tile % ntiles;
+    // Each XCD (workgroups b, b + 8, ...) takes a contiguous run of tiles, so that those resident on it share rows and weights:
+    // dense, row tiles of the same columns; experts, column tiles of the same rows.
+    if (GROUPED) mtiles = R.tiles[-1];
+    const int total = mtiles * ntiles * split.parts, run = (total + 7) / 8, id = (blockIdx.x & 7) * run + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= run || id >= total) return;
+    const int part = id % split.parts, tile = id / split.parts;
+    const int mt0 = GROUPED ? tile / ntiles : tile % mtiles, nt0 = GROUPED ? tile % ntiles : tile / mtiles;
     int first, count, e = 0;
     if (GROUPED) {
-        if (mt0 >= R.tiles[-1]) return;
         e = R.tiles[2 * mt0], first = R.tiles[2 * mt0 + 1];
         count = min(MT * 16, R.off[e + 1] - first);
     } else
         first = mt0 * MT * 16, count = min(MT * 16, R.M - first);
-    const int col0 = (nt0 * 8 + wv) * NT;   // first row tile of W
+    const int col0 = (nt0 * NV + wv) * NT;   // first row tile of W
     f32x4 acc[NW][NT][MT];
 #pragma unroll
     for (int q = 0; q < NW; q++)
@@ -323,123 +338,142 @@ __global__ void __launch_bounds__(512) mx4_gemm_few_kernel(Rows R, Mx4View W, Mx
 #pragma unroll
         for (int n = 0; n < NT; n++) top[q][n] = 0;
     if (!GROUPED || e < experts) {
-        const int quad = threadIdx.x & 31;
-        const T *row[MT];   // rows past the last repeat it and are not stored
+        const int at_k = (int)threadIdx.x % PR * U;
+        const T *row[NL];   // rows past the last repeat it and are not stored
 #pragma unroll
-        for (int u = 0; u < MT; u++) {
-            const int i = first + min(u * 16 + (int)(threadIdx.x >> 5), count - 1);
+        for (int u = 0; u < NL; u++) {
+            const int i = first + min(u * (NTH / PR) + (int)threadIdx.x / PR, count - 1);
             long long at;
             if (GROUPED) {
                 const int slot = R.order[i];
                 at = slot / R.S * R.ldt + slot % R.S * R.lds;
             } else
                 at = (long long)i * R.ldt;
-            row[u] = (const T *)R.A + at;
+            row[u] = (const T *)R.A + at + at_k;
         }
-        const u32x4 *wc[NW][NT];
-        const uint8_t *ws[NW][NT];
+        const u32x4 *wc[NW][NT];   // uniform: the lane is added to each load's offset
+        const uint8_t *ws[NW][NT], *tops[NW * NT];
 #pragma unroll
         for (int q = 0; q < NW; q++)
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 const Mx4View &V = q ? G : W;
                 const long long t = (long long)e * W.rt + min(col0 + n, W.rt - 1);
-                wc[q][n] = reinterpret_cast<const u32x4 *>(V.codes) + t * W.kc * 64 + lane;
-                ws[q][n] = V.scales + t * W.kg * 256 + lane * 4;
-                if (P == 1) top[q][n] = row_top(V.top + (t * 16 + r) * W.kt, W.kt);
+                wc[q][n] = reinterpret_cast<const u32x4 *>(V.codes) + t * W.kc * 64;
+                ws[q][n] = V.scales + t * W.kg * 256;
+                tops[q * NT + n] = V.top + (t * 16 + r) * W.kt;
             }
+        if (P == 1) row_tops<NW * NT>(tops, W.kt, &top[0][0]);
         const int whole = W.K / 128;
         const int c1 = (int)((long long)whole * part / split.parts), end = (int)((long long)whole * (part + 1) / split.parts);
         u32x4 w[D][NW][NT];
         unsigned s[D][NW][NT];
-        T4 raw[D][MT];
+        TU raw[D][NL];
         auto fetch_weights = [&](int c, int d) {
 #pragma unroll
             for (int q = 0; q < NW; q++)
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    w[d][q][n] = __builtin_nontemporal_load(wc[q][n] + (long long)c * 64);
-                    s[d][q][n] = ws[q][n][c / 4 * 256 + c % 4];
+                    w[d][q][n] = __builtin_nontemporal_load(wc[q][n] + (long long)c * 64 + (unsigned)lane);
+                    s[d][q][n] = (ws[q][n] + (c / 4 * 256 + c % 4))[(unsigned)lane * 4];
                 }
         };
         auto fetch = [&](int c, int d) {   // chunk c to the registers of place d
             fetch_weights(c, d);
 #pragma unroll
-            for (int u = 0; u < MT; u++) raw[d][u] = *reinterpret_cast<const T4 *>(row[u] + c * 128 + quad * 4);
+            for (int u = 0; u < NL; u++) raw[d][u] = *reinterpret_cast<const TU *>(row[u] + c * 128);
         };
         auto stage = [&](int d, int buf) {   // the rows in place d to LDS
 #pragma unroll
-            for (int u = 0; u < MT; u++) {
-                const int m = u * 16 + (threadIdx.x >> 5);
-                G9_LDS unsigned char *at = (G9_LDS unsigned char *)smem + buf * P * PLANE + m * 256 + (((quad >> 1) ^ (m & 15)) << 4) + (quad & 1) * 8;
-                unsigned long long h[P];
-                X::split4(raw[d][u], h);
+            for (int u = 0; u < NL; u++) {
+                const int m = u * (NTH / PR) + threadIdx.x / PR;
+                G9_LDS unsigned char *at = (G9_LDS unsigned char *)smem + buf * P * PLANE + m * 256 + (((at_k >> 3) ^ swizzle(m)) << 4) + (at_k & 7) * 2;
+                typename X::template Piece<U> h[P];
+                X::template split_unit<U>(raw[d][u], h);
 #pragma unroll
-                for (int p = 0; p < P; p++) *reinterpret_cast<G9_LDS unsigned long long *>(at + p * PLANE) = h[p];
+                for (int p = 0; p < P; p++) *reinterpret_cast<G9_LDS typename X::template Piece<U> *>(at + p * PLANE) = h[p];
             }
         };
-        auto multiply = [&](int d, int buf) {
+        const int sw_r = swizzle(r);
+        // Steps of eight k and one piece: a step's fragments are read (and its weights converted) while the step before it is
+        // multiplied. `half` is called half way.
+        auto multiply = [&](int d, int buf, auto half) {
             const G9_LDS unsigned char *base = (const G9_LDS unsigned char *)smem + buf * P * PLANE + r * 256;
             float sc[NW][NT];
 #pragma unroll
             for (int q = 0; q < NW; q++)
 #pragma unroll
                 for (int n = 0; n < NT; n++) sc[q][n] = X::scale(s[d][q][n], top[q][n]);
+            Frag a[2][MT], b[2][NW][NT];
+            auto prepare = [&](int t) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                Frag b[NW][NT];
+                for (int m = 0; m < MT; m++) a[t & 1][m] = *reinterpret_cast<const G9_LDS Frag *>(base + t % P * PLANE + m * 4096 + (((4 * g + t / P) ^ sw_r) << 4));
+                if (t % P == 0)
 #pragma unroll
-                for (int q = 0; q < NW; q++)
+                    for (int q = 0; q < NW; q++)
 #pragma unroll
-                    for (int n = 0; n < NT; n++) b[q][n] = X::weights(w[d][q][n][i], sc[q][n]);
+                        for (int n = 0; n < NT; n++) b[t / P & 1][q][n] = X::weights(w[d][q][n][t / P], sc[q][n]);
+            };
+            prepare(0);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int t = 0; t < 4 * P; t++) {
+                if (t + 1 < 4 * P) prepare(t + 1);
 #pragma unroll
                 for (int m = 0; m < MT; m++)
 #pragma unroll
-                    for (int p = 0; p < P; p++) {
-                        const Frag a = *reinterpret_cast<const G9_LDS Frag *>(base + p * PLANE + m * 4096 + (((4 * g + i) ^ r) << 4));
+                    for (int q = 0; q < NW; q++)
 #pragma unroll
-                        for (int q = 0; q < NW; q++)
+                        for (int n = 0; n < NT; n++) acc[q][n][m] = X::mfma(b[t / P & 1][q][n], a[t & 1][m], acc[q][n][m]);
+                // the next reads first, then a conversion after each matrix instruction
+                __builtin_amdgcn_sched_group_barrier(0x100, MT, 0);
 #pragma unroll
-                            for (int n = 0; n < NT; n++) acc[q][n][m] = X::mfma(b[q][n], a, acc[q][n][m]);
-                    }
+                for (int j = 0; j < MT * NW * NT; j++) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 1, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (t == 2 * P - 1) half();
             }
         };
         if (c1 < end) {
             // No load is conditional (past the end the last chunk is loaded again): a wait then leaves all younger loads on their way.
-            // Buffer d & 1 (D is even) holds chunk c + d; the barrier before a chunk is multiplied is the one after it was staged.
-            static_assert(D % 2 == 0, "two LDS buffers");
+            // A chunk is staged while the one before it is multiplied; the barrier between them is the one that ends that.
 #pragma unroll
             for (int d = 0; d < D; d++) fetch(min(c1 + d, end - 1), d);
+            int buf = 0;
             stage(0, 0);
             lds_barrier();
             int c = c1;
             for (; c + D < end; c += D) {
 #pragma unroll
                 for (int d = 0; d < D; d++) {
-                    stage((d + 1) % D, (d + 1) & 1);
-                    multiply(d, d & 1);
+                    multiply(d, buf, [&] { stage((d + 1) % D, buf ^ 1); });
                     fetch(min(c + d + D, end - 1), d);
+                    buf ^= 1;
                     lds_barrier();
                 }
             }
 #pragma unroll
             for (int d = 0; d < D; d++) {
                 if (c + d >= end) break;
-                if (d + 1 < D && c + d + 1 < end) stage(d + 1, (d + 1) & 1);
-                multiply(d, d & 1);
+                multiply(d, buf, [&] {
+                    if (d + 1 < D && c + d + 1 < end) stage((d + 1) % D, buf ^ 1);
+                });
+                buf ^= 1;
                 lds_barrier();
             }
         }
         if (W.K % 128 && part == split.parts - 1) {   // the chunk in which the rows end
             fetch_weights(whole, 0);
-            const int k = whole * 128 + quad * 4;
+            const int k = whole * 128;
 #pragma unroll
-            for (int u = 0; u < MT; u++)
+            for (int u = 0; u < NL; u++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) raw[0][u][j] = k + j < W.K ? row[u][k + j] : T(0);
+                for (int j = 0; j < U; j++) raw[0][u][j] = k + at_k + j < W.K ? row[u][k + j] : T(0);
             stage(0, 0);
             __syncthreads();
-            multiply(0, 0);
+            multiply(0, 0, [] {});
         }
     }
 #pragma unroll

@@ -1,6 +1,6 @@
-// Products of many rows with MX4 weights: tiles of BM rows × 256 columns on the FP16 or BF16 matrix cores.
+// Products of many rows with MX4 weights: tiles of 64 rows × 256 columns on the FP16 or BF16 matrix cores.
 #pragma once
-#include "mx4_gemm_kernel.h"
+#include "mx4_rows_kernel.h"
 
 namespace g9llm {
 
@@ -10,34 +10,30 @@ struct Planes {
     long long ld, plane;   // row stride and plane stride (elements)
 };
 
-// One 16-byte global→LDS copy per lane, lane L to lds + 16·L, from 64-bit addresses (see lds_dma16 for the waits).
-__device__ __forceinline__ void lds_dma16_ptr(const void *p, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "s"(lds) : "memory");
-}
-
-// A workgroup's 4 waves lie side by side in n: each makes all BM = 16·MT rows × 64 columns (4 column tiles; gated: 2 of W and
-// 2 of the gate). Per 128 k and wave that is 16·MT matrix instructions to 64 conversions, and the weights, which no other
-// wave needs, go from global memory to registers and are converted there. The rows are staged in LDS by direct copies, two
-// stages: stage s + 1 is on its way while s is multiplied. 16-byte piece q of row m lies at q ^ (m & 15): eight lanes that
-// read together then cover all banks.
-template <class T, class O, int MT, bool GROUPED, bool GATED>
-__global__ void __launch_bounds__(256, 2) mx4_gemm_tile_kernel(Planes A, Rows R, Mx4View W, Mx4View G, int experts, int mtiles, int ntiles) {
+// 64 rows × 256 columns a workgroup, 4 waves side by side in n: each all rows × 64 columns (4 column tiles; gated: 2 of W and 2
+// of the gate), three workgroups a CU. Per 128 k and wave that is 64 matrix instructions to 64 conversions, which run beside
+// them, and the weights, which no other wave needs, go from global memory to registers and are converted there. The rows are
+// staged in LDS by direct copies, two stages: stage s + 1 is on its way while s is multiplied. Their fragments are read three
+// ahead of the one that is multiplied: ds_read_b128 gives 64 bytes a clock and CU, what the matrix cores take here at their full rate.
+template <class T, class O, bool GROUPED, bool GATED>
+__global__ void __launch_bounds__(256, 3) mx4_gemm_tile_kernel(Planes A, Rows R, Mx4View W, Mx4View G, int experts, int mtiles, int ntiles, Split split) {
     typedef Act<T> X;
     typedef typename X::Frag Frag;
-    constexpr int P = X::P, BM = MT * 16, NT = 4, PER = BM / 16;   // PER: copies per thread and stage
-    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * BM * 256];
+    constexpr int P = X::P, MT = 4, NT = 4, STAGE = MT * 4096;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     // Each XCD (workgroups b, b + 8, ...) takes a contiguous run of tiles, so that those resident on it share rows and weights.
     if (GROUPED) mtiles = R.tiles[-1];
-    const int total = mtiles * ntiles, run = (total + 7) / 8, id = (blockIdx.x & 7) * run + (blockIdx.x >> 3);
+    const int total = mtiles * ntiles * split.parts, run = (total + 7) / 8, id = (blockIdx.x & 7) * run + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= run || id >= total) return;
-    const int mt0 = GROUPED ? id / ntiles : id % mtiles, nt0 = GROUPED ? id % ntiles : id / mtiles;
+    const int part = id % split.parts, tl = id / split.parts;
+    const int mt0 = GROUPED ? tl / ntiles : tl % mtiles, nt0 = GROUPED ? tl % ntiles : tl / mtiles;
     int first, count, e = 0;
     if (GROUPED) {
         e = R.tiles[2 * mt0], first = R.tiles[2 * mt0 + 1];
-        count = min(BM, R.off[e + 1] - first);
+        count = min(MT * 16, R.off[e + 1] - first);
     } else
-        first = mt0 * BM, count = min(BM, R.M - first);
+        first = mt0 * MT * 16, count = min(MT * 16, R.M - first);
     int tile[NT];   // row tiles of W (gated: 2 of W, the same 2 of G)
 #pragma unroll
     for (int n = 0; n < NT; n++) tile[n] = GATED ? (nt0 * 4 + wv) * 2 + n % 2 : (nt0 * 4 + wv) * 4 + n;
@@ -50,41 +46,55 @@ __global__ void __launch_bounds__(256, 2) mx4_gemm_tile_kernel(Planes A, Rows R,
     int top[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) top[n] = 0;
+    const int c1 = (int)((long long)W.kc * part / split.parts), c2 = (int)((long long)W.kc * (part + 1) / split.parts);
 
-    if (!GROUPED || e < experts) {
-        const u32x4 *wc[NT];
-        const unsigned *ws[NT];
+    if ((!GROUPED || e < experts) && c1 < c2) {
+        const u32x4 *wc[NT];   // uniform: the lane is added to each load's offset
+        const uint8_t *ws[NT], *tops[NT];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             const Mx4View &V = GATED && n >= 2 ? G : W;
             const long long t = (long long)e * W.rt + min(tile[n], W.rt - 1);   // columns past the last repeat it and are not stored
-            wc[n] = reinterpret_cast<const u32x4 *>(V.codes) + t * W.kc * 64 + lane;
-            ws[n] = reinterpret_cast<const unsigned *>(V.scales) + t * W.kg * 64 + lane;
-            top[n] = row_top(V.top + (t * 16 + r) * W.kt, W.kt);
+            wc[n] = reinterpret_cast<const u32x4 *>(V.codes) + t * W.kc * 64;
+            ws[n] = V.scales + t * W.kg * 256;
+            tops[n] = V.top + (t * 16 + r) * W.kt;
         }
-        // copy j of a thread: row (wv·PER + j)·4 + lane/16 of the tile, piece (lane & 15) ^ (row & 15); rows past the last repeat it
-        const uint16_t *src[PER];
+        if (P == 1) row_tops<NT>(tops, W.kt, top);
+        // copy j of a thread: row (wv·MT + j)·4 + lane/16 of the tile, piece (lane & 15) ^ swizzle(row); rows past the last repeat it
+        const uint16_t *src[MT];
 #pragma unroll
-        for (int j = 0; j < PER; j++) {
-            const int m = (wv * PER + j) * 4 + (lane >> 4), i = first + min(m, count - 1);
+        for (int j = 0; j < MT; j++) {
+            const int m = (wv * MT + j) * 4 + g, i = first + min(m, count - 1);
             long long row = i;
             if (GROUPED) row = R.lds ? R.order[i] : R.order[i] / R.S;
-            src[j] = A.p + row * A.ld + ((lane & 15) ^ (m & 15)) * 8;
+            src[j] = A.p + row * A.ld + (r ^ swizzle(m)) * 8;
         }
-        const unsigned lds0 = (unsigned)(uintptr_t)(const G9_LDS unsigned char *)smem + wv * PER * 1024;
-        auto issue = [&](int stage, int buf) {   // stage = chunk·P + plane
-            const long long at = (long long)(stage / P) * 128 + (stage % P) * A.plane;
+        const unsigned lds0 = (unsigned)(uintptr_t)(const G9_LDS unsigned char *)smem + wv * MT * 1024;
+        auto issue = [&](int s) {   // the rows of stage s = chunk · P + plane
+            const long long at = (long long)(s / P) * 128 + s % P * A.plane;
 #pragma unroll
-            for (int j = 0; j < PER; j++) lds_dma16_ptr(src[j] + at, __builtin_amdgcn_readfirstlane(lds0 + buf * BM * 256 + j * 1024));
+            for (int j = 0; j < MT; j++)
+                asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+                             : : "v"(src[j] + at), "s"(__builtin_amdgcn_readfirstlane(lds0 + (s & 1) * STAGE + j * 1024)) : "memory");
         };
         u32x4 w[NT], wn[NT];
-        unsigned sw[NT], sn[NT];
-        issue(0, 0);
-#pragma unroll
-        for (int n = 0; n < NT; n++) wn[n] = wc[n][0], sn[n] = ws[n][0];
-        const int stages = W.kc * P;
+        unsigned sn[NT];
         float sc[NT];
-        for (int s = 0; s < stages; s++) {
+        auto fetch = [&](int c) {
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                wn[n] = (wc[n] + (long long)c * 64)[(unsigned)lane];
+                sn[n] = (ws[n] + (c / 4 * 256 + c % 4))[(unsigned)lane * 4];
+            }
+        };
+        const int s1 = c1 * P, s2 = c2 * P, sw_r = swizzle(r);
+        const G9_LDS unsigned char *base = (const G9_LDS unsigned char *)smem + r * 256;
+        int q[4];   // where this lane's pieces of a step lie in its row
+#pragma unroll
+        for (int i = 0; i < 4; i++) q[i] = ((4 * g + i) ^ sw_r) << 4;
+        issue(s1);
+        fetch(c1);
+        for (int s = s1; s < s2; s++) {
             const int c = s / P;
             g9::wait_vm<0>();
             __syncthreads();
@@ -92,67 +102,41 @@ __global__ void __launch_bounds__(256, 2) mx4_gemm_tile_kernel(Planes A, Rows R,
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     w[n] = wn[n];
-                    if (c % 4 == 0) sw[n] = sn[n];
-                    sc[n] = X::scale(sw[n] >> (c % 4 * 8) & 255u, top[n]);
+                    sc[n] = X::scale(sn[n], top[n]);
                 }
             }
-            if (s + 1 < stages) {
-                issue(s + 1, (s + 1) & 1);
-                if ((P == 1 || s % P == 0) && c + 1 < W.kc) {
-#pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        wn[n] = wc[n][(c + 1) * 64];
-                        if (c % 4 == 3) sn[n] = ws[n][(c + 1) / 4 * 64];
-                    }
-                }
+            if (s + 1 < s2) {
+                issue(s + 1);
+                if (P == 1 || s % P == 0) fetch(min(c + 1, c2 - 1));
             }
-            const G9_LDS unsigned char *base = (const G9_LDS unsigned char *)smem + (s & 1) * BM * 256 + r * 256;
+            const G9_LDS unsigned char *st = base + (s & 1) * STAGE;
+            Frag a[4], b[NT];
+            auto read = [&](int t) { a[t & 3] = *reinterpret_cast<const G9_LDS Frag *>(st + t % MT * 4096 + q[t / MT]); };
+            read(0);
+            read(1);
+            read(2);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                Frag a[MT], b[NT];
+            for (int t = 0; t < 4 * MT; t++) {
+                if (t + 3 < 4 * MT) read(t + 3);
+                if (t % MT == 0)
 #pragma unroll
-                for (int m = 0; m < MT; m++) a[m] = *reinterpret_cast<const G9_LDS Frag *>(base + m * 4096 + (((4 * g + i) ^ r) << 4));
+                    for (int n = 0; n < NT; n++) b[n] = X::weights(w[n][t / MT], sc[n]);
 #pragma unroll
-                for (int n = 0; n < NT; n++) b[n] = X::weights(w[n][i], sc[n]);
-#pragma unroll
-                for (int m = 0; m < MT; m++)
-#pragma unroll
-                    for (int n = 0; n < NT; n++) acc[n][m] = X::mfma(b[n], a[m], acc[n][m]);
+                for (int n = 0; n < NT; n++) acc[n][t % MT] = X::mfma(b[n], a[t & 3], acc[n][t % MT]);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
-    int tn[NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; n++)
+    for (int n = 0; n < (GATED ? 2 : NT); n++) {
+        int ty[4], tz[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) tn[n][j] = __shfl(top[n], 4 * g + j);
+        for (int j = 0; j < 4; j++) ty[j] = __shfl(top[n], 4 * g + j), tz[j] = GATED ? __shfl(top[(n + 2) % NT], 4 * g + j) : 0;
 #pragma unroll
-    for (int m = 0; m < MT; m++) {
-        const int i = m * 16 + r;
-        if (i >= count) continue;
-        O *c;
-        if (GROUPED) {
-            const int slot = R.order[first + i];
-            c = (O *)R.C + (slot / R.S) * R.ldct + (slot % R.S) * R.ldcs;
-        } else
-            c = (O *)R.C + (long long)(first + i) * R.ldct;
-#pragma unroll
-        for (int n = 0; n < (GATED ? 2 : NT); n++) {
-            float y[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                y[j] = X::finish(acc[n][m][j], tn[n][j]);
-                if (GATED) y[j] *= silu(X::finish(acc[(n + 2) % NT][m][j], tn[(n + 2) % NT][j]));
-            }
-            const int col = tile[n] * 16 + 4 * g;
-            if (col + 4 <= W.rows) {
-                typedef O O4 __attribute__((ext_vector_type(4), aligned(sizeof(O))));
-                *reinterpret_cast<O4 *>(c + col) = O4{(O)y[0], (O)y[1], (O)y[2], (O)y[3]};
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (col + j < W.rows) c[col + j] = (O)y[j];
-            }
+        for (int m = 0; m < MT; m++) {
+            const int i = m * 16 + r;
+            if (i < count) finish4<T, O, GROUPED, GATED>(R, W, split, part, first, i, tile[n] * 16 + 4 * g, acc[n][m], acc[(n + 2) % NT][m], ty, tz);
         }
     }
 }
