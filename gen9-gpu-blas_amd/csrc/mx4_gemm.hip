@@ -7,9 +7,10 @@ namespace g9llm {
 
 // Both operands MX4, any shape: a workgroup makes 64 rows × 16 columns, its 4 waves every fourth group of 512 k.
 template <class O>
-__global__ void __launch_bounds__(256) mx4_gemm_q_any_kernel(Mx4View A, Mx4View W, O *__restrict__ C, long long ldc) {
+__global__ void __launch_bounds__(256) mx4_gemm_q_any_kernel(Mx4View A, Mx4View W, O *__restrict__ C, long long ldc, int mtiles, int) {
     constexpr int MT = 4;
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    if ((int)blockIdx.x >= mtiles * W.rt) return;
     const int nt = blockIdx.x % W.rt, mt = blockIdx.x / W.rt * MT;
     f32x4 acc[MT];
 #pragma unroll
@@ -62,24 +63,16 @@ __global__ void __launch_bounds__(256) mx4_gemm_q_any_kernel(Mx4View A, Mx4View 
     }
 }
 
-template <class O, int T> static int launch_q_tiles(const Mx4View &A, const Mx4View &W, O *C, long long ldc) {
-    constexpr int LDS = 4 * 4 * T * 1024 + 2 * 4 * T * 256;
-    static hipError_t allowed = hipFuncSetAttribute((const void *)mx4_gemm_q_tile_kernel<O, T>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-    G9_HIP(allowed);
-    const long long mtiles = cdiv(A.rt, 2 * T), ntiles = cdiv(W.rt, 2 * T), wgs = cdiv(mtiles * ntiles, 8) * 8;
-    if (wgs > 0xffffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm_q: more tiles than one launch can index");
-    hipLaunchKernelGGL((mx4_gemm_q_tile_kernel<O, T>), dim3((unsigned)wgs), dim3(256), LDS, stream, A, W, C, ldc, (int)mtiles, (int)ntiles);
-    G9_HIP(hipGetLastError());
-    return 0;
-}
-
 template <class O> static int launch_q(const Mx4View &A, const Mx4View &W, O *C, long long ldc) {
-    if (A.rt > 4) return cdiv(A.rt, 16) * cdiv(W.rt, 16) >= num_cus ? launch_q_tiles<O, 8>(A, W, C, ldc) : launch_q_tiles<O, 4>(A, W, C, ldc);
-    const long long wgs = cdiv(A.rt, 4) * W.rt;
-    if (wgs > 0xffffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm_q: more tiles than one launch can index");
-    hipLaunchKernelGGL((mx4_gemm_q_any_kernel<O>), dim3((unsigned)wgs), dim3(256), 0, stream, A, W, C, ldc);
-    G9_HIP(hipGetLastError());
-    return 0;
+    auto run = [&](auto kernel, int rows, int cols) -> int {   // of row tiles
+        const long long mtiles = cdiv(A.rt, rows), ntiles = cdiv(W.rt, cols), wgs = cdiv(mtiles * ntiles, 8) * 8;
+        if (wgs > 0xffffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm_q: more tiles than one launch can index");
+        hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(256), 0, stream, A, W, C, ldc, (int)mtiles, (int)ntiles);
+        G9_HIP(hipGetLastError());
+        return 0;
+    };
+    if (A.rt > 4) return cdiv(A.rt, 16) * cdiv(W.rt, 16) >= num_cus ? run(mx4_gemm_q_tile_kernel<O>, 16, 16) : run(mx4_gemm_q_ring_kernel<O>, 8, 8);
+    return run(mx4_gemm_q_any_kernel<O>, 4, 1);
 }
 
 static int split_space(const Rows &R, const Mx4View &W, Split *s) {

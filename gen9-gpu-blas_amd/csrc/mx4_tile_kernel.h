@@ -20,7 +20,7 @@ __global__ void __launch_bounds__(256, 3) mx4_gemm_tile_kernel(Planes A, Rows R,
     typedef Act<T> X;
     typedef typename X::Frag Frag;
     constexpr int P = X::P, MT = 4, NT = 4, STAGE = MT * 4096;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE];
+    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE + 1024];   // two stages, or a finished tile of FP16 with its rows 16 bytes apart
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     // Each XCD (workgroups b, b + 8, ...) takes a contiguous run of tiles, so that those resident on it share rows and weights.
     if (GROUPED) mtiles = R.tiles[-1];
@@ -128,17 +128,50 @@ __global__ void __launch_bounds__(256, 3) mx4_gemm_tile_kernel(Planes A, Rows R,
             }
         }
     }
+    constexpr int NO = GATED ? NT / 2 : NT, COLS = NO * 64;   // column tiles a wave, columns a workgroup
+    int ty[NO][4], tz[NO][4];
 #pragma unroll
-    for (int n = 0; n < (GATED ? 2 : NT); n++) {
-        int ty[4], tz[4];
+    for (int n = 0; n < NO; n++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) ty[j] = __shfl(top[n], 4 * g + j), tz[j] = GATED ? __shfl(top[(n + 2) % NT], 4 * g + j) : 0;
+        for (int j = 0; j < 4; j++) ty[n][j] = __shfl(top[n], 4 * g + j), tz[n][j] = GATED ? __shfl(top[(n + 2) % NT], 4 * g + j) : 0;
+    // the tile through LDS in one piece (FP16) or two (FP32)
+    auto store = [&](auto zero, auto row) {
+        typedef decltype(zero) E;
+        typedef E E4 __attribute__((ext_vector_type(4)));
+        constexpr int PIECE = sizeof(E) == 2 ? 64 : 32, PITCH = COLS * sizeof(E) + 16;
+        static_assert(PIECE * PITCH <= sizeof(smem), "a piece of the tile");
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-            const int i = m * 16 + r;
-            if (i < count) finish4<T, O, GROUPED, GATED>(R, W, split, part, first, i, tile[n] * 16 + 4 * g, acc[n][m], acc[(n + 2) % NT][m], ty, tz);
+        for (int p = 0; p < 64; p += PIECE) {
+            __syncthreads();
+#pragma unroll
+            for (int m = p / 16; m < (p + PIECE) / 16; m++)
+#pragma unroll
+                for (int n = 0; n < NO; n++) {
+                    E4 v;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        float y = X::finish(acc[n][m][j], ty[n][j]);
+                        if (GATED) y *= silu(X::finish(acc[(n + 2) % NT][m][j], tz[n][j]));
+                        v[j] = (E)y;
+                    }
+                    *reinterpret_cast<G9_LDS E4 *>((G9_LDS unsigned char *)smem + (m * 16 + r - p) * PITCH + ((wv * NO + n) * 16 + 4 * g) * sizeof(E)) = v;
+                }
+            __syncthreads();
+            store_rows<E, 256, PIECE, COLS, PITCH>((const G9_LDS unsigned char *)smem, W.rows - nt0 * COLS, [&](int i) { return p + i < count ? row(p + i) : (E *)nullptr; });
         }
-    }
+    };
+    if (!GROUPED && split.parts > 1)
+        store(0.f, [&](int i) { return split.sums + ((long long)part * split.rows + first + i) * split.ld + nt0 * COLS; });
+    else
+        store(O(0), [&](int i) {
+            long long at;
+            if (GROUPED) {
+                const int slot = R.order[first + i];
+                at = slot / R.S * R.ldct + slot % R.S * R.ldcs;
+            } else
+                at = (long long)(first + i) * R.ldct;
+            return (O *)R.C + at + nt0 * COLS;
+        });
 }
 
 // Rows of activations to planes: T·S rows at X + t·ldt + s·lds, each thread eight k.
