@@ -22,19 +22,34 @@ __device__ __forceinline__ unsigned ordered(float x) {
     const unsigned u = __builtin_bit_cast(unsigned, x + 0.f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+// Reductions over the 64 lanes by DPP: within rows of 16, then from each row to the next; lane 63 has the result, which all get.
+// (Six exchanges through LDS permutes, for each of k choices, were most of 8192 tokens' 21 µs.)
+template <int CTRL, int ROWS> __device__ __forceinline__ unsigned dpp(unsigned old, unsigned v) {
+    return (unsigned)__builtin_amdgcn_update_dpp((int)old, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <class F> __device__ __forceinline__ unsigned wave_reduce(unsigned v, unsigned identity, F op) {
+    v = op(v, dpp<0x111, 0xf>(identity, v));   // row_shr 1, 2, 4, 8
+    v = op(v, dpp<0x112, 0xf>(identity, v));
+    v = op(v, dpp<0x114, 0xf>(identity, v));
+    v = op(v, dpp<0x118, 0xf>(identity, v));
+    v = op(v, dpp<0x142, 0xa>(identity, v));   // lane 15 of rows 0 and 2 to rows 1 and 3
+    v = op(v, dpp<0x143, 0xc>(identity, v));   // lane 31 to rows 2 and 3
+    return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ unsigned as_u(float v) { return __builtin_bit_cast(unsigned, v); }
+__device__ __forceinline__ float as_f(unsigned v) { return __builtin_bit_cast(float, v); }
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-    return v;
+    return as_f(wave_reduce(as_u(v), as_u(-__builtin_inff()), [](unsigned a, unsigned b) { return as_u(fmaxf(as_f(a), as_f(b))); }));
 }
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    return v;
+    return as_f(wave_reduce(as_u(v), 0u, [](unsigned a, unsigned b) { return as_u(as_f(a) + as_f(b)); }));
+}
+__device__ __forceinline__ unsigned wave_max(unsigned v) {
+    return wave_reduce(v, 0u, [](unsigned a, unsigned b) { return a > b ? a : b; });
 }
 
-// A wave routes a token: lane l holds the experts l, l + 64, ... The choice of the k experts is k rounds of a wave's
-// maximum over (choice, lowest index).
+// A wave routes a token: lane l holds the NL experts from l·NL on, so that of equal choices the lowest lane's, and there the
+// first, is the lowest index. The k experts are k rounds of a wave's maximum over ordered choices (0: not to be chosen).
 template <class T, int NL>
 __global__ void __launch_bounds__(256) moe_route_kernel(RouteArgs a) {
     const float ninf = -__builtin_inff();
@@ -45,13 +60,19 @@ __global__ void __launch_bounds__(256) moe_route_kernel(RouteArgs a) {
     const T *row = (const T *)a.logits + t * a.ldl;
     float score[NL], choice[NL];
     bool nan = false;
+    if (lane * NL + NL <= a.E) {
+        typedef T TV __attribute__((ext_vector_type(NL), aligned(sizeof(T))));
+        if constexpr (NL > 1) {
+            const TV v = *reinterpret_cast<const TV *>(row + lane * NL);
 #pragma unroll
-    for (int i = 0; i < NL; i++) {
-        const int e = i * 64 + lane;
-        score[i] = e < a.E ? (float)row[e] : ninf;
-        nan |= score[i] != score[i];
-    }
-    nan = __ballot(nan) != 0;
+            for (int i = 0; i < NL; i++) score[i] = (float)v[i];
+        } else
+            score[0] = (float)row[lane];
+    } else
+#pragma unroll
+        for (int i = 0; i < NL; i++) score[i] = lane * NL + i < a.E ? (float)row[lane * NL + i] : ninf;
+#pragma unroll
+    for (int i = 0; i < NL; i++) nan |= score[i] != score[i];
     if (a.sigmoid) {
 #pragma unroll
         for (int i = 0; i < NL; i++) {
@@ -81,65 +102,71 @@ __global__ void __launch_bounds__(256) moe_route_kernel(RouteArgs a) {
     if (a.bias)
 #pragma unroll
         for (int i = 0; i < NL; i++) {
-            const int e = i * 64 + lane;
+            const int e = lane * NL + i;
             if (e < a.E && choice[i] > ninf) choice[i] += a.bias[e];
             if (choice[i] != choice[i]) choice[i] = ninf, nan = true;
         }
     nan = __ballot(nan) != 0;
+    unsigned key[NL];
+#pragma unroll
+    for (int i = 0; i < NL; i++) key[i] = choice[i] > ninf ? ordered(choice[i]) : 0;
     if (a.groups > 1) {
+        // `per` lanes a group (a power of two) take its choices in turn and join their two largest
         float *mine = lds + wv * a.E;
         const int size = a.E / a.groups;
+        int per = 64;
+        while (per * a.groups > 64) per >>= 1;
 #pragma unroll
         for (int i = 0; i < NL; i++)
-            if (i * 64 + lane < a.E) mine[i * 64 + lane] = choice[i];
+            if (lane * NL + i < a.E) mine[lane * NL + i] = choice[i];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // other lanes read what these wrote
         __builtin_amdgcn_wave_barrier();
+        const int group = lane / per;
         float best = ninf, second = ninf;
-        if (lane < a.groups)
-            for (int i = 0; i < size; i++) {
-                const float c = mine[lane * size + i];
-                second = fmaxf(second, fminf(best, c));
-                best = fmaxf(best, c);
-            }
+        auto take = [&](float c) {
+            second = fmaxf(second, fminf(best, c));
+            best = fmaxf(best, c);
+        };
+        if (group < a.groups)
+            for (int i = lane % per; i < size; i += per) take(mine[group * size + i]);
+        for (int d = per >> 1; d; d >>= 1) {
+            const float b = __shfl_xor(best, d), c = __shfl_xor(second, d);
+            take(b);
+            take(c);
+        }
         // a group with one expert left counts as that one; one with none is never chosen
-        const unsigned key = ordered(a.sigmoid && second > ninf ? best + second : best);
+        const unsigned mark = ordered(a.sigmoid && second > ninf ? best + second : best);
         int rank = 0;
         for (int j = 0; j < a.groups; j++) {
-            const unsigned other = __shfl(key, j);
-            rank += other > key || (other == key && j < lane);
+            const unsigned other = (unsigned)__builtin_amdgcn_readlane((int)mark, j * per);
+            rank += other > mark || (other == mark && j < group);
         }
-        const unsigned long long keep = __ballot(lane < a.groups && rank < a.top_groups);
+        const unsigned long long keep = __ballot(group < a.groups && rank < a.top_groups);   // of each group `per` bits
 #pragma unroll
         for (int i = 0; i < NL; i++) {
-            const int e = i * 64 + lane;
-            if (e < a.E && !(keep >> (e / size) & 1)) choice[i] = ninf;
+            const int e = lane * NL + i;
+            if (e < a.E && !(keep >> (e / size * per) & 1)) key[i] = 0;
         }
     }
     int id = -1;      // lane j: the j-th choice
     float w = 0.f;
     for (int j = 0; j < a.k; j++) {
-        unsigned long long best = 0;   // (choice, lowest index first); 0: none left
+        unsigned best = key[0];
+        int at = 0;
+        float s = score[0];
 #pragma unroll
-        for (int i = 0; i < NL; i++) {
-            const unsigned long long key = (unsigned long long)ordered(choice[i]) << 32 | (0xffffffffu - (i * 64 + lane));
-            if (choice[i] > ninf && key > best) best = key;
-        }
+        for (int i = 1; i < NL; i++)
+            if (key[i] > best) best = key[i], at = i, s = score[i];
+        const unsigned top = wave_max(best);
+        if (!top) break;   // none left
+        const int from = __builtin_ctzll(__ballot(best == top));
+        const int e = from * NL + __builtin_amdgcn_readlane(at, from);
+        const float ws = as_f((unsigned)__builtin_amdgcn_readlane((int)as_u(s), from));
+        if (lane == from)
 #pragma unroll
-        for (int d = 32; d; d >>= 1) {
-            const unsigned long long other = __shfl_xor(best, d);
-            best = other > best ? other : best;
-        }
-        if (!best) break;
-        const int e = (int)(0xffffffffu - (unsigned)best);
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < NL; i++)
-            if (i == e / 64) {
-                s = score[i];
-                if (lane == e % 64) choice[i] = ninf;
-            }
-        s = __shfl(s, e % 64);
-        if (lane == j) id = e, w = s;
+            for (int i = 0; i < NL; i++)
+                if (i == at) key[i] = 0;
+        if (lane == j) id = e, w = ws;
     }
     if (a.renorm) {
         const float sum = wave_sum(w);
@@ -207,17 +234,30 @@ __global__ void __launch_bounds__(1024) moe_plan_kernel(const int *__restrict__ 
     each([&](int e, int i) { order[atomicAdd(&base[e], 1)] = i; });
 }
 
-// C(t) = Σ_s weights(t, s) · y(t, s), in the order of s; places that are no expert's are left out.
+// C(t) = Σ_s weights(t, s) · y(t, s), in the order of s; places that are no expert's are left out. A thread for four columns
+// of a token; y has rows of ld, whole 16-byte pieces.
 template <class T>
-__global__ void __launch_bounds__(256) moe_join_kernel(const float *__restrict__ y, const int *__restrict__ ids, const float *__restrict__ weights,
+__global__ void __launch_bounds__(256) moe_join_kernel(const float *__restrict__ y, long long ld, const int *__restrict__ ids, const float *__restrict__ weights,
                                                        int S, int E, int N, T *__restrict__ C, long long ldct) {
     const long long t = blockIdx.y;
-    const int n = blockIdx.x * 256 + threadIdx.x;
+    const int n = (blockIdx.x * 256 + threadIdx.x) * 4;
     if (n >= N) return;
-    float sum = 0.f;
-    for (int s = 0; s < S; s++)
-        if ((unsigned)ids[t * S + s] < (unsigned)E) sum += weights[t * S + s] * y[(t * S + s) * N + n];
-    C[t * ldct + n] = (T)sum;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < S; s++) {
+        const bool is = (unsigned)ids[t * S + s] < (unsigned)E;
+        const float w = is ? weights[t * S + s] : 0.f;
+        const f32x4 v = *reinterpret_cast<const f32x4 *>(y + (t * S + s) * ld + n);
+        if (is) sum += w * v;
+    }
+    T *c = C + t * ldct + n;
+    if (n + 4 <= N) {
+        typedef T T4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+        *reinterpret_cast<T4 *>(c) = T4{(T)sum[0], (T)sum[1], (T)sum[2], (T)sum[3]};
+    } else
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (n + j < N) c[j] = (T)sum[j];
 }
 
 template <class T> static int launch_route(const RouteArgs &a) {
@@ -275,7 +315,8 @@ static int experts(int Tn, int S, const int *ids, const void *X, int64_t ldt, in
         G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "moe_gemm: more tiles than one launch can index");
     void *plan = nullptr, *slots = nullptr;
     G9_TRY(scratch(SLOT_PLAN, (size_t)(n + E + 3 + 2 * most) * 4, &plan));
-    if (weights) G9_TRY(scratch(SLOT_SLOTS, (size_t)n * N * 4, &slots));
+    const long long ld = (N + 3) / 4 * 4LL;
+    if (weights) G9_TRY(scratch(SLOT_SLOTS, (size_t)n * ld * 4, &slots));
     int *order = (int *)plan, *off = order + n, *tiles = off + E + 3;
     hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(1024), 0, stream, ids, (int)n, E, rows, order, off, tiles, (int)most);
     G9_HIP(hipGetLastError());
@@ -283,12 +324,12 @@ static int experts(int Tn, int S, const int *ids, const void *X, int64_t ldt, in
     const Mx4View w = view(W), g = gate ? view(gate) : w;
     if (!weights)
         return gate ? launch_grouped<T, T, true>(R, w, g, E, (int)most, rows, Tn, n) : launch_grouped<T, T, false>(R, w, g, E, (int)most, rows, Tn, n);
-    R.C = slots, R.ldct = (long long)S * N, R.ldcs = N;
+    R.C = slots, R.ldct = S * ld, R.ldcs = ld;
     G9_TRY((gate ? launch_grouped<T, float, true>(R, w, g, E, (int)most, rows, Tn, n) : launch_grouped<T, float, false>(R, w, g, E, (int)most, rows, Tn, n)));
     for (int t0 = 0; t0 < Tn; t0 += 65535) {   // the grid's y limit
         const int rowsy = min(Tn - t0, 65535);
-        hipLaunchKernelGGL((moe_join_kernel<T>), dim3((unsigned)cdiv(N, 256), (unsigned)rowsy), dim3(256), 0, stream,
-                           (const float *)slots + (long long)t0 * S * N, ids + (long long)t0 * S, weights + (long long)t0 * S, S, E, N,
+        hipLaunchKernelGGL((moe_join_kernel<T>), dim3((unsigned)cdiv(N, 1024), (unsigned)rowsy), dim3(256), 0, stream,
+                           (const float *)slots + t0 * S * ld, ld, ids + (long long)t0 * S, weights + (long long)t0 * S, S, E, N,
                            (T *)C + t0 * ldct, (long long)ldct);
     }
     G9_HIP(hipGetLastError());

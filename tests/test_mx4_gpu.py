@@ -145,6 +145,37 @@ def test_gemm_quantized(g9, torch_dev, out, M, N, K):
     check_product(torch_dev, got, values(*quantize(a)), values(codes, scales))
 
 
+def check_large(torch, got, a, w, out):
+    """check_product with the 64-bit products on the GPU."""
+    ref, mag = a @ w.t(), a.abs() @ w.abs().t()
+    tol = sum_bound(a.shape[1]) * mag + (2.0 ** -11 * ref.abs() + 2.0 ** -25 if out == torch.float16 else 2.0 ** -24 * ref.abs())
+    assert got.dtype == out and bool(((got.double() - ref).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("K", [96, 200, 384, 512, 640, 1100, 1536])
+def test_gemm_quantized_large(g9, torch_dev, K):
+    """Enough tiles for one of 256 × 256 a CU, ragged at both ends, for every number of 128-k stages up to a few groups."""
+    torch = torch_dev
+    g = torch.Generator(device="cuda").manual_seed(K)
+    qa = g9.mx4_quantize(torch.randn((4100, K), generator=g, device="cuda"))
+    qw = g9.mx4_quantize(torch.randn((4117, K), generator=g, device="cuda") / 8)
+    a, w = g9.mx4_dequantize(qa).double(), g9.mx4_dequantize(qw).double()
+    for out, t in ((np.float16, torch.float16), (np.float32, torch.float32)):
+        check_large(torch, g9.mx4_gemm(qa, qw, dtype=out), a, w, t)
+
+
+@pytest.mark.parametrize("M,N,K", [(1000, 5000, 256), (513, 4099, 1000), (2050, 2050, 640)])
+def test_gemm_large(g9, torch_dev, M, N, K):
+    """More tiles than CUs: k is not split."""
+    torch = torch_dev
+    g = torch.Generator(device="cuda").manual_seed(M)
+    W = g9.mx4_quantize(torch.randn((N, K), generator=g, device="cuda") / 8)
+    w = g9.mx4_dequantize(W).double()
+    for t in (torch.float16, torch.float32):
+        a = torch.randn((M, K), generator=g, device="cuda").to(t)
+        check_large(torch, g9.mx4_gemm(a, W), a.double(), w, t)
+
+
 @pytest.mark.parametrize("dtype", [np.float16, np.float32])
 @pytest.mark.parametrize("M", [1, 7, 33, 90, 260])
 def test_gemm_strides(g9, torch_dev, dtype, M):
