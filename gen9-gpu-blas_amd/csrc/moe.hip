@@ -286,19 +286,19 @@ template <class T, class O, bool GATED> static int launch_grouped(const Rows &R,
     const Split whole = {1, nullptr, 0, 0};
     // few: 8 waves share the rows of a chunk, 128·NT columns a workgroup; rows: each wave has its own, 16·NT columns
     auto few = [&](auto kernel, int cols) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(cdiv(most * cdiv(W.rt, cols), 8) * 8)), dim3(512), 0, stream, R, W, G, E, 0, (int)cdiv(W.rt, cols), whole);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(cdiv(most * cdiv(W.rt, cols), 8) * 8)), dim3(512), 0, stream, R, W, G, E, most, (int)cdiv(W.rt, cols), whole);
     };
     if (rows == 32)
         // gated, FP16 44 × 4 places of 16 experts, 832 × 1664, and FP32 21 × 8, 768 × 4096: 16.6 and 49.5 µs; two column tiles a
         // wave 24.3 and 75.3, the rows kernel 17.1 and 55.4
         few(mx4_gemm_few_kernel<T, O, 2, 1, 8, 4, true, GATED>, 8);
-    else if (sizeof(T) == 2 || std::min<long long>(n, E) * cdiv(W.rt, 8) < num_cus)
-        // FP16 gated, 8 places, 1536 × 4096: 15.3 µs; few kernel 20.6 and more. FP32 gated, 7 places, 864 × 3840: 16 µs a call,
-        // the few kernel, whose 49 workgroups leave most CUs idle, 29
-        hipLaunchKernelGGL((mx4_gemm_rows_kernel<T, O, 1, 1, 1, 2, true, GATED>), dim3((unsigned)((long long)most * W.rt)), dim3(256), 0, stream, R, W, G, E, W.rt, whole);
     else if (std::min<long long>(n, E) * cdiv(W.rt, 16) >= 2LL * num_cus)
-        // 24 × 4 places of 64 experts, 4096 × 1536: 35.6 µs; one column tile a wave 41.3, the rows kernel 63
+        // FP32 joined, 24 × 4 places of 64 experts, 4096 × 1536: 35.6 µs; one column tile a wave 41.3, the rows kernel 63
         few(mx4_gemm_few_kernel<T, O, 1, 2, 8, 4, true, GATED>, 16);
+    else if (std::min<long long>(n, E) * cdiv(W.rt, 8) < num_cus)
+        // FP16 gated, 8 places, 1536 × 4096: 13.6 µs; few kernel 20.6 and more. FP32 gated, 7 places, 864 × 3840: 14.2 µs, the few
+        // kernel, whose 49 workgroups leave most CUs idle, 24
+        hipLaunchKernelGGL((mx4_gemm_rows_kernel<T, O, 1, 1, 1, 2, true, GATED>), dim3((unsigned)((long long)most * W.rt)), dim3(256), 0, stream, R, W, G, E, W.rt, whole);
     else
         few(mx4_gemm_few_kernel<T, O, 1, 1, 8, 4, true, GATED>, 8);
     G9_HIP(hipGetLastError());
@@ -309,18 +309,23 @@ template <class T>
 static int experts(int Tn, int S, const int *ids, const void *X, int64_t ldt, int64_t lds, const gen9blas_mx4 *W, const gen9blas_mx4 *gate,
                    const float *weights, void *C, int64_t ldct, int64_t ldcs) {
     const long long n = (long long)Tn * S;
-    const int E = W->count, N = W->rows, rows = n > 16LL * E ? 64 : n > 8LL * E ? 32 : 16;
-    const long long most = cdiv(n, rows) + E + 1;
+    const int E = W->count, N = W->rows, rows = n > 64 && n > 16LL * E ? 64 : n > 8LL * E ? 32 : 16;
+    // Few places: each workgroup finds its rows among the ids itself (8 places 17.5 µs a call with a plan, whose kernel comes first)
+    const bool direct = n <= 64;
+    const long long most = direct ? n : cdiv(n, rows) + E + 1;
     if (most * W->rt > 0xffffff || n > 0x7fffffff)
         G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "moe_gemm: more tiles than one launch can index");
     void *plan = nullptr, *slots = nullptr;
-    G9_TRY(scratch(SLOT_PLAN, (size_t)(n + E + 3 + 2 * most) * 4, &plan));
     const long long ld = (N + 3) / 4 * 4LL;
     if (weights) G9_TRY(scratch(SLOT_SLOTS, (size_t)n * ld * 4, &slots));
-    int *order = (int *)plan, *off = order + n, *tiles = off + E + 3;
-    hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(1024), 0, stream, ids, (int)n, E, rows, order, off, tiles, (int)most);
-    G9_HIP(hipGetLastError());
-    Rows R = {X, C, ldt, lds, ldct, ldcs, 0, S, tiles, order, off};
+    Rows R = {X, C, ldt, lds, ldct, ldcs, (int)n, S, nullptr, nullptr, nullptr, direct ? ids : nullptr};
+    if (!direct) {
+        G9_TRY(scratch(SLOT_PLAN, (size_t)(n + E + 3 + 2 * most) * 4, &plan));
+        int *order = (int *)plan, *off = order + n, *tiles = off + E + 3;
+        hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(1024), 0, stream, ids, (int)n, E, rows, order, off, tiles, (int)most);
+        G9_HIP(hipGetLastError());
+        R.tiles = tiles, R.order = order, R.off = off;
+    }
     const Mx4View w = view(W), g = gate ? view(gate) : w;
     if (!weights)
         return gate ? launch_grouped<T, T, true>(R, w, g, E, (int)most, rows, Tn, n) : launch_grouped<T, T, false>(R, w, g, E, (int)most, rows, Tn, n);

@@ -166,7 +166,7 @@ int gen9blas_mx4_gemm(int type, int M, const void *A, int lda, const gen9blas_mx
     const int es = elem_size(type);
     G9_TRY(need_device(A, ((size_t)(M - 1) * lda + W->K) * es, "mx4_gemm: A"));
     G9_TRY(need_device(C, ((size_t)(M - 1) * ldc + W->rows) * es, "mx4_gemm: C"));
-    const Rows R = {A, C, lda, 0, ldc, 0, M, 1, nullptr, nullptr, nullptr};
+    const Rows R = {A, C, lda, 0, ldc, 0, M, 1, nullptr, nullptr, nullptr, nullptr};
     return type == GEN9BLAS_H ? launch_dense<_Float16>(R, view(W)) : launch_dense<float>(R, view(W));
 }
 

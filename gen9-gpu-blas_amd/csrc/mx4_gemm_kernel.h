@@ -131,6 +131,7 @@ struct Rows {
     long long ldt, lds, ldct, ldcs;
     int M, S;
     const int *tiles, *order, *off;
+    const int *ids;   // not null: no plan, M places with these experts
 };
 
 // Rows of a finished tile from LDS (ROWS rows of COLS elements, PITCH bytes apart) to memory: consecutive threads take

@@ -4,6 +4,42 @@
 
 namespace g9llm {
 
+// The rows of a tile, to `slots` in LDS: of the plan's tile t, or (ids: few places, no plan) of place t's expert, if t is the first,
+// 17th (ROWS + 1st), ... place with that expert; count 0 otherwise. e = experts: places without one. All threads of a workgroup
+// call it; a wave finds the places 64 at a time.
+struct TileRows {
+    int e, first, count;
+};
+template <int ROWS> __device__ __forceinline__ TileRows tile_rows(const Rows &R, int t, int experts, int *slots) {
+    TileRows o;
+    if (!R.ids) {
+        o.e = R.tiles[2 * t], o.first = R.tiles[2 * t + 1];
+        o.count = min(ROWS, R.off[o.e + 1] - o.first);
+        if ((int)threadIdx.x < o.count) slots[threadIdx.x] = R.order[o.first + threadIdx.x];
+    } else {
+        const int lane = threadIdx.x & 63, n = R.M;
+        auto expert = [&](int i) { return i < n ? (int)min((unsigned)R.ids[i], (unsigned)experts) : -1; };   // ids outside 0..E−1: E
+        o.e = expert(t), o.first = 0;
+        int before = 0, all = 0;
+        for (int c = 0; c < n; c += 64) {
+            const unsigned long long mask = __ballot(expert(c + lane) == o.e);
+            all += __builtin_popcountll(mask);
+            if (c <= t) before += __builtin_popcountll(t - c < 64 ? mask & ((1ull << (t - c)) - 1) : mask);
+        }
+        o.count = before % ROWS ? 0 : min(ROWS, all - before);
+        int rank = -before;
+        for (int c = 0; o.count && c < n; c += 64) {
+            const bool mine = expert(c + lane) == o.e;
+            const unsigned long long mask = __ballot(mine);
+            const int at = rank + __builtin_popcountll(mask & ((1ull << lane) - 1));
+            if (threadIdx.x < 64 && mine && at >= 0 && at < o.count) slots[at] = c + lane;
+            rank += __builtin_popcountll(mask);
+        }
+    }
+    __syncthreads();
+    return o;
+}
+
 // 32 consecutive k of a row in MFMA fragments: f[i][p] the i-th eight, piece p.
 template <class T> struct Row32;
 template <> struct Row32<_Float16> {
@@ -78,8 +114,8 @@ template <> struct Row32<float> {
 
 // The end of a row's four columns col .. col + 3 (y: the sum with W, z: with the gate): to C, or as a part's sums.
 template <class T, class O, bool GROUPED, bool GATED>
-__device__ __forceinline__ void finish4(const Rows &R, const Mx4View &W, const Split &split, int part, int first, int i, int col, f32x4 y, f32x4 z, const int *ty,
-                                        const int *tz) {
+__device__ __forceinline__ void finish4(const Rows &R, const Mx4View &W, const Split &split, int part, int first, const int *slots, int i, int col, f32x4 y, f32x4 z,
+                                        const int *ty, const int *tz) {
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         y[j] = Act<T>::finish(y[j], ty[j]);
@@ -94,7 +130,7 @@ __device__ __forceinline__ void finish4(const Rows &R, const Mx4View &W, const S
     }
     O *c;
     if (GROUPED) {
-        const int slot = R.order[first + i];
+        const int slot = slots[i];
         c = (O *)R.C + slot / R.S * R.ldct + slot % R.S * R.ldcs;
     } else
         c = (O *)R.C + (long long)(first + i) * R.ldct;
@@ -150,11 +186,13 @@ __global__ void __launch_bounds__(256) mx4_gemm_rows_kernel(Rows R, Mx4View W, M
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const int part = blockIdx.x % split.parts, tile = blockIdx.x / split.parts;
     const int mt0 = tile / ntiles, nt0 = tile % ntiles;
+    __shared__ int slots[GROUPED ? MT * 16 : 1];
     int first, count, e = 0;
     if (GROUPED) {
-        if (mt0 >= R.tiles[-1]) return;
-        e = R.tiles[2 * mt0], first = R.tiles[2 * mt0 + 1];
-        count = min(MT * 16, R.off[e + 1] - first);
+        if (!R.ids && mt0 >= R.tiles[-1]) return;
+        const TileRows o = tile_rows<MT * 16>(R, mt0, experts, slots);
+        e = o.e, first = o.first, count = o.count;
+        if (count == 0) return;
     } else
         first = mt0 * MT * 16, count = min(MT * 16, R.M - first);
     const int col0 = (nt0 * WN + wv % WN) * NT;   // first row tile of W
@@ -174,13 +212,13 @@ __global__ void __launch_bounds__(256) mx4_gemm_rows_kernel(Rows R, Mx4View W, M
         const T *row[MT];   // rows past the last repeat it and are not stored
 #pragma unroll
         for (int m = 0; m < MT; m++) {
-            const int i = first + min(m * 16 + r, count - 1);
+            const int i = min(m * 16 + r, count - 1);
             long long at;
             if (GROUPED) {
-                const int slot = R.order[i];
+                const int slot = slots[i];
                 at = slot / R.S * R.ldt + slot % R.S * R.lds;
             } else
-                at = (long long)i * R.ldt;
+                at = (long long)(first + i) * R.ldt;
             row[m] = (const T *)R.A + at + g * 32;
         }
         const u32x4 *wc[NW][NT];
@@ -284,7 +322,7 @@ __global__ void __launch_bounds__(256) mx4_gemm_rows_kernel(Rows R, Mx4View W, M
 #pragma unroll
         for (int m = 0; m < MT; m++) {
             const int i = m * 16 + r;
-            if (i < count) finish4<T, O, GROUPED, GATED>(R, W, split, part, first, i, col, acc[0][n][m], acc[NW - 1][n][m], tn[0], tn[NW - 1]);
+            if (i < count) finish4<T, O, GROUPED, GATED>(R, W, split, part, first, slots, i, col, acc[0][n][m], acc[NW - 1][n][m], tn[0], tn[NW - 1]);
         }
     }
 }
@@ -313,15 +351,19 @@ __global__ void __launch_bounds__(NV * 64, 2) mx4_gemm_few_kernel(Rows R, Mx4Vie
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     // Each XCD (workgroups b, b + 8, ...) takes a contiguous run of tiles, so that those resident on it share rows and weights:
     // dense, row tiles of the same columns; experts, column tiles of the same rows.
-    if (GROUPED) mtiles = R.tiles[-1];
-    const int total = mtiles * ntiles * split.parts, run = (total + 7) / 8, id = (blockIdx.x & 7) * run + (blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= run || id >= total) return;
+    // Without a plan the places that come first have most of the work, so they are dealt out to the XCDs in turn.
+    const bool deal = GROUPED && R.ids;
+    if (GROUPED && !deal) mtiles = R.tiles[-1];
+    const int total = mtiles * ntiles * split.parts, run = (total + 7) / 8, id = deal ? (int)blockIdx.x : (blockIdx.x & 7) * run + (blockIdx.x >> 3);
+    if ((!deal && (int)(blockIdx.x >> 3) >= run) || id >= total) return;
     const int part = id % split.parts, tile = id / split.parts;
     const int mt0 = GROUPED ? tile / ntiles : tile % mtiles, nt0 = GROUPED ? tile % ntiles : tile / mtiles;
+    __shared__ int slots[GROUPED ? MT * 16 : 1];
     int first, count, e = 0;
     if (GROUPED) {
-        e = R.tiles[2 * mt0], first = R.tiles[2 * mt0 + 1];
-        count = min(MT * 16, R.off[e + 1] - first);
+        const TileRows o = tile_rows<MT * 16>(R, mt0, experts, slots);
+        e = o.e, first = o.first, count = o.count;
+        if (count == 0) return;
     } else
         first = mt0 * MT * 16, count = min(MT * 16, R.M - first);
     const int col0 = (nt0 * NV + wv) * NT;   // first row tile of W
@@ -342,13 +384,13 @@ __global__ void __launch_bounds__(NV * 64, 2) mx4_gemm_few_kernel(Rows R, Mx4Vie
         const T *row[NL];   // rows past the last repeat it and are not stored
 #pragma unroll
         for (int u = 0; u < NL; u++) {
-            const int i = first + min(u * (NTH / PR) + (int)threadIdx.x / PR, count - 1);
+            const int i = min(u * (NTH / PR) + (int)threadIdx.x / PR, count - 1);
             long long at;
             if (GROUPED) {
-                const int slot = R.order[i];
+                const int slot = slots[i];
                 at = slot / R.S * R.ldt + slot % R.S * R.lds;
             } else
-                at = (long long)i * R.ldt;
+                at = (long long)(first + i) * R.ldt;
             row[u] = (const T *)R.A + at + at_k;
         }
         const u32x4 *wc[NW][NT];   // uniform: the lane is added to each load's offset
@@ -487,7 +529,7 @@ __global__ void __launch_bounds__(NV * 64, 2) mx4_gemm_few_kernel(Rows R, Mx4Vie
 #pragma unroll
         for (int m = 0; m < MT; m++) {
             const int i = m * 16 + r;
-            if (i < count) finish4<T, O, GROUPED, GATED>(R, W, split, part, first, i, col, acc[0][n][m], acc[NW - 1][n][m], tn[0], tn[NW - 1]);
+            if (i < count) finish4<T, O, GROUPED, GATED>(R, W, split, part, first, slots, i, col, acc[0][n][m], acc[NW - 1][n][m], tn[0], tn[NW - 1]);
         }
     }
 }
