@@ -49,7 +49,9 @@ __device__ __forceinline__ unsigned wave_max(unsigned v) {
 }
 
 // A wave routes a token: lane l holds the NL experts from l·NL on, so that of equal choices the lowest lane's, and there the
-// first, is the lowest index. The k experts are k rounds of a wave's maximum over ordered choices (0: not to be chosen).
+// first, is the lowest index. A lane sorts its choices (as ordered numbers; 0: not to be chosen) once, neighbours only, which keeps
+// equal ones in their order; the k experts are k rounds of the wave's maximum over the lanes' first, and the lane that had it moves
+// its own up. Instructions bound it: 8192 tokens of 256 experts, 8 chosen, 10.4 µs a call; 12.1 with each round over all of a lane's choices.
 template <class T, int NL>
 __global__ void __launch_bounds__(256) moe_route_kernel(RouteArgs a) {
     const float ninf = -__builtin_inff();
@@ -57,20 +59,22 @@ __global__ void __launch_bounds__(256) moe_route_kernel(RouteArgs a) {
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const long long t = (long long)blockIdx.x * 4 + wv;
     if (t >= a.T) return;   // whole waves: nothing below waits for another wave
-    const T *row = (const T *)a.logits + t * a.ldl;
-    float score[NL], choice[NL];
-    bool nan = false;
-    if (lane * NL + NL <= a.E) {
-        typedef T TV __attribute__((ext_vector_type(NL), aligned(sizeof(T))));
-        if constexpr (NL > 1) {
-            const TV v = *reinterpret_cast<const TV *>(row + lane * NL);
+    float *mine = lds + wv * 64 * NL;
+    float score[NL], choice[NL], bias[NL];
+    auto load = [&](auto *row, float *v, float none) {
+        typedef std::remove_cv_t<std::remove_reference_t<decltype(*row)>> E;
+        if (lane * NL + NL <= a.E) {
+            E e[NL];
+            __builtin_memcpy(e, row + lane * NL, sizeof e);
 #pragma unroll
-            for (int i = 0; i < NL; i++) score[i] = (float)v[i];
+            for (int i = 0; i < NL; i++) v[i] = (float)e[i];
         } else
-            score[0] = (float)row[lane];
-    } else
 #pragma unroll
-        for (int i = 0; i < NL; i++) score[i] = lane * NL + i < a.E ? (float)row[lane * NL + i] : ninf;
+            for (int i = 0; i < NL; i++) v[i] = lane * NL + i < a.E ? (float)row[lane * NL + i] : none;
+    };
+    load((const T *)a.logits + t * a.ldl, score, ninf);
+    if (a.bias) load(a.bias, bias, 0.f);
+    bool nan = false;
 #pragma unroll
     for (int i = 0; i < NL; i++) nan |= score[i] != score[i];
     if (a.sigmoid) {
@@ -102,72 +106,94 @@ __global__ void __launch_bounds__(256) moe_route_kernel(RouteArgs a) {
     if (a.bias)
 #pragma unroll
         for (int i = 0; i < NL; i++) {
-            const int e = lane * NL + i;
-            if (e < a.E && choice[i] > ninf) choice[i] += a.bias[e];
+            if (choice[i] > ninf) choice[i] += bias[i];
             if (choice[i] != choice[i]) choice[i] = ninf, nan = true;
         }
     nan = __ballot(nan) != 0;
     unsigned key[NL];
+    int at[NL];
 #pragma unroll
-    for (int i = 0; i < NL; i++) key[i] = choice[i] > ninf ? ordered(choice[i]) : 0;
+    for (int i = 0; i < NL; i++) key[i] = choice[i] > ninf ? ordered(choice[i]) : 0, at[i] = i;
     if (a.groups > 1) {
-        // `per` lanes a group (a power of two) take its choices in turn and join their two largest
-        float *mine = lds + wv * a.E;
+        // `per` lanes a group (a power of two) take its choices, their own where those are the group's, and join their two largest
         const int size = a.E / a.groups;
         int per = 64;
         while (per * a.groups > 64) per >>= 1;
-#pragma unroll
-        for (int i = 0; i < NL; i++)
-            if (lane * NL + i < a.E) mine[lane * NL + i] = choice[i];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // other lanes read what these wrote
-        __builtin_amdgcn_wave_barrier();
+        const bool own = per * NL == size;
         const int group = lane / per;
         float best = ninf, second = ninf;
-        auto take = [&](float c) {
-            second = fmaxf(second, fminf(best, c));
-            best = fmaxf(best, c);
+        auto take = [&](float b, float s) {
+            second = fmaxf(fmaxf(second, s), fminf(best, b));
+            best = fmaxf(best, b);
         };
-        if (group < a.groups)
-            for (int i = lane % per; i < size; i += per) take(mine[group * size + i]);
-        for (int d = per >> 1; d; d >>= 1) {
-            const float b = __shfl_xor(best, d), c = __shfl_xor(second, d);
-            take(b);
-            take(c);
+        if (own) {
+#pragma unroll
+            for (int i = 0; i < NL; i++) take(choice[i], ninf);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NL; i++) mine[lane * NL + i] = choice[i];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // other lanes read what these wrote
+            __builtin_amdgcn_wave_barrier();
+            if (group < a.groups)
+                for (int i = lane % per; i < size; i += per) take(mine[group * size + i], ninf);
         }
+        auto join = [&](auto other) {
+            const float b = as_f(other(as_u(best))), s = as_f(other(as_u(second)));
+            take(b, s);
+        };
+        if (per > 1) join([](unsigned v) { return dpp<0xb1, 0xf>(0, v); });    // lanes 1 apart
+        if (per > 2) join([](unsigned v) { return dpp<0x4e, 0xf>(0, v); });    // 2 apart
+        if (per > 4) join([](unsigned v) { return dpp<0x141, 0xf>(0, v); });   // the other four of eight
+        if (per > 8) join([](unsigned v) { return dpp<0x140, 0xf>(0, v); });   // the other eight of sixteen
+        if (per > 16) join([](unsigned v) { return (unsigned)__shfl_xor((int)v, 16); });
         // a group with one expert left counts as that one; one with none is never chosen
         const unsigned mark = ordered(a.sigmoid && second > ninf ? best + second : best);
         int rank = 0;
         for (int j = 0; j < a.groups; j++) {
             const unsigned other = (unsigned)__builtin_amdgcn_readlane((int)mark, j * per);
-            rank += other > mark || (other == mark && j < group);
+            rank += other >= mark + (j >= group);   // of equal groups the first; no mark is the largest number
         }
         const unsigned long long keep = __ballot(group < a.groups && rank < a.top_groups);   // of each group `per` bits
-#pragma unroll
-        for (int i = 0; i < NL; i++) {
-            const int e = lane * NL + i;
-            if (e < a.E && !(keep >> (e / size * per) & 1)) key[i] = 0;
-        }
-    }
-    int id = -1;      // lane j: the j-th choice
-    float w = 0.f;
-    for (int j = 0; j < a.k; j++) {
-        unsigned best = key[0];
-        int at = 0;
-        float s = score[0];
-#pragma unroll
-        for (int i = 1; i < NL; i++)
-            if (key[i] > best) best = key[i], at = i, s = score[i];
-        const unsigned top = wave_max(best);
-        if (!top) break;   // none left
-        const int from = __builtin_ctzll(__ballot(best == top));
-        const int e = from * NL + __builtin_amdgcn_readlane(at, from);
-        const float ws = as_f((unsigned)__builtin_amdgcn_readlane((int)as_u(s), from));
-        if (lane == from)
+        if (own) {
 #pragma unroll
             for (int i = 0; i < NL; i++)
-                if (i == at) key[i] = 0;
-        if (lane == j) id = e, w = ws;
+                if (!(keep >> lane & 1)) key[i] = 0;
+        } else
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const int e = lane * NL + i;
+                if (e < a.E && !(keep >> (e / size * per) & 1)) key[i] = 0;
+            }
+        __builtin_amdgcn_wave_barrier();   // the choices in LDS have been read
     }
+#pragma unroll
+    for (int i = 0; i < NL; i++) mine[lane * NL + i] = score[i];
+#pragma unroll
+    for (int n = 0; n < NL; n++)
+#pragma unroll
+        for (int i = n & 1; i + 1 < NL; i += 2) {
+            const bool swap = key[i + 1] > key[i];
+            const unsigned high = swap ? key[i + 1] : key[i], low = swap ? key[i] : key[i + 1];
+            const int first = swap ? at[i + 1] : at[i], last = swap ? at[i] : at[i + 1];
+            key[i] = high, key[i + 1] = low, at[i] = first, at[i + 1] = last;
+        }
+    int id = -1;      // lane j: the j-th choice
+    for (int j = 0; j < a.k; j++) {
+        const unsigned top = wave_max(key[0]);
+        if (!top) break;   // none left
+        const int from = __builtin_ctzll(__ballot(key[0] == top));
+        const int e = from * NL + __builtin_amdgcn_readlane(at[0], from);
+        if (lane == j) id = e;
+        const bool moves = lane == from;
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            key[i] = moves ? i + 1 < NL ? key[i + 1] : 0 : key[i];
+            if (i + 1 < NL) at[i] = moves ? at[i + 1] : at[i];
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    float w = id >= 0 ? mine[id] : 0.f;
     if (a.renorm) {
         const float sum = wave_sum(w);
         w = sum == 0.f ? 0.f : w / sum;
@@ -182,8 +208,8 @@ __global__ void __launch_bounds__(256) moe_route_kernel(RouteArgs a) {
 
 // The plan of a grouped product: slots by expert (order; places whose id is no expert come last, as expert E), off[e] where
 // expert e's begin, and the tiles of `rows` slots: (expert, first place), (−1, 0) past the last, their number in front. One
-// workgroup: the ids are counted in LDS, a scan gives each expert's place, and the ids are read again to be placed. The order
-// of a group's slots varies from call to call; no result depends on it.
+// workgroup: the ids are counted in LDS, which gives each its rank among its expert's (kept in memory), a scan gives each expert's
+// place, and the ids are read again to be placed. The order of a group's slots varies from call to call; no result depends on it.
 __device__ __forceinline__ int2 scan_pair(int2 v, int lane) {   // sums over the lanes up to this one
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -192,7 +218,7 @@ __device__ __forceinline__ int2 scan_pair(int2 v, int lane) {   // sums over the
     }
     return v;
 }
-__global__ void __launch_bounds__(1024) moe_plan_kernel(const int *__restrict__ ids, int n, int E, int rows, int *order, int *off, int *tiles, int most) {
+__global__ void __launch_bounds__(1024) moe_plan_kernel(const int *__restrict__ ids, int n, int E, int rows, int *rank, int *order, int *off, int *tiles, int most) {
     __shared__ int count[MAX_EXPERTS + 1], base[MAX_EXPERTS + 1];
     __shared__ int2 waves[16];
     const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
@@ -209,7 +235,7 @@ __global__ void __launch_bounds__(1024) moe_plan_kernel(const int *__restrict__ 
                 if (i0 + j * 1024 < n) use((unsigned)id[j] < (unsigned)E ? id[j] : E, (int)(i0 + j * 1024));
         }
     };
-    each([&](int e, int) { atomicAdd(&count[e], 1); });
+    each([&](int e, int i) { rank[i] = atomicAdd(&count[e], 1); });
     __syncthreads();
     const int mine = t < E ? count[t] : 0, own = (mine + rows - 1) / rows;
     const int2 s = scan_pair({mine, own}, lane);
@@ -231,7 +257,7 @@ __global__ void __launch_bounds__(1024) moe_plan_kernel(const int *__restrict__ 
     }
     for (int i = last + t; i < most; i += 1024) tiles[2 * i] = -1, tiles[2 * i + 1] = 0;
     __syncthreads();
-    each([&](int e, int i) { order[atomicAdd(&base[e], 1)] = i; });
+    each([&](int e, int i) { order[base[e] + rank[i]] = i; });
 }
 
 // C(t) = Σ_s weights(t, s) · y(t, s), in the order of s; places that are no expert's are left out. A thread for four columns
@@ -262,12 +288,12 @@ __global__ void __launch_bounds__(256) moe_join_kernel(const float *__restrict__
 
 template <class T> static int launch_route(const RouteArgs &a) {
     const dim3 grid((unsigned)cdiv(a.T, 4)), block(256);
-    const size_t lds = a.groups > 1 ? (size_t)a.E * 16 : 0;
-    if (a.E <= 64) hipLaunchKernelGGL((moe_route_kernel<T, 1>), grid, block, lds, stream, a);
-    else if (a.E <= 128) hipLaunchKernelGGL((moe_route_kernel<T, 2>), grid, block, lds, stream, a);
-    else if (a.E <= 256) hipLaunchKernelGGL((moe_route_kernel<T, 4>), grid, block, lds, stream, a);
-    else if (a.E <= 512) hipLaunchKernelGGL((moe_route_kernel<T, 8>), grid, block, lds, stream, a);
-    else hipLaunchKernelGGL((moe_route_kernel<T, 16>), grid, block, lds, stream, a);
+    auto run = [&](auto kernel, int experts) { hipLaunchKernelGGL(kernel, grid, block, (size_t)experts * 16, stream, a); };
+    if (a.E <= 64) run(moe_route_kernel<T, 1>, 64);
+    else if (a.E <= 128) run(moe_route_kernel<T, 2>, 128);
+    else if (a.E <= 256) run(moe_route_kernel<T, 4>, 256);
+    else if (a.E <= 512) run(moe_route_kernel<T, 8>, 512);
+    else run(moe_route_kernel<T, 16>, 1024);
     G9_HIP(hipGetLastError());
     return 0;
 }
@@ -320,9 +346,9 @@ static int experts(int Tn, int S, const int *ids, const void *X, int64_t ldt, in
     if (weights) G9_TRY(scratch(SLOT_SLOTS, (size_t)n * ld * 4, &slots));
     Rows R = {X, C, ldt, lds, ldct, ldcs, (int)n, S, nullptr, nullptr, nullptr, direct ? ids : nullptr};
     if (!direct) {
-        G9_TRY(scratch(SLOT_PLAN, (size_t)(n + E + 3 + 2 * most) * 4, &plan));
-        int *order = (int *)plan, *off = order + n, *tiles = off + E + 3;
-        hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(1024), 0, stream, ids, (int)n, E, rows, order, off, tiles, (int)most);
+        G9_TRY(scratch(SLOT_PLAN, (size_t)(2 * n + E + 3 + 2 * most) * 4, &plan));
+        int *rank = (int *)plan, *order = rank + n, *off = order + n, *tiles = off + E + 3;
+        hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(1024), 0, stream, ids, (int)n, E, rows, rank, order, off, tiles, (int)most);
         G9_HIP(hipGetLastError());
         R.tiles = tiles, R.order = order, R.off = off;
     }
