@@ -324,7 +324,7 @@ template <class T, class O, bool GATED> static int launch_grouped(const Rows &R,
     else if (std::min<long long>(n, E) * cdiv(W.rt, 8) < num_cus)
         // FP16 gated, 8 places, 1536 × 4096: 13.6 µs; few kernel 20.6 and more. FP32 gated, 7 places, 864 × 3840: 14.2 µs, the few
         // kernel, whose 49 workgroups leave most CUs idle, 24
-        hipLaunchKernelGGL((mx4_gemm_rows_kernel<T, O, 1, 1, 1, 2, true, GATED>), dim3((unsigned)((long long)most * W.rt)), dim3(256), 0, stream, R, W, G, E, W.rt, whole);
+        hipLaunchKernelGGL((mx4_gemm_rows_kernel<T, O, 2, true, GATED>), dim3((unsigned)((long long)most * W.rt)), dim3(256), 0, stream, R, W, G, E, whole);
     else
         few(mx4_gemm_few_kernel<T, O, 1, 1, 8, 4, true, GATED>, 8);
     G9_HIP(hipGetLastError());

@@ -86,18 +86,16 @@ template <class O> static int sum_parts(const Rows &R, const Mx4View &W, const S
     return 0;
 }
 
-// Tiles of MT·16 rows × WN·NT·16 columns; k is split until there is about a workgroup a CU.
-template <class T, int MT, int NT, int WN, int D> static int launch_rows(const Rows &R, const Mx4View &W, int mtiles) {
-    const int ntiles = (int)cdiv(W.rt, NT * WN);
-    const long long tiles = (long long)mtiles * ntiles;
+// Up to 16 rows in tiles of 16 columns; k is split until there is about a workgroup a CU.
+template <class T> static int launch_rows(const Rows &R, const Mx4View &W) {
     Split split = {1, nullptr, 0, 0};
-    const int ways = (int)(num_cus / tiles), most = W.kc / (4 / WN * 2);
+    const int ways = num_cus / W.rt, most = W.kc / 8;
     if (ways > 1 && most > 1) {
         split.parts = ways < most ? ways : most;
         G9_TRY(split_space(R, W, &split));
     }
-    if (tiles * split.parts > 0xffffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm: more tiles than one launch can index");
-    hipLaunchKernelGGL((mx4_gemm_rows_kernel<T, T, MT, NT, WN, D, false, false>), dim3((unsigned)(tiles * split.parts)), dim3(256), 0, stream, R, W, W, 1, ntiles, split);
+    if ((long long)W.rt * split.parts > 0xffffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm: more tiles than one launch can index");
+    hipLaunchKernelGGL((mx4_gemm_rows_kernel<T, T, 4, false, false>), dim3((unsigned)(W.rt * split.parts)), dim3(256), 0, stream, R, W, W, 1, split);
     G9_HIP(hipGetLastError());
     return sum_parts<T>(R, W, split);
 }
@@ -139,15 +137,16 @@ template <class T> static int launch_tiles(const Rows &R, const Mx4View &W) {
 
 template <class T> static int launch_dense(const Rows &R, const Mx4View &W) {
     if (R.M > 64) return launch_tiles<T>(R, W);
-    constexpr bool F = sizeof(T) == 4;
     // µs of the product alone, FP16 1 × 11008 × 4096 and FP32 8 × 4096 × 11008: rows kernel 9.4 and 13.2, few kernel 8.8 to
     // 9.5 and 10.7: FP32 rows are taken apart once a workgroup there, and once a wave in the rows kernel.
     if (R.M <= 16) {
-        if (F) return launch_few<T, 1, 2, 8, 4>(R, W);
-        else return launch_rows<T, 1, 1, 1, 4>(R, W, 1);
+        if constexpr (sizeof(T) == 4) return launch_few<T, 1, 2, 8, 4>(R, W);
+        else return launch_rows<T>(R, W);
     }
-    // 24 × 4096 × 11008: 128 columns a workgroup 10.4 FP16 and 17.3 FP32, 256 columns 13.0 and 16.7
-    if (R.M <= 32) return launch_few<T, 2, F ? 2 : 1, 8, 4>(R, W);
+    // 128 columns a workgroup; with 256, which reads the rows from LDS half as often but leaves twice the parts to be summed or half
+    // the workgroups: FP32 24 × 4096 × 11008 19.6 µs and 20.0, 24 × 11008 × 4096 21.6 and 20.5, 28 × 2048 × 2048 9.5 and 11.9
+    if (R.M <= 32) return launch_few<T, 2, 1, 8, 4>(R, W);
+    // FP32 64 × 4096 × 4096 18.6 µs, 56 × 8192 × 8192 40.0, 33 × 1000 × 4992 14.3; 256 columns 21.9, 36.3, 18.1
     return launch_few<T, 4, 1, 8, 2>(R, W);
 }
 

@@ -175,102 +175,78 @@ __global__ void __launch_bounds__(256) mx4_sum_parts_kernel(Rows R, Split split,
     ((O *)R.C)[row * R.ldct + col] = (O)y;
 }
 
-// A workgroup has WN × WK waves (WN · WK = 4): WN side by side in n, each 16·NT columns (gated: of W and of the gate) of MT·16
-// rows, and WK along k; `split` workgroups share the k of a tile. Weights and rows of the next D chunks of 128 k are
-// on their way in registers. Lane 16g + r multiplies columns' row r of each weight tile, activations' row r.
-template <class T, class O, int MT, int NT, int WN, int D, bool GROUPED, bool GATED>
-__global__ void __launch_bounds__(256) mx4_gemm_rows_kernel(Rows R, Mx4View W, Mx4View G, int experts, int ntiles, Split split) {
+// A workgroup makes 16 rows of 16 columns (gated: of W and of the gate) by 4 waves along k; `split` workgroups share the k of
+// a tile. Weights and rows of the next D chunks of 128 k are on their way in registers. Lane 16g + r multiplies columns' row r of
+// each weight tile, activations' row r.
+template <class T, class O, int D, bool GROUPED, bool GATED>
+__global__ void __launch_bounds__(256) mx4_gemm_rows_kernel(Rows R, Mx4View W, Mx4View G, int experts, Split split) {
     typedef Act<T> X;
     typedef typename X::Frag Frag;
-    constexpr int NW = GATED ? 2 : 1, WK = 4 / WN, NA = NW * NT * MT;
+    constexpr int NW = GATED ? 2 : 1, WAVES = 4;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const int part = blockIdx.x % split.parts, tile = blockIdx.x / split.parts;
-    const int mt0 = tile / ntiles, nt0 = tile % ntiles;
-    __shared__ int slots[GROUPED ? MT * 16 : 1];
-    int first, count, e = 0;
+    const int mt = tile / W.rt, nt = tile % W.rt;
+    __shared__ int slots[GROUPED ? 16 : 1];
+    int first = 0, count = min(16, R.M), e = 0;   // dense: one tile of rows
     if (GROUPED) {
-        if (!R.ids && mt0 >= R.tiles[-1]) return;
-        const TileRows o = tile_rows<MT * 16>(R, mt0, experts, slots);
+        if (!R.ids && mt >= R.tiles[-1]) return;
+        const TileRows o = tile_rows<16>(R, mt, experts, slots);
         e = o.e, first = o.first, count = o.count;
         if (count == 0) return;
-    } else
-        first = mt0 * MT * 16, count = min(MT * 16, R.M - first);
-    const int col0 = (nt0 * WN + wv % WN) * NT;   // first row tile of W
-    f32x4 acc[NW][NT][MT];
+    }
+    f32x4 acc[NW];
+    int top[NW];
 #pragma unroll
-    for (int q = 0; q < NW; q++)
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int m = 0; m < MT; m++) acc[q][n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-    int top[NW][NT];
-#pragma unroll
-    for (int q = 0; q < NW; q++)
-#pragma unroll
-        for (int n = 0; n < NT; n++) top[q][n] = 0;
+    for (int q = 0; q < NW; q++) acc[q] = f32x4{0.f, 0.f, 0.f, 0.f}, top[q] = 0;
     if (!GROUPED || e < experts) {
-        const T *row[MT];   // rows past the last repeat it and are not stored
+        const int i = min(r, count - 1);   // rows past the last repeat it and are not stored
+        long long at;
+        if (GROUPED) {
+            const int slot = slots[i];
+            at = slot / R.S * R.ldt + slot % R.S * R.lds;
+        } else
+            at = i * R.ldt;
+        const T *row = (const T *)R.A + at + g * 32;
+        const u32x4 *wc[NW];
+        const uint8_t *ws[NW], *tops[NW];
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-            const int i = min(m * 16 + r, count - 1);
-            long long at;
-            if (GROUPED) {
-                const int slot = slots[i];
-                at = slot / R.S * R.ldt + slot % R.S * R.lds;
-            } else
-                at = (long long)(first + i) * R.ldt;
-            row[m] = (const T *)R.A + at + g * 32;
+        for (int q = 0; q < NW; q++) {
+            const Mx4View &V = q ? G : W;
+            const long long t = (long long)e * W.rt + nt;
+            wc[q] = reinterpret_cast<const u32x4 *>(V.codes) + t * W.kc * 64 + lane;
+            ws[q] = V.scales + t * W.kg * 256 + lane * 4;
+            tops[q] = V.top + (t * 16 + r) * W.kt;
         }
-        const u32x4 *wc[NW][NT];
-        const uint8_t *ws[NW][NT], *tops[NW * NT];
-#pragma unroll
-        for (int q = 0; q < NW; q++)
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                const Mx4View &V = q ? G : W;
-                const long long t = (long long)e * W.rt + min(col0 + n, W.rt - 1);
-                wc[q][n] = reinterpret_cast<const u32x4 *>(V.codes) + t * W.kc * 64 + lane;
-                ws[q][n] = V.scales + t * W.kg * 256 + lane * 4;
-                tops[q * NT + n] = V.top + (t * 16 + r) * W.kt;
-            }
-        if (X::P == 1) row_tops<NW * NT>(tops, W.kt, &top[0][0]);
-        const int ways = split.parts * WK, way = part * WK + wv / WN, whole = W.K / 128;
+        if (X::P == 1) row_tops<NW>(tops, W.kt, top);
+        const int ways = split.parts * WAVES, way = part * WAVES + wv, whole = W.K / 128;
         const int c1 = (int)((long long)whole * way / ways), end = (int)((long long)whole * (way + 1) / ways);
-        u32x4 w[D][NW][NT];
-        unsigned s[D][NW][NT];
-        Row32<T> a[D][MT];
+        u32x4 w[D][NW];
+        unsigned s[D][NW];
+        Row32<T> a[D];
         auto fetch_weights = [&](int c, int d) {
 #pragma unroll
-            for (int q = 0; q < NW; q++)
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    w[d][q][n] = __builtin_nontemporal_load(wc[q][n] + (long long)c * 64);
-                    s[d][q][n] = ws[q][n][c / 4 * 256 + c % 4];
-                }
+            for (int q = 0; q < NW; q++) {
+                w[d][q] = __builtin_nontemporal_load(wc[q] + (long long)c * 64);
+                s[d][q] = ws[q][c / 4 * 256 + c % 4];
+            }
         };
         auto fetch = [&](int c, int d) {   // chunk c to the registers of place d
             fetch_weights(c, d);
-#pragma unroll
-            for (int m = 0; m < MT; m++) a[d][m].load(row[m] + c * 128);
+            a[d].load(row + c * 128);
         };
         auto multiply = [&](int d) {
-            Frag f[MT][4][X::P];
+            Frag f[4][X::P];
+            a[d].fragments(f);
 #pragma unroll
-            for (int m = 0; m < MT; m++) a[d][m].fragments(f[m]);
+            for (int q = 0; q < NW; q++) {
+                const float sc = X::scale(s[d][q], top[q]);
 #pragma unroll
-            for (int q = 0; q < NW; q++)
+                for (int i = 0; i < 4; i++) {
+                    const Frag b = X::weights(w[d][q][i], sc);
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    const float sc = X::scale(s[d][q][n], top[q][n]);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const Frag b = X::weights(w[d][q][n][i], sc);
-#pragma unroll
-                        for (int m = 0; m < MT; m++)
-#pragma unroll
-                            for (int p = 0; p < X::P; p++) acc[q][n][m] = X::mfma(b, f[m][i][p], acc[q][n][m]);
-                    }
+                    for (int p = 0; p < X::P; p++) acc[q] = X::mfma(b, f[i][p], acc[q]);
                 }
+            }
         };
         if (c1 < end) {
             // No load is conditional (past the end the last chunk is loaded again): a wait then leaves all younger loads on their way.
@@ -290,41 +266,28 @@ __global__ void __launch_bounds__(256) mx4_gemm_rows_kernel(Rows R, Mx4View W, M
         }
         if (W.K % 128 && way == ways - 1) {   // the chunk in which the rows end
             fetch_weights(whole, 0);
-#pragma unroll
-            for (int m = 0; m < MT; m++) a[0][m].load_tail(row[m] - g * 32, whole * 128 + g * 32, W.K);
+            a[0].load_tail(row - g * 32, whole * 128 + g * 32, W.K);
             multiply(0);
         }
     }
     // the sums of the waves along k, in their order
-    if (WK > 1) {
-        __shared__ f32x4 sums[(WK - 1) * WN * NA * 64];
-        if (wv >= WN) {
+    __shared__ f32x4 sums[(WAVES - 1) * NW * 64];
+    if (wv) {
 #pragma unroll
-            for (int i = 0; i < NA; i++) sums[((wv - WN) * NA + i) * 64 + lane] = acc[i / (NT * MT)][i / MT % NT][i % MT];
-        }
-        __syncthreads();
-        if (wv < WN) {
-#pragma unroll
-            for (int k = 1; k < WK; k++)
-#pragma unroll
-                for (int i = 0; i < NA; i++) acc[i / (NT * MT)][i / MT % NT][i % MT] += sums[(((k - 1) * WN + wv) * NA + i) * 64 + lane];
-        }
+        for (int q = 0; q < NW; q++) sums[((wv - 1) * NW + q) * 64 + lane] = acc[q];
     }
-    if (wv >= WN) return;
+    __syncthreads();
+    if (wv) return;
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        int tn[NW][4];
+    for (int k = 1; k < WAVES; k++)
 #pragma unroll
-        for (int q = 0; q < NW; q++)
+        for (int q = 0; q < NW; q++) acc[q] += sums[((k - 1) * NW + q) * 64 + lane];
+    int tn[NW][4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) tn[q][j] = __shfl(top[q][n], 4 * g + j);
-        const int col = (col0 + n) * 16 + 4 * g;
+    for (int q = 0; q < NW; q++)
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-            const int i = m * 16 + r;
-            if (i < count) finish4<T, O, GROUPED, GATED>(R, W, split, part, first, slots, i, col, acc[0][n][m], acc[NW - 1][n][m], tn[0], tn[NW - 1]);
-        }
-    }
+        for (int j = 0; j < 4; j++) tn[q][j] = __shfl(top[q], 4 * g + j);
+    if (r < count) finish4<T, O, GROUPED, GATED>(R, W, split, part, first, slots, r, nt * 16 + 4 * g, acc[0], acc[NW - 1], tn[0], tn[NW - 1]);
 }
 
 // A barrier for what waves pass each other in LDS: their loads from memory stay on their way (__syncthreads waits for them).
