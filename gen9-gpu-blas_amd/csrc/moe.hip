@@ -303,9 +303,8 @@ template <class T, class O, bool GATED> static int launch_grouped(const Rows &R,
         Planes A;
         G9_TRY(stage_planes<T>(R, Tn, W.K, W.kc, &A));
         const int ntiles = (int)cdiv(W.rt, GATED ? 8 : 16);
-        const Split whole = {1, nullptr, 0, 0};
         hipLaunchKernelGGL((mx4_gemm_tile_kernel<T, O, true, GATED>), dim3((unsigned)(cdiv((long long)most * ntiles, 8) * 8)), dim3(256), 0, stream, A, R, W, G, E, 0,
-                           ntiles, whole);
+                           ntiles);
         G9_HIP(hipGetLastError());
         return 0;
     }
@@ -314,11 +313,20 @@ template <class T, class O, bool GATED> static int launch_grouped(const Rows &R,
     auto few = [&](auto kernel, int cols) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)(cdiv(most * cdiv(W.rt, cols), 8) * 8)), dim3(512), 0, stream, R, W, G, E, most, (int)cdiv(W.rt, cols), whole);
     };
-    if (rows == 32)
-        // gated, FP16 44 × 4 places of 16 experts, 832 × 1664, and FP32 21 × 8, 768 × 4096: 16.6 and 49.5 µs; two column tiles a
-        // wave 24.3 and 75.3, the rows kernel 17.1 and 55.4
-        few(mx4_gemm_few_kernel<T, O, 2, 1, 8, 4, true, GATED>, 8);
-    else if (std::min<long long>(n, E) * cdiv(W.rt, 16) >= 2LL * num_cus)
+    const bool many = std::min<long long>(n, E) * cdiv(W.rt, 16) >= 2LL * num_cus;   // workgroups of 256 columns
+    if constexpr (sizeof(T) == 2) {
+        if (rows == 32) {
+            // FP16 128 × 4 places of 64 experts, 4096 × 1536, not gated: 51.0 µs; one column tile a wave 56.4. Gated, 1536 × 4096, 87.7
+            // and 77.1; 64 × 4 places of 16 experts 44.3 and 29.5
+            if constexpr (!GATED) {
+                if (many) few(mx4_gemm_few_kernel<T, O, 2, 2, 8, 4, true, GATED>, 16);
+            }
+            if (GATED || !many) few(mx4_gemm_few_kernel<T, O, 2, 1, 8, 4, true, GATED>, 8);
+            G9_HIP(hipGetLastError());
+            return 0;
+        }
+    }
+    if (many)
         // FP32 joined, 24 × 4 places of 64 experts, 4096 × 1536: 35.6 µs; one column tile a wave 41.3, the rows kernel 63
         few(mx4_gemm_few_kernel<T, O, 1, 2, 8, 4, true, GATED>, 16);
     else if (std::min<long long>(n, E) * cdiv(W.rt, 8) < num_cus)
@@ -335,7 +343,14 @@ template <class T>
 static int experts(int Tn, int S, const int *ids, const void *X, int64_t ldt, int64_t lds, const gen9blas_mx4 *W, const gen9blas_mx4 *gate,
                    const float *weights, void *C, int64_t ldct, int64_t ldcs) {
     const long long n = (long long)Tn * S;
-    const int E = W->count, N = W->rows, rows = n > 64 && n > 16LL * E ? 64 : n > 8LL * E ? 32 : 16;
+    const int E = W->count, N = W->rows;
+    // The rows of a tile, by places an expert: 64 go to the tile kernel, fewer to the kernels that read the weights once. µs with 16, 32
+    // and 64, of 64 experts: FP16 gated 1536 × 4096, 6 places each 74.7, 75.9 and more, 8 81.9, 77.1 and 102, 32 149, 117 and 126, 48 200, 153
+    // and 147; not gated 4096 × 1536, 6 48.7, 48.9, 8 53.9, 51.0 and 64, 32 106, 82 and 83, 48 148, 109 and 97. FP32, whose three pieces
+    // of 32 rows LDS passes no faster than 16 twice: gated 32 208, 216 and 268, 64 364, 308 and 338; not gated 48 173, 185 and 181, 64 219,
+    // 215 and 206.
+    constexpr bool F = sizeof(T) == 4;
+    const int rows = n > 64 && n > (F ? 56LL : 40LL) * E ? 64 : !F && n >= 7LL * E ? 32 : 16;
     // Few places: each workgroup finds its rows among the ids itself (8 places 17.5 µs a call with a plan, whose kernel comes first)
     const bool direct = n <= 64;
     const long long most = direct ? n : cdiv(n, rows) + E + 1;

@@ -5,62 +5,41 @@
 
 namespace g9llm {
 
-// Both operands MX4, any shape: a workgroup makes 64 rows × 16 columns, its 4 waves every fourth group of 512 k.
+// Both operands MX4, few rows: a workgroup makes a tile of 16 rows × 16 columns, its 4 waves every fourth group of 512 k.
 template <class O>
-__global__ void __launch_bounds__(256) mx4_gemm_q_any_kernel(Mx4View A, Mx4View W, O *__restrict__ C, long long ldc, int mtiles, int) {
-    constexpr int MT = 4;
+__global__ void __launch_bounds__(256) mx4_gemm_q_few_kernel(Mx4View A, Mx4View W, O *__restrict__ C, long long ldc, int mtiles, int) {
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
     if ((int)blockIdx.x >= mtiles * W.rt) return;
-    const int nt = blockIdx.x % W.rt, mt = blockIdx.x / W.rt * MT;
-    f32x4 acc[MT];
-#pragma unroll
-    for (int m = 0; m < MT; m++) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int nt = blockIdx.x % W.rt, mt = blockIdx.x / W.rt;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    const u32x4 *ac = reinterpret_cast<const u32x4 *>(A.codes) + (long long)mt * A.kc * 64 + lane;
     const u32x4 *wc = reinterpret_cast<const u32x4 *>(W.codes) + (long long)nt * W.kc * 64 + lane;
+    const int *as = reinterpret_cast<const int *>(A.scales) + (long long)mt * A.kg * 64 + lane;
     const int *ws = reinterpret_cast<const int *>(W.scales) + (long long)nt * W.kg * 64 + lane;
     for (int grp = wv; grp < W.kg; grp += 4) {
-        const int sw = ws[grp * 64];
-        int sa[MT];
-#pragma unroll
-        for (int m = 0; m < MT; m++)
-            sa[m] = reinterpret_cast<const int *>(A.scales)[((long long)min(mt + m, A.rt - 1) * A.kg + grp) * 64 + lane];
+        const int sa = as[grp * 64], sw = ws[grp * 64];
         auto step = [&](auto J) {
             constexpr int j = decltype(J)::value;
             const int c = grp * 4 + j;
             if (c >= W.kc) return;
-            const u32x4 w = wc[(long long)c * 64];
-            const i32x8 wf = {(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
-#pragma unroll
-            for (int m = 0; m < MT; m++) {
-                const u32x4 a = reinterpret_cast<const u32x4 *>(A.codes)[((long long)min(mt + m, A.rt - 1) * A.kc + c) * 64 + lane];
-                const i32x8 af = {(int)a[0], (int)a[1], (int)a[2], (int)a[3]};
-                acc[m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, af, acc[m], 4, 4, j, sw, j, sa[m]);
-            }
+            acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(wc[(long long)c * 64]), fp4_operand(ac[(long long)c * 64]), acc, 4, 4, j, sw, j, sa);
         };
         step(std::integral_constant<int, 0>());
         step(std::integral_constant<int, 1>());
         step(std::integral_constant<int, 2>());
         step(std::integral_constant<int, 3>());
     }
-    __shared__ f32x4 part[3][MT][64];
-    if (wv) {
-#pragma unroll
-        for (int m = 0; m < MT; m++) part[wv - 1][m][lane] = acc[m];
-    }
+    __shared__ f32x4 part[3][64];
+    if (wv) part[wv - 1][lane] = acc;
     __syncthreads();
     if (wv) return;
 #pragma unroll
-    for (int m = 0; m < MT; m++) {
-        f32x4 v = acc[m];
+    for (int w = 0; w < 3; w++) acc += part[w][lane];
+    const int row = mt * 16 + r, n = nt * 16 + 4 * g;
+    if (row >= A.rows) return;
 #pragma unroll
-        for (int w = 0; w < 3; w++) v += part[w][m][lane];
-        const int row = (mt + m) * 16 + r;
-        if (row >= A.rows) continue;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int n = nt * 16 + 4 * g + j;
-            if (n < W.rows) C[row * ldc + n] = (O)v[j];
-        }
-    }
+    for (int j = 0; j < 4; j++)
+        if (n + j < W.rows) C[row * ldc + n + j] = (O)acc[j];
 }
 
 template <class O> static int launch_q(const Mx4View &A, const Mx4View &W, O *C, long long ldc) {
@@ -71,8 +50,13 @@ template <class O> static int launch_q(const Mx4View &A, const Mx4View &W, O *C,
         G9_HIP(hipGetLastError());
         return 0;
     };
-    if (A.rt > 4) return cdiv(A.rt, 16) * cdiv(W.rt, 16) >= num_cus ? run(mx4_gemm_q_tile_kernel<O>, 16, 16) : run(mx4_gemm_q_ring_kernel<O>, 8, 8);
-    return run(mx4_gemm_q_any_kernel<O>, 4, 1);
+    // µs with the quantisation of A's rows: few kernel 100 × 4096 × 4096 11.3 and 100 × 4096 × 11008 17.5, ring kernel 12.8 and 21.8;
+    // 64 × 11008 × 4096 and 200 × 4096 × 4096 15.1 and 15.8, ring kernel 13.0 and 13.2
+    if ((long long)A.rt * W.rt <= 8 * num_cus) return run(mx4_gemm_q_few_kernel<O>, 1, 1);
+    // ring kernel 2000 × 6000 × 4096 (192 tiles of 256 × 256) 37.8, tile kernel 40.4; 2300 × 6100 × 4096 (216) 45.2 and 43.4,
+    // 3000 × 5000 × 4096 (240) 50.3 and 42.7
+    if (cdiv(A.rt, 16) * cdiv(W.rt, 16) * 5 < 4 * num_cus) return run(mx4_gemm_q_ring_kernel<O>, 8, 8);
+    return run(mx4_gemm_q_tile_kernel<O>, 16, 16);
 }
 
 static int split_space(const Rows &R, const Mx4View &W, Split *s) {
@@ -116,38 +100,38 @@ template <class T, int MT, int NT, int NV, int D> static int launch_few(const Ro
     return sum_parts<T>(R, W, split);
 }
 
-// Tiles of 64 rows × 256 columns; k is split until there is about a workgroup a CU.
+// Tiles of 64 rows × 256 columns.
 template <class T> static int launch_tiles(const Rows &R, const Mx4View &W) {
     Planes A;
     G9_TRY(stage_planes<T>(R, R.M, W.K, W.kc, &A));
-    const int mtiles = (int)cdiv(R.M, 64), ntiles = (int)cdiv(W.rt, 16);
-    const long long tiles = (long long)mtiles * ntiles;
-    Split split = {1, nullptr, 0, 0};
-    const int ways = (int)(num_cus / tiles), most = W.kc / 4;
-    if (ways > 1 && most > 1) {
-        split.parts = ways < most ? ways : most;
-        G9_TRY(split_space(R, W, &split));
-    }
-    if (tiles * split.parts > 0xffffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm: more tiles than one launch can index");
-    hipLaunchKernelGGL((mx4_gemm_tile_kernel<T, T, false, false>), dim3((unsigned)(cdiv(tiles * split.parts, 8) * 8)), dim3(256), 0, stream, A, R, W, W, 1, mtiles,
-                       ntiles, split);
+    const long long mtiles = cdiv(R.M, 64), ntiles = cdiv(W.rt, 16);
+    if (mtiles * ntiles > 0xfffff0) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm: more tiles than one launch can index");
+    hipLaunchKernelGGL((mx4_gemm_tile_kernel<T, T, false, false>), dim3((unsigned)(cdiv(mtiles * ntiles, 8) * 8)), dim3(256), 0, stream, A, R, W, W, 1, (int)mtiles,
+                       (int)ntiles);
     G9_HIP(hipGetLastError());
-    return sum_parts<T>(R, W, split);
+    return 0;
 }
 
 template <class T> static int launch_dense(const Rows &R, const Mx4View &W) {
-    if (R.M > 64) return launch_tiles<T>(R, W);
+    constexpr bool F = sizeof(T) == 4;
     // µs of the product alone, FP16 1 × 11008 × 4096 and FP32 8 × 4096 × 11008: rows kernel 9.4 and 13.2, few kernel 8.8 to
     // 9.5 and 10.7: FP32 rows are taken apart once a workgroup there, and once a wave in the rows kernel.
     if (R.M <= 16) {
-        if constexpr (sizeof(T) == 4) return launch_few<T, 1, 2, 8, 4>(R, W);
+        if constexpr (F) return launch_few<T, 1, 2, 8, 4>(R, W);
         else return launch_rows<T>(R, W);
     }
     // 128 columns a workgroup; with 256, which reads the rows from LDS half as often but leaves twice the parts to be summed or half
     // the workgroups: FP32 24 × 4096 × 11008 19.6 µs and 20.0, 24 × 11008 × 4096 21.6 and 20.5, 28 × 2048 × 2048 9.5 and 11.9
     if (R.M <= 32) return launch_few<T, 2, 1, 8, 4>(R, W);
-    // FP32 64 × 4096 × 4096 18.6 µs, 56 × 8192 × 8192 40.0, 33 × 1000 × 4992 14.3; 256 columns 21.9, 36.3, 18.1
-    return launch_few<T, 4, 1, 8, 2>(R, W);
+    // 64 rows: 128 columns, 256 columns, or the tile kernel, which has 64 × 256 too but fills the GPU with 768 workgroups, not 256.
+    // FP16 512 × 4096 × 4096 (256 workgroups of 128 columns) 24.8, 29.1 and 33.1 µs, 1000 × 4096 × 4096 (512) 42.7, 37.1 and 40.5,
+    // 400 × 11008 × 4096 (301 of 256 columns) 55.2, 65.0 and 54.8. FP32, where LDS gives three pieces of the rows: 100 × 4096 × 4096 (64 of 128
+    // columns) 23.6, 25.6 and 26.6, 192 × 4096 × 4096 (96) 36.3, 30.8 and 36.0, 1000 × 4096 × 4096 (256 of 256 columns) 121, 87 and 98,
+    // 400 × 11008 × 4096 156, 148 and 124.
+    const long long mtiles = cdiv(R.M, 64);
+    if (mtiles * cdiv(W.rt, 8) <= num_cus / (F ? 3 : 1)) return launch_few<T, 4, 1, 8, 2>(R, W);
+    if (mtiles * cdiv(W.rt, 16) <= num_cus) return launch_few<T, 4, 2, 8, 2>(R, W);
+    return launch_tiles<T>(R, W);
 }
 
 }  // namespace g9llm

@@ -220,6 +220,24 @@ def test_experts(g9, torch_dev, dtype, T, S, E, N, K):
 
 
 @pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("T,S,E,N,K", [(30, 2, 4, 100, 300), (150, 4, 64, 2070, 160), (16, 4, 9, 300, 260)])
+def test_experts_of_seven_places_and_more(g9, torch_dev, dtype, T, S, E, N, K):
+    """Tiles of 32 rows (FP16), without a plan and with one; enough experts and columns for 256 columns a workgroup."""
+    r = np.random.default_rng(T + N)
+    ids = np.argsort(r.random((T, E)), 1)[:, :S].astype(np.int32)
+    ids[r.random(ids.shape) < 0.1] = -1
+    W, w = weights(r, torch_dev, g9, E, N, K)
+    G, g = weights(r, torch_dev, g9, E, N, K)
+    share = r.random((T, S)).astype(np.float32)
+    x = r.standard_normal((T, S, K)).astype(dtype)
+    for gate in (False, True):
+        for join in (False, True):
+            got = g9.moe_gemm(gpu(torch_dev, x), gpu(torch_dev, ids), W, gate=G if gate else None, weights=gpu(torch_dev, share) if join else None)
+            ref, tol = experts64(x, ids, w, g if gate else None, share if join else None)
+            check_experts(torch_dev, got, ref, tol)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
 def test_experts_unbalanced(g9, torch_dev, dtype):
     """All tokens at one expert, none at the others; every place empty; an expert twice in a token's places."""
     r = np.random.default_rng(9)

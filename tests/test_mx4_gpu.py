@@ -176,6 +176,43 @@ def test_gemm_large(g9, torch_dev, M, N, K):
         check_large(torch, g9.mx4_gemm(a, W), a.double(), w, t)
 
 
+@pytest.mark.parametrize("K", [96, 200, 384, 512, 640, 1100, 1536])
+def test_gemm_quantized_middle(g9, torch_dev, K):
+    """More tiles of 16 × 16 than eight a CU, too few of 256 × 256."""
+    torch = torch_dev
+    g = torch.Generator(device="cuda").manual_seed(K)
+    qa = g9.mx4_quantize(torch.randn((700, K), generator=g, device="cuda"))
+    qw = g9.mx4_quantize(torch.randn((1301, K), generator=g, device="cuda") / 8)
+    a, w = g9.mx4_dequantize(qa).double(), g9.mx4_dequantize(qw).double()
+    for out, t in ((np.float16, torch.float16), (np.float32, torch.float32)):
+        check_large(torch, g9.mx4_gemm(qa, qw, dtype=out), a, w, t)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+@pytest.mark.parametrize("M,N,K", [(300, 5000, 200), (700, 4099, 129), (1100, 4099, 645)])
+def test_gemm_large_strides_and_nan(g9, torch_dev, dtype, M, N, K):
+    """Tiles of 64 rows by 128 and 256 columns: A at any alignment, nothing written beside C, an infinity or NaN stays in its row."""
+    torch = torch_dev
+    t = getattr(torch, dtype)
+    g = torch.Generator(device="cuda").manual_seed(M)
+    W = g9.mx4_quantize(torch.randn((N, K), generator=g, device="cuda") / 8)
+    w = g9.mx4_dequantize(W).double()
+    big = torch.randn((M, K + 5), generator=g, device="cuda").to(t)
+    for off in (0, 1, 2):
+        a = big[:, off:off + K]
+        out = torch.full((M + 2, N + 7), 3.0, dtype=t, device="cuda")
+        g9.mx4_gemm(a, W, C=out[1:M + 1, 2:N + 2])
+        check_large(torch, out[1:M + 1, 2:N + 2], a.double(), w, t)
+        out[1:M + 1, 2:N + 2] = 3.0
+        assert bool((out == 3.0).all())
+    a = big[:, :K].clone()
+    a[5, 7], a[M - 2, K - 1] = float("nan"), float("inf")
+    rest = [i for i in range(M) if i not in (5, M - 2)]
+    got = g9.mx4_gemm(a, W)
+    check_large(torch, got[rest], a[rest].double(), w, t)
+    assert bool(got[5].isnan().all()) and not bool(got[M - 2].isfinite().any())
+
+
 @pytest.mark.parametrize("dtype", [np.float16, np.float32])
 @pytest.mark.parametrize("M", [1, 7, 33, 90, 260])
 def test_gemm_strides(g9, torch_dev, dtype, M):
