@@ -208,8 +208,10 @@ __global__ void __launch_bounds__(256) moe_route_kernel(RouteArgs a) {
 
 // The plan of a grouped product: slots by expert (order; places whose id is no expert come last, as expert E), off[e] where
 // expert e's begin, and the tiles of `rows` slots: (expert, first place), (−1, 0) past the last, their number in front. One
-// workgroup: the ids are counted in LDS, which gives each its rank among its expert's (kept in memory), a scan gives each expert's
-// place, and the ids are read again to be placed. The order of a group's slots varies from call to call; no result depends on it.
+// workgroup: the ids are counted in LDS, a scan gives each expert's place, and the ids (the first 8192 from registers) are placed.
+// Latencies bound it, so a thread has eight loads or LDS atomics on their way, none of them conditional (a rank that the count
+// gives, kept in memory for the placing, took longer than counting twice: 8192 ids 14.6 µs and 8.1). The order of a group's slots
+// varies from call to call; no result depends on it.
 __device__ __forceinline__ int2 scan_pair(int2 v, int lane) {   // sums over the lanes up to this one
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -218,38 +220,49 @@ __device__ __forceinline__ int2 scan_pair(int2 v, int lane) {   // sums over the
     }
     return v;
 }
-__global__ void __launch_bounds__(1024) moe_plan_kernel(const int *__restrict__ ids, int n, int E, int rows, int *rank, int *order, int *off, int *tiles, int most) {
-    __shared__ int count[MAX_EXPERTS + 1], base[MAX_EXPERTS + 1];
+__global__ void __launch_bounds__(1024) moe_plan_kernel(const int *__restrict__ ids, int n, int E, int rows, int *order, int *off, int *tiles, int most) {
+    __shared__ int count[MAX_EXPERTS + 65], base[MAX_EXPERTS + 65];   // the last 64: lanes without an id
     __shared__ int2 waves[16];
     const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+    auto load = [&](long long i0, int *e) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) e[j] = ids[min(i0 + j * 1024, (long long)n - 1)];
+#pragma unroll
+        for (int j = 0; j < 8; j++) e[j] = i0 + j * 1024 < n ? (int)min((unsigned)e[j], (unsigned)E) : E + 1 + lane;
+    };
+    int mine8[8];
+    load(t, mine8);
     for (int i = t; i <= E; i += 1024) count[i] = 0;
     __syncthreads();
-    // eight ids of a thread are on their way at a time
     auto each = [&](auto use) {
-        for (long long i0 = t; i0 < n; i0 += 8 * 1024) {
-            int id[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) id[j] = i0 + j * 1024 < n ? ids[i0 + j * 1024] : 0;
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (i0 + j * 1024 < n) use((unsigned)id[j] < (unsigned)E ? id[j] : E, (int)(i0 + j * 1024));
+        use((long long)t, mine8);
+        for (long long i0 = 8 * 1024 + t; i0 - t < n; i0 += 8 * 1024) {
+            int e[8];
+            load(i0, e);
+            use(i0, e);
         }
     };
-    each([&](int e, int i) { rank[i] = atomicAdd(&count[e], 1); });
+    each([&](long long, const int *e) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) atomicAdd(&count[e[j]], 1);
+    });
     __syncthreads();
     const int mine = t < E ? count[t] : 0, own = (mine + rows - 1) / rows;
     const int2 s = scan_pair({mine, own}, lane);
     if (lane == 63) waves[wv] = s;
     __syncthreads();
-    int2 before = {s.x - mine, s.y - own};
-    for (int w = 0; w < wv; w++) before.x += waves[w].x, before.y += waves[w].y;
+    int2 before = {s.x - mine, s.y - own}, all = {0, 0};
+#pragma unroll
+    for (int w = 0; w < 16; w++) {
+        const int2 v = waves[w];
+        if (w < wv) before.x += v.x, before.y += v.y;
+        all.x += v.x, all.y += v.y;
+    }
     auto put = [&](int e, int first, int tile, int c) {
         base[e] = first, off[e] = first;
         for (int i = 0; i * rows < c; i++) tiles[2 * (tile + i)] = e, tiles[2 * (tile + i) + 1] = first + i * rows;
     };
     if (t < E) put(t, before.x, before.y, mine);
-    int2 all = {0, 0};
-    for (int w = 0; w < 16; w++) all.x += waves[w].x, all.y += waves[w].y;
     const int last = all.y + (count[E] + rows - 1) / rows;
     if (t == 0) {
         put(E, all.x, all.y, count[E]);
@@ -257,7 +270,14 @@ __global__ void __launch_bounds__(1024) moe_plan_kernel(const int *__restrict__ 
     }
     for (int i = last + t; i < most; i += 1024) tiles[2 * i] = -1, tiles[2 * i + 1] = 0;
     __syncthreads();
-    each([&](int e, int i) { order[base[e] + rank[i]] = i; });
+    each([&](long long i0, const int *e) {
+        int at[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) at[j] = atomicAdd(&base[e[j]], 1);
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (e[j] <= E) order[at[j]] = (int)i0 + j * 1024;
+    });
 }
 
 // C(t) = Σ_s weights(t, s) · y(t, s), in the order of s; places that are no expert's are left out. A thread for four columns
@@ -361,9 +381,9 @@ static int experts(int Tn, int S, const int *ids, const void *X, int64_t ldt, in
     if (weights) G9_TRY(scratch(SLOT_SLOTS, (size_t)n * ld * 4, &slots));
     Rows R = {X, C, ldt, lds, ldct, ldcs, (int)n, S, nullptr, nullptr, nullptr, direct ? ids : nullptr};
     if (!direct) {
-        G9_TRY(scratch(SLOT_PLAN, (size_t)(2 * n + E + 3 + 2 * most) * 4, &plan));
-        int *rank = (int *)plan, *order = rank + n, *off = order + n, *tiles = off + E + 3;
-        hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(1024), 0, stream, ids, (int)n, E, rows, rank, order, off, tiles, (int)most);
+        G9_TRY(scratch(SLOT_PLAN, (size_t)(n + E + 3 + 2 * most) * 4, &plan));
+        int *order = (int *)plan, *off = order + n, *tiles = off + E + 3;
+        hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(1024), 0, stream, ids, (int)n, E, rows, order, off, tiles, (int)most);
         G9_HIP(hipGetLastError());
         R.tiles = tiles, R.order = order, R.off = off;
     }
