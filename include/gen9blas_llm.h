@@ -6,7 +6,7 @@
 //
 // Rules shared by every entry point
 // - Operands are device memory, used in place at any element alignment. One in host memory, or one that runs past the
-//   end of its allocation, is INVALID_ARG before anything runs.
+//   end of its allocation, is INVALID_ARG before anything runs. A result overlaps no operand.
 // - A call queues its kernels on the library's stream and returns; gen9blas_flush() waits for them. The stream orders
 //   itself after work on the legacy null stream and before work queued there later.
 // - Return value: 0, or a negative gen9blas_status with the text in gen9blas_llm_error(). Functions returning pointers

@@ -3,7 +3,8 @@
 // The reference's lib/gen9blas_ml.h declares its ggml operator set (norms, RoPE, attention, packed activations,
 // fused FFN, copies). Of it, this build provides the small-batch product on packed FP16 weights with FP32
 // activations, and the queued-work pair gen9blas_set_nowait / gen9blas_flush (declared with the MI355X additions in
-// gen9blas_hip.h, included here). The other operators are not part of this library.
+// gen9blas_hip.h, included here). The reference's other operators are not part of this library. 4-bit weights and
+// mixtures of experts, which it does not have, are in gen9blas_llm.h.
 #pragma once
 #include "gen9blas.h"
 #include "gen9blas_hip.h"
