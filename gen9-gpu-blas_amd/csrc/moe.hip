@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(1024) moe_plan_kernel(const int *__restrict__ 
 }
 
 // C(t) = Σ_s weights(t, s) · y(t, s), in the order of s; places that are no expert's are left out. A thread for four columns
-// of a token; y has rows of ld, whole 16-byte pieces.
+// of a token; y has rows of ld, whole 16-byte pieces. 2047 × 4 places, 4096 columns, FP16: 22 µs, 6.8 TB/s from HBM and the last cache.
 template <class T>
 __global__ void __launch_bounds__(256) moe_join_kernel(const float *__restrict__ y, long long ld, const int *__restrict__ ids, const float *__restrict__ weights,
                                                        int S, int E, int N, T *__restrict__ C, long long ldct) {
@@ -339,22 +339,22 @@ template <class T, class O, bool GATED> static int launch_grouped(const Rows &R,
             // FP16 128 × 4 places of 64 experts, 4096 × 1536, not gated: 51.0 µs; one column tile a wave 56.4. Gated, 1536 × 4096, 87.7
             // and 77.1; 64 × 4 places of 16 experts 44.3 and 29.5
             if constexpr (!GATED) {
-                if (many) few(mx4_gemm_few_kernel<T, O, 2, 2, 8, 4, true, GATED>, 16);
+                if (many) few(mx4_gemm_few_kernel<T, O, 2, 2, 4, true, GATED>, 16);
             }
-            if (GATED || !many) few(mx4_gemm_few_kernel<T, O, 2, 1, 8, 4, true, GATED>, 8);
+            if (GATED || !many) few(mx4_gemm_few_kernel<T, O, 2, 1, 4, true, GATED>, 8);
             G9_HIP(hipGetLastError());
             return 0;
         }
     }
     if (many)
         // FP32 joined, 24 × 4 places of 64 experts, 4096 × 1536: 35.6 µs; one column tile a wave 41.3, the rows kernel 63
-        few(mx4_gemm_few_kernel<T, O, 1, 2, 8, 4, true, GATED>, 16);
+        few(mx4_gemm_few_kernel<T, O, 1, 2, 4, true, GATED>, 16);
     else if (std::min<long long>(n, E) * cdiv(W.rt, 8) < num_cus)
         // FP16 gated, 8 places, 1536 × 4096: 13.6 µs; few kernel 20.6 and more. FP32 gated, 7 places, 864 × 3840: 14.2 µs, the few
         // kernel, whose 49 workgroups leave most CUs idle, 24
         hipLaunchKernelGGL((mx4_gemm_rows_kernel<T, O, 2, true, GATED>), dim3((unsigned)((long long)most * W.rt)), dim3(256), 0, stream, R, W, G, E, whole);
     else
-        few(mx4_gemm_few_kernel<T, O, 1, 1, 8, 4, true, GATED>, 8);
+        few(mx4_gemm_few_kernel<T, O, 1, 1, 4, true, GATED>, 8);
     G9_HIP(hipGetLastError());
     return 0;
 }

@@ -62,7 +62,8 @@ __device__ __forceinline__ void write_scales(unsigned char (*sc)[64], unsigned c
     }
 }
 
-// A workgroup makes one row tile's group of 512 k, wave j its tile j: lane 16g + r the block of row r, k = 32g.
+// A workgroup makes one row tile's group of 512 k, wave j its tile j: lane 16g + r the block of row r, k = 32g. HBM bounds it:
+// 11008 × 4096 FP32 43 µs, 4.7 TB/s.
 template <class T>
 __global__ void __launch_bounds__(256) mx4_quantize_kernel(const T *__restrict__ X, long long ldx, long long sX, Mx4View q,
                                                            uint8_t *codes, uint8_t *scales, uint8_t *top) {
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(256) mx4_load_kernel(const uint8_t *__restrict
 }
 
 // A wave's tile of 16 rows × 128 k: the codes through LDS, so that 32 lanes write 512 consecutive bytes of a row, four values
-// each (a lane that wrote its block's 128 bytes: 11008 × 4096 54 µs).
+// each (11008 × 4096 30 µs, 6.8 TB/s into HBM and the last cache; a lane that wrote its block's 128 bytes 54).
 __global__ void __launch_bounds__(256) mx4_dequantize_kernel(Mx4View q, float *__restrict__ X, long long ldx, long long sX) {
     __shared__ u32x4 codes[4][64];
     __shared__ unsigned char sc[4][64];

@@ -6,6 +6,8 @@
 namespace g9llm {
 
 // Both operands MX4, few rows: a workgroup makes a tile of 16 rows × 16 columns, its 4 waves every fourth group of 512 k.
+// The operands go to the matrix cores as they lie, both read by every tile (W once from memory, then from L2): few rows leave the time to
+// latency, and the many small workgroups hide it.
 template <class O>
 __global__ void __launch_bounds__(256) mx4_gemm_q_few_kernel(Mx4View A, Mx4View W, O *__restrict__ C, long long ldc, int mtiles, int) {
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
@@ -84,9 +86,9 @@ template <class T> static int launch_rows(const Rows &R, const Mx4View &W) {
     return sum_parts<T>(R, W, split);
 }
 
-// Tiles of MT·16 rows × 16·NT·NV columns; k is split until there is about a workgroup a CU.
-template <class T, int MT, int NT, int NV, int D> static int launch_few(const Rows &R, const Mx4View &W) {
-    const int ntiles = (int)cdiv(W.rt, NT * NV), mtiles = (int)cdiv(R.M, MT * 16);
+// Tiles of MT·16 rows × 128·NT columns; k is split until there is about a workgroup a CU.
+template <class T, int MT, int NT, int D> static int launch_few(const Rows &R, const Mx4View &W) {
+    const int ntiles = (int)cdiv(W.rt, NT * 8), mtiles = (int)cdiv(R.M, MT * 16);
     const long long tiles = (long long)mtiles * ntiles;
     Split split = {1, nullptr, 0, 0};
     const int ways = (int)(num_cus / tiles), most = W.kc / 4;
@@ -95,7 +97,7 @@ template <class T, int MT, int NT, int NV, int D> static int launch_few(const Ro
         G9_TRY(split_space(R, W, &split));
     }
     if (tiles * split.parts > 0x7fffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "mx4_gemm: more tiles than one launch can index");
-    hipLaunchKernelGGL((mx4_gemm_few_kernel<T, T, MT, NT, NV, D, false, false>), dim3((unsigned)(cdiv(tiles * split.parts, 8) * 8)), dim3(NV * 64), 0, stream, R, W, W, 1, mtiles, ntiles, split);
+    hipLaunchKernelGGL((mx4_gemm_few_kernel<T, T, MT, NT, D, false, false>), dim3((unsigned)(cdiv(tiles * split.parts, 8) * 8)), dim3(512), 0, stream, R, W, W, 1, mtiles, ntiles, split);
     G9_HIP(hipGetLastError());
     return sum_parts<T>(R, W, split);
 }
@@ -117,20 +119,20 @@ template <class T> static int launch_dense(const Rows &R, const Mx4View &W) {
     // µs of the product alone, FP16 1 × 11008 × 4096 and FP32 8 × 4096 × 11008: rows kernel 9.4 and 13.2, few kernel 8.8 to
     // 9.5 and 10.7: FP32 rows are taken apart once a workgroup there, and once a wave in the rows kernel.
     if (R.M <= 16) {
-        if constexpr (F) return launch_few<T, 1, 2, 8, 4>(R, W);
+        if constexpr (F) return launch_few<T, 1, 2, 4>(R, W);
         else return launch_rows<T>(R, W);
     }
     // 128 columns a workgroup; with 256, which reads the rows from LDS half as often but leaves twice the parts to be summed or half
     // the workgroups: FP32 24 × 4096 × 11008 19.6 µs and 20.0, 24 × 11008 × 4096 21.6 and 20.5, 28 × 2048 × 2048 9.5 and 11.9
-    if (R.M <= 32) return launch_few<T, 2, 1, 8, 4>(R, W);
+    if (R.M <= 32) return launch_few<T, 2, 1, 4>(R, W);
     // 64 rows: 128 columns, 256 columns, or the tile kernel, which has 64 × 256 too but fills the GPU with 768 workgroups, not 256.
     // FP16 512 × 4096 × 4096 (256 workgroups of 128 columns) 24.8, 29.1 and 33.1 µs, 1000 × 4096 × 4096 (512) 42.7, 37.1 and 40.5,
     // 400 × 11008 × 4096 (301 of 256 columns) 55.2, 65.0 and 54.8. FP32, where LDS gives three pieces of the rows: 100 × 4096 × 4096 (64 of 128
     // columns) 23.6, 25.6 and 26.6, 192 × 4096 × 4096 (96) 36.3, 30.8 and 36.0, 1000 × 4096 × 4096 (256 of 256 columns) 121, 87 and 98,
     // 400 × 11008 × 4096 156, 148 and 124.
     const long long mtiles = cdiv(R.M, 64);
-    if (mtiles * cdiv(W.rt, 8) <= num_cus / (F ? 3 : 1)) return launch_few<T, 4, 1, 8, 2>(R, W);
-    if (mtiles * cdiv(W.rt, 16) <= num_cus) return launch_few<T, 4, 2, 8, 2>(R, W);
+    if (mtiles * cdiv(W.rt, 8) <= num_cus / (F ? 3 : 1)) return launch_few<T, 4, 1, 2>(R, W);
+    if (mtiles * cdiv(W.rt, 16) <= num_cus) return launch_few<T, 4, 2, 2>(R, W);
     return launch_tiles<T>(R, W);
 }
 
