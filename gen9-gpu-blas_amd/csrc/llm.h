@@ -7,9 +7,10 @@
 // wave that walks k streams consecutive KiB. Scales: for each row tile and group of 512 k a word per lane, byte j the
 // scale of tile 4·group + j. Codes past K and past the last row are zero, their scales 0.
 //
-// Row exponents. `top`: for each row and group of 512 k the largest scale byte of a block with a non-zero code. FP16
-// products scale a row's weights by its largest one, e: code · 2^(s−e+13) is exact in FP16 (49152 at most, and down to
-// s = e − 36), and the sums are multiplied by 2^(e−140) at the end.
+// Row exponents. A block of zeros has scale 0 (or 255: a NaN block, whatever its codes). `top`: for each row and group of
+// 512 k the largest scale byte, so no scale of a row but NaN's lies above its largest, e. FP16 products scale a row's weights
+// by it: code · 2^(s−e+13) is exact in FP16 (49152 at most, and down to s = e − 36), and the sums are multiplied by 2^(e−140)
+// at the end.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stddef.h>

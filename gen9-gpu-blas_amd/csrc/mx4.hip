@@ -48,14 +48,13 @@ template <class T> __device__ __forceinline__ unsigned quantize32(const T *v, u3
 }
 
 // Scale bytes of a row tile's 512-k group: sc[j] of wave j's lanes, written as one word per lane with the row's largest.
-__device__ __forceinline__ void write_scales(unsigned char (*sc)[64], unsigned char (*tp)[64], uint8_t *scales, uint8_t *top,
-                                             int kt, int grp) {
+__device__ __forceinline__ void write_scales(unsigned char (*sc)[64], uint8_t *scales, uint8_t *top, int kt, int grp) {
     __syncthreads();
     const int t = threadIdx.x;
     if (t < 64) {
         const unsigned w = sc[0][t] | sc[1][t] << 8 | sc[2][t] << 16 | (unsigned)sc[3][t] << 24;
         reinterpret_cast<unsigned *>(scales)[t] = w;
-        int m = max(max(tp[0][t], tp[1][t]), max(tp[2][t], tp[3][t]));
+        int m = max(max(sc[0][t], sc[1][t]), max(sc[2][t], sc[3][t]));
         m = max(m, __shfl_xor(m, 16));
         m = max(m, __shfl_xor(m, 32));
         if (t < 16) top[t * kt + grp] = (uint8_t)m;
@@ -67,37 +66,36 @@ __device__ __forceinline__ void write_scales(unsigned char (*sc)[64], unsigned c
 template <class T>
 __global__ void __launch_bounds__(256) mx4_quantize_kernel(const T *__restrict__ X, long long ldx, long long sX, Mx4View q,
                                                            uint8_t *codes, uint8_t *scales, uint8_t *top) {
-    __shared__ unsigned char sc[4][64], tp[4][64];
+    __shared__ unsigned char sc[4][64];
     const int lane = threadIdx.x & 63, j = threadIdx.x >> 6;
     const int grp = blockIdx.x % q.kg;
     const long long tile = blockIdx.x / q.kg;   // over all matrices
     const int b = (int)(tile / q.rt), row = (int)(tile % q.rt) * 16 + (lane & 15), c = grp * 4 + j;
-    unsigned s = 0, t = 0;
+    unsigned s = 0;
     if (c < q.kc) {
         const long long k = (long long)c * 128 + (lane >> 4) * 32;
         u32x4 w = {0, 0, 0, 0};
         if (row < q.rows && k < q.K) {
             T v[32];
             load32(X + b * sX + row * ldx, k, q.K, v);
-            s = quantize32(v, w);
-            t = (w[0] | w[1] | w[2] | w[3]) & 0x77777777u || s == 255 ? s : 0;
+            s = quantize32(v, w);   // of a block of zeros: 0, as every other scale leaves the largest at 4 or more
         }
         reinterpret_cast<u32x4 *>(codes)[(tile * q.kc + c) * 64 + lane] = w;
     }
     sc[j][lane] = (unsigned char)s;
-    tp[j][lane] = (unsigned char)t;
-    write_scales(sc, tp, scales + (tile * q.kg + grp) * 256, top + tile * 16 * q.kt, q.kt, grp);
+    write_scales(sc, scales + (tile * q.kg + grp) * 256, top + tile * 16 * q.kt, q.kt, grp);
 }
 
-// The same from a checkpoint's rows of codes and scales. Codes past K are cleared.
+// The same from a checkpoint's rows of codes and scales. Codes past K are cleared; a block of zeros, which may come with any
+// scale, gets scale 0 (NaN blocks, 255, stay).
 __global__ void __launch_bounds__(256) mx4_load_kernel(const uint8_t *__restrict__ in, long long ldc, const uint8_t *__restrict__ sin,
                                                        long long lds, Mx4View q, uint8_t *codes, uint8_t *scales, uint8_t *top) {
-    __shared__ unsigned char sc[4][64], tp[4][64];
+    __shared__ unsigned char sc[4][64];
     const int lane = threadIdx.x & 63, j = threadIdx.x >> 6;
     const int grp = blockIdx.x % q.kg;
     const long long tile = blockIdx.x / q.kg;
     const int b = (int)(tile / q.rt), row = (int)(tile % q.rt) * 16 + (lane & 15), c = grp * 4 + j;
-    unsigned s = 0, t = 0;
+    unsigned s = 0;
     if (c < q.kc) {
         const int k = c * 128 + (lane >> 4) * 32;
         union { u32x4 v; uint8_t e[16]; } w;
@@ -113,13 +111,12 @@ __global__ void __launch_bounds__(256) mx4_load_kernel(const uint8_t *__restrict
 #pragma unroll
                 for (int i = 0; i < 16; i++) w.e[i] = 2 * i + 1 < n ? p[i] : 2 * i < n ? p[i] & 15 : 0;
             }
-            t = (w.v[0] | w.v[1] | w.v[2] | w.v[3]) & 0x77777777u || s == 255 ? s : 0;
+            if (!((w.v[0] | w.v[1] | w.v[2] | w.v[3]) & 0x77777777u) && s != 255) s = 0;
         }
         reinterpret_cast<u32x4 *>(codes)[(tile * q.kc + c) * 64 + lane] = w.v;
     }
     sc[j][lane] = (unsigned char)s;
-    tp[j][lane] = (unsigned char)t;
-    write_scales(sc, tp, scales + (tile * q.kg + grp) * 256, top + tile * 16 * q.kt, q.kt, grp);
+    write_scales(sc, scales + (tile * q.kg + grp) * 256, top + tile * 16 * q.kt, q.kt, grp);
 }
 
 // A wave's tile of 16 rows × 128 k: the codes through LDS, so that 32 lanes write 512 consecutive bytes of a row, four values

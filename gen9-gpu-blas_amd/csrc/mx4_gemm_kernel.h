@@ -15,7 +15,8 @@ template <class T> struct Act;
 template <> struct Act<_Float16> {
     static constexpr int P = 1;
     typedef f16x8 Frag;
-    // 8 codes of a word to FP16, scale byte s of a block of a row whose largest is e
+    // 8 codes of a word to FP16, scale byte s of a block of a row whose largest is e: s <= e, or s = 255, which makes every
+    // code a NaN, zeros too
     static __device__ __forceinline__ float scale(unsigned s, int e) {
         const int r = s == 255 ? 255 : max((int)s - e + 140, 0);
         return __builtin_bit_cast(float, r << 23);

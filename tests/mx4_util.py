@@ -44,3 +44,25 @@ def sum_bound(K, pieces=3):
     """Rounding of an FP32 sum of K products in chains of 32-product matrix instructions, of which each adds at most two
     units of 2^-24 of a partial sum, over the sum of the magnitudes: `pieces` chains of K/32 steps and a few joins."""
     return (pieces * -(-K // 32) + 16) * 2.0 ** -23
+
+
+def zero_block_rows(r, K):
+    """Codes and scales of 1122 rows (K at least 576) with blocks of zeros, of both signs, under scales of their own: for rows of the largest
+    scales 0, 60, 100, 120 and 130 every scale from there to 254, in the second and the eighteenth block; rows of zeros with each
+    scale 0..254; and two rows with a NaN block (scale 255), of codes zero and others."""
+    n = -(-K // 32)
+    rows = [(e, s) for e in (0, 60, 100, 120, 130) for s in range(e, 255)]
+    e, s = np.array(rows).T
+    codes = r.integers(0, 16, (len(rows), K)).astype(np.uint8)
+    codes[:, 0] |= 1                                       # no accident leaves the row's largest block empty
+    scales = np.maximum(e[:, None] - r.integers(0, 4, (len(rows), n)), 0)
+    scales[:, 0] = e
+    for b in (1, 17):
+        codes[:, 32 * b:32 * b + 32] &= 8
+        scales[:, b] = s
+    zeros = 8 * r.integers(0, 2, (255, K))
+    nan, nan_scales = codes[-2:].copy(), scales[-2:].copy()
+    nan[0, 64:96] = 0
+    nan_scales[:, 2] = 255
+    return (np.concatenate([codes, zeros, nan]).astype(np.uint8),
+            np.concatenate([scales, np.repeat(np.arange(255)[:, None], n, 1), nan_scales]).astype(np.uint8))

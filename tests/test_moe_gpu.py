@@ -7,7 +7,7 @@ argument with a slope of at most 1.1, and adds a few units of 2^-23 of its own."
 import numpy as np
 import pytest
 
-from mx4_util import packed, quantize, sum_bound, values
+from mx4_util import packed, quantize, sum_bound, values, zero_block_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -250,6 +250,32 @@ def test_experts_unbalanced(g9, torch_dev, dtype):
         for join in (None, share):
             got = g9.moe_gemm(gpu(torch_dev, x), gpu(torch_dev, ids), W, weights=None if join is None else gpu(torch_dev, join))
             check_experts(torch_dev, got, *experts64(x, ids, w, None, join))
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("T,S", [(1, 2), (8, 2), (20, 2), (60, 2), (100, 2)])
+def test_experts_blocks_of_zeros_with_any_scale(g9, torch_dev, dtype, T, S):
+    """Blocks and rows of zeros under any scale, NaN blocks beside them: few places without a plan, tiles of 16, 32 and 64 rows.
+    X in steps of 2^-10: no sum of a row is rounded. Products of two such sums may be FP32 subnormals, of 2^-149 steps."""
+    torch = torch_dev
+    r = np.random.default_rng(T)
+    E, K = 3, 640
+
+    def experts():
+        codes, scales = (np.stack(p) for p in zip(*(zero_block_rows(r, K) for _ in range(E))))
+        return g9.mx4_load(gpu(torch, packed(codes)), gpu(torch, scales), K=K), values(codes, scales)
+
+    (W, w), (G, g) = experts(), experts()
+    nan = np.isnan(w).any((0, 2))           # the same rows of every expert
+    ids = np.argsort(r.random((T, E)), 1)[:, :S].astype(np.int32)
+    share = r.random((T, S)).astype(np.float32)
+    x = (r.integers(-64, 65, (T, K)) / 1024).astype(dtype)
+    for gate in (False, True):
+        for join in (False, True):
+            got = g9.moe_gemm(gpu(torch, x), gpu(torch, ids), W, gate=G if gate else None, weights=gpu(torch, share) if join else None)
+            assert bool(got[..., gpu(torch, nan)].isnan().all())
+            ref, tol = experts64(x, ids, w[:, ~nan], g[:, ~nan] if gate else None, share if join else None)
+            check_experts(torch, got[..., gpu(torch, ~nan)], ref, tol + 2.0 ** -146)
 
 
 @pytest.mark.parametrize("T", [1, 5, 90])

@@ -9,7 +9,7 @@ import ctypes
 import numpy as np
 import pytest
 
-from mx4_util import packed, quantize, sum_bound, values
+from mx4_util import packed, quantize, sum_bound, values, zero_block_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -271,6 +271,37 @@ def test_gemm_scales_of_any_size(g9, torch_dev, M):
     ref = values(codes, scales)
     assert np.abs(h.astype(np.float64) @ ref.T).max() < 6e4
     check_product(torch_dev, g9.mx4_gemm(gpu(torch_dev, h), W), h, ref)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("M", [1, 20, 100, 500, 1000])
+def test_gemm_blocks_of_zeros_with_any_scale(g9, torch_dev, dtype, M):
+    """A block of zeros is zeros whatever its scale says, in rows of any largest scale and in rows of nothing but zeros; a NaN block
+    (scale 255) stays NaN. Rows enough for every kernel that takes these M. A in steps of 2^-10, so that no sum of FP32 is rounded, the
+    subnormal ones of the least scales among them."""
+    torch = torch_dev
+    r = rng(M)
+    parts = [zero_block_rows(r, 640) for _ in range(4)]
+    codes, scales = (np.concatenate([p[i] for p in parts]) for i in (0, 1))
+    nan = (scales == 255).any(1)
+    W = g9.mx4_load(gpu(torch, packed(codes)), gpu(torch, scales), K=640)
+    a = gpu(torch, (r.integers(-64, 65, (M, 640)) / 1024).astype(dtype))
+    got = g9.mx4_gemm(a, W)
+    assert bool(got[:, gpu(torch, nan)].isnan().all())
+    assert bool(got[:, gpu(torch, ~nan)].isfinite().all())
+    check_large(torch, got[:, gpu(torch, ~nan)], a.double(), gpu(torch, values(codes[~nan], scales[~nan])), got.dtype)
+
+
+@pytest.mark.parametrize("M", [1, 20, 100, 500, 1000])
+def test_gemm_quantized_nan_block_stays_nan(g9, torch_dev, M):
+    """The codes of a NaN block are zeros: a block of zeros must not be taken for it, nor it for one."""
+    torch = torch_dev
+    w = torch.zeros((4500, 640), device="cuda")
+    w[7, 100], w[4499, 639], w[300, 40] = float("nan"), float("inf"), 1.0
+    got = g9.mx4_gemm(torch.ones((M, 640), dtype=torch.float16, device="cuda"), g9.mx4_quantize(w))
+    want = torch.zeros((M, 4500), dtype=torch.float16, device="cuda")
+    want[:, 7], want[:, 4499], want[:, 300] = float("nan"), float("nan"), 1.0
+    assert same(got.cpu().numpy(), want.cpu().numpy())
 
 
 @pytest.mark.parametrize("dtype", [np.float16, np.float32])
