@@ -16,8 +16,9 @@ __device__ __forceinline__ i32x8 fp4_operand(u32x4 v) { return i32x8{(int)v[0], 
 // Four stages of A are on the ring: while stage s is multiplied, its fragments for s + 1 are read and s + 2 to s + 4 are on their
 // way (s + 4 into the place of s, whose fragments every wave has by then). A fragment of W is loaded as soon as its registers are
 // free, a stage or more ahead. The scales of 512 k (a word per lane and row tile) come with every fourth stage, A's through
-// LDS on a ring of two, W's to registers. Each wait counts the copies and loads behind what it waits for: none is conditional, past
-// the end the last ones are fetched again.
+// LDS on a ring of two, W's to registers. In whole groups each wait counts the copies and loads behind what it waits for: none of them is
+// conditional (past the end the last ones are fetched again), and the next group takes what they bring. The stages after the last
+// whole group count nothing.
 template <class O>
 __global__ void __launch_bounds__(256, 1) mx4_gemm_q_tile_kernel(Mx4View A, Mx4View W, O *__restrict__ C, long long ldc, int mtiles, int ntiles) {
     constexpr int T = 8, STAGE = 2 * T * 1024, NS = 4, SCALES = 2 * T * 256, T2 = T / 2, CP = T2, OPS = CP + T;   // copies of A, and all copies and loads, a stage and wave
@@ -107,18 +108,13 @@ __global__ void __launch_bounds__(256, 1) mx4_gemm_q_tile_kernel(Mx4View A, Mx4V
     read_scales(0);
     // A stage. With the matrix instructions of each fragment of A go a copy (in the first half), a fragment of the next stage, and
     // a load into the registers of W that the last half has left: the second half of the next stage, then the first of the one after.
-    auto step = [&](int c0, auto J, bool first) {
+    auto multiply = [&](int c0, auto J, auto COPY) __attribute__((always_inline)) {   // called seven times: what it refers to must stay in registers
         constexpr int j = decltype(J)::value;
         constexpr std::integral_constant<int, (j & 1)> here{};
         constexpr std::integral_constant<int, ((j + 1) & 1)> next{};
-        // what the two stages before this one have queued may be on its way, with the scales if one of them began a group; in
-        // the first group the copies of stage 2 (and 3) stand for them
-        if (first && j < 2) arrive(std::integral_constant<int, j == 0 ? 2 * CP : CP + OPS + 1 + T>());
-        else arrive(std::integral_constant<int, 2 * OPS + (j == 1 || j == 2 ? 1 + T : 0)>());
-        if (j == 0) scales(c0 + 4);
 #pragma unroll
         for (int t = 0; t < T; t++) {
-            if (t < CP) issue_one(c0 + j + 4, t);
+            if (decltype(COPY)::value && t < CP) issue_one(c0 + j + 4, t);
             read_one(std::integral_constant<int, (j + 1) % 4>(), t);
             if (j == 3 && t == T - 1) read_scales(c0 / 4 + 1);
             const int u = t / T2, m = t % T2;
@@ -131,25 +127,40 @@ __global__ void __launch_bounds__(256, 1) mx4_gemm_q_tile_kernel(Mx4View A, Mx4V
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    auto group = [&](int c0, bool first) {
-#pragma unroll
-        for (int t = 0; t < T; t++) sa[t] = sa_next[t], sw[t] = sw_next[t];
-        step(c0, std::integral_constant<int, 0>(), first);
-        if (c0 + 1 < A.kc) step(c0, std::integral_constant<int, 1>(), first);
-        if (c0 + 2 < A.kc) step(c0, std::integral_constant<int, 2>(), first);
-        if (c0 + 3 < A.kc) step(c0, std::integral_constant<int, 3>(), first);
+    auto step = [&](int c0, auto J, bool first) __attribute__((always_inline)) {
+        constexpr int j = decltype(J)::value;
+        // what the two stages before this one have queued may be on its way, with the scales if one of them began a group; in
+        // the first group the copies of stage 2 (and 3) stand for them
+        if (first && j < 2) arrive(std::integral_constant<int, j == 0 ? 2 * CP : CP + OPS + 1 + T>());
+        else arrive(std::integral_constant<int, 2 * OPS + (j == 1 || j == 2 ? 1 + T : 0)>());
+        if (j == 0) scales(c0 + 4);
+        multiply(c0, J, std::true_type());
     };
-    group(0, true);
-    int c0 = 4;
-    for (; c0 + 4 <= A.kc; c0 += 4) {
+    auto take_scales = [&] {
 #pragma unroll
         for (int t = 0; t < T; t++) sa[t] = sa_next[t], sw[t] = sw_next[t];
-        step(c0, std::integral_constant<int, 0>(), false);
-        step(c0, std::integral_constant<int, 1>(), false);
-        step(c0, std::integral_constant<int, 2>(), false);
-        step(c0, std::integral_constant<int, 3>(), false);
+    };
+    auto group = [&](int c0, bool first) __attribute__((always_inline)) {
+        take_scales();
+        step(c0, std::integral_constant<int, 0>(), first);
+        step(c0, std::integral_constant<int, 1>(), first);
+        step(c0, std::integral_constant<int, 2>(), first);
+        step(c0, std::integral_constant<int, 3>(), first);
+    };
+    int c0 = 0;
+    if (A.kc >= 4) {
+        group(0, true);
+        for (c0 = 4; c0 + 4 <= A.kc; c0 += 4) group(c0, false);
     }
-    if (c0 < A.kc) group(c0, false);
+    // The last one to three stages. Their copies are on their way, so nothing is queued but what they still take of W, and one wait
+    // for all of it stands before them: a count would be wrong here, as the compiler drops loads that no stage uses.
+    if (c0 < A.kc) {
+        arrive(std::integral_constant<int, 0>());
+        take_scales();
+        multiply(c0, std::integral_constant<int, 0>(), std::false_type());
+        if (c0 + 1 < A.kc) multiply(c0, std::integral_constant<int, 1>(), std::false_type());
+        if (c0 + 2 < A.kc) multiply(c0, std::integral_constant<int, 2>(), std::false_type());
+    }
     g9::wait_vm<0>();   // no copy may land after the workgroup has gone
     // lane l: row l % 32, and of register 4q + j column 8q + 4·(l / 32) + j. Both halves' 32-row tiles m go through LDS together.
     constexpr int COLS = 32 * T, PITCH = COLS * sizeof(O) + 16;

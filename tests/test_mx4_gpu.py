@@ -188,6 +188,19 @@ def test_gemm_quantized_middle(g9, torch_dev, K):
         check_large(torch, g9.mx4_gemm(qa, qw, dtype=out), a, w, t)
 
 
+@pytest.mark.parametrize("M,N", [(4100, 4117), (700, 1301)])
+@pytest.mark.parametrize("K", [768, 870, 1280, 1400])
+def test_gemm_quantized_stages_after_whole_groups(g9, torch_dev, M, N, K):
+    """Six, seven, ten and eleven 128-k stages: two and three of them after the last whole group of four, in both tilings."""
+    torch = torch_dev
+    g = torch.Generator(device="cuda").manual_seed(K + M)
+    qa = g9.mx4_quantize(torch.randn((M, K), generator=g, device="cuda"))
+    qw = g9.mx4_quantize(torch.randn((N, K), generator=g, device="cuda") / 8)
+    a, w = g9.mx4_dequantize(qa).double(), g9.mx4_dequantize(qw).double()
+    for out, t in ((np.float16, torch.float16), (np.float32, torch.float32)):
+        check_large(torch, g9.mx4_gemm(qa, qw, dtype=out), a, w, t)
+
+
 @pytest.mark.parametrize("dtype", ["float16", "float32"])
 @pytest.mark.parametrize("M,N,K", [(300, 5000, 200), (700, 4099, 129), (1100, 4099, 645)])
 def test_gemm_large_strides_and_nan(g9, torch_dev, dtype, M, N, K):
