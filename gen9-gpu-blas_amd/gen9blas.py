@@ -1102,8 +1102,9 @@ def moe_gemm(X, ids, W, gate=None, weights=None, C=None):
     torch = _torch
     x = _device_rows(X, (2, 3))
     i = ids if isinstance(ids, torch.Tensor) and ids.is_cuda else torch.as_tensor(ids).cuda()
-    if i.dtype is not torch.int32 or not i.is_contiguous():
-        i = i.to(torch.int32).contiguous()
+    if i.dtype is not torch.int32:
+        i = i.to(torch.int64).clamp(-1, 0x7fffffff).to(torch.int32)   # past 32 bits: no expert's
+    i = i.contiguous()
     if i.dim() != 2 or len(W.shape) != 3 or x.shape[-1] != W.shape[2] or x.shape[0] != i.shape[0] or \
             (x.dim() == 3 and x.shape[1] != i.shape[1]) or (gate is not None and gate.shape != W.shape):
         raise ValueError(f"incompatible shapes: X {tuple(x.shape)}, ids {tuple(i.shape)}, W {W.shape}"

@@ -278,6 +278,26 @@ def test_experts_blocks_of_zeros_with_any_scale(g9, torch_dev, dtype, T, S):
             check_experts(torch, got[..., gpu(torch, ~nan)], ref, tol + 2.0 ** -146)
 
 
+@pytest.mark.parametrize("T", [3, 70])
+def test_experts_ids_of_other_types(g9, torch_dev, T):
+    """Ids of 64 bits, beyond 32 bits too, are no expert's unless they are 0..E-1; other integer types as they are."""
+    torch = torch_dev
+    r = np.random.default_rng(T)
+    S, E, N, K = 6, 4, 40, 96
+    W, w = weights(r, torch, g9, E, N, K)
+    x = r.standard_normal((T, K)).astype(np.float32)
+    ids = r.integers(0, E, (T, S))
+    ids[:, 1], ids[:, 3] = 1 << 32, -(1 << 32) + 2
+    ids[0, 0], ids[1, 2], ids[2, 5] = (1 << 31) + 1, np.iinfo(np.int64).min, np.iinfo(np.int64).max
+    want = experts64(x, ids, w)
+    assert (want[0][:, (1, 3)] == 0).all()
+    check_experts(torch, g9.moe_gemm(gpu(torch, x), gpu(torch, ids), W), *want)
+    check_experts(torch, torch.from_numpy(g9.moe_gemm(x, ids, W)), *want)
+    small = r.integers(0, E, (T, S))
+    for t in (torch.int64, torch.int16, torch.uint8):
+        check_experts(torch, g9.moe_gemm(gpu(torch, x), gpu(torch, small).to(t), W), *experts64(x, small, w))
+
+
 @pytest.mark.parametrize("T", [1, 5, 90])
 def test_experts_strides(g9, torch_dev, T):
     """Rows of X and C with strides of tokens and places, at odd alignments; nothing written beside C; NaN in one token's row
