@@ -360,6 +360,16 @@ template <class T, class O, bool GATED> static int launch_grouped(const Rows &R,
 }
 
 template <class T>
+static int join(const float *y, long long ld, const int *ids, const float *weights, int Tn, int S, int E, int N, T *C, long long ldct) {
+    for (long long t0 = 0; t0 < Tn; t0 += 65535) {   // the grid's y limit
+        const dim3 grid((unsigned)cdiv(N, 1024), (unsigned)std::min(Tn - t0, 65535LL));
+        hipLaunchKernelGGL((moe_join_kernel<T>), grid, dim3(256), 0, stream, y + t0 * S * ld, ld, ids + t0 * S, weights + t0 * S, S, E, N, C + t0 * ldct, ldct);
+    }
+    G9_HIP(hipGetLastError());
+    return 0;
+}
+
+template <class T>
 static int experts(int Tn, int S, const int *ids, const void *X, int64_t ldt, int64_t lds, const gen9blas_mx4 *W, const gen9blas_mx4 *gate,
                    const float *weights, void *C, int64_t ldct, int64_t ldcs) {
     const long long n = (long long)Tn * S;
@@ -392,14 +402,7 @@ static int experts(int Tn, int S, const int *ids, const void *X, int64_t ldt, in
         return gate ? launch_grouped<T, T, true>(R, w, g, E, (int)most, rows, Tn, n) : launch_grouped<T, T, false>(R, w, g, E, (int)most, rows, Tn, n);
     R.C = slots, R.ldct = S * ld, R.ldcs = ld;
     G9_TRY((gate ? launch_grouped<T, float, true>(R, w, g, E, (int)most, rows, Tn, n) : launch_grouped<T, float, false>(R, w, g, E, (int)most, rows, Tn, n)));
-    for (int t0 = 0; t0 < Tn; t0 += 65535) {   // the grid's y limit
-        const int rowsy = min(Tn - t0, 65535);
-        hipLaunchKernelGGL((moe_join_kernel<T>), dim3((unsigned)cdiv(N, 1024), (unsigned)rowsy), dim3(256), 0, stream,
-                           (const float *)slots + t0 * S * ld, ld, ids + (long long)t0 * S, weights + (long long)t0 * S, S, E, N,
-                           (T *)C + t0 * ldct, (long long)ldct);
-    }
-    G9_HIP(hipGetLastError());
-    return 0;
+    return join((const float *)slots, ld, ids, weights, Tn, S, E, N, (T *)C, ldct);
 }
 
 }  // namespace g9llm
@@ -433,8 +436,13 @@ int gen9blas_moe_gemm(int type, int T, int S, const int *ids, const void *X, int
     if (!W || W->count > MAX_EXPERTS) G9_FAIL(GEN9BLAS_ERR_INVALID_ARG, "moe_gemm: %s", W ? "more than 1024 experts" : "no W");
     if (gate && (gate->count != W->count || gate->rows != W->rows || gate->K != W->K))
         G9_FAIL(GEN9BLAS_ERR_INVALID_ARG, "moe_gemm: the gate's shape is not W's");
-    if (T <= 0 || S <= 0) return 0;
+    if (T <= 0 || (S <= 0 && !weights)) return 0;
     const int K = W->K, N = W->rows, es = elem_size(type);
+    if (S <= 0) {   // sums of nothing
+        if (ldct < N) G9_FAIL(GEN9BLAS_ERR_INVALID_ARG, "moe_gemm: rows of C overlap (ldct %lld, N %d)", (long long)ldct, N);
+        G9_TRY(need_device(C, ((size_t)(T - 1) * ldct + N) * es, "moe_gemm: C"));
+        return type == GEN9BLAS_H ? join(nullptr, 0, nullptr, nullptr, T, 0, 0, N, (_Float16 *)C, ldct) : join(nullptr, 0, nullptr, nullptr, T, 0, 0, N, (float *)C, ldct);
+    }
     if (lds < 0 || (lds > 0 && lds < K) || ldt < (lds ? (S - 1) * lds + K : K))
         G9_FAIL(GEN9BLAS_ERR_INVALID_ARG, "moe_gemm: rows of X overlap (ldt %lld, lds %lld, K %d)", (long long)ldt, (long long)lds, K);
     if (weights ? ldct < N : (ldcs < N || ldct < (S - 1) * ldcs + N))

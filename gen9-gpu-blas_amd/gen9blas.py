@@ -1120,5 +1120,6 @@ def moe_gemm(X, ids, W, gate=None, weights=None, C=None):
     ldcs = N if weights is not None else _row_step(out, 1)
     ldct = out.stride(0) if T > 1 else ldcs * max(S, 1)
     _llm_call(lib.gen9blas_moe_gemm, 1 if x.dtype == torch.float32 else 0, T, S, i.data_ptr(), x.data_ptr(), ldt, lds, W._handle,
-              None if gate is None else gate._handle, None if weights is None else weights.data_ptr(), out.data_ptr(), ldct, ldcs)
+              None if gate is None else gate._handle, None if weights is None else weights.data_ptr() or out.data_ptr(),   # empty: no address
+              out.data_ptr(), ldct, ldcs)
     return _host_like(X, out) if C is None else out

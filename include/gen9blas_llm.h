@@ -70,7 +70,8 @@ GEN9BLAS_API int gen9blas_moe_route(int type, int T, int E, const void *logits, 
 // The row of token t, place s is X + t·ldt + s·lds (lds = 0: one row for all places of a token); y(t, s) = row · W[ids(t, s)]ᵀ.
 // - gate != NULL (as W): y(t, s) = silu(row · gate[ids(t, s)]ᵀ) · (row · W[ids(t, s)]ᵀ), silu(z) = z / (1 + e^−z).
 // - weights == NULL: C(t, s) = y(t, s) at C + t·ldct + s·ldcs (ldcs >= N, ldct >= S·ldcs).
-// - weights (T×S floats, dense): C(t) = Σ_s weights(t, s) · y(t, s) at C + t·ldct, in the order of s; ldcs is not read.
+// - weights (T×S floats, dense): C(t) = Σ_s weights(t, s) · y(t, s) at C + t·ldct, in the order of s; ldcs is not read. S = 0: zeros
+//   (weights still not NULL, ids and X not read).
 // An id outside 0..E−1 is an empty place: its y is 0, and its weight is not read.
 GEN9BLAS_API int gen9blas_moe_gemm(int type, int T, int S, const int *ids, const void *X, int64_t ldt, int64_t lds,
                                    const gen9blas_mx4 *W, const gen9blas_mx4 *gate, const float *weights, void *C,

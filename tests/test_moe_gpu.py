@@ -298,6 +298,32 @@ def test_experts_ids_of_other_types(g9, torch_dev, T):
         check_experts(torch, g9.moe_gemm(gpu(torch, x), gpu(torch, small).to(t), W), *experts64(x, small, w))
 
 
+def test_experts_no_places(g9, torch_dev):
+    """A token without places has nothing to join: its row of the result is zero."""
+    torch = torch_dev
+    W = g9.mx4_quantize(torch.ones((3, 40, 96), device="cuda"))
+    ids, share = torch.empty((5, 0), dtype=torch.int32, device="cuda"), torch.empty((5, 0), device="cuda")
+    for t in (torch.float16, torch.float32):
+        x = torch.ones((5, 96), dtype=t, device="cuda")
+        out = torch.full((7, 50), 3.0, dtype=t, device="cuda")
+        assert g9.moe_gemm(x, ids, W, weights=share, C=out[1:6, 2:42]) is not None
+        assert bool((out[1:6, 2:42] == 0).all())
+        out[1:6, 2:42] = 3.0
+        assert bool((out == 3.0).all())
+        assert g9.moe_gemm(x, ids, W).shape == (5, 0, 40)
+    assert (g9.moe_gemm(np.ones((5, 96), np.float32), np.empty((5, 0), np.int32), W, weights=np.empty((5, 0), np.float32)) == 0).all()
+    L = g9._llm_library()
+    C = torch.full((5, 40), 3.0, device="cuda")
+    x = torch.ones((5, 96), device="cuda")
+    call = lambda S, weights, C: L.gen9blas_moe_gemm(1, 5, S, None, x.data_ptr(), 96, 0, W._handle, None, weights, C, 40, 40)   # noqa: E731
+    assert call(0, None, None) == 0 and call(0, None, C.data_ptr()) == 0 and call(0, x.data_ptr(), None) == -3
+    torch.cuda.synchronize()
+    assert bool((C == 3).all())
+    assert call(0, x.data_ptr(), C.data_ptr()) == 0
+    g9.flush()
+    assert bool((C == 0).all())
+
+
 @pytest.mark.parametrize("T", [1, 5, 90])
 def test_experts_strides(g9, torch_dev, T):
     """Rows of X and C with strides of tokens and places, at odd alignments; nothing written beside C; NaN in one token's row
