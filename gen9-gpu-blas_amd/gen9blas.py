@@ -947,16 +947,31 @@ def _llm_call(fn, *args):
         flush()
 
 
-def _device_rows(X, dims):
-    """X as a GPU tensor of float16 or float32 whose rows are contiguous, of one of the numbers of dimensions in `dims`."""
+def _on_gpu(X):
+    """X as a GPU tensor: itself, or a copy of an array, tensor or list in host memory."""
     torch = _torch
-    if not (isinstance(X, torch.Tensor) and X.is_cuda):
-        X = torch.as_tensor(X).cuda()
+    if not isinstance(X, torch.Tensor):
+        if isinstance(X, np.ndarray) and any(step < 0 for step in X.strides):
+            X = X.copy()                                    # torch takes no negative strides
+        X = torch.as_tensor(X)
+    return X if X.is_cuda else X.cuda()
+
+
+def _device_rows(X, dims, shared=False):
+    """X as a GPU tensor of float16 or float32, of one of the numbers of dimensions in `dims`, whose rows are contiguous and do not
+    overlap; X in another layout is copied. shared: one row for all places of a token (a stride of 0) is one too."""
+    torch = _torch
+    X = _on_gpu(X)
     if X.dim() not in dims:
         raise ValueError(f"expected {' or '.join(map(str, dims))} dimensions, got {X.dim()}")
     if X.dtype is not torch.float16 and X.dtype is not torch.float32:
         X = X.float()
-    return X if X.stride(-1) == 1 or X.shape[-1] <= 1 else X.contiguous()
+    shape, step = X.shape, X.stride()
+    if step[-1] != 1 and shape[-1] > 1:
+        return X.contiguous()
+    if len(shape) > 1 and step[-2] < shape[-1] and shape[-2] > 1 and not (shared and len(shape) == 3 and step[1] == 0):
+        return X.contiguous()
+    return X
 
 
 def _host_like(X, result):
@@ -1020,7 +1035,7 @@ def mx4_load(codes, scales, K=None):
     in the low half; scales (..., rows, K/32), the exponent + 127. K defaults to twice the width of codes."""
     lib = _llm_library()
     torch = _torch
-    c, s = (x if _is_tensor(x) and x.is_cuda else torch.as_tensor(x).cuda() for x in (codes, scales))
+    c, s = _on_gpu(codes), _on_gpu(scales)
     if c.dtype != torch.uint8 or s.dtype != torch.uint8:
         raise TypeError("codes and scales are uint8")
     K = 2 * c.shape[-1] if K is None else int(K)
@@ -1100,8 +1115,7 @@ def moe_gemm(X, ids, W, gate=None, weights=None, C=None):
     weights[t, s]·y[t, s] (T, N). An id that is no expert's (-1) is an empty place, its y is zero."""
     lib = _llm_library()
     torch = _torch
-    x = _device_rows(X, (2, 3))
-    i = ids if isinstance(ids, torch.Tensor) and ids.is_cuda else torch.as_tensor(ids).cuda()
+    x, i = _device_rows(X, (2, 3), shared=True), _on_gpu(ids)
     if i.dtype is not torch.int32:
         i = i.to(torch.int64).clamp(-1, 0x7fffffff).to(torch.int32)   # past 32 bits: no expert's
     i = i.contiguous()
@@ -1116,6 +1130,9 @@ def moe_gemm(X, ids, W, gate=None, weights=None, C=None):
             raise ValueError(f"weights {tuple(weights.shape)} for ids {tuple(i.shape)}")
     out = _llm_out(C, (T, N) if weights is not None else (T, S, N), x.dtype)
     lds = 0 if x.dim() == 2 else _row_step(x, 1)
+    if T > 1 and x.stride(0) < max(S - 1, 0) * lds + x.shape[-1]:   # tokens share rows, or lie within each other's
+        x = x.contiguous()
+        lds = 0 if x.dim() == 2 else x.shape[-1]
     ldt = x.stride(0) if T > 1 else max(lds * S, x.shape[-1])
     ldcs = N if weights is not None else _row_step(out, 1)
     ldct = out.stride(0) if T > 1 else ldcs * max(S, 1)

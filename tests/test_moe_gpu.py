@@ -324,6 +324,34 @@ def test_experts_no_places(g9, torch_dev):
     assert bool((C == 0).all())
 
 
+def test_inputs_of_any_layout(g9, torch_dev):
+    """Layouts that the C entry points do not take are copied: repeated and overlapping rows, permuted dimensions, NumPy's negative
+    strides."""
+    torch = torch_dev
+    r = np.random.default_rng(6)
+    E, S, N, K, T = 5, 3, 40, 96, 7
+    W, _ = weights(r, torch, g9, E, N, K)
+    ids = gpu(torch, np.argsort(r.random((T, E)), 1)[:, :S].astype(np.int32))
+    share = gpu(torch, r.random((T, S)).astype(np.float32))
+    for dtype in (torch.float16, torch.float32):
+        x = gpu(torch, r.standard_normal((S, T, K))).to(dtype)
+        flat = x.reshape(-1)
+        for v in (x[0, :1].expand(T, K), flat.as_strided((T, K), (3, 1)), x.transpose(0, 1), x[:, :1].transpose(0, 1).expand(T, S, K),
+                  x[0, :, None].expand(T, S, K), flat.as_strided((T, S, K), (K, 5, 1)), x[0].t().contiguous().t()):
+            for kw in (dict(), dict(weights=share), dict(gate=W)):
+                assert bool((g9.moe_gemm(v, ids, W, **kw) == g9.moe_gemm(v.contiguous(), ids, W, **kw)).all())
+        logits = flat.as_strided((T, 8), (2, 1))
+        for v in (logits, flat[:8].expand(T, 8)):
+            got, want = g9.moe_route(v, 2), g9.moe_route(v.contiguous(), 2)
+            assert bool((got[0] == want[0]).all()) and bool((got[1] == want[1]).all())
+    x, l, b = (r.standard_normal(n).astype(np.float32) for n in ((T, K), (T, 8), 8))
+    i, w = ids.cpu().numpy(), share.cpu().numpy()
+    got = g9.moe_gemm(x[::-1, ::-1], i[::-1], W, weights=w[::-1, ::-1])
+    assert np.array_equal(got, g9.moe_gemm(x[::-1, ::-1].copy(), i[::-1].copy(), W, weights=w[::-1, ::-1].copy()))
+    got, want = g9.moe_route(l[:, ::-1], 2, bias=b[::-1]), g9.moe_route(l[:, ::-1].copy(), 2, bias=b[::-1].copy())
+    assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
 @pytest.mark.parametrize("T", [1, 5, 90])
 def test_experts_strides(g9, torch_dev, T):
     """Rows of X and C with strides of tokens and places, at odd alignments; nothing written beside C; NaN in one token's row

@@ -249,6 +249,27 @@ def test_gemm_strides(g9, torch_dev, dtype, M):
     assert bool((out[:, 0] == 3.0).all()) and bool((out[:, N + 1:] == 3.0).all())
 
 
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+def test_inputs_of_any_layout(g9, torch_dev, dtype):
+    """Layouts that the C entry points do not take are copied: repeated and overlapping rows, permuted dimensions, NumPy's negative
+    strides."""
+    torch = torch_dev
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn((6, 5, 96), generator=g, device="cuda").to(getattr(torch, dtype))
+    flat = x.reshape(-1)
+    W = g9.mx4_quantize(torch.randn((40, 96), generator=g, device="cuda"))
+    for a in (x[0, :1].expand(9, 96), flat.as_strided((9, 96), (7, 1)), x[:, 0], x[0, :, :48].expand(2, 5, 48).reshape(5, 96), x[0].t().contiguous().t()):
+        assert bool((g9.mx4_gemm(a, W) == g9.mx4_gemm(a.contiguous(), W)).all())
+        assert bool((g9.mx4_dequantize(g9.mx4_quantize(a)) == g9.mx4_dequantize(g9.mx4_quantize(a.contiguous()))).all())
+    for a in (x.transpose(0, 1), x[:1].expand(3, 5, 96), x[:, :1].expand(6, 4, 96), flat.as_strided((3, 5, 40), (11, 2, 1)), x.transpose(1, 2)):
+        assert bool((g9.mx4_dequantize(g9.mx4_quantize(a)) == g9.mx4_dequantize(g9.mx4_quantize(a.contiguous()))).all())
+    n = x[0].cpu().numpy()
+    for a in (n[::-1], n[:, ::-1], n[::2], n.T[::-1].T):
+        assert np.array_equal(g9.mx4_gemm(a, W), g9.mx4_gemm(a.copy(), W))
+    c, s = np.arange(4 * 48, dtype=np.uint8).reshape(4, 48), np.arange(120, 132, dtype=np.uint8).reshape(4, 3)
+    assert same(g9.mx4_dequantize(g9.mx4_load(c[::-1], s[::-1])).cpu(), g9.mx4_dequantize(g9.mx4_load(c[::-1].copy(), s[::-1].copy())).cpu())
+
+
 @pytest.mark.parametrize("M", [1, 16, 40, 70, 130, 300])
 def test_gemm_fp32_is_fp32(g9, torch_dev, M):
     """FP32 activations keep their 24 bits: over 32 products of one sign the relative error is a few units of 2^-24, where
