@@ -959,7 +959,8 @@ def _on_gpu(X):
 
 def _device_rows(X, dims, shared=False):
     """X as a GPU tensor of float16 or float32, of one of the numbers of dimensions in `dims`, whose rows are contiguous and do not
-    overlap; X in another layout is copied. shared: one row for all places of a token (a stride of 0) is one too."""
+    overlap, with a row stride that is a C int; X in another layout is copied. shared (the rows of experts' products): one row
+    for all places of a token (a stride of 0) is taken too, and strides of any length are."""
     torch = _torch
     X = _on_gpu(X)
     if X.dim() not in dims:
@@ -969,8 +970,11 @@ def _device_rows(X, dims, shared=False):
     shape, step = X.shape, X.stride()
     if step[-1] != 1 and shape[-1] > 1:
         return X.contiguous()
-    if len(shape) > 1 and step[-2] < shape[-1] and shape[-2] > 1 and not (shared and len(shape) == 3 and step[1] == 0):
-        return X.contiguous()
+    if len(shape) > 1 and shape[-2] > 1:
+        if step[-2] < shape[-1] and not (shared and len(shape) == 3 and step[1] == 0):
+            return X.contiguous()
+        if step[-2] > _LONGEST_STEP and not shared:
+            return X.contiguous()
     return X
 
 
@@ -990,9 +994,20 @@ def _llm_out(C, shape, dtype, what="C"):
     return C
 
 
+_LONGEST_STEP = 0x7fffffff
+
+
 def _row_step(X, dim=-2):
     """Stride between rows, at least the row's length (a dimension of one has any stride)."""
     return X.stride(dim) if X.shape[dim] > 1 else max(X.shape[-1], 1)
+
+
+def _out_step(X, what="C"):
+    """The same of a result whose row stride is a C int."""
+    step = _row_step(X)
+    if step > _LONGEST_STEP:
+        raise ValueError(f"{what} has a row stride of {step} elements; the longest is {_LONGEST_STEP}")
+    return step
 
 
 class MX4:
@@ -1052,7 +1067,7 @@ def mx4_dequantize(Q, out=None):
     """The values of an MX4 matrix in float32."""
     lib = _llm_library()
     X = _llm_out(out, Q.shape, _torch.float32, "out")
-    _llm_call(lib.gen9blas_mx4_dequantize, Q._handle, X.data_ptr(), _row_step(X), X.stride(0) if X.dim() == 3 else 0)
+    _llm_call(lib.gen9blas_mx4_dequantize, Q._handle, X.data_ptr(), _out_step(X, "out"), X.stride(0) if X.dim() == 3 else 0)
     return X
 
 
@@ -1071,14 +1086,14 @@ def mx4_gemm(A, W, C=None, dtype=None):
         if t != torch.float16 and t != torch.float32:
             raise TypeError("C must be float16 or float32")
         C = _llm_out(C, (A.shape[0], W.shape[0]), t)
-        _llm_call(lib.gen9blas_mx4_gemm_q, 1 if t == torch.float32 else 0, A._handle, W._handle, C.data_ptr(), _row_step(C))
+        _llm_call(lib.gen9blas_mx4_gemm_q, 1 if t == torch.float32 else 0, A._handle, W._handle, C.data_ptr(), _out_step(C))
         return C
     a = _device_rows(A, (2,))
     if len(W.shape) != 2 or a.shape[1] != W.shape[1]:
         raise ValueError(f"incompatible dimensions: {tuple(a.shape)} · {W.shape}ᵀ")
     out = _llm_out(C, (a.shape[0], W.shape[0]), a.dtype)
     _llm_call(lib.gen9blas_mx4_gemm, 1 if a.dtype == torch.float32 else 0, a.shape[0], a.data_ptr(), _row_step(a), W._handle,
-              out.data_ptr(), _row_step(out))
+              out.data_ptr(), _out_step(out))
     return _host_like(A, out) if C is None else out
 
 

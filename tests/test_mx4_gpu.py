@@ -270,6 +270,29 @@ def test_inputs_of_any_layout(g9, torch_dev, dtype):
     assert same(g9.mx4_dequantize(g9.mx4_load(c[::-1], s[::-1])).cpu(), g9.mx4_dequantize(g9.mx4_load(c[::-1].copy(), s[::-1].copy())).cpu())
 
 
+def test_row_strides_past_32_bits(g9, torch_dev):
+    """The C entry points have row strides of 31 bits: inputs of longer ones are copied, such results are refused."""
+    torch = torch_dev
+    far = (1 << 32) + 64
+    buf = torch.zeros(far + 64, dtype=torch.float16, device="cuda")
+    a = buf.as_strided((2, 64), (far, 1))
+    buf[:128] = torch.arange(128, device="cuda") / 16
+    a[1] = 1.0
+    W = g9.mx4_quantize(torch.ones((64, 64), device="cuda"))
+    assert bool((g9.mx4_gemm(a, W) == g9.mx4_gemm(a.contiguous(), W)).all())
+    assert bool((g9.mx4_dequantize(g9.mx4_quantize(a)) == g9.mx4_dequantize(g9.mx4_quantize(a.contiguous()))).all())
+    got, want = g9.moe_route(a, 2), g9.moe_route(a.contiguous(), 2)
+    assert bool((got[0] == want[0]).all()) and bool((got[1] == want[1]).all())
+    with pytest.raises(ValueError):
+        g9.mx4_gemm(a.contiguous(), W, C=a)
+    stack = g9.mx4_quantize(torch.ones((2, 64, 64), device="cuda"))    # strides of tokens are of 64 bits
+    ids = torch.ones((2, 1), dtype=torch.int32, device="cuda")
+    y = g9.moe_gemm(a, ids, stack)
+    assert bool((y == g9.moe_gemm(a.contiguous(), ids, stack)).all())
+    g9.moe_gemm(a.contiguous(), ids, stack, C=buf.as_strided((2, 1, 64), (far, 64, 1)))
+    assert bool((a == y[:, 0]).all()) and bool((buf[64:128] == torch.arange(64, 128, device="cuda") / 16).all())
+
+
 @pytest.mark.parametrize("M", [1, 16, 40, 70, 130, 300])
 def test_gemm_fp32_is_fp32(g9, torch_dev, M):
     """FP32 activations keep their 24 bits: over 32 products of one sign the relative error is a few units of 2^-24, where
