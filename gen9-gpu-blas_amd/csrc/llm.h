@@ -47,6 +47,8 @@ G9_HIDDEN int need_device(const void *p, size_t bytes, const char *what);
 // Device scratch, grown on demand and kept; growing waits for queued work.
 enum Slot { SLOT_A = 0, SLOT_PART, SLOT_PLAN, SLOT_SLOTS, NSLOTS };
 G9_HIDDEN int scratch(int slot, size_t bytes, void **p);
+// The longest rows: kernels count k in an int, up to the end of the last 128-k chunk.
+constexpr int MAX_COLS = 0x7fffff80;
 inline int elem_size(int type) { return type == GEN9BLAS_S ? 4 : 2; }
 inline long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
 

@@ -172,6 +172,10 @@ gen9blas_mx4 *gen9blas_mx4_create(int count, int rows, int K) {
         fail(GEN9BLAS_ERR_INVALID_ARG, "mx4_create: count = %d, rows = %d, K = %d", count, rows, K);
         return nullptr;
     }
+    if (K > MAX_COLS) {
+        fail(GEN9BLAS_ERR_UNSUPPORTED, "mx4_create: K = %d, rows have at most %d values", K, MAX_COLS);
+        return nullptr;
+    }
     gen9blas_mx4 q;
     q.count = count, q.rows = rows, q.K = K;
     q.rt = (int)cdiv(rows, 16), q.kc = (int)cdiv(K, 128), q.kg = (int)cdiv(q.kc, 4), q.kt = (int)cdiv(q.kg, 16) * 16;

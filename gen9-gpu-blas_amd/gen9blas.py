@@ -968,12 +968,14 @@ def _device_rows(X, dims, shared=False):
     if X.dtype is not torch.float16 and X.dtype is not torch.float32:
         X = X.float()
     shape, step = X.shape, X.stride()
+    if X.numel() > _LONGEST and max(shape) > _LONGEST:
+        raise ValueError(f"dimensions {tuple(shape)} past {_LONGEST}")
     if step[-1] != 1 and shape[-1] > 1:
         return X.contiguous()
     if len(shape) > 1 and shape[-2] > 1:
         if step[-2] < shape[-1] and not (shared and len(shape) == 3 and step[1] == 0):
             return X.contiguous()
-        if step[-2] > _LONGEST_STEP and not shared:
+        if step[-2] > _LONGEST and not shared:
             return X.contiguous()
     return X
 
@@ -994,7 +996,7 @@ def _llm_out(C, shape, dtype, what="C"):
     return C
 
 
-_LONGEST_STEP = 0x7fffffff
+_LONGEST = 0x7fffffff   # the C entry points' int; ctypes would cut longer numbers
 
 
 def _row_step(X, dim=-2):
@@ -1005,8 +1007,8 @@ def _row_step(X, dim=-2):
 def _out_step(X, what="C"):
     """The same of a result whose row stride is a C int."""
     step = _row_step(X)
-    if step > _LONGEST_STEP:
-        raise ValueError(f"{what} has a row stride of {step} elements; the longest is {_LONGEST_STEP}")
+    if step > _LONGEST:
+        raise ValueError(f"{what} has a row stride of {step} elements; the longest is {_LONGEST}")
     return step
 
 
@@ -1020,6 +1022,8 @@ class MX4:
         self.shape = tuple(int(n) for n in shape)
         if len(self.shape) not in (2, 3):
             raise ValueError("MX4 matrices have a shape (rows, K) or (count, rows, K)")
+        if max(self.shape) > _LONGEST:
+            raise ValueError(f"dimensions {self.shape} past {_LONGEST}")
         self.count = self.shape[0] if len(self.shape) == 3 else 1
         self._handle = lib.gen9blas_mx4_create(self.count, *self.shape[-2:])
         if not self._handle:

@@ -29,7 +29,8 @@ GEN9BLAS_API int gen9blas_llm_last_status(void);
 // Rows of E2M1 values (±0, 0.5, 1, 1.5, 2, 3, 4, 6), each 32 consecutive values of a row sharing one E8M0 scale 2^(s−127),
 // s = 0..254 (255: every value of the block is NaN), as in the OCP Microscaling Formats specification (MXFP4).
 // `count` matrices of `rows` × K in one object (count > 1: the weights of `count` experts), in device memory that the
-// object owns, in the order in which the matrix cores take them. Limits: count, rows, K ≥ 1.
+// object owns, in the order in which the matrix cores take them. Limits: count, rows, K ≥ 1, K ≤ 2^31 − 128, and
+// count · ⌈rows/16⌉ · ⌈K/512⌉ < 2^24 (137 G values).
 typedef struct gen9blas_mx4 gen9blas_mx4;
 // A matrix (or `count` of them) of zeros.
 GEN9BLAS_API gen9blas_mx4 *gen9blas_mx4_create(int count, int rows, int K);

@@ -293,6 +293,32 @@ def test_row_strides_past_32_bits(g9, torch_dev):
     assert bool((a == y[:, 0]).all()) and bool((buf[64:128] == torch.arange(64, 128, device="cuda") / 16).all())
 
 
+def test_rows_of_two_billion(g9, torch_dev):
+    """The longest rows that a matrix has; longer ones are refused."""
+    torch = torch_dev
+    K = (1 << 31) - 128
+    L = g9._llm_library()
+    for k in (K + 1, K + 127):
+        assert L.gen9blas_mx4_create(1, 1, k) is None and L.gen9blas_llm_last_status() == -2
+    x = torch.zeros((1, K), dtype=torch.float16, device="cuda")
+    at, v = torch.tensor([0, 12345, K // 2 + 1, K - 1], device="cuda"), torch.tensor([2.0, -1.0, 0.5, 3.0], device="cuda")
+    x[0, at] = v.half()
+    q = g9.mx4_quantize(x)
+    d = g9.mx4_dequantize(q)
+    assert bool((d[0, at] == v).all()) and int(torch.count_nonzero(d)) == 4
+    del d
+    assert float(g9.mx4_gemm(x, q)) == float((v * v).sum())
+    del x, q
+    for shape in ((1, (1 << 32) + 5), ((1 << 32) + 1, 4), ((1 << 32) + 1, 2, 2)):    # not cut to their low 32 bits
+        with pytest.raises(ValueError):
+            g9.MX4(*shape)
+    tall = torch.empty(((1 << 31) + 1, 1), dtype=torch.float16, device="cuda")
+    with pytest.raises(ValueError):
+        g9.mx4_gemm(tall, g9.MX4(4, 1))
+    with pytest.raises(ValueError):
+        g9.moe_route(tall, 1)
+
+
 @pytest.mark.parametrize("M", [1, 16, 40, 70, 130, 300])
 def test_gemm_fp32_is_fp32(g9, torch_dev, M):
     """FP32 activations keep their 24 bits: over 32 products of one sign the relative error is a few units of 2^-24, where
