@@ -318,20 +318,32 @@ template <class T> static int launch_route(const RouteArgs &a) {
     return 0;
 }
 
+// The workgroups of a launch, or an error if their threads are more than it can index.
+static int grid_of(long long workgroups, int threads, dim3 *grid) {
+    if (workgroups * threads > 0xffffffffLL) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "moe_gemm: more tiles than one launch can index");
+    *grid = dim3((unsigned)workgroups);
+    return 0;
+}
+
 template <class T, class O, bool GATED> static int launch_grouped(const Rows &R, const Mx4View &W, const Mx4View &G, int E, int most, int rows, int Tn, long long n) {
+    dim3 grid;
     if (rows > 32) {
         Planes A;
-        G9_TRY(stage_planes<T>(R, Tn, W.K, W.kc, &A));
         const int ntiles = (int)cdiv(W.rt, GATED ? 8 : 16);
-        hipLaunchKernelGGL((mx4_gemm_tile_kernel<T, O, true, GATED>), dim3((unsigned)(cdiv((long long)most * ntiles, 8) * 8)), dim3(256), 0, stream, A, R, W, G, E, 0,
-                           ntiles);
+        G9_TRY(grid_of(cdiv((long long)most * ntiles, 8) * 8, 256, &grid));
+        G9_TRY(stage_planes<T>(R, Tn, W.K, W.kc, &A));
+        hipLaunchKernelGGL((mx4_gemm_tile_kernel<T, O, true, GATED>), grid, dim3(256), 0, stream, A, R, W, G, E, 0, ntiles);
         G9_HIP(hipGetLastError());
         return 0;
     }
     const Split whole = {1, nullptr, 0, 0};
     // few: 8 waves share the rows of a chunk, 128·NT columns a workgroup; rows: each wave has its own, 16·NT columns
-    auto few = [&](auto kernel, int cols) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(cdiv(most * cdiv(W.rt, cols), 8) * 8)), dim3(512), 0, stream, R, W, G, E, most, (int)cdiv(W.rt, cols), whole);
+    auto few = [&](auto kernel, int cols) -> int {
+        const int ntiles = (int)cdiv(W.rt, cols);
+        G9_TRY(grid_of(cdiv((long long)most * ntiles, 8) * 8, 512, &grid));
+        hipLaunchKernelGGL(kernel, grid, dim3(512), 0, stream, R, W, G, E, most, ntiles, whole);
+        G9_HIP(hipGetLastError());
+        return 0;
     };
     const bool many = std::min<long long>(n, E) * cdiv(W.rt, 16) >= 2LL * num_cus;   // workgroups of 256 columns
     if constexpr (sizeof(T) == 2) {
@@ -339,22 +351,18 @@ template <class T, class O, bool GATED> static int launch_grouped(const Rows &R,
             // FP16 128 × 4 places of 64 experts, 4096 × 1536, not gated: 51.0 µs; one column tile a wave 56.4. Gated, 1536 × 4096, 87.7
             // and 77.1; 64 × 4 places of 16 experts 44.3 and 29.5
             if constexpr (!GATED) {
-                if (many) few(mx4_gemm_few_kernel<T, O, 2, 2, 4, true, GATED>, 16);
+                if (many) return few(mx4_gemm_few_kernel<T, O, 2, 2, 4, true, GATED>, 16);
             }
-            if (GATED || !many) few(mx4_gemm_few_kernel<T, O, 2, 1, 4, true, GATED>, 8);
-            G9_HIP(hipGetLastError());
-            return 0;
+            return few(mx4_gemm_few_kernel<T, O, 2, 1, 4, true, GATED>, 8);
         }
     }
-    if (many)
-        // FP32 joined, 24 × 4 places of 64 experts, 4096 × 1536: 35.6 µs; one column tile a wave 41.3, the rows kernel 63
-        few(mx4_gemm_few_kernel<T, O, 1, 2, 4, true, GATED>, 16);
-    else if (std::min<long long>(n, E) * cdiv(W.rt, 8) < num_cus)
-        // FP16 gated, 8 places, 1536 × 4096: 13.6 µs; few kernel 20.6 and more. FP32 gated, 7 places, 864 × 3840: 14.2 µs, the few
-        // kernel, whose 49 workgroups leave most CUs idle, 24
-        hipLaunchKernelGGL((mx4_gemm_rows_kernel<T, O, 2, true, GATED>), dim3((unsigned)((long long)most * W.rt)), dim3(256), 0, stream, R, W, G, E, whole);
-    else
-        few(mx4_gemm_few_kernel<T, O, 1, 1, 4, true, GATED>, 8);
+    // FP32 joined, 24 × 4 places of 64 experts, 4096 × 1536: 35.6 µs; one column tile a wave 41.3, the rows kernel 63
+    if (many) return few(mx4_gemm_few_kernel<T, O, 1, 2, 4, true, GATED>, 16);
+    // FP16 gated, 8 places, 1536 × 4096: 13.6 µs; few kernel 20.6 and more. FP32 gated, 7 places, 864 × 3840: 14.2 µs, the few
+    // kernel, whose 49 workgroups leave most CUs idle, 24
+    if (std::min<long long>(n, E) * cdiv(W.rt, 8) >= num_cus) return few(mx4_gemm_few_kernel<T, O, 1, 1, 4, true, GATED>, 8);
+    G9_TRY(grid_of((long long)most * W.rt, 256, &grid));
+    hipLaunchKernelGGL((mx4_gemm_rows_kernel<T, O, 2, true, GATED>), grid, dim3(256), 0, stream, R, W, G, E, whole);
     G9_HIP(hipGetLastError());
     return 0;
 }
@@ -384,8 +392,7 @@ static int experts(int Tn, int S, const int *ids, const void *X, int64_t ldt, in
     // Few places: each workgroup finds its rows among the ids itself (8 places 17.5 µs a call with a plan, whose kernel comes first)
     const bool direct = n <= 64;
     const long long most = direct ? n : cdiv(n, rows) + E + 1;
-    if (most * W->rt > 0xffffff || n > 0x7fffffff)
-        G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "moe_gemm: more tiles than one launch can index");
+    if (n > 0x7fffffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "moe_gemm: T = %d tokens of S = %d places", Tn, S);
     void *plan = nullptr, *slots = nullptr;
     const long long ld = (N + 3) / 4 * 4LL;
     if (weights) G9_TRY(scratch(SLOT_SLOTS, (size_t)n * ld * 4, &slots));

@@ -352,6 +352,20 @@ def test_inputs_of_any_layout(g9, torch_dev):
     assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
 
 
+def test_experts_of_many_places_and_columns(g9, torch_dev):
+    """2^18 places of 65536 columns: offsets past 32 bits, and more tiles of 16 columns than a launch takes (it has wider ones)."""
+    torch = torch_dev
+    g = torch.Generator(device="cuda").manual_seed(1)
+    T, E, N, K = 1 << 18, 2, 1 << 16, 32
+    w = torch.randint(-2, 3, (E, N, K), generator=g, device="cuda").half()
+    x = torch.randint(-2, 3, (T, K), generator=g, device="cuda").half()
+    ids = torch.randint(0, E, (T, 1), generator=g, device="cuda", dtype=torch.int32)
+    y = g9.moe_gemm(x, ids, g9.mx4_quantize(w))
+    for e in range(E):
+        for t in torch.nonzero(ids[:, 0] == e)[:, 0].split(4096):
+            assert bool((y[t, 0] == x[t] @ w[e].t()).all())
+
+
 @pytest.mark.parametrize("T", [1, 5, 90])
 def test_experts_strides(g9, torch_dev, T):
     """Rows of X and C with strides of tokens and places, at odd alignments; nothing written beside C; NaN in one token's row
