@@ -1077,24 +1077,26 @@ def mx4_dequantize(Q, out=None):
 
 def mx4_gemm(A, W, C=None, dtype=None):
     """C = A·Wᵀ, W an MX4 matrix (N, K). A (M, K): float16 or float32, and C in the same type; or MX4, and C in `dtype`
-    (np.float16 by default, or the type of a given C)."""
+    (np.float16 by default, or the type of a given C). A dtype that is not the result's is refused with TypeError."""
     lib = _llm_library()
     torch = _torch
+    want = None if dtype is None else _torch_dtype(np.dtype(dtype))
     if isinstance(A, MX4):
         if len(A.shape) != 2 or len(W.shape) != 2 or A.shape[1] != W.shape[1]:
             raise ValueError(f"incompatible dimensions: {A.shape} · {W.shape}ᵀ")
-        if C is not None:
-            t = C.dtype
-        else:
-            t = _torch_dtype(np.dtype(np.float16 if dtype is None else dtype))
+        t = C.dtype if C is not None else want or torch.float16
         if t != torch.float16 and t != torch.float32:
             raise TypeError("C must be float16 or float32")
+        if want not in (None, t):
+            raise TypeError(f"C is of {t}, not of {want}")
         C = _llm_out(C, (A.shape[0], W.shape[0]), t)
         _llm_call(lib.gen9blas_mx4_gemm_q, 1 if t == torch.float32 else 0, A._handle, W._handle, C.data_ptr(), _out_step(C))
         return C
     a = _device_rows(A, (2,))
     if len(W.shape) != 2 or a.shape[1] != W.shape[1]:
         raise ValueError(f"incompatible dimensions: {tuple(a.shape)} · {W.shape}ᵀ")
+    if want not in (None, a.dtype):
+        raise TypeError(f"the result is of A's type, {a.dtype}, not of {want}")
     out = _llm_out(C, (a.shape[0], W.shape[0]), a.dtype)
     _llm_call(lib.gen9blas_mx4_gemm, 1 if a.dtype == torch.float32 else 0, a.shape[0], a.data_ptr(), _row_step(a), W._handle,
               out.data_ptr(), _out_step(out))

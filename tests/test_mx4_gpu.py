@@ -319,6 +319,21 @@ def test_rows_of_two_billion(g9, torch_dev):
         g9.moe_route(tall, 1)
 
 
+def test_dtype_that_contradicts_is_refused(g9, torch_dev):
+    """dtype chooses the result's type of two MX4 operands; where it is given already, another dtype is not ignored."""
+    torch = torch_dev
+    a = torch.ones((4, 64), dtype=torch.float16, device="cuda")
+    W = g9.mx4_quantize(torch.ones((8, 64), device="cuda"))
+    q = g9.mx4_quantize(a)
+    assert g9.mx4_gemm(a, W, dtype=np.float16).dtype == torch.float16
+    C = torch.empty((4, 8), device="cuda")
+    assert g9.mx4_gemm(q, W, C=C, dtype=np.float32) is C
+    with pytest.raises(TypeError):
+        g9.mx4_gemm(a, W, dtype=np.float32)
+    with pytest.raises(TypeError):
+        g9.mx4_gemm(q, W, C=C, dtype=np.float16)
+
+
 @pytest.mark.parametrize("M", [1, 16, 40, 70, 130, 300])
 def test_gemm_fp32_is_fp32(g9, torch_dev, M):
     """FP32 activations keep their 24 bits: over 32 products of one sign the relative error is a few units of 2^-24, where
