@@ -366,6 +366,22 @@ def test_experts_of_many_places_and_columns(g9, torch_dev):
             assert bool((y[t, 0] == x[t] @ w[e].t()).all())
 
 
+@pytest.mark.parametrize("step", [256, 260, 262, 263])
+def test_experts_rows_in_place(g9, torch_dev, step):
+    """More than 40 places an expert, whole 128-k chunks of FP16: rows that the tile kernel copies to LDS from where they lie, at any
+    multiple of four bytes, and those that go by way of the work space."""
+    torch = torch_dev
+    r = np.random.default_rng(step)
+    T, S, E, N, K = 100, 2, 3, 300, 256
+    W, w = weights(r, torch, g9, E, N, K)
+    ids = np.argsort(r.random((T, E)), 1)[:, :S].astype(np.int32)
+    flat = gpu(torch, r.standard_normal(T * (S + 1) * step + 8).astype(np.float16))
+    for off in (0, 1, 2, 4, 6):
+        for x in (flat.as_strided((T, K), (step, 1), off), flat.as_strided((T, 1, K), (step, step, 1), off).expand(T, S, K),
+                  flat.as_strided((T, S, K), (S * step, step, 1), off), flat.as_strided((T, S, K), ((S + 1) * step, step, 1), off)):
+            check_experts(torch, g9.moe_gemm(x, gpu(torch, ids), W), *experts64(x.cpu().numpy(), ids, w))
+
+
 @pytest.mark.parametrize("T", [1, 5, 90])
 def test_experts_strides(g9, torch_dev, T):
     """Rows of X and C with strides of tokens and places, at odd alignments; nothing written beside C; NaN in one token's row

@@ -226,6 +226,21 @@ def test_gemm_large_strides_and_nan(g9, torch_dev, dtype, M, N, K):
     assert bool(got[5].isnan().all()) and not bool(got[M - 2].isfinite().any())
 
 
+@pytest.mark.parametrize("step", [256, 260, 262, 263])
+def test_gemm_large_rows_in_place(g9, torch_dev, step):
+    """Whole 128-k chunks of FP16 rows for the tile kernel, which copies them to LDS from where they lie if all rows begin at multiples of
+    four bytes, of any sixteen; from odd elements, and at odd strides, by way of the work space."""
+    torch = torch_dev
+    M, N, K = 1000, 4400, 256
+    g = torch.Generator(device="cuda").manual_seed(step)
+    W = g9.mx4_quantize(torch.randn((N, K), generator=g, device="cuda") / 8)
+    w = g9.mx4_dequantize(W).double()
+    flat = torch.randn(M * step + 8, generator=g, device="cuda").half()
+    for off in (0, 1, 2, 4, 6):
+        a = flat.as_strided((M, K), (step, 1), off)
+        check_large(torch, g9.mx4_gemm(a, W), a.double(), w, torch.float16)
+
+
 @pytest.mark.parametrize("dtype", [np.float16, np.float32])
 @pytest.mark.parametrize("M", [1, 7, 33, 90, 260])
 def test_gemm_strides(g9, torch_dev, dtype, M):
