@@ -59,8 +59,8 @@ struct Mx4View {
 };
 inline Mx4View view(const gen9blas_mx4 *q) { return {q->codes, q->scales, q->top, q->rows, q->K, q->rt, q->kc, q->kg, q->kt}; }
 
-// A product whose k is split among `parts` workgroups: each leaves its FP32 sums in a plane of rows × ld (gated: two, W's and
-// the gate's), and a second kernel adds the planes in their order.
+// A dense product whose k is split among `parts` workgroups: each leaves its FP32 sums in a plane of rows × ld, and a second kernel
+// adds the planes in their order. (The experts' have enough workgroups: parts = 1.)
 struct Split {
     int parts;
     float *sums;

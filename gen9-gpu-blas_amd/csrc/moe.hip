@@ -388,9 +388,9 @@ static int experts(int Tn, int S, const int *ids, const void *X, int64_t ldt, in
     // of 32 rows LDS passes no faster than 16 twice: gated 32 208, 216 and 268, 64 364, 308 and 338; not gated 48 173, 185 and 181, 64 219,
     // 215 and 206.
     constexpr bool F = sizeof(T) == 4;
-    const int rows = n > 64 && n > (F ? 56LL : 40LL) * E ? 64 : !F && n >= 7LL * E ? 32 : 16;
+    const int rows = n > FEW_PLACES && n > (F ? 56LL : 40LL) * E ? 64 : !F && n >= 7LL * E ? 32 : 16;
     // Few places: each workgroup finds its rows among the ids itself (8 places 17.5 µs a call with a plan, whose kernel comes first)
-    const bool direct = n <= 64;
+    const bool direct = n <= FEW_PLACES;
     const long long most = direct ? n : cdiv(n, rows) + E + 1;
     if (n > 0x7fffffff) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "moe_gemm: T = %d tokens of S = %d places", Tn, S);
     void *plan = nullptr, *slots = nullptr;

@@ -4,9 +4,10 @@
 
 namespace g9llm {
 
-// The rows of a tile, to `slots` in LDS: of the plan's tile t, or (ids: few places, no plan) of place t's expert, if t is the first,
-// 17th (ROWS + 1st), ... place with that expert; count 0 otherwise. e = experts: places without one. All threads of a workgroup
-// call it; a wave finds the places 64 at a time.
+// The rows of a tile, to `slots` in LDS: of the plan's tile t, or (ids: at most FEW_PLACES places, no plan) of place t's expert, if t is
+// the first, 17th (ROWS + 1st), ... place with that expert; count 0 otherwise. e = experts: places without one. All threads of a
+// workgroup call it.
+constexpr int FEW_PLACES = 64;   // a place a lane
 struct TileRows {
     int e, first, count;
 };
@@ -17,24 +18,14 @@ template <int ROWS> __device__ __forceinline__ TileRows tile_rows(const Rows &R,
         o.count = min(ROWS, R.off[o.e + 1] - o.first);
         if ((int)threadIdx.x < o.count) slots[threadIdx.x] = R.order[o.first + threadIdx.x];
     } else {
-        const int lane = threadIdx.x & 63, n = R.M;
-        auto expert = [&](int i) { return i < n ? (int)min((unsigned)R.ids[i], (unsigned)experts) : -1; };   // ids outside 0..E−1: E
-        o.e = expert(t), o.first = 0;
-        int before = 0, all = 0;
-        for (int c = 0; c < n; c += 64) {
-            const unsigned long long mask = __ballot(expert(c + lane) == o.e);
-            all += __builtin_popcountll(mask);
-            if (c <= t) before += __builtin_popcountll(t - c < 64 ? mask & ((1ull << (t - c)) - 1) : mask);
-        }
-        o.count = before % ROWS ? 0 : min(ROWS, all - before);
-        int rank = -before;
-        for (int c = 0; o.count && c < n; c += 64) {
-            const bool mine = expert(c + lane) == o.e;
-            const unsigned long long mask = __ballot(mine);
-            const int at = rank + __builtin_popcountll(mask & ((1ull << lane) - 1));
-            if (threadIdx.x < 64 && mine && at >= 0 && at < o.count) slots[at] = c + lane;
-            rank += __builtin_popcountll(mask);
-        }
+        const int lane = threadIdx.x & 63;
+        const int expert = lane < R.M ? (int)min((unsigned)R.ids[lane], (unsigned)experts) : -1;   // ids outside 0..E−1: E
+        o.e = __builtin_amdgcn_readlane(expert, t), o.first = 0;
+        const unsigned long long mask = __ballot(expert == o.e);
+        const int before = __builtin_popcountll(mask & ((1ull << t) - 1));
+        o.count = before % ROWS ? 0 : min(ROWS, __builtin_popcountll(mask) - before);
+        const int at = __builtin_popcountll(mask & ((1ull << lane) - 1)) - before;
+        if (threadIdx.x < 64 && expert == o.e && at >= 0 && at < o.count) slots[at] = lane;
     }
     __syncthreads();
     return o;
@@ -112,7 +103,7 @@ template <> struct Row32<float> {
     }
 };
 
-// The end of a row's four columns col .. col + 3 (y: the sum with W, z: with the gate): to C, or as a part's sums.
+// The end of a row's four columns col .. col + 3 (y: the sum with W, z: with the gate): to C, or (dense) as a part's sums.
 template <class T, class O, bool GROUPED, bool GATED>
 __device__ __forceinline__ void finish4(const Rows &R, const Mx4View &W, const Split &split, int part, int first, const int *slots, int i, int col, f32x4 y, f32x4 z,
                                         const int *ty, const int *tz) {
@@ -121,11 +112,9 @@ __device__ __forceinline__ void finish4(const Rows &R, const Mx4View &W, const S
         y[j] = Act<T>::finish(y[j], ty[j]);
         if (GATED) z[j] = Act<T>::finish(z[j], tz[j]);
     }
-    if (split.parts > 1) {
+    if (!GROUPED && split.parts > 1) {
         if (col >= W.rows) return;   // ld is whole column tiles
-        float *p = split.sums + ((long long)part * (GATED ? 2 : 1) * split.rows + first + i) * split.ld + col;
-        *reinterpret_cast<f32x4 *>(p) = y;
-        if (GATED) *reinterpret_cast<f32x4 *>(p + split.rows * split.ld) = z;
+        *reinterpret_cast<f32x4 *>(split.sums + ((long long)part * split.rows + first + i) * split.ld + col) = y;
         return;
     }
     O *c;
