@@ -116,11 +116,19 @@ template <class T> static int launch_tiles(const Rows &R, const Mx4View &W) {
 
 template <class T> static int launch_dense(const Rows &R, const Mx4View &W) {
     constexpr bool F = sizeof(T) == 4;
-    // µs of the product alone, FP16 1 × 11008 × 4096 and FP32 8 × 4096 × 11008: rows kernel 9.4 and 13.2, few kernel 8.8 to
-    // 9.5 and 10.7: FP32 rows are taken apart once a workgroup there, and once a wave in the rows kernel.
     if (R.M <= 16) {
+        // FP32 rows are taken apart once a workgroup in the few kernel, once a wave in the rows kernel: 8 × 4096 × 11008 10.7 µs and 13.2
         if constexpr (F) return launch_few<T, 1, 2, 4>(R, W);
-        else return launch_rows<T>(R, W);
+        // FP16: each 16 columns of the rows kernel read all rows again, from L2; the few kernel, eight times as wide, splits k where it has
+        // fewer workgroups than CUs, and a second launch adds the parts. µs a call, rows kernel and few kernel: 1 × 11008 × 4096
+        // 9.2 and 10.7, 8 × 11008 × 4096 (`again`, the elements read, 23 M) 11.1 and 11.1, 16 × 4096 × 8192 (34 M) 11.0 and 10.4,
+        // 16 × 11008 × 4096 (45 M) 15.2 and 11.6. Where the rows kernel splits k too: 4 × 2048 × 8192 (4 M) 7.9 and 8.3, 8 × 2048 × 8192
+        // (8 M) 8.5 and 8.3, 16 × 2048 × 8192 (17 M) 10.2 and 8.6. Where the few kernel need not: 1 × 16384 × 4096 (split) 11.5 and 11.9,
+        // 1 × 17000 × 4096 (whole) 13.0 and 12.0, 16 × 22016 × 4096 27.0 and 12.6.
+        const long long again = (long long)W.rt * W.K * R.M;
+        const bool few_whole = cdiv(W.rt, 8) * 2 > num_cus, rows_whole = W.rt * 2 > num_cus;
+        if (!few_whole && again <= (rows_whole ? 26000000 : 8000000)) return launch_rows<T>(R, W);
+        return launch_few<T, 1, 1, 4>(R, W);
     }
     // 128 columns a workgroup; with 256, which reads the rows from LDS half as often but leaves twice the parts to be summed or half
     // the workgroups: FP32 24 × 4096 × 11008 19.6 µs and 20.0, 24 × 11008 × 4096 21.6 and 20.5, 28 × 2048 × 2048 9.5 and 11.9

@@ -176,6 +176,22 @@ def test_gemm_large(g9, torch_dev, M, N, K):
         check_large(torch, g9.mx4_gemm(a, W), a.double(), w, t)
 
 
+@pytest.mark.parametrize("M,N,K", [(16, 8192, 4096), (16, 2048, 8192), (9, 2050, 8200), (1, 16400, 200), (5, 17003, 129), (16, 22016, 96)])
+def test_gemm_few_rows_large(g9, torch_dev, M, N, K):
+    """Up to 16 rows of products that read much, or whose columns fill the GPU without a split of k: 128 columns a workgroup."""
+    torch = torch_dev
+    g = torch.Generator(device="cuda").manual_seed(N)
+    W = g9.mx4_quantize(torch.randn((N, K), generator=g, device="cuda") / 8)
+    w = g9.mx4_dequantize(W).double()
+    for t in (torch.float16, torch.float32):
+        big = torch.randn((M, K + 3), generator=g, device="cuda").to(t)
+        for a in (big[:, :K], big[:, 1:K + 1]):
+            out = torch.full((M, N + 5), 3.0, dtype=t, device="cuda")
+            g9.mx4_gemm(a, W, C=out[:, 2:N + 2])
+            check_large(torch, out[:, 2:N + 2], a.double(), w, t)
+            assert bool((out[:, :2] == 3.0).all()) and bool((out[:, N + 2:] == 3.0).all())
+
+
 @pytest.mark.parametrize("K", [96, 200, 384, 512, 640, 1100, 1536])
 def test_gemm_quantized_middle(g9, torch_dev, K):
     """More tiles of 16 × 16 than eight a CU, too few of 256 × 256."""
