@@ -959,25 +959,28 @@ def _on_gpu(X):
 
 def _device_rows(X, dims, shared=False):
     """X as a GPU tensor of float16 or float32, of one of the numbers of dimensions in `dims`, whose rows are contiguous and do not
-    overlap, with a row stride that is a C int; X in another layout is copied. shared (the rows of experts' products): one row
+    overlap, and its row stride, which is a C int; X in another layout is copied. shared (the rows of experts' products): one row
     for all places of a token (a stride of 0) is taken too, and strides of any length are."""
     torch = _torch
-    X = _on_gpu(X)
-    if X.dim() not in dims:
-        raise ValueError(f"expected {' or '.join(map(str, dims))} dimensions, got {X.dim()}")
+    if not (isinstance(X, torch.Tensor) and X.is_cuda):
+        X = _on_gpu(X)
     if X.dtype is not torch.float16 and X.dtype is not torch.float32:
         X = X.float()
     shape, step = X.shape, X.stride()
-    if X.numel() > _LONGEST and max(shape) > _LONGEST:
+    n = len(shape)
+    if n not in dims:
+        raise ValueError(f"expected {' or '.join(map(str, dims))} dimensions, got {n}")
+    K = shape[-1]
+    if shape[0] > _LONGEST or K > _LONGEST:
         raise ValueError(f"dimensions {tuple(shape)} past {_LONGEST}")
-    if step[-1] != 1 and shape[-1] > 1:
-        return X.contiguous()
-    if len(shape) > 1 and shape[-2] > 1:
-        if step[-2] < shape[-1] and not (shared and len(shape) == 3 and step[1] == 0):
-            return X.contiguous()
-        if step[-2] > _LONGEST and not shared:
-            return X.contiguous()
-    return X
+    if step[-1] != 1 and K > 1:
+        return X.contiguous(), K
+    if n == 1 or shape[-2] <= 1:   # a dimension of one has any stride
+        return X, K or 1
+    ld = step[-2]
+    if (ld < K and not (shared and n == 3 and ld == 0)) or (ld > _LONGEST and not shared):
+        return X.contiguous(), K
+    return X, ld
 
 
 def _host_like(X, result):
@@ -999,9 +1002,10 @@ def _llm_out(C, shape, dtype, what="C"):
 _LONGEST = 0x7fffffff   # the C entry points' int; ctypes would cut longer numbers
 
 
-def _row_step(X, dim=-2):
+def _row_step(X):
     """Stride between rows, at least the row's length (a dimension of one has any stride)."""
-    return X.stride(dim) if X.shape[dim] > 1 else max(X.shape[-1], 1)
+    shape = X.shape
+    return X.stride(-2) if shape[-2] > 1 else max(shape[-1], 1)
 
 
 def _out_step(X, what="C"):
@@ -1039,12 +1043,12 @@ def mx4_quantize(X, out=None):
     """X, (rows, K) or (count, rows, K), rounded to MX4 (a new one, or `out` of the same shape). A block's scale is
     2^(floor(log2 max|x|) - 2); values round to the nearest, ties to even codes, beyond 6 scales to 6."""
     lib = _llm_library()
-    X = _device_rows(X, (2, 3))
+    X, ld = _device_rows(X, (2, 3))
     if out is None:
         out = MX4(*X.shape)
     elif out.shape != tuple(X.shape):
         raise ValueError(f"X has shape {tuple(X.shape)}, the MX4 matrix {out.shape}")
-    _llm_call(lib.gen9blas_mx4_quantize, 1 if X.dtype == _torch.float32 else 0, X.data_ptr(), _row_step(X),
+    _llm_call(lib.gen9blas_mx4_quantize, 1 if X.dtype == _torch.float32 else 0, X.data_ptr(), ld,
               X.stride(0) if X.dim() == 3 else 0, out._handle)
     return out
 
@@ -1071,7 +1075,7 @@ def mx4_dequantize(Q, out=None):
     """The values of an MX4 matrix in float32."""
     lib = _llm_library()
     X = _llm_out(out, Q.shape, _torch.float32, "out")
-    _llm_call(lib.gen9blas_mx4_dequantize, Q._handle, X.data_ptr(), _out_step(X, "out"), X.stride(0) if X.dim() == 3 else 0)
+    _llm_call(lib.gen9blas_mx4_dequantize, Q._handle, X.data_ptr(), Q.shape[-1] if out is None else _out_step(X, "out"), X.stride(0) if X.dim() == 3 else 0)
     return X
 
 
@@ -1092,14 +1096,16 @@ def mx4_gemm(A, W, C=None, dtype=None):
         C = _llm_out(C, (A.shape[0], W.shape[0]), t)
         _llm_call(lib.gen9blas_mx4_gemm_q, 1 if t == torch.float32 else 0, A._handle, W._handle, C.data_ptr(), _out_step(C))
         return C
-    a = _device_rows(A, (2,))
-    if len(W.shape) != 2 or a.shape[1] != W.shape[1]:
+    a, lda = _device_rows(A, (2,))
+    (M, K), t = a.shape, a.dtype
+    if len(W.shape) != 2 or K != W.shape[1]:
         raise ValueError(f"incompatible dimensions: {tuple(a.shape)} · {W.shape}ᵀ")
-    if want not in (None, a.dtype):
-        raise TypeError(f"the result is of A's type, {a.dtype}, not of {want}")
-    out = _llm_out(C, (a.shape[0], W.shape[0]), a.dtype)
-    _llm_call(lib.gen9blas_mx4_gemm, 1 if a.dtype == torch.float32 else 0, a.shape[0], a.data_ptr(), _row_step(a), W._handle,
-              out.data_ptr(), _out_step(out))
+    if want not in (None, t):
+        raise TypeError(f"the result is of A's type, {t}, not of {want}")
+    N = W.shape[0]
+    out = _llm_out(C, (M, N), t)
+    _llm_call(lib.gen9blas_mx4_gemm, 1 if t is torch.float32 else 0, M, a.data_ptr(), lda, W._handle, out.data_ptr(),
+              N if C is None else _out_step(out))
     return _host_like(A, out) if C is None else out
 
 
@@ -1113,49 +1119,55 @@ def moe_route(logits, k, bias=None, score="softmax", groups=1, top_groups=1, ren
     chosen; places left over get id -1 and weight 0. `out`: (ids, weights) to write into."""
     lib = _llm_library()
     torch = _torch
-    x = _device_rows(logits, (2,))
+    x, ldl = _device_rows(logits, (2,))
     T, E = x.shape
     if bias is not None:
-        bias = _device_rows(bias, (1,)).float().contiguous()
+        bias = _device_rows(bias, (1,))[0].float().contiguous()
         if bias.shape[0] != E:
             raise ValueError(f"bias has {bias.shape[0]} elements for {E} experts")
     ids = _llm_out(out[0] if out else None, (T, k), torch.int32, "ids")
     w = _llm_out(out[1] if out else None, (T, k), torch.float32, "weights")
-    if not (ids.is_contiguous() and w.is_contiguous()):
+    if out and not (ids.is_contiguous() and w.is_contiguous()):
         raise ValueError("ids and weights must be contiguous")
-    _llm_call(lib.gen9blas_moe_route, 1 if x.dtype == torch.float32 else 0, T, E, x.data_ptr(), _row_step(x),
+    _llm_call(lib.gen9blas_moe_route, 1 if x.dtype == torch.float32 else 0, T, E, x.data_ptr(), ldl,
               None if bias is None else bias.data_ptr(), _SCORE_CODE[score], groups, top_groups, k, bool(renorm), scale,
               ids.data_ptr(), w.data_ptr())
     return (ids, w) if out else (_host_like(logits, ids), _host_like(logits, w))
 
 
 def moe_gemm(X, ids, W, gate=None, weights=None, C=None):
-    """The products of each token's rows with its experts' weights: W an MX4 stack (experts, N, K), ids (T, S) int32.
+    """The products of each token's rows with its experts' weights: W an MX4 stack (experts, N, K), ids (T, S) integers.
     X (T, K): one row for all places of a token, or (T, S, K). y[t, s] = X[t(, s)]·W[ids[t, s]]ᵀ, and with `gate` (as W)
     silu(X[t(, s)]·gate[ids[t, s]]ᵀ)·y[t, s]. The result is y (T, S, N), or with weights (T, S) float32 the sum over s of
     weights[t, s]·y[t, s] (T, N). An id that is no expert's (-1) is an empty place, its y is zero."""
     lib = _llm_library()
     torch = _torch
-    x, i = _device_rows(X, (2, 3), shared=True), _on_gpu(ids)
+    x, lds = _device_rows(X, (2, 3), shared=True)
+    i = ids if isinstance(ids, torch.Tensor) and ids.is_cuda else _on_gpu(ids)
     if i.dtype is not torch.int32:
-        i = i.to(torch.int64).clamp(-1, 0x7fffffff).to(torch.int32)   # past 32 bits: no expert's
-    i = i.contiguous()
-    if i.dim() != 2 or len(W.shape) != 3 or x.shape[-1] != W.shape[2] or x.shape[0] != i.shape[0] or \
-            (x.dim() == 3 and x.shape[1] != i.shape[1]) or (gate is not None and gate.shape != W.shape):
-        raise ValueError(f"incompatible shapes: X {tuple(x.shape)}, ids {tuple(i.shape)}, W {W.shape}"
+        i = i.to(torch.int64).clamp(-1, _LONGEST).to(torch.int32)   # past 32 bits: no expert's
+    if not i.is_contiguous():
+        i = i.contiguous()
+    shape = x.shape
+    if i.dim() != 2 or len(W.shape) != 3 or shape[-1] != W.shape[2] or shape[0] != i.shape[0] or \
+            (len(shape) == 3 and shape[1] != i.shape[1]) or (gate is not None and gate.shape != W.shape):
+        raise ValueError(f"incompatible shapes: X {tuple(shape)}, ids {tuple(i.shape)}, W {W.shape}"
                          + (f", gate {gate.shape}" if gate is not None else ""))
     (T, S), N = i.shape, W.shape[1]
     if weights is not None:
-        weights = _device_rows(weights, (2,)).float().contiguous()
+        weights = _device_rows(weights, (2,))[0].float().contiguous()
         if weights.shape != i.shape:
             raise ValueError(f"weights {tuple(weights.shape)} for ids {tuple(i.shape)}")
     out = _llm_out(C, (T, N) if weights is not None else (T, S, N), x.dtype)
-    lds = 0 if x.dim() == 2 else _row_step(x, 1)
-    if T > 1 and x.stride(0) < max(S - 1, 0) * lds + x.shape[-1]:   # tokens share rows, or lie within each other's
+    K = shape[-1]
+    if len(shape) == 2:
+        lds = 0
+    ldt = x.stride(0) if T > 1 else max(lds * S, K)
+    if ldt < (S - 1) * lds + K:   # tokens share rows, or lie within each other's
         x = x.contiguous()
-        lds = 0 if x.dim() == 2 else x.shape[-1]
-    ldt = x.stride(0) if T > 1 else max(lds * S, x.shape[-1])
-    ldcs = N if weights is not None else _row_step(out, 1)
+        lds = 0 if len(shape) == 2 else K
+        ldt = x.stride(0)
+    ldcs = N if weights is not None else _row_step(out)
     ldct = out.stride(0) if T > 1 else ldcs * max(S, 1)
     _llm_call(lib.gen9blas_moe_gemm, 1 if x.dtype == torch.float32 else 0, T, S, i.data_ptr(), x.data_ptr(), ldt, lds, W._handle,
               None if gate is None else gate._handle, None if weights is None else weights.data_ptr() or out.data_ptr(),   # empty: no address
