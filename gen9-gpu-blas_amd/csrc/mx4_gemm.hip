@@ -55,8 +55,8 @@ template <class O> static int launch_q(const Mx4View &A, const Mx4View &W, O *C,
     // µs with the quantisation of A's rows: few kernel 100 × 4096 × 4096 11.3 and 100 × 4096 × 11008 17.5, ring kernel 12.8 and 21.8;
     // 64 × 11008 × 4096 and 200 × 4096 × 4096 15.1 and 15.8, ring kernel 13.0 and 13.2
     if ((long long)A.rt * W.rt <= 8 * num_cus) return run(mx4_gemm_q_few_kernel<O>, 1, 1);
-    // ring kernel 2000 × 6000 × 4096 (192 tiles of 256 × 256) 37.8, tile kernel 40.4; 2300 × 6100 × 4096 (216) 45.2 and 43.4,
-    // 3000 × 5000 × 4096 (240) 50.3 and 42.7
+    // ring kernel 2000 × 6000 × 4096 (192 tiles of 256 × 256) 38.5, tile kernel 39.3; 2300 × 6100 × 4096 (216) 45.7 and 42.8,
+    // 3000 × 5000 × 4096 (240) 50.3 and 42.6
     if (cdiv(A.rt, 16) * cdiv(W.rt, 16) * 5 < 4 * num_cus) return run(mx4_gemm_q_ring_kernel<O>, 8, 8);
     return run(mx4_gemm_q_tile_kernel<O>, 16, 16);
 }
@@ -131,7 +131,8 @@ template <class T> static int launch_dense(const Rows &R, const Mx4View &W) {
         return launch_few<T, 1, 1, 4>(R, W);
     }
     // 128 columns a workgroup; with 256, which reads the rows from LDS half as often but leaves twice the parts to be summed or half
-    // the workgroups: FP32 24 × 4096 × 11008 19.6 µs and 20.0, 24 × 11008 × 4096 21.6 and 20.5, 28 × 2048 × 2048 9.5 and 11.9
+    // the workgroups, µs a call: FP32 24 × 4096 × 11008 17.8 and 19.0, 24 × 11008 × 4096 20.2 and 19.1, 28 × 2048 × 2048 9.5 and 11.8; FP16
+    // 24 × 4096 × 11008 13.0 and 15.1, 24 × 11008 × 4096 12.5 and 14.2
     if (R.M <= 32) return launch_few<T, 2, 1, 4>(R, W);
     // 64 rows: 128 columns, 256 columns, or the tile kernel, which has 64 × 256 too but fills the GPU with 768 workgroups, not 256.
     // FP16 512 × 4096 × 4096 (256 workgroups of 128 columns) 24.8, 29.1 and 33.1 µs, 1000 × 4096 × 4096 (512) 42.7, 37.1 and 40.5,

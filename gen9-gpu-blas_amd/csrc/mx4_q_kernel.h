@@ -10,9 +10,9 @@ __device__ __forceinline__ i32x8 fp4_operand(u32x4 v) { return i32x8{(int)v[0], 
 
 // A workgroup of 2 × 2 waves makes 256 rows × 256 columns, each wave 128 × 128 (T = 8 row tiles), with v_mfma_scale_f32_32x32x64 (37 clocks in
 // a loop of one wave a SIMD, where 16x16x128 takes 29 for half the products): lane l holds row l % 32 of two row tiles and block
-// 2u + l / 32 of a stage's 128 k, u = 0, 1. 32 instructions a stage and wave leave LDS and the path from L2 about 1100 clocks,
-// and either passes 57 to 64 bytes a clock and CU. So A, which two waves share in turn, goes through LDS, its tiles as they
-// lie (16 KiB in, 32 KiB read), and W goes from L2 to registers (32 KiB).
+// 2u + l / 32 of a stage's 128 k, u = 0, 1. 32 instructions a stage and wave leave the path from L2 about 1100 clocks, and
+// it passes 57 to 64 bytes a clock and CU. So A, which two waves share in turn, goes through LDS, its tiles as they lie (16 KiB in,
+// 32 KiB read), and W goes from L2 to registers (32 KiB). 4096 × 11008 × 4096: 98 to 101 µs, matrix cores 56 % busy.
 // Four stages of A are on the ring: while stage s is multiplied, its fragments for s + 1 are read and s + 2 to s + 4 are on their
 // way (s + 4 into the place of s, whose fragments every wave has by then). A fragment of W is loaded as soon as its registers are
 // free, a stage or more ahead. The scales of 512 k (a word per lane and row tile) come with every fourth stage, A's through

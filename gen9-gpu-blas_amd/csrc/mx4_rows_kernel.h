@@ -290,8 +290,9 @@ __device__ __forceinline__ void lds_barrier() {
 // 8 waves side by side in n, each 16·NT columns (gated: of W and of the gate) of MT·16 rows. The rows of each 128 k are taken
 // apart once for the whole workgroup, into FP16 or BF16 planes in LDS (two buffers). A thread loads U elements at a time. Weights and rows of the next D
 // chunks are on their way in registers; both, as loads return in order and the wait for the nearest rows would be a wait for
-// all older weights too. FP32 24 × 4096 × 11008 in 8 parts of k: 16 µs for 24 MB of weights, a chain of a split, a barrier and LDS reads for each
-// of 11 chunks; 4 waves of 64 columns, two workgroups a CU, which read LDS half as often, took 18 to 20.
+// all older weights too. FP32 24 × 4096 × 11008 in 8 parts of k: 15 to 16.5 µs for 24 MB of weights, 11 chunks of
+// 1.4 µs. Of these the matrix cores are busy 0.3; each wave reads all rows in three planes for its 16 columns, 192 KiB a chunk, 0.6 µs at
+// the 320 bytes a ns that eight waves read at if they do nothing else; the rest is the chain of split, barrier and first reads. 4 waves of 64 columns, two workgroups a CU, which read LDS half as often, took 18 to 20.
 template <class T, class O, int MT, int NT, int D, bool GROUPED, bool GATED>
 __global__ void __launch_bounds__(512, 2) mx4_gemm_few_kernel(Rows R, Mx4View W, Mx4View G, int experts, int mtiles, int ntiles, Split split) {
     typedef Act<T> X;

@@ -46,8 +46,9 @@ GEN9BLAS_API int gen9blas_mx4_quantize(int type, const void *X, int ldx, int64_t
 GEN9BLAS_API int gen9blas_mx4_load(const uint8_t *codes, int ldc, const uint8_t *scales, int lds, gen9blas_mx4 *Q);
 // X = the values of Q, in FP32 (exact but for values past 2^128, which are infinite there).
 GEN9BLAS_API int gen9blas_mx4_dequantize(const gen9blas_mx4 *Q, float *X, int ldx, int64_t sX);
-// C (M×N) = A (M×K, FP16 or FP32) · Wᵀ, W (N×K) a single MX4 matrix. The products are exact; FP16: terms of a row of W
-// more than 2^36 below its largest scale may be rounded. C in the type of A.
+// C (M×N) = A (M×K, FP16 or FP32) · Wᵀ, W (N×K) a single MX4 matrix. The products are exact, but for: FP16, terms of a row
+// of W more than 2^36 below its largest scale may be rounded; FP32, elements of A below 2^−110 lose the bits below 2^−133,
+// products are FP32 numbers (nothing below 2^−149), and a value of W past 2^128 is infinite. C in the type of A.
 GEN9BLAS_API int gen9blas_mx4_gemm(int type, int M, const void *A, int lda, const gen9blas_mx4 *W, void *C, int ldc);
 // C (M×N, FP16 or FP32 as `type` says) = A · Wᵀ, both MX4 (M×K, N×K): products on the 4-bit matrix cores.
 GEN9BLAS_API int gen9blas_mx4_gemm_q(int type, const gen9blas_mx4 *A, const gen9blas_mx4 *W, void *C, int ldc);
@@ -63,14 +64,15 @@ enum { GEN9BLAS_SOFTMAX = 0, GEN9BLAS_SIGMOID = 1 };
 //   experts are chosen; a group counts as the sum of its two largest choices (sigmoid) or its largest one (softmax).
 // - weights: the chosen experts' scores (without bias), divided by their sum if renorm, times scale.
 // - A logit of −inf is an expert that is masked: never chosen. Places that are left over get id −1 and weight 0. A NaN
-//   logit is not chosen either, and makes the row's weights NaN. Scores whose sum is 0 renormalise to weights 0.
+//   logit is not chosen either, and makes the row's weights NaN (softmax with a bias: all scores of the row are NaN, so all
+//   its ids are −1). Scores whose sum is 0 renormalise to weights 0.
 // ids and weights are T×k, dense.
 GEN9BLAS_API int gen9blas_moe_route(int type, int T, int E, const void *logits, int ldl, const float *bias, int score,
                                     int groups, int top_groups, int k, int renorm, float scale, int *ids, float *weights);
 // The products of each token's rows with its experts' weights. ids: T×S, dense; W: E = count matrices N×K (E <= 1024).
 // The row of token t, place s is X + t·ldt + s·lds (lds = 0: one row for all places of a token); y(t, s) = row · W[ids(t, s)]ᵀ.
 // - gate != NULL (as W): y(t, s) = silu(row · gate[ids(t, s)]ᵀ) · (row · W[ids(t, s)]ᵀ), silu(z) = z / (1 + e^−z).
-// - weights == NULL: C(t, s) = y(t, s) at C + t·ldct + s·ldcs (ldcs >= N, ldct >= S·ldcs).
+// - weights == NULL: C(t, s) = y(t, s) at C + t·ldct + s·ldcs (ldcs >= N, ldct >= (S − 1)·ldcs + N).
 // - weights (T×S floats, dense): C(t) = Σ_s weights(t, s) · y(t, s) at C + t·ldct, in the order of s; ldcs is not read. S = 0: zeros
 //   (weights still not NULL, ids and X not read).
 // An id outside 0..E−1 is an empty place: its y is 0, and its weight is not read.
