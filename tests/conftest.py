@@ -62,5 +62,12 @@ def torch_dev():
     return torch
 
 
+@pytest.fixture
+def torch_roomy(torch_dev):
+    """torch_dev for a test of many GiB: what torch keeps of them is given back to the device afterwards."""
+    yield torch_dev
+    torch_dev.cuda.empty_cache()
+
+
 def seeded(seed):
     return np.random.default_rng(seed)

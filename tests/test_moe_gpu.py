@@ -352,9 +352,9 @@ def test_inputs_of_any_layout(g9, torch_dev):
     assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
 
 
-def test_experts_of_many_places_and_columns(g9, torch_dev):
+def test_experts_of_many_places_and_columns(g9, torch_roomy):
     """2^18 places of 65536 columns: offsets past 32 bits, and more tiles of 16 columns than a launch takes (it has wider ones)."""
-    torch = torch_dev
+    torch = torch_roomy
     g = torch.Generator(device="cuda").manual_seed(1)
     T, E, N, K = 1 << 18, 2, 1 << 16, 32
     w = torch.randint(-2, 3, (E, N, K), generator=g, device="cuda").half()

@@ -301,9 +301,9 @@ def test_inputs_of_any_layout(g9, torch_dev, dtype):
     assert same(g9.mx4_dequantize(g9.mx4_load(c[::-1], s[::-1])).cpu(), g9.mx4_dequantize(g9.mx4_load(c[::-1].copy(), s[::-1].copy())).cpu())
 
 
-def test_row_strides_past_32_bits(g9, torch_dev):
+def test_row_strides_past_32_bits(g9, torch_roomy):
     """The C entry points have row strides of 31 bits: inputs of longer ones are copied, such results are refused."""
-    torch = torch_dev
+    torch = torch_roomy
     far = (1 << 32) + 64
     buf = torch.zeros(far + 64, dtype=torch.float16, device="cuda")
     a = buf.as_strided((2, 64), (far, 1))
@@ -324,9 +324,9 @@ def test_row_strides_past_32_bits(g9, torch_dev):
     assert bool((a == y[:, 0]).all()) and bool((buf[64:128] == torch.arange(64, 128, device="cuda") / 16).all())
 
 
-def test_rows_of_two_billion(g9, torch_dev):
+def test_rows_of_two_billion(g9, torch_roomy):
     """The longest rows that a matrix has; longer ones are refused."""
-    torch = torch_dev
+    torch = torch_roomy
     K = (1 << 31) - 128
     L = g9._llm_library()
     for k in (K + 1, K + 127):
