@@ -1,4 +1,4 @@
-"""Builds libgen9blas.so (HIP, gfx950), libgen9blas_llm.so (MX4 and mixture-of-experts operators, HIP) and
+"""Builds libgen9blas.so (HIP, gfx950), libgen9blas_llm.so (operators of large language models, HIP) and
 libgen9blas_blas.so (CBLAS/BLAS shim) in this directory.
 
     python gen9-gpu-blas_amd/build.py            # rebuild what changed
@@ -31,7 +31,7 @@ HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++20", "-fPIC", "-fvisibilit
              "-Wall", "-Wno-unused-function"]
 HIP_SOURCES = ["runtime.hip", "gemm.hip", "gemm_kernels.hip", "skinny.hip", "level12.hip", "level12_kernels.hip",
                "packed.hip", "level3.hip", "level2.hip", "noalloc.hip"]
-LLM_SOURCES = ["llm_runtime.hip", "mx4.hip", "mx4_gemm.hip", "moe.hip"]
+LLM_SOURCES = ["llm_runtime.hip", "mx4.hip", "mx4_gemm.hip", "moe.hip", "linear.hip", "norm.hip", "dropout.hip", "embedding.hip"]
 # every header of csrc/ counts as a dependency of every object: a new header cannot be left out
 HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith(".h"))
 

@@ -1,0 +1,34 @@
+// Sums over rows for the gradients of a bias or a norm's weights: kernels leave the sums of blocks of rows in a work buffer, and
+// this adds the blocks in a fixed order, so results do not vary from call to call.
+#pragma once
+#include "llm.h"
+
+namespace g9llm {
+
+// out[n] (+)= Σ_b parts[b·ld + n]: 64 columns a workgroup, 16 threads a column, each with every sixteenth block.
+static __global__ void __launch_bounds__(1024) column_sums_kernel(const float *__restrict__ parts, long long blocks, int N, long long ld, float *__restrict__ out, int accumulate) {
+    __shared__ float part[16][64];
+    const int c = threadIdx.x & 63, r = threadIdx.x >> 6, n = blockIdx.x * 64 + c;
+    float s[4] = {};
+    if (n < N) {
+        long long b = r;
+        for (; b + 48 < blocks; b += 64)
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[i] += parts[(b + 16 * i) * ld + n];
+        for (; b < blocks; b += 16) s[0] += parts[b * ld + n];
+    }
+    part[r][c] = (s[0] + s[1]) + (s[2] + s[3]);
+    __syncthreads();
+    if (r || n >= N) return;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) sum += part[i][c];
+    out[n] = accumulate ? out[n] + sum : sum;
+}
+static int column_sums(const float *parts, long long blocks, int N, long long ld, float *out, int accumulate) {
+    hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)cdiv(N, 64)), dim3(1024), 0, stream, parts, blocks, N, ld, out, accumulate);
+    G9_HIP(hipGetLastError());
+    return 0;
+}
+
+}  // namespace g9llm

@@ -41,7 +41,8 @@
 // - the workgroup → tile mapping gives each XCD a contiguous range of tiles, ordered in groups of 4 tile rows, so
 //   one XCD's L2 serves the A and B panels its tiles share.
 #pragma once
-#include "internal.h"
+#include <hip/hip_runtime.h>
+#include <stdint.h>
 #include "lds_dma.h"
 #include <type_traits>
 
@@ -251,9 +252,10 @@ __device__ __forceinline__ void store8(f16 *c, f32x4 lo, f32x4 hi, float alpha, 
 // copy directly (EDGE in Loader) is taken first, through registers.
 // SPLIT: blockIdx.y is a slice of K (count 1); each workgroup leaves its unscaled FP32 sums in P, accumulator by
 // accumulator (64 lanes × 16 bytes), for split_sum.
+// Par: Params, or one derived from it with a member `epilogue` (linear_epilogue.h) that takes the sums instead of alpha, beta and C.
 template <int BM, int BN, int WM, int WN, int KB, int NS, bool AK, bool BKC, bool RA = false, bool EDGE = false,
-          bool SPLIT = false>
-__global__ void __launch_bounds__(WM *WN * 64) hgemm_kernel(Params p) {
+          bool SPLIT = false, class Par = Params>
+__global__ void __launch_bounds__(WM *WN * 64) hgemm_kernel(Par p) {
     constexpr int NW = WM * WN;
     constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
     constexpr int ABYTES = BM * KB * 2, BBYTES = BN * KB * 2, SBYTES = ABYTES + BBYTES;
@@ -344,6 +346,7 @@ __global__ void __launch_bounds__(WM *WN * 64) hgemm_kernel(Params p) {
         // the compiler wait for all LDS reads of a substep at once (scalar loads and LDS reads share a counter). The
         // accumulators' zeros are hidden from the compiler: as one shared constant they cost register copies per k-step.
         asm volatile("" : "+s"(C), "+s"(p.P), "+s"(p.ldc), "+s"(p.M), "+s"(p.N));
+        if constexpr (requires { p.epilogue; }) p.epilogue.pin();
         wait_lgkm0();
 #pragma unroll
         for (int i = 0; i < TN; i++)
@@ -499,8 +502,23 @@ __global__ void __launch_bounds__(WM *WN * 64) hgemm_kernel(Params p) {
             }
         return;
     }
-    const float alpha = p.alpha, beta = p.beta;
     const int g = lane >> 4;
+    if constexpr (requires { p.epilogue; }) {
+        p.epilogue.each([&](auto kind) {
+#pragma unroll
+            for (int pp = 0; pp < TN / 2; pp++) {
+                const int n = n0 + wn * WTN + 32 * pp + 8 * g;
+                const auto cols = p.epilogue.template columns<8>(n, p.N - n);
+#pragma unroll
+                for (int j = 0; j < TM; j++) {
+                    const int m = m0 + wm * WTM + j * 16 + (lane & 15);
+                    if (m < p.M) p.epilogue.template row<f16, 8>(kind, C, p.ldc, m, n, cols, p.N - n, acc[2 * pp][j], acc[2 * pp + 1][j]);
+                }
+            }
+        });
+        return;
+    }
+    const float alpha = p.alpha, beta = p.beta;
 #pragma unroll
     for (int pp = 0; pp < TN / 2; pp++)
 #pragma unroll
@@ -526,8 +544,8 @@ __global__ void __launch_bounds__(WM *WN * 64) hgemm_kernel(Params p) {
 // Finish of a SPLIT product on BM × BN tiles of WM × WN waves: the slices' sums added in slice order, then alpha / beta and
 // one rounding. A workgroup of 256 takes four (wave tile, pair of n tiles, m tile) groups of 64 lanes, each lane the 8
 // consecutive n of one row that it held in the product.
-template <int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(256) split_sum(Params p, int slices) {
+template <int BM, int BN, int WM, int WN, class Par = Params>
+__global__ void __launch_bounds__(256) split_sum(Par p, int slices) {
     constexpr int NW = WM * WN, WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16, PER = NW * TM * (TN / 2);
     const int lane = threadIdx.x & 63;
     const long long q = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), tiles = (long long)p.tiles_m * p.tiles_n;
@@ -544,7 +562,9 @@ __global__ void __launch_bounds__(256) split_sum(Params p, int slices) {
         lo += P[s * slice];
         hi += P[s * slice + 64];
     }
-    store8(p.C + (long long)m * p.ldc + n, lo, hi, p.alpha, p.beta, p.N - n);
+    if constexpr (requires { p.epilogue; })
+        p.epilogue.each([&](auto kind) { p.epilogue.template row<f16, 8>(kind, p.C, p.ldc, m, n, p.epilogue.template columns<8>(n, p.N - n), p.N - n, lo, hi); });
+    else store8(p.C + (long long)m * p.ldc + n, lo, hi, p.alpha, p.beta, p.N - n);
 }
 
 }  // namespace hg

@@ -1,0 +1,115 @@
+// What a linear layer does with a product's sums before they are stored: Z = sum + bias, Y = R + dropout(act(Z)), all in FP32,
+// Y and Z each rounded once.
+//
+// Three kinds of activation, chosen once outside the loops over a tile: z < low ? low : z (none: low = −∞, ReLU: 0);
+// z·σ(a·z + b·z³) (SiLU: a = 1, b = 0; GELU's tanh form, 0.5·z·(1 + tanh(c·(z + 0.044715·z³))) with c = √(2/π): a = 2c, b =
+// 2c·0.044715, as 0.5·(1 + tanh x) = σ(2x)); and z·Φ(z), GELU itself.
+#pragma once
+#include "dropout.h"
+#include "rows.h"
+#include <type_traits>
+
+namespace g9llm {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+enum Kind { KIND_CLIP, KIND_SIGMOID, KIND_ERF };
+
+struct Activation {
+    int kind;
+    float low, a, b;
+};
+inline Activation make_act(int act) {
+    switch (act) {
+    case 1: return {KIND_CLIP, 0.f, 0.f, 0.f};
+    case 2: return {KIND_ERF, 0.f, 0.f, 0.f};
+    case 3: return {KIND_SIGMOID, 0.f, 1.5957691216057308f, 0.0713548162726009f};
+    case 4: return {KIND_SIGMOID, 0.f, 1.f, 0.f};
+    }
+    return {KIND_CLIP, -INFINITY, 0.f, 0.f};
+}
+
+// T: the type of the result. For FP16 the hardware's exponential and reciprocal are enough (2^-21 of the value and less).
+template <class T> __device__ __forceinline__ float sigmoid(float x) {
+    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
+    else return 1.f / (1.f + expf(-x));
+}
+// The normal distribution function.
+template <class T> __device__ __forceinline__ float phi(float z) { return 0.5f * erfcf(-0.7071067811865476f * z); }
+
+// z² with an end, so that its product with b = 0, or with the zero of a slope far out, is none of infinity's.
+__device__ __forceinline__ float square(float z) { return fminf(z * z, 1e30f); }
+
+template <class T, int KIND> __device__ __forceinline__ float activate(const Activation &act, float z) {
+    if constexpr (KIND == KIND_CLIP) return z < act.low ? act.low : z;
+    if constexpr (KIND == KIND_SIGMOID) return z * sigmoid<T>(z * (act.a + act.b * square(z)));
+    return z * phi<T>(z);
+}
+// d activate / dz
+template <class T, int KIND> __device__ __forceinline__ float slope(const Activation &act, float z) {
+    if constexpr (KIND == KIND_CLIP) return z > act.low || z != z ? 1.f : 0.f;
+    if constexpr (KIND == KIND_SIGMOID) {
+        const float q = square(z), s = sigmoid<T>(z * (act.a + act.b * q));
+        return s + z * s * (1.f - s) * (act.a + 3.f * act.b * q);
+    }
+    return phi<T>(z) + z * 0.3989422804014327f * expf(-0.5f * z * z);
+}
+
+template <class T> struct Epilogue {
+    const float *bias;   // or null
+    T *Z;                // or null
+    const T *R;          // or null
+    long long ldz, ldr;
+    Activation act;
+    Dropout dropout;
+
+    template <int V> struct Cols { float bias[V]; };
+
+    // Keeps the loads of these kernel arguments before this place.
+    __device__ __forceinline__ void pin() {
+        asm volatile("" : "+s"(bias), "+s"(Z), "+s"(R), "+s"(ldz), "+s"(ldr), "+s"(act.kind), "+s"(act.low), "+s"(act.a), "+s"(act.b));
+        asm volatile("" : "+s"(dropout.limit), "+s"(dropout.scale), "+s"(dropout.seed[0]), "+s"(dropout.seed[1]), "+s"(dropout.offset[0]), "+s"(dropout.offset[1]));
+    }
+    template <class F> __device__ __forceinline__ void each(F f) const {
+        if (act.kind == KIND_CLIP) f(std::integral_constant<int, KIND_CLIP>{});
+        else if (act.kind == KIND_SIGMOID) f(std::integral_constant<int, KIND_SIGMOID>{});
+        else f(std::integral_constant<int, KIND_ERF>{});
+    }
+    // Columns n .. n + V − 1, of which `valid` exist (also none: nothing is read then).
+    template <int V> __device__ __forceinline__ Cols<V> columns(int n, int valid) const {
+        Cols<V> c;
+        if (bias) load_some<V>(bias + n, valid, c.bias);
+        else
+#pragma unroll
+            for (int e = 0; e < V; e++) c.bias[e] = 0.f;
+        return c;
+    }
+    // Row m, columns n .. n + V − 1 (n a multiple of V) from their sums: four, or eight in `v` and `hi`.
+    template <class O, int V, class K> __device__ __forceinline__ void row(K, O *Y, long long ldy, int m, int n, const Cols<V> &cols, int valid, f32x4 v, f32x4 hi = {}) const {
+        if (valid <= 0) return;
+        float x[V];
+#pragma unroll
+        for (int e = 0; e < V; e++) x[e] = (e < 4 ? v[e & 3] : hi[e & 3]) + cols.bias[e];
+        if (Z) store_some<V>(Z + m * ldz + n, valid, x);
+#pragma unroll
+        for (int e = 0; e < V; e++) x[e] = activate<T, K::value>(act, x[e]);
+        if (dropout.limit) drop<V>(dropout, m, n, x);
+        if (R) {
+            float r[V];
+            load_some<V>(R + m * ldr + n, valid, r);
+#pragma unroll
+            for (int e = 0; e < V; e++) x[e] += r[e];
+        }
+        store_some<V>(Y + m * ldy + n, valid, x);
+    }
+    // One element.
+    template <class O> __device__ __forceinline__ void one(O *Y, long long ldy, int m, int n, float sum) const {
+        float x = sum + (bias ? bias[n] : 0.f);
+        if (Z) Z[m * ldz + n] = (T)x;
+        each([&](auto kind) { x = activate<T, decltype(kind)::value>(act, x); });
+        if (dropout.limit) x = kept(dropout, philox(dropout, (unsigned)n >> 3, m), n & 7) ? x * dropout.scale : 0.f;
+        if (R) x += (float)R[m * ldr + n];
+        Y[m * ldy + n] = (T)x;
+    }
+};
+
+}  // namespace g9llm

@@ -45,8 +45,10 @@ G9_HIDDEN int begin();
 // 0 if [p, p + bytes) is device memory of one allocation, else INVALID_ARG naming `what`.
 G9_HIDDEN int need_device(const void *p, size_t bytes, const char *what);
 // Device scratch, grown on demand and kept; growing waits for queued work.
-enum Slot { SLOT_A = 0, SLOT_PART, SLOT_PLAN, SLOT_SLOTS, NSLOTS };
+enum Slot { SLOT_A = 0, SLOT_PART, SLOT_PLAN, SLOT_SLOTS, SLOT_X, SLOT_W, SLOT_DZ, SLOT_SUMS, SLOT_SORT, NSLOTS };
 G9_HIDDEN int scratch(int slot, size_t bytes, void **p);
+// Clears `rows` rows of `bytes` bytes (a multiple of 2), `ld` bytes apart.
+G9_HIDDEN int zero_rows(void *p, long long ld, long long rows, long long bytes);
 // The longest rows: kernels count k in an int, up to the end of the last 128-k chunk.
 constexpr int MAX_COLS = 0x7fffff80;
 inline int elem_size(int type) { return type == GEN9BLAS_S ? 4 : 2; }

@@ -130,8 +130,8 @@ template <int TRI, int BM> __device__ __forceinline__ void tri_tile(int bid, int
 }
 
 template <int BM, int BN, int WM, int WN, int NS, bool AK, bool BKC, int BLK = 1, int TRI = 0, int KLIM = 0,
-          bool MSKIP = false, bool EDGE = false, bool SPLIT = false>
-__global__ void __launch_bounds__(WM *WN * 64) sgemm_kernel(Params p) {
+          bool MSKIP = false, bool EDGE = false, bool SPLIT = false, class Par = Params>
+__global__ void __launch_bounds__(WM *WN * 64) sgemm_kernel(Par p) {
     constexpr int NW = WM * WN, KB = 32;
     constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 32, TN = WTN / 32;
     constexpr int ABYTES = BM * KB * 4, BBYTES = BN * KB * 4, SBYTES = ABYTES + BBYTES;
@@ -284,6 +284,7 @@ __global__ void __launch_bounds__(WM *WN * 64) sgemm_kernel(Params p) {
         // as in the FP16 kernel: the epilogue's kernel arguments are loaded here, so that none is on its way when the loop
         // begins, and the accumulators' zeros are hidden from the compiler
         asm volatile("" : "+s"(C), "+s"(p.P), "+s"(p.ldc), "+s"(p.M), "+s"(p.N));
+        if constexpr (requires { p.epilogue; }) p.epilogue.pin();
         wait_lgkm0();
 #pragma unroll
         for (int i = 0; i < TN; i++)
@@ -378,6 +379,24 @@ __global__ void __launch_bounds__(WM *WN * 64) sgemm_kernel(Params p) {
             }
         return;
     }
+    if constexpr (requires { p.epilogue; }) {   // as in the FP16 kernel
+        p.epilogue.each([&](auto kind) {
+#pragma unroll
+            for (int i = 0; i < TN; i++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int n = n0 + wn * WTN + 32 * i + 8 * q + 4 * h;
+                    const auto cols = p.epilogue.template columns<4>(n, p.N - n);
+#pragma unroll
+                    for (int j = 0; j < TM; j++) {
+                        const int m = m0 + wm * WTM + 32 * j + (lane & 31);
+                        const f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                        if (m < p.M) p.epilogue.template row<float, 4>(kind, C, p.ldc, m, n, cols, p.N - n, v);
+                    }
+                }
+        });
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < TN; i++)
 #pragma unroll
@@ -418,8 +437,8 @@ __global__ void __launch_bounds__(WM *WN * 64) sgemm_kernel(Params p) {
 // Finish of a SPLIT product on BM × BN tiles of WM × WN waves (TRI: the tiles of a triangle): the slices' sums added in
 // slice order, then alpha / beta. A wave takes one run of 4 n of a 32×32 MFMA tile, each lane the 4 consecutive n of one
 // row that it held in the product. In the plain mode tile indices go group by group of 4 tile rows, as in the product.
-template <int BM, int BN, int WM, int WN, int TRI>
-__global__ void __launch_bounds__(256) split_sum(Params p, int slices, int tiles) {
+template <int BM, int BN, int WM, int WN, int TRI, class Par = Params>
+__global__ void __launch_bounds__(256) split_sum(Par p, int slices, int tiles) {
     constexpr int NW = WM * WN, WTM = BM / WM, WTN = BN / WN, TM = WTM / 32, TN = WTN / 32, PER = NW * TM * TN * 4;
     const int lane = threadIdx.x & 63;
     const long long u = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -441,7 +460,9 @@ __global__ void __launch_bounds__(256) split_sum(Params p, int slices, int tiles
     const long long slice = (long long)tiles * PER * 64;
     f32x4 v = P[0];
     for (int s = 1; s < slices; s++) v += P[s * slice];
-    store4<TRI>(p.C + (long long)m * p.ldc + n, v, p.alpha, p.beta, m, n, p.N, TRI != 0 && m0 == n0);
+    if constexpr (requires { p.epilogue; })
+        p.epilogue.each([&](auto kind) { p.epilogue.template row<float, 4>(kind, p.C, p.ldc, m, n, p.epilogue.template columns<4>(n, p.N - n), p.N - n, v); });
+    else store4<TRI>(p.C + (long long)m * p.ldc + n, v, p.alpha, p.beta, m, n, p.N, TRI != 0 && m0 == n0);
 }
 
 }  // namespace sg

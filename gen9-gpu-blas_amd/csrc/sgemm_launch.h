@@ -1,17 +1,12 @@
-// Host side of the FP32 GEMM on direct global→LDS loads (sgemm_kernel.h): which products it takes, their tiles and their
-// split of K, the triangle and k-limited modes of the level-3 routines. Part of gemm_kernels.hip.
+// Host side of the FP32 GEMM on direct global→LDS loads (sgemm_kernel.h): which products it takes, their tiles (with
+// their split of K in sgemm_tiles.h), the triangle and k-limited modes of the level-3 routines. Part of gemm_kernels.hip.
 // Against the general kernel that served ragged products before, with checked loads in every k-step and whole-tile interiors
 // (µs): 1000³ 37.4 → 25.0, 64 × 250³ 46.1 → 27.7, 141×3840×3712 TN 205 → 60, 6192×192×5910 NT 413 → 143, 1512×362×738
 // 43.4 → 19.5.
-//
-// Tile configurations, with rates on MI355X (TFLOP/s, sustained): 128×256, 8 waves of 64×64, two stages, sums blocked per
-// 128 k: n = 4096 NN 144.9, NT 144.3, 8192×8192×2048 144.1 (three stages 142.6; blocks of 32 k 134.3, 64 k 140.3, 256 k
-// 142.6; 256×128 tiles 142.7). 128×128, 8 waves of 64×32, three stages: n = 2048 133-134 (4 waves of 64×64 129.7).
-// 64×64, 4 waves of 32×32, four stages, sums blocked per 256 k: n = 2048 137, n = 1024 102.6 (three stages 94.0, six 93.0,
-// eight 92.2; 128-k blocks 101.9, 32-k 90.9). 64×128 and 128×64, 4 waves of 32×64 (64×32), three stages:
-// 2386×1512×1920 120.5 µs against 121.1 on 64×64 and 122.1 on 128×128 tiles, 3000×3000×150 42.6 against 43.1 and 46.5.
 #pragma once
+#include "internal.h"
 #include "sgemm_kernel.h"
+#include "sgemm_tiles.h"
 #include <stdlib.h>
 #include <string.h>
 #include <algorithm>
@@ -19,56 +14,6 @@
 
 namespace g9 {
 namespace sgl {
-
-constexpr int KB = 32;   // k per k-step
-// ns: time per k of a 64×64 share of the tile, for cost(); per_cu: workgroups that share a CU
-struct SgCfg { int BM, BN, WM, WN, NS, BLK; double ns; int per_cu; };
-constexpr SgCfg CFG[] = {{128, 256, 2, 4, 2, 4, 14.4, 1}, {128, 128, 2, 4, 3, 4, 14.8, 1}, {64, 64, 2, 2, 4, 8, 14.8, 2},
-                         {64, 128, 2, 2, 3, 4, 14.8, 2}, {128, 64, 2, 2, 3, 4, 14.8, 2}};
-constexpr int NCFG = sizeof CFG / sizeof CFG[0];
-struct Choice { int cfg, slices; double us; };
-
-static int slices_of(int K, int s, int &kper) {
-    kper = std::max(((K + s - 1) / s + KB - 1) / KB * KB, 2 * KB);
-    return (K + kper - 1) / kper;
-}
-// Estimated time (µs) of `tiles` tiles of a configuration in ns slices of kper k: the launch, the most loaded CU's tiles at
-// the matrix cores' rate, a fixed part for each round of tiles that share a CU, and for slices the second kernel and
-// their sums written and read. Constants fitted to 29 products (K 100 to 20000, 100 to 8000 rows, batches, whole and
-// ragged, every layout), timed with every configuration and 1-24 slices: the choice is the fastest or within 2 % of it for
-// 27 of them, within 7 % for all. A few (µs, chosen / others): 500³ 64×64 in 3 slices 10.2 / unsplit 12.1; 130×130×5000
-// 64×64 in 16-24 slices 16.9 / in 4 24; 64 × 256³ 128×128 24.8 / 64×64 27.4; 245 × 144×64×264 64×64 25.5 / 128×128 48.5.
-static double cost(const SgCfg &g, long long tiles, int kper, int ns) {
-    const double per_cu = (double)(tiles * ns) / num_cus, area = (double)g.BM * g.BN / 4096;
-    double t = 5.4 + std::max(1.0, std::ceil(per_cu)) * area * g.ns * 1e-3 * kper + 3.4 * std::ceil(per_cu / g.per_cu);
-    if (ns > 1) t += 0.8 + (double)(ns * tiles) * g.BM * g.BN * 8 / 1e7;
-    return t;
-}
-// The cheapest configuration and split of K into slices that fit `work` bytes; tri: the tiles of a triangle of side M
-// (square tiles only); big: 128×256 tiles may be taken (their edge-capable variant would need more registers than a wave
-// has).
-static Choice choose(const GemmCall &c, size_t work, bool tri, bool big) {
-    static constexpr int SLICES[] = {1, 2, 3, 4, 6, 8, 12, 16, 24};
-    Choice best{2, 1, 1e30};
-    for (int i = 0; i < NCFG; i++) {
-        const SgCfg &g = CFG[i];
-        // a triangle that no whole tiles fill: 128×128 tiles lose half of each on the diagonal, and on this kernel they
-        // were slower throughout (2000×200 22.1 µs against 20.0, 5000×160 50.8 against 40.3)
-        if ((tri && (g.BM != g.BN || (g.BM == 128 && c.M % 64))) || (i == 0 && !big)) continue;
-        const long long tm = (c.M + g.BM - 1) / g.BM, tn = (c.N + g.BN - 1) / g.BN;
-        const long long tiles = (tri ? tm * (tm + 1) / 2 : tm * tn) * c.count;
-        for (const int s : SLICES) {
-            int kper;
-            const int ns = s == 1 ? 1 : slices_of(c.K, s, kper);
-            if (s == 1) kper = (c.K + KB - 1) / KB * KB;
-            if (s > 1 && (i == 0 || kper < 4 * KB || tiles * s > 5LL * num_cus ||
-                          (size_t)(ns * tiles) * g.BM * g.BN * sizeof(float) > work)) break;
-            const double t = cost(g, tiles, kper, ns);
-            if (t < best.us) best = Choice{i, ns, t};
-        }
-    }
-    return best;
-}
 
 // TRI: 0 plain, 1 lower, 2 upper triangle (square tiles). EDGE as in the kernel; slices > 1 needs p.P.
 template <int I, bool AK, bool BKC, int TRI, bool EDGE>
@@ -188,7 +133,7 @@ static bool sg_tri(const GemmCall &c, bool lower, int *rc) {
     if (c.K <= 128 && side * (side + 1) / 2 > 2LL * num_cus) return false;
     size_t work;
     const sg::Params p = sg_work(c, false, work);
-    const sgl::Choice ch = sgl::choose(c, work, true, false);
+    const sgl::Choice ch = sgl::choose({c.M, c.N, c.K, c.count}, work, true, false, num_cus);
     // whole tiles (sums blocked per 128 or 256 k, as whole_block) where they fill the CUs, 64×64 ones unless 128×128 fill
     // their last round as well
     const long long s64 = c.M / 64, s128 = c.M / 128, t64 = s64 * (s64 + 1) / 2, t128 = s128 * (s128 + 1) / 2;
@@ -253,7 +198,7 @@ static bool sg_strip(const GemmCall &c, const sg::Params &p0, double us, int *rc
     const int Mi = c.M / big.BM * big.BM, r = c.M - Mi, Ms = (r + 63) / 64 * 64;
     if (c.count != 1 || r == 0 || Ms > c.M || c.N % big.BN || (c.tA && (c.M - Ms) % 4) || !sgemm_tiles_ok(c)) return false;
     const long long tiles = (long long)(Mi / big.BM) * (c.N / big.BN), strip = (long long)(Ms / 64) * (c.N / 64);
-    if (tiles < 2LL * num_cus || sgl::cost(big, tiles, c.K, 1) + sgl::cost(small, strip, c.K, 1) - 5.4 >= us) return false;
+    if (tiles < 2LL * num_cus || sgl::cost(big, tiles, c.K, 1, num_cus) + sgl::cost(small, strip, c.K, 1, num_cus) - 5.4 >= us) return false;
     sg::Params p = p0, s = p0;
     p.M = Mi;
     s.A += c.tA ? (long long)(c.M - Ms) : (long long)(c.M - Ms) * c.lda;
@@ -288,7 +233,7 @@ static bool launch_sgemm_direct(const GemmCall &c, int *rc) {
     const sg::Params p = sg_work(c, batch, work);
     const bool tiles_ok = sgemm_tiles_ok(c);
     const int block = tiles_ok ? whole_block(c) : 0;
-    const sgl::Choice ch = sgl::choose(c, work, false, block >= sgl::CFG[0].BLK && c.M % 128 == 0 && c.N % 256 == 0);
+    const sgl::Choice ch = sgl::choose({c.M, c.N, c.K, c.count}, work, false, block >= sgl::CFG[0].BLK && c.M % 128 == 0 && c.N % 256 == 0, num_cus);
     const sgl::SgCfg &g = sgl::CFG[ch.cfg];
     if ((long long)((c.M + g.BM - 1) / g.BM) * ((c.N + g.BN - 1) / g.BN) > 0x7fffffffLL) return false;
     if (sg_strip(c, p, ch.us, rc)) return true;

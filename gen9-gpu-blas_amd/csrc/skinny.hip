@@ -5,6 +5,7 @@
 // with one template over the M tile. Per M tile, the weight rows per workgroup (RW), the waves splitting K (KS) and
 // the chunks prefetched per lane (NC) are the fastest of a sweep over 155 configurations on MI355X for
 // C = A·Wᵀ with W 4096×4096 FP16 rotated over 32 copies (1 GiB, beyond the 256 MB MALL).
+#include "internal.h"
 #include "skinny_kernel.h"
 #include <algorithm>
 

@@ -12,7 +12,8 @@
 //   distance the lane keeps half of its values and adds its partner's copy of them, so 64 sums cost about one
 //   exchange per value instead of six; then the KS waves combine through LDS.
 #pragma once
-#include "internal.h"
+#include <hip/hip_runtime.h>
+#include <stdint.h>
 #include "lds_dma.h"
 #include "wave.h"
 
@@ -62,8 +63,9 @@ template <class T, bool VEC, bool NTL = false> __device__ __forceinline__ u32x4 
     return u.v;
 }
 
-template <class T, int MT, int RW, int KS, int NC, bool VEC>
-__global__ void __launch_bounds__(KS * 64) skinny_kernel(Params p) {
+// Par: Params, or one derived from it with a member `epilogue` (linear_epilogue.h) that takes the sums; C's rows are scm apart then.
+template <class T, int MT, int RW, int KS, int NC, bool VEC, class Par = Params>
+__global__ void __launch_bounds__(KS * 64) skinny_kernel(Par p) {
     constexpr int V = 16 / (int)sizeof(T);
     constexpr int NV = RW * MT;
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
@@ -126,6 +128,10 @@ __global__ void __launch_bounds__(KS * 64) skinny_kernel(Params p) {
     auto emit = [&](int idx, float s) {
         const int n = n0 + idx / MT, m = m0 + idx % MT;
         if (n < p.N && m < p.M) {
+            if constexpr (requires { p.epilogue; }) {
+                p.epilogue.one(C, p.scm, m, n, s);
+                return;
+            }
             T *c = C + (long long)m * p.scm + (long long)n * p.scn;
             const float r = p.beta == 0.f ? p.alpha * s : __builtin_fmaf(p.alpha, s, p.beta * (float)*c);
             *c = (T)r;
@@ -164,8 +170,8 @@ __global__ void __launch_bounds__(KS * 64) skinny_kernel(Params p) {
 // - the 16×16 FP32 partial tiles of the KS waves are summed through LDS, then alpha (and beta·C, C not read when
 //   beta = 0) is applied and rounded once to FP16, as in the dot-product kernel.
 // Requires K % 256 == 0 and 16-byte aligned rows of a and w (the launcher checks; other shapes take the kernel above).
-template <int MT, int KS, int NS>
-__global__ void __launch_bounds__(KS * 64) skinny_mfma_kernel(Params p) {
+template <int MT, int KS, int NS, class Par = Params>
+__global__ void __launch_bounds__(KS * 64) skinny_mfma_kernel(Par p) {
     typedef f16 f16x8 __attribute__((ext_vector_type(8)));
     typedef float f32x4 __attribute__((ext_vector_type(4)));
     constexpr int GK = 256, ROWB = GK * 2;                 // 512 bytes of a row per group
@@ -254,6 +260,10 @@ __global__ void __launch_bounds__(KS * 64) skinny_mfma_kernel(Params p) {
         for (int q = 0; q < KS; q++) sum += part[(q * 16 + n) * 16 + m];
         const int gm = m0 + m, gn = n0 + n;
         if (gm < p.M && gn < p.N) {
+            if constexpr (requires { p.epilogue; }) {
+                p.epilogue.one(C, p.scm, gm, gn, sum);
+                continue;
+            }
             f16 *c = C + (long long)gm * p.scm + (long long)gn * p.scn;
             const float r = p.beta == 0.f ? p.alpha * sum : __builtin_fmaf(p.alpha, sum, p.beta * (float)*c);
             *c = (f16)r;

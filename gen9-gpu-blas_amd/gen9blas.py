@@ -9,6 +9,7 @@
     C = gen9blas.mx4_gemm(A, W)               # A float16, float32 or MX4
     ids, w = gen9blas.moe_route(logits, 8)    # a mixture of experts: its router, and
     y = gen9blas.moe_gemm(x, ids, We, weights=w)   # its experts' products on MX4 weights
+    y = gen9blas.linear(x, Wf, bias=b, act="gelu") # a linear layer; layer_norm, dropout, embedding and their gradients
 
 API contract (reference lib/gen9blas.py:96-610): the same public names, positional arguments and defaults.
 - The compute type follows the data: float16, float64, and float32 for every other element type.
@@ -897,14 +898,16 @@ def spr2(alpha, x, y, Ap, uplo="L"):
 
 
 # ------------------------------------------------------------------------------------------------------------------
-# 4-bit weights (MX4) and mixtures of experts: libgen9blas_llm.so
+# Operators of large language models: libgen9blas_llm.so
 # ------------------------------------------------------------------------------------------------------------------
 # These operators work on GPU memory: torch GPU tensors in place, and NumPy arrays (or CPU tensors) through a copy to
 # the GPU and back. float16 computes from float16 and gives float16; every other type is converted to float32.
 _LLM_SIGNATURES = """
     llm_error=s:  llm_last_status=i:  mx4_create=p:iii  mx4_free=v:p  mx4_quantize=i:ipilp  mx4_load=i:pipip
     mx4_dequantize=i:ppil  mx4_gemm=i:iipippi  mx4_gemm_q=i:ipppi  moe_route=i:iiipipiiiiifpp
-    moe_gemm=i:iiippllppppll
+    moe_gemm=i:iiippllppppll  linear=i:iiiipipipipidllpipi  linear_backward=i:iiiipipiidllpipipipipi
+    layer_norm=i:iiipippfpip  layer_norm_backward=i:iiipipipppippi  dropout=i:iiipidllpipi
+    embedding=i:iiiipipifpi  embedding_backward=i:iiiipipifipii
 """
 _llm = None
 _llm_device = 0        # torch's index of the library's device
@@ -1173,3 +1176,194 @@ def moe_gemm(X, ids, W, gate=None, weights=None, C=None):
               None if gate is None else gate._handle, None if weights is None else weights.data_ptr() or out.data_ptr(),   # empty: no address
               out.data_ptr(), ldct, ldcs)
     return _host_like(X, out) if C is None else out
+
+
+# ---- linear layers, layer norm, dropout, embeddings ----
+_ACT_CODE = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+_U64 = (1 << 64) - 1
+
+
+def _act_code(act):
+    if act not in _ACT_CODE:
+        raise ValueError(f"activation {act!r}; known: {', '.join(map(repr, _ACT_CODE))}")
+    return _ACT_CODE[act]
+
+
+def _matrix_like(X, shape, t, what):
+    """X as _device_rows gives it, of this shape and type."""
+    x, ld = _device_rows(X, (2,))
+    if tuple(x.shape) != tuple(shape):
+        raise ValueError(f"{what} has shape {tuple(x.shape)}, expected {tuple(shape)}")
+    if x.dtype is not t:
+        raise TypeError(f"{what} is of {x.dtype}, the others of {t}")
+    return x, ld
+
+
+def _floats(v, n, what):
+    """A vector of n float32 on the GPU, or None."""
+    if v is None:
+        return None
+    v = _device_rows(v, (1,))[0].float().contiguous()
+    if v.shape[0] != n:
+        raise ValueError(f"{what} has {v.shape[0]} elements, expected {n}")
+    return v
+
+
+def _float_sums(v, n, wanted, accumulate, what):
+    """Where the sums over the rows go: float32 (n,), the given ones or new; None if they are not wanted."""
+    if not wanted:
+        return None
+    if v is None and accumulate:
+        raise ValueError(f"accumulate needs {what}")
+    return _llm_out(v, (n,), _torch.float32, what)
+
+
+def _ptr(X):
+    return None if X is None else X.data_ptr()
+
+
+def linear(X, W, bias=None, act=None, dropout=0.0, seed=0, offset=0, residual=None, Z=None, C=None):
+    """residual + dropout(act(X·Wᵀ + bias)): X (M, K) and W (N, K) float16 or both float32, bias (N,) float32, residual (M, N).
+    act: None, "relu", "gelu", "gelu_tanh" or "silu". dropout, seed, offset: as in dropout(). Z, if given, takes the
+    pre-activations X·Wᵀ + bias, which linear_backward needs for an activation."""
+    lib = _llm_library()
+    a = _act_code(act)
+    x, ldx = _device_rows(X, (2,))
+    (M, K), t = x.shape, x.dtype
+    w, ldw = _device_rows(W, (2,))
+    N = w.shape[0]
+    if w.shape[1] != K:
+        raise ValueError(f"incompatible dimensions: {tuple(x.shape)} · {tuple(w.shape)}ᵀ")
+    if w.dtype is not t:
+        raise TypeError(f"W is of {w.dtype}, X of {t}")
+    b = _floats(bias, N, "bias")
+    r, ldr = (None, 0) if residual is None else _matrix_like(residual, (M, N), t, "residual")
+    z = None if Z is None else _llm_out(Z, (M, N), t, "Z")
+    out = _llm_out(C, (M, N), t)
+    _llm_call(lib.gen9blas_linear, 1 if t is _torch.float32 else 0, M, N, K, x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(b), a,
+              _ptr(z), 0 if z is None else _out_step(z, "Z"), dropout, seed & _U64, offset & _U64, _ptr(r), ldr,
+              out.data_ptr(), N if C is None else _out_step(out))
+    return _host_like(X, out) if C is None else out
+
+
+def linear_backward(dY, X, W, Z=None, act=None, dropout=0.0, seed=0, offset=0, dX=None, dW=None, db=None, accumulate=False, grads="xwb"):
+    """The gradients of linear() from dY (M, N), its X, W and Z (Z only for an activation) and the same act, dropout, seed and
+    offset: (dX, dW, db), db in float32. residual's gradient is dY itself. accumulate: dW and db are added to the given ones.
+    grads: those wanted ("x", "w", "b"); the others are None."""
+    lib = _llm_library()
+    a = _act_code(act)
+    dy, lddy = _device_rows(dY, (2,))
+    (M, N), t = dy.shape, dy.dtype
+    w, ldw = _device_rows(W, (2,))
+    K = w.shape[1]
+    w, ldw = _matrix_like(w, (N, K), t, "W")
+    x, ldx = _matrix_like(X, (M, K), t, "X")
+    if a and Z is None:
+        raise ValueError("an activation's gradient needs Z")
+    z, ldz = _matrix_like(Z, (M, N), t, "Z") if a else (None, 0)
+    if not set(grads) <= set("xwb"):
+        raise ValueError(f"grads {grads!r}: of 'x', 'w' and 'b'")
+    gx = _llm_out(dX, (M, K), t, "dX") if "x" in grads else None
+    if "w" in grads and dW is None and accumulate:
+        raise ValueError("accumulate needs dW")
+    gw = _llm_out(dW, (N, K), t, "dW") if "w" in grads else None
+    gb = _float_sums(db, N, "b" in grads, accumulate, "db")
+    _llm_call(lib.gen9blas_linear_backward, 1 if t is _torch.float32 else 0, M, N, K, dy.data_ptr(), lddy, _ptr(z), ldz, a, dropout,
+              seed & _U64, offset & _U64, x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(gx), 0 if gx is None else _out_step(gx, "dX"),
+              _ptr(gw), 0 if gw is None else _out_step(gw, "dW"), _ptr(gb), bool(accumulate))
+    return tuple(g if g is None or given is not None else _host_like(dY, g) for g, given in ((gx, dX), (gw, dW), (gb, db)))
+
+
+def layer_norm(X, gamma=None, beta=None, eps=1e-5, out=None, stats=None):
+    """(X - mean)·rstd·gamma + beta over each row of X (M, N), rstd = 1 / sqrt(variance + eps); gamma and beta (N,) float32.
+    stats, a GPU tensor (M, 2) of float32 if given, takes each row's mean and rstd, for layer_norm_backward."""
+    lib = _llm_library()
+    x, ldx = _device_rows(X, (2,))
+    M, N = x.shape
+    g, b = _floats(gamma, N, "gamma"), _floats(beta, N, "beta")
+    y = _llm_out(out, (M, N), x.dtype, "out")
+    if stats is not None and not _llm_out(stats, (M, 2), _torch.float32, "stats").is_contiguous():
+        raise ValueError("stats must be contiguous")
+    _llm_call(lib.gen9blas_layer_norm, 1 if x.dtype is _torch.float32 else 0, M, N, x.data_ptr(), ldx, _ptr(g), _ptr(b), eps,
+              y.data_ptr(), N if out is None else _out_step(y, "out"), _ptr(stats))
+    return _host_like(X, y) if out is None else y
+
+
+def layer_norm_backward(dY, X, stats, gamma=None, dX=None, dgamma=None, dbeta=None, accumulate=False, grads="xgb"):
+    """The gradients of layer_norm() from dY and its X, stats and gamma: (dX, dgamma, dbeta), the sums in float32. accumulate:
+    dgamma and dbeta are added to the given ones. grads: those wanted ("x", "g", "b"); the others are None."""
+    lib = _llm_library()
+    dy, lddy = _device_rows(dY, (2,))
+    (M, N), t = dy.shape, dy.dtype
+    x, ldx = _matrix_like(X, (M, N), t, "X")
+    stats = _matrix_like(stats, (M, 2), _torch.float32, "stats")[0].contiguous()
+    g = _floats(gamma, N, "gamma")
+    if not set(grads) <= set("xgb"):
+        raise ValueError(f"grads {grads!r}: of 'x', 'g' and 'b'")
+    gx = _llm_out(dX, (M, N), t, "dX") if "x" in grads else None
+    gg, gb = _float_sums(dgamma, N, "g" in grads, accumulate, "dgamma"), _float_sums(dbeta, N, "b" in grads, accumulate, "dbeta")
+    _llm_call(lib.gen9blas_layer_norm_backward, 1 if t is _torch.float32 else 0, M, N, dy.data_ptr(), lddy, x.data_ptr(), ldx,
+              stats.data_ptr(), _ptr(g), _ptr(gx), 0 if gx is None else _out_step(gx, "dX"), _ptr(gg), _ptr(gb), bool(accumulate))
+    return tuple(v if v is None or given is not None else _host_like(dY, v) for v, given in ((gx, dX), (gg, dgamma), (gb, dbeta)))
+
+
+def dropout(X, p, seed=0, offset=0, residual=None, out=None):
+    """residual + X with a share p of its elements zeroed and the others scaled by 1 / (1 - p), p to the nearest of 2^-16. The mask
+    is a function of place, seed and offset (Philox4x32-10, include/gen9blas_llm.h): the same call on the gradient of the
+    result gives X's. Take another offset for each layer and step."""
+    lib = _llm_library()
+    x, ldx = _device_rows(X, (2,))
+    M, N = x.shape
+    r, ldr = (None, 0) if residual is None else _matrix_like(residual, (M, N), x.dtype, "residual")
+    y = _llm_out(out, (M, N), x.dtype, "out")
+    _llm_call(lib.gen9blas_dropout, 1 if x.dtype is _torch.float32 else 0, M, N, x.data_ptr(), ldx, p, seed & _U64, offset & _U64,
+              _ptr(r), ldr, y.data_ptr(), N if out is None else _out_step(y, "out"))
+    return _host_like(X, y) if out is None else y
+
+
+def _token_ids(ids):
+    """Tokens as a dense GPU vector of int32 or int64."""
+    i = ids if isinstance(ids, _torch.Tensor) and ids.is_cuda else _on_gpu(ids)
+    if i.is_floating_point() or i.is_complex() or i.dtype is _torch.bool:
+        raise TypeError(f"ids are integers, not {i.dtype}")
+    if i.dim() != 1:
+        raise ValueError(f"ids of {i.dim()} dimensions, expected 1")
+    if i.shape[0] > _LONGEST:
+        raise ValueError(f"{i.shape[0]} ids; the most are {_LONGEST}")
+    if i.dtype is not _torch.int64 and i.dtype is not _torch.int32:
+        i = i.to(_torch.int64)
+    return i.contiguous()
+
+
+def embedding(table, ids, scale=1.0, out=None):
+    """scale · table[ids]: table (V, D), ids (T,) integers; one outside 0..V-1 (-1) has a row of zeros."""
+    lib = _llm_library()
+    x, ldt = _device_rows(table, (2,))
+    V, D = x.shape
+    i = _token_ids(ids)
+    T = i.shape[0]
+    y = _llm_out(out, (T, D), x.dtype, "out")
+    _llm_call(lib.gen9blas_embedding, 1 if x.dtype is _torch.float32 else 0, T, V, D, x.data_ptr(), ldt, i.data_ptr(), i.element_size(),
+              scale, y.data_ptr(), D if out is None else _out_step(y, "out"))
+    return _host_like(table, y) if out is None else y
+
+
+def embedding_backward(dY, ids, rows, scale=1.0, out=None, accumulate=False):
+    """The gradient of embedding()'s table of `rows` rows from dY (T, D) and its ids: row v is scale times the sum of dY over the
+    tokens that are v, in their order; rows without tokens are zeros. out may be float32 for float16 dY. accumulate: added
+    to the given out, where rows without tokens stay as they are."""
+    lib = _llm_library()
+    dy, lddy = _device_rows(dY, (2,))
+    (T, D), t = dy.shape, dy.dtype
+    i = _token_ids(ids)
+    if i.shape[0] != T:
+        raise ValueError(f"{i.shape[0]} ids for {T} rows of dY")
+    if rows > _LONGEST:
+        raise ValueError(f"{rows} rows; the most are {_LONGEST}")
+    if out is None and accumulate:
+        raise ValueError("accumulate needs out")
+    f32 = _torch.float32
+    g = _llm_out(out, (rows, D), f32 if out is not None and out.dtype is f32 else t, "out")
+    _llm_call(lib.gen9blas_embedding_backward, 1 if t is f32 else 0, T, rows, D, dy.data_ptr(), lddy, i.data_ptr(), i.element_size(), scale,
+              1 if g.dtype is f32 else 0, g.data_ptr(), D if out is None else _out_step(g, "out"), bool(accumulate))
+    return _host_like(dY, g) if out is None else g

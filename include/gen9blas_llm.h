@@ -1,4 +1,6 @@
-// gen9blas MI355X: operators of large language models on 4-bit weights and mixtures of experts (libgen9blas_llm.so).
+// gen9blas MI355X: operators of large language models (libgen9blas_llm.so): 4-bit weights, mixtures of experts, and what
+// stands around the products of a transformer's layer: linear layers with their bias, activation, dropout and residual, layer
+// norm, dropout and embeddings, each with its gradients.
 //
 // These entry points have no counterpart in the reference. They live in a library of their own, beside libgen9blas.so
 // (which exports the reference's surface only), and run on its stream and device: gen9blas_init opens the device,
@@ -79,6 +81,50 @@ GEN9BLAS_API int gen9blas_moe_route(int type, int T, int E, const void *logits, 
 GEN9BLAS_API int gen9blas_moe_gemm(int type, int T, int S, const int *ids, const void *X, int64_t ldt, int64_t lds,
                                    const gen9blas_mx4 *W, const gen9blas_mx4 *gate, const float *weights, void *C,
                                    int64_t ldct, int64_t ldcs);
+
+// ---- Linear layers ----
+// Weights are N×K (a row for each output); biases, norms' weights and their gradients are FP32 whatever the type is.
+enum { GEN9BLAS_ACT_NONE = 0, GEN9BLAS_ACT_RELU = 1, GEN9BLAS_ACT_GELU = 2, GEN9BLAS_ACT_GELU_TANH = 3, GEN9BLAS_ACT_SILU = 4 };
+// Y (M×N) = R + dropout(act(Z)), Z = X·Wᵀ + bias (X M×K, W N×K, 1 <= K < 2^22), in FP32, rounded once.
+// - bias (N floats), R (M×N) and Z may be NULL; Z: where the pre-activations go, which the gradients need if there is an activation.
+// - act: max(z, 0); z·Φ(z); its tanh form 0.5·z·(1 + tanh(√(2/π)·(z + 0.044715·z³))); z / (1 + e^−z).
+// - p, seed, offset: as in gen9blas_dropout (p = 0: none).
+GEN9BLAS_API int gen9blas_linear(int type, int M, int N, int K, const void *X, int ldx, const void *W, int ldw, const float *bias, int act,
+                                 void *Z, int ldz, double p, uint64_t seed, uint64_t offset, const void *R, int ldr, void *Y, int ldy);
+// Its gradients: dZ = act'(Z)·dropout(dY), rounded to the type for the products; dX (M×K) = dZ·W; dW (N×K) = dZᵀ·X; db (N floats) =
+// the column sums of dZ before that rounding. Each may be NULL, and what only it needs is not read then (Z: without an activation).
+// R's gradient is dY. accumulate: dW and db are added to what is there. M = 0: dW and db are zeros, or stay. The products are
+// gen9blas_gemm's, which wait unless gen9blas_set_nowait is on.
+GEN9BLAS_API int gen9blas_linear_backward(int type, int M, int N, int K, const void *dY, int lddy, const void *Z, int ldz, int act, double p,
+                                          uint64_t seed, uint64_t offset, const void *X, int ldx, const void *W, int ldw, void *dX, int lddx,
+                                          void *dW, int lddw, float *db, int accumulate);
+
+// ---- Layer norm ----
+// Y = (X − mean)·rstd·gamma + beta for each of M rows of N values, rstd = 1 / √(variance + eps) (of the population). gamma and beta
+// (N floats) may be NULL: ones and zeros. stats (M×2 floats, or NULL): mean and rstd of each row, for the gradients.
+GEN9BLAS_API int gen9blas_layer_norm(int type, int M, int N, const void *X, int ldx, const float *gamma, const float *beta, float eps, void *Y,
+                                     int ldy, float *stats);
+// Its gradients from dY, X and stats: dX, and sums over the rows in dgamma and dbeta (N floats); each may be NULL. accumulate: dgamma and
+// dbeta are added to what is there. M = 0: they are zeros, or stay.
+GEN9BLAS_API int gen9blas_layer_norm_backward(int type, int M, int N, const void *dY, int lddy, const void *X, int ldx, const float *stats,
+                                              const float *gamma, void *dX, int lddx, float *dgamma, float *dbeta, int accumulate);
+
+// ---- Dropout ----
+// Y (M×N) = R + X with a share p of its elements (0 <= p <= 1) replaced by zeros, whatever they were, and the others scaled; R may
+// be NULL. The mask is a function of place, seed and offset, so that the same call on the gradient is the backward pass: columns 8c ..
+// 8c+7 of row m take the 16-bit parts, low ones first, of Philox4x32-10 with the counter (c, m, offset, offset >> 32) and the
+// key (seed, seed >> 32); parts below limit = round(65536 p) are lost, the others scaled by 65536 / (65536 − limit).
+GEN9BLAS_API int gen9blas_dropout(int type, int M, int N, const void *X, int ldx, double p, uint64_t seed, uint64_t offset, const void *R,
+                                  int ldr, void *Y, int ldy);
+
+// ---- Embeddings ----
+// Y(t) = scale · table(ids[t]) for T tokens; table V×D; ids: T integers of id_bytes (4 or 8), dense. One outside 0..V−1 has a row of zeros.
+GEN9BLAS_API int gen9blas_embedding(int type, int T, int V, int D, const void *table, int ldt, const void *ids, int id_bytes, float scale,
+                                    void *Y, int ldy);
+// The table's gradient: dT(v) = scale · Σ dY(t) over the tokens t with ids[t] = v, in their order, summed in FP32; rows without tokens
+// are zeros. accumulate: added to what is there, rows without tokens stay. out_type, dT's: type, or GEN9BLAS_S.
+GEN9BLAS_API int gen9blas_embedding_backward(int type, int T, int V, int D, const void *dY, int lddy, const void *ids, int id_bytes, float scale,
+                                             int out_type, void *dT, int lddt, int accumulate);
 
 #ifdef __cplusplus
 }
