@@ -5,10 +5,13 @@
 
 namespace g9llm {
 
-// out[n] (+)= Σ_b parts[b·ld + n]: 64 columns a workgroup, 16 threads a column, each with every sixteenth block.
-static __global__ void __launch_bounds__(1024) column_sums_kernel(const float *__restrict__ parts, long long blocks, int N, long long ld, float *__restrict__ out, int accumulate) {
+// out[n] (+)= Σ_b parts[b·ld + n], and, blockIdx.y = 1, out2 of the N columns behind: 64 columns a workgroup, 16 threads a column, each
+// with every sixteenth block.
+static __global__ void __launch_bounds__(1024) column_sums_kernel(const float *__restrict__ parts, long long blocks, int N, long long ld, float *out, float *out2, int accumulate) {
     __shared__ float part[16][64];
     const int c = threadIdx.x & 63, r = threadIdx.x >> 6, n = blockIdx.x * 64 + c;
+    if (blockIdx.y) parts += N, out = out2;
+    if (!out) return;
     float s[4] = {};
     if (n < N) {
         long long b = r;
@@ -25,8 +28,8 @@ static __global__ void __launch_bounds__(1024) column_sums_kernel(const float *_
     for (int i = 0; i < 16; i++) sum += part[i][c];
     out[n] = accumulate ? out[n] + sum : sum;
 }
-static int column_sums(const float *parts, long long blocks, int N, long long ld, float *out, int accumulate) {
-    hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)cdiv(N, 64)), dim3(1024), 0, stream, parts, blocks, N, ld, out, accumulate);
+static int column_sums(const float *parts, long long blocks, int N, long long ld, float *out, float *out2, int accumulate) {
+    hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)cdiv(N, 64), out2 ? 2 : 1), dim3(1024), 0, stream, parts, blocks, N, ld, out, out2, accumulate);
     G9_HIP(hipGetLastError());
     return 0;
 }

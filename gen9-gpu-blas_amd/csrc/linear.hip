@@ -236,7 +236,7 @@ static int backward(int type, int M, int N, int K, const T *dY, int lddy, const 
         else if (a.kind == KIND_SIGMOID) run(linear_back_kernel<T, KIND_SIGMOID>);
         else run(linear_back_kernel<T, KIND_ERF>);
         G9_HIP(hipGetLastError());
-        if (db) G9_TRY(column_sums(sums, blocks, N, N, db, accumulate));
+        if (db) G9_TRY(column_sums(sums, blocks, N, N, db, nullptr, accumulate));
     }
     const T *g = own ? dZ : dY;
     auto product = [&](int tA, int m, int n, int k, const void *A, int lda, const void *B, int ldb, double beta, void *C, int ldc) -> int {

@@ -3,103 +3,362 @@
 #include "colsum.h"
 #include "rows.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace g9llm {
 
-// The sum of `v` over the workgroup's 256 threads, in all of them. `part`: four floats that no other sum still uses.
-__device__ __forceinline__ float block_sum(float v, float *part) {
+// A row is in the registers of L threads, C pieces of 16 bytes each, so that it is read once: its mean, the squares around it (the
+// second pass that a variance needs, without a second read) and its result come from there. L is 16, a wave, 256 or 1024.
+template <class T> struct Piece {
+    static constexpr int V = 16 / sizeof(T);
+    typedef T Vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+    // Elements n .. n + V − 1 of a row of N, zeros past its end. TAIL: the row may end inside a piece.
+    template <bool TAIL = true> static __device__ __forceinline__ Vec load(const T *row, int n, int N) {
+        if (n + V <= N) return *reinterpret_cast<const Vec *>(row + n);
+        Vec v = {};
+        if constexpr (TAIL)
 #pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return (part[0] + part[1]) + (part[2] + part[3]);
+            for (int e = 0; e < V; e++) v[e] = n + e < N ? row[n + e] : T(0);
+        return v;
+    }
+};
+// How many of V elements are left to a loop that has some left.
+template <bool TAIL, int V> __device__ __forceinline__ int some(int valid) { return TAIL ? valid : V; }
+// Sums of `v` over the L threads of a row, in all of them. part: the row's L / 64 · K floats of LDS, that no other sum uses before a barrier.
+template <int L, int K> __device__ __forceinline__ void row_sum(float *v, float *part) {
+#pragma unroll
+    for (int d = 1; d < (L < 64 ? L : 64); d <<= 1)
+#pragma unroll
+        for (int k = 0; k < K; k++) v[k] += __shfl_xor(v[k], d);
+    if constexpr (L > 64) {
+        const int w = (threadIdx.x >> 6) % (L / 64);
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int k = 0; k < K; k++) part[w * K + k] = v[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            v[k] = 0.f;
+#pragma unroll
+            for (int i = 0; i < L / 64; i++) v[k] += part[i * K + k];
+        }
+    }
 }
 
 // y = (x − mean)·rstd·gamma + beta, rstd = 1 / √(mean((x − mean)²) + eps). The mean of x − mean, what rounding has left of it, is
 // taken off again: a row whose mean is large against its values loses nothing that x has.
+template <class T, int L, int C, bool TAIL>
+__global__ void __launch_bounds__(L > 256 ? L : 256) norm_kernel(const T *__restrict__ X, long long ldx, const float *__restrict__ gamma, const float *__restrict__ beta, float eps,
+                                                                 int M, int N, T *__restrict__ Y, long long ldy, float *__restrict__ stats) {
+    using P = Piece<T>;
+    constexpr int V = P::V, ROWS = (L > 256 ? L : 256) / L;
+    __shared__ float part[L > 64 ? 3 * (L / 64) : 1];
+    const int t = threadIdx.x % L;
+    const long long m = (long long)blockIdx.x * ROWS + threadIdx.x / L;
+    if (L <= 64 && m >= M) return;   // whole rows of threads, and no barrier below
+    const T *x = X + m * ldx;
+    typename P::Vec v[C];
+#pragma unroll
+    for (int c = 0; c < C; c++) v[c] = P::template load<TAIL>(x, (c * L + t) * V, N);
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int e = 0; e < V; e++) s[0] += (float)v[c][e];
+    row_sum<L, 1>(s, part);
+    const float inv = 1.f / N, mean = s[0] * inv;
+    s[0] = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        const int valid = N - (c * L + t) * V;
+        if (valid <= 0) break;
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            const float d = !TAIL || e < valid ? (float)v[c][e] - mean : 0.f;
+            s[0] += d, s[1] = __builtin_fmaf(d, d, s[1]);
+        }
+    }
+    row_sum<L, 2>(s, part + (L > 64 ? L / 64 : 0));
+    const float left = s[0] * inv, rstd = 1.f / sqrtf(fmaxf(s[1] * inv - left * left, 0.f) + eps);
+    if (stats && t == 0) *reinterpret_cast<float2 *>(stats + 2 * m) = float2{mean + left, rstd};
+    T *y = Y + m * ldy;
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        const int n = (c * L + t) * V, valid = some<TAIL, V>(N - n);
+        if (n >= N) break;
+        float g[V], b[V];
+        if (gamma) load_some<V>(gamma + n, valid, g);
+        if (beta) load_some<V>(beta + n, valid, b);
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            const float z = (((float)v[c][e] - mean) - left) * rstd;
+            b[e] = (gamma ? z * g[e] : z) + (beta ? b[e] : 0.f);
+        }
+        store_some<V>(y + n, valid, b);
+    }
+}
+// Rows too long for the registers of a workgroup: three passes over memory.
 template <class T>
-__global__ void __launch_bounds__(256) norm_kernel(const T *__restrict__ X, long long ldx, const float *__restrict__ gamma, const float *__restrict__ beta, float eps, int N,
-                                                   T *__restrict__ Y, long long ldy, float *__restrict__ stats) {
-    __shared__ float part[3][4];
+__global__ void __launch_bounds__(1024) norm_long_kernel(const T *__restrict__ X, long long ldx, const float *__restrict__ gamma, const float *__restrict__ beta, float eps, int N,
+                                                         T *__restrict__ Y, long long ldy, float *__restrict__ stats) {
+    using P = Piece<T>;
+    constexpr int V = P::V;
+    __shared__ float part[48];
     const T *x = X + (long long)blockIdx.x * ldx;
     T *y = Y + (long long)blockIdx.x * ldy;
-    float s = 0.f;
-    for (int n = threadIdx.x; n < N; n += 256) s += (float)x[n];
-    const float mean = block_sum(s, part[0]) / N;
-    float d = 0.f, q = 0.f;
-    for (int n = threadIdx.x; n < N; n += 256) {
-        const float v = (float)x[n] - mean;
-        d += v, q = __builtin_fmaf(v, v, q);
+    float s[2] = {0.f, 0.f};
+    for (long long n = threadIdx.x * V; n < N; n += 1024 * V) {
+        const typename P::Vec v = P::load(x, (int)n, N);
+#pragma unroll
+        for (int e = 0; e < V; e++) s[0] += (float)v[e];
     }
-    const float left = block_sum(d, part[1]) / N, var = block_sum(q, part[2]) / N - left * left, rstd = 1.f / sqrtf(fmaxf(var, 0.f) + eps);
-    for (int n = threadIdx.x; n < N; n += 256) {
-        const float v = ((float)x[n] - mean - left) * rstd;
-        y[n] = (T)(v * (gamma ? gamma[n] : 1.f) + (beta ? beta[n] : 0.f));
+    row_sum<1024, 1>(s, part);
+    const float inv = 1.f / N, mean = s[0] * inv;
+    s[0] = 0.f;
+    for (long long n = threadIdx.x * V; n < N; n += 1024 * V) {
+        const typename P::Vec v = P::load(x, (int)n, N);
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            const float d = n + e < N ? (float)v[e] - mean : 0.f;
+            s[0] += d, s[1] = __builtin_fmaf(d, d, s[1]);
+        }
     }
-    if (stats && threadIdx.x == 0) stats[2LL * blockIdx.x] = mean + left, stats[2LL * blockIdx.x + 1] = rstd;
+    row_sum<1024, 2>(s, part + 16);
+    const float left = s[0] * inv, rstd = 1.f / sqrtf(fmaxf(s[1] * inv - left * left, 0.f) + eps);
+    if (stats && threadIdx.x == 0) *reinterpret_cast<float2 *>(stats + 2LL * blockIdx.x) = float2{mean + left, rstd};
+    for (long long n = threadIdx.x * V; n < N; n += 1024 * V) {
+        const typename P::Vec v = P::load(x, (int)n, N);
+        const int valid = (int)(N - n);
+        float g[V], b[V];
+        if (gamma) load_some<V>(gamma + n, valid, g);
+        if (beta) load_some<V>(beta + n, valid, b);
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            const float z = (((float)v[e] - mean) - left) * rstd;
+            b[e] = (gamma ? z * g[e] : z) + (beta ? b[e] : 0.f);
+        }
+        store_some<V>(y + n, valid, b);
+    }
 }
 
-// dx = rstd·(g − mean(g) − x̂·mean(g·x̂)), g = dy·gamma, x̂ = (x − mean)·rstd.
-template <class T>
-__global__ void __launch_bounds__(256) norm_back_kernel(const T *__restrict__ dY, long long lddy, const T *__restrict__ X, long long ldx, const float *__restrict__ stats,
-                                                        const float *__restrict__ gamma, int N, T *__restrict__ dX, long long lddx) {
-    __shared__ float part[2][4];
-    const T *x = X + (long long)blockIdx.x * ldx, *dy = dY + (long long)blockIdx.x * lddy;
-    T *dx = dX + (long long)blockIdx.x * lddx;
-    const float mean = stats[2LL * blockIdx.x], rstd = stats[2LL * blockIdx.x + 1];
-    float a = 0.f, b = 0.f;
-    for (int n = threadIdx.x; n < N; n += 256) {
-        const float g = (float)dy[n] * (gamma ? gamma[n] : 1.f);
-        a += g, b = __builtin_fmaf(g, ((float)x[n] - mean) * rstd, b);
+struct BackArgs {
+    const void *dY, *X;
+    long long lddy, ldx;
+    const float *stats, *gamma;
+    int M, N;
+    void *dX;              // or null
+    long long lddx;
+    float *sums;           // or null: rows of 2N, the sums of dy·x̂ and of dy of each workgroup's rows
+    float *dgamma, *dbeta; // where one workgroup has all rows: the results (each may be null), and no sums
+    int accumulate;
+};
+// dx = rstd·(g − mean(g) − x̂·mean(g·x̂)), g = dy·gamma, x̂ = (x − mean)·rstd, and the sums over the rows that dgamma and dbeta
+// need, from one read of x and dy. The workgroups go through the rows with a stride; a thread adds up its own columns, and the
+// row groups of a workgroup are added in their order.
+template <class T, int L, int C, int B, bool TAIL>
+__global__ void __launch_bounds__(B) norm_back_kernel(BackArgs a) {
+    using P = Piece<T>;
+    constexpr int V = P::V, ROWS = B / L;
+    __shared__ float part[2][L > 64 ? 2 * (B / 64) : 1];
+    __shared__ float join[ROWS > 1 ? L * V * 2 : 1];
+    const int t = threadIdx.x % L, group = threadIdx.x / L, N = a.N;
+    const float inv = 1.f / N;
+    float sg[C][V] = {}, sb[C][V] = {};
+    int flip = 0;
+    for (long long m0 = (long long)blockIdx.x * ROWS; m0 < a.M; m0 += (long long)gridDim.x * ROWS, flip ^= 1) {
+        const bool is = ROWS == 1 || m0 + group < a.M;   // a row group without a row goes along where the others wait for it
+        if (L <= 64 && !is) break;
+        const long long m = is ? m0 + group : a.M - 1;
+        const T *x = (const T *)a.X + m * a.ldx, *dy = (const T *)a.dY + m * a.lddy;
+        const float2 st = *reinterpret_cast<const float2 *>(a.stats + 2 * m);
+        const float mean = st.x, rstd = st.y;
+        typename P::Vec vx[C], vd[C];
+#pragma unroll
+        for (int c = 0; c < C; c++) vx[c] = P::template load<TAIL>(x, (c * L + t) * V, N), vd[c] = P::template load<TAIL>(dy, (c * L + t) * V, N);
+        float s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const int n = (c * L + t) * V, valid = some<TAIL, V>(N - n);
+            if (n >= N || (L > 64 && !is)) break;
+            float g[V];
+            if (a.gamma) load_some<V>(a.gamma + n, valid, g);
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const float d = (float)vd[c][e], xh = ((float)vx[c][e] - mean) * rstd, w = a.gamma ? d * g[e] : d;
+                s[0] += w, s[1] = __builtin_fmaf(w, xh, s[1]);
+                sg[c][e] = __builtin_fmaf(d, xh, sg[c][e]), sb[c][e] += d;
+            }
+        }
+        if (!a.dX) continue;
+        row_sum<L, 2>(s, part[flip] + (L > 64 ? group * (L / 64) * 2 : 0));
+        const float p = s[0] * inv, q = s[1] * inv;
+        T *dx = (T *)a.dX + m * a.lddx;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const int n = (c * L + t) * V, valid = some<TAIL, V>(N - n);
+            if (n >= N || (L > 64 && !is)) break;
+            float g[V];
+            if (a.gamma) load_some<V>(a.gamma + n, valid, g);
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const float d = (float)vd[c][e], xh = ((float)vx[c][e] - mean) * rstd;
+                g[e] = rstd * ((a.gamma ? d * g[e] : d) - p - xh * q);
+            }
+            store_some<V>(dx + n, valid, g);
+        }
     }
-    a = block_sum(a, part[0]) / N, b = block_sum(b, part[1]) / N;
-    for (int n = threadIdx.x; n < N; n += 256) {
-        const float g = (float)dy[n] * (gamma ? gamma[n] : 1.f);
-        dx[n] = (T)(rstd * (g - a - ((float)x[n] - mean) * rstd * b));
+    if (!a.sums && !a.dgamma && !a.dbeta) return;
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        const int n = (c * L + t) * V, valid = some<TAIL, V>(N - n);
+        if constexpr (ROWS > 1) {
+            for (int r = 1; r < ROWS; r++) {
+                __syncthreads();
+                if (group == r)
+#pragma unroll
+                    for (int e = 0; e < V; e++) join[e * L + t] = sg[c][e], join[(V + e) * L + t] = sb[c][e];
+                __syncthreads();
+                if (group == 0)
+#pragma unroll
+                    for (int e = 0; e < V; e++) sg[c][e] += join[e * L + t], sb[c][e] += join[(V + e) * L + t];
+            }
+        }
+        if (group || n >= N) continue;
+        if (a.sums) {
+            store_some<V>(a.sums + 2LL * blockIdx.x * N + n, valid, sg[c]);
+            store_some<V>(a.sums + (2LL * blockIdx.x + 1) * N + n, valid, sb[c]);
+            continue;
+        }
+        auto put = [&](float *out, float *v) {
+            if (!out) return;
+            float old[V];
+            if (a.accumulate) {
+                load_some<V>(out + n, valid, old);
+#pragma unroll
+                for (int e = 0; e < V; e++) v[e] += old[e];
+            }
+            store_some<V>(out + n, valid, v);
+        };
+        put(a.dgamma, sg[c]);
+        put(a.dbeta, sb[c]);
     }
 }
 
-// Sums of dy·x̂ and of dy over blocks of rows: part 2b and 2b + 1 of N.
+// Rows too long for that: dx alone, from two passes over x and dy, and the sums by themselves.
 template <class T>
-__global__ void __launch_bounds__(256) norm_sums_kernel(const T *__restrict__ dY, long long lddy, const T *__restrict__ X, long long ldx, const float *__restrict__ stats,
-                                                        int M, int N, int rows, float *__restrict__ sums) {
+__global__ void __launch_bounds__(1024) norm_back_long_kernel(BackArgs a) {
+    using P = Piece<T>;
+    constexpr int V = P::V;
+    __shared__ float part[32];
+    const T *x = (const T *)a.X + blockIdx.x * a.ldx, *dy = (const T *)a.dY + blockIdx.x * a.lddy;
+    T *dx = (T *)a.dX + blockIdx.x * a.lddx;
+    const float mean = a.stats[2LL * blockIdx.x], rstd = a.stats[2LL * blockIdx.x + 1], inv = 1.f / a.N;
+    float s[2] = {0.f, 0.f};
+    auto each = [&](auto use) {
+        for (long long n = threadIdx.x * V; n < a.N; n += 1024 * V) {
+            const typename P::Vec vx = P::load(x, (int)n, a.N), vd = P::load(dy, (int)n, a.N);
+            const int valid = (int)(a.N - n);
+            float g[V], xh[V];
+            if (a.gamma) load_some<V>(a.gamma + n, valid, g);
+#pragma unroll
+            for (int e = 0; e < V; e++) g[e] = a.gamma ? (float)vd[e] * g[e] : (float)vd[e], xh[e] = ((float)vx[e] - mean) * rstd;
+            use(n, valid, g, xh);
+        }
+    };
+    each([&](long long, int valid, const float *g, const float *xh) {
+#pragma unroll
+        for (int e = 0; e < V; e++) s[0] += g[e], s[1] += e < valid ? g[e] * xh[e] : 0.f;
+    });
+    row_sum<1024, 2>(s, part);
+    const float p = s[0] * inv, q = s[1] * inv;
+    each([&](long long n, int valid, float *g, const float *xh) {
+#pragma unroll
+        for (int e = 0; e < V; e++) g[e] = rstd * (g[e] - p - xh[e] * q);
+        store_some<V>(dx + n, valid, g);
+    });
+}
+template <class T>
+__global__ void __launch_bounds__(256) norm_sums_long_kernel(BackArgs a, int rows) {
     const int n = blockIdx.x * 256 + threadIdx.x;
-    if (n >= N) return;
-    const long long m0 = (long long)blockIdx.y * rows, m1 = min(m0 + rows, (long long)M);
-    float a = 0.f, b = 0.f;
+    if (n >= a.N) return;
+    const long long m0 = (long long)blockIdx.y * rows, m1 = min(m0 + rows, (long long)a.M);
+    float g = 0.f, b = 0.f;
     for (long long m = m0; m < m1; m++) {
-        const float g = (float)dY[m * lddy + n];
-        a = __builtin_fmaf(g, ((float)X[m * ldx + n] - stats[2 * m]) * stats[2 * m + 1], a), b += g;
+        const float d = (float)((const T *)a.dY)[m * a.lddy + n];
+        g = __builtin_fmaf(d, ((float)((const T *)a.X)[m * a.ldx + n] - a.stats[2 * m]) * a.stats[2 * m + 1], g), b += d;
     }
-    sums[2LL * blockIdx.y * N + n] = a;
-    sums[(2LL * blockIdx.y + 1) * N + n] = b;
+    a.sums[2LL * blockIdx.y * a.N + n] = g;
+    a.sums[(2LL * blockIdx.y + 1) * a.N + n] = b;
+}
+
+// f(L, C, TAIL) for rows of N elements of T by the first pair of threads and pieces that holds them, or false.
+template <int L_, int C_> struct Shape { static constexpr int L = L_, C = C_; };
+template <class T, class F, class... S> static bool by_length(int N, F f, S... shapes) {
+    constexpr int V = 16 / (int)sizeof(T);
+    auto take = [&](auto s) {
+        if (cdiv(N, V) > s.L * s.C) return false;
+        if (N % V) f(s, std::true_type{});
+        else f(s, std::false_type{});
+        return true;
+    };
+    return (take(shapes) || ...);
 }
 
 template <class T>
 static int norm(int M, int N, const T *X, int ldx, const float *gamma, const float *beta, float eps, T *Y, int ldy, float *stats) {
-    return by_rows(M, 256, [&](long long m0, unsigned rows) -> int {
-        hipLaunchKernelGGL((norm_kernel<T>), dim3(rows), dim3(256), 0, stream, X + m0 * ldx, ldx, gamma, beta, eps, N, Y + m0 * ldy, ldy, stats ? stats + 2 * m0 : nullptr);
+    int rc = 0;
+    const bool fits = by_length<T>(N, [&](auto shape, auto tail) {
+        constexpr int L = shape.L, C = shape.C, ROWS = 256 / L;
+        rc = by_rows(cdiv(M, ROWS), 256, [&](long long b0, unsigned blocks) -> int {
+            const long long m0 = b0 * ROWS;
+            hipLaunchKernelGGL((norm_kernel<T, L, C, tail()>), dim3(blocks), dim3(256), 0, stream, X + m0 * ldx, ldx, gamma, beta, eps, (int)(M - m0), N, Y + m0 * ldy, ldy, stats ? stats + 2 * m0 : nullptr);
+            G9_HIP(hipGetLastError());
+            return 0;
+        });
+    }, Shape<16, 1>(), Shape<16, 2>(), Shape<64, 1>(), Shape<64, 2>(), Shape<64, 4>(), Shape<64, 8>(), Shape<256, 4>(), Shape<256, 8>());
+    if (fits) return rc;
+    return by_rows(M, 1024, [&](long long m0, unsigned rows) -> int {
+        hipLaunchKernelGGL((norm_long_kernel<T>), dim3(rows), dim3(1024), 0, stream, X + m0 * ldx, ldx, gamma, beta, eps, N, Y + m0 * ldy, ldy, stats ? stats + 2 * m0 : nullptr);
         G9_HIP(hipGetLastError());
         return 0;
     });
 }
-template <class T>
-static int norm_back(int M, int N, const T *dY, int lddy, const T *X, int ldx, const float *stats, const float *gamma, T *dX, int lddx, float *dgamma, float *dbeta, int accumulate) {
-    if (dX)
-        G9_TRY(by_rows(M, 256, [&](long long m0, unsigned rows) -> int {
-            hipLaunchKernelGGL((norm_back_kernel<T>), dim3(rows), dim3(256), 0, stream, dY + m0 * lddy, lddy, X + m0 * ldx, ldx, stats + 2 * m0, gamma, N, dX + m0 * lddx, lddx);
+template <class T> static int norm_back(BackArgs a) {
+    int rc = 0;
+    void *sums = nullptr;
+    float *dgamma = a.dgamma, *dbeta = a.dbeta;
+    const bool both = dgamma || dbeta;
+    const bool fits = by_length<T>(a.N, [&](auto shape, auto tail) {
+        constexpr int L = shape.L, C = shape.C, B = L > 512 ? L : 512, ROWS = B / L;
+        const int blocks = (int)std::min(cdiv(a.M, 4LL * ROWS), (long long)num_cus * (1024 / B));
+        auto run = [&]() -> int {
+            if (both && blocks > 1) {
+                G9_TRY(scratch(SLOT_SUMS, (size_t)blocks * 2 * a.N * 4, &sums));
+                a.sums = (float *)sums;
+            }
+            hipLaunchKernelGGL((norm_back_kernel<T, L, C, B, tail()>), dim3(blocks), dim3(B), 0, stream, a);
+            G9_HIP(hipGetLastError());
+            return a.sums ? column_sums((float *)sums, blocks, a.N, 2LL * a.N, dgamma, dbeta, a.accumulate) : 0;
+        };
+        rc = run();
+    }, Shape<16, 1>(), Shape<16, 2>(), Shape<64, 1>(), Shape<64, 2>(), Shape<64, 4>(), Shape<256, 2>(), Shape<256, 4>(), Shape<1024, 2>());
+    if (fits) return rc;
+    if (a.dX)
+        G9_TRY(by_rows(a.M, 1024, [&](long long m0, unsigned rows) -> int {
+            BackArgs b = a;
+            b.dY = (const T *)a.dY + m0 * a.lddy, b.X = (const T *)a.X + m0 * a.ldx, b.stats = a.stats + 2 * m0, b.dX = (T *)a.dX + m0 * a.lddx;
+            hipLaunchKernelGGL((norm_back_long_kernel<T>), dim3(rows), dim3(1024), 0, stream, b);
             G9_HIP(hipGetLastError());
             return 0;
         }));
-    if (dgamma || dbeta) {
-        const int rows = (int)std::max(32LL, cdiv(M, 512));
-        const long long blocks = cdiv(M, rows);
-        void *sums;
-        G9_TRY(scratch(SLOT_SUMS, (size_t)blocks * 2 * N * 4, &sums));
-        hipLaunchKernelGGL((norm_sums_kernel<T>), dim3((unsigned)cdiv(N, 256), (unsigned)blocks), dim3(256), 0, stream, dY, lddy, X, ldx, stats, M, N, rows, (float *)sums);
+    if (both) {
+        const int rows = (int)std::max(32LL, cdiv(a.M, 512));
+        const long long blocks = cdiv(a.M, rows);
+        G9_TRY(scratch(SLOT_SUMS, (size_t)blocks * 2 * a.N * 4, &sums));
+        a.sums = (float *)sums;
+        hipLaunchKernelGGL((norm_sums_long_kernel<T>), dim3((unsigned)cdiv(a.N, 256), (unsigned)blocks), dim3(256), 0, stream, a, rows);
         G9_HIP(hipGetLastError());
-        if (dgamma) G9_TRY(column_sums((float *)sums, blocks, N, 2LL * N, dgamma, accumulate));
-        if (dbeta) G9_TRY(column_sums((float *)sums + N, blocks, N, 2LL * N, dbeta, accumulate));
+        G9_TRY(column_sums((float *)sums, blocks, a.N, 2LL * a.N, dgamma, dbeta, a.accumulate));
     }
     return 0;
 }
@@ -146,8 +405,8 @@ int gen9blas_layer_norm_backward(int type, int M, int N, const void *dY, int ldd
         if (dgamma) G9_TRY(zero_rows(dgamma, 4LL * N, 1, 4LL * N));
         return dbeta ? zero_rows(dbeta, 4LL * N, 1, 4LL * N) : 0;
     }
-    return type == GEN9BLAS_H ? norm_back(M, N, (const _Float16 *)dY, lddy, (const _Float16 *)X, ldx, stats, gamma, (_Float16 *)dX, lddx, dgamma, dbeta, accumulate)
-                              : norm_back(M, N, (const float *)dY, lddy, (const float *)X, ldx, stats, gamma, (float *)dX, lddx, dgamma, dbeta, accumulate);
+    const BackArgs a = {dY, X, lddy, ldx, stats, gamma, M, N, dX, lddx, nullptr, dgamma, dbeta, accumulate};
+    return type == GEN9BLAS_H ? norm_back<_Float16>(a) : norm_back<float>(a);
 }
 
 }  // extern "C"
