@@ -509,11 +509,13 @@ __global__ void __launch_bounds__(WM *WN * 64) hgemm_kernel(Par p) {
             for (int pp = 0; pp < TN / 2; pp++) {
                 const int n = n0 + wn * WTN + 32 * pp + 8 * g;
                 const auto cols = p.epilogue.template columns<8>(n, p.N - n);
+                const auto row = [&](int j) { return m0 + wm * WTM + j * 16 + (lane & 15); };
+                decltype(p.epilogue.template residual<8>(0, 0, 0, 0)) res[TM];
 #pragma unroll
-                for (int j = 0; j < TM; j++) {
-                    const int m = m0 + wm * WTM + j * 16 + (lane & 15);
-                    if (m < p.M) p.epilogue.template row<f16, 8>(kind, C, p.ldc, m, n, cols, p.N - n, acc[2 * pp][j], acc[2 * pp + 1][j]);
-                }
+                for (int j = 0; j < TM; j++) res[j] = p.epilogue.template residual<8>(row(j), p.M, n, p.N - n);
+#pragma unroll
+                for (int j = 0; j < TM; j++)
+                    if (row(j) < p.M) p.epilogue.template row<f16, 8>(kind, C, p.ldc, row(j), n, cols, res[j], p.N - n, acc[2 * pp][j], acc[2 * pp + 1][j]);
             }
         });
         return;
@@ -563,7 +565,7 @@ __global__ void __launch_bounds__(256) split_sum(Par p, int slices) {
         hi += P[s * slice + 64];
     }
     if constexpr (requires { p.epilogue; })
-        p.epilogue.each([&](auto kind) { p.epilogue.template row<f16, 8>(kind, p.C, p.ldc, m, n, p.epilogue.template columns<8>(n, p.N - n), p.N - n, lo, hi); });
+        p.epilogue.each([&](auto kind) { p.epilogue.template row<f16, 8>(kind, p.C, p.ldc, m, n, p.epilogue.template columns<8>(n, p.N - n), p.epilogue.template residual<8>(m, p.M, n, p.N - n), p.N - n, lo, hi); });
     else store8(p.C + (long long)m * p.ldc + n, lo, hi, p.alpha, p.beta, p.N - n);
 }
 

@@ -11,6 +11,7 @@
 #include "sgemm_kernel.h"
 #include "sgemm_tiles.h"
 #include "skinny_kernel.h"
+#include "linear_rows_kernel.h"
 #include "colsum.h"
 #include <algorithm>
 
@@ -20,20 +21,22 @@ struct HParams : g9::hg::Params { Epilogue<_Float16> epilogue; };
 struct SParams : g9::sg::Params { Epilogue<float> epilogue; };
 template <class T> struct FewParams : g9::sk::Params { Epilogue<T> epilogue; };
 
-// Rows of K elements into rows of ldd (zeros past K).
+// Rows of K elements into rows of ldd, a multiple of 8 (zeros past K); a thread has eight of them.
 template <class T>
-__global__ void __launch_bounds__(256) pad_rows_kernel(const T *__restrict__ X, long long ldx, int K, T *__restrict__ D, int ldd, long long total) {
+__global__ void __launch_bounds__(256) pad_rows_kernel(const T *__restrict__ X, long long ldx, int K, T *__restrict__ D, int groups, long long total) {
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const long long r = i / ldd;
-        const int k = (int)(i % ldd);
-        D[i] = k < K ? X[r * ldx + k] : T(0);
+        const long long r = i / groups;
+        const int k = (int)(i % groups) * 8;
+        float v[8];
+        load_some<8>(X + r * ldx + k, K - k, v);
+        store_some<8>(D + i * 8, 8, v);
     }
 }
 template <class T> static int pad_rows(const void *X, long long ldx, long long rows, int K, int ldd, int slot, const T **D) {
     void *d;
-    const long long total = rows * ldd;
-    G9_TRY(scratch(slot, (size_t)total * sizeof(T), &d));
-    hipLaunchKernelGGL((pad_rows_kernel<T>), dim3((unsigned)std::min(cdiv(total, 256), 32LL * num_cus)), dim3(256), 0, stream, (const T *)X, ldx, K, (T *)d, ldd, total);
+    const long long total = rows * (ldd / 8);
+    G9_TRY(scratch(slot, (size_t)total * 8 * sizeof(T), &d));
+    hipLaunchKernelGGL((pad_rows_kernel<T>), dim3((unsigned)std::min(cdiv(total, 256), 32LL * num_cus)), dim3(256), 0, stream, (const T *)X, ldx, K, (T *)d, ldd / 8, total);
     G9_HIP(hipGetLastError());
     *D = (const T *)d;
     return 0;
@@ -47,8 +50,7 @@ static int check_grid(long long workgroups, int threads) {
 // The partial sums of a split k, 64 MiB: what the FP16 and FP32 products of libgen9blas.so have.
 constexpr size_t SPLIT_BYTES = 64u << 20;
 
-template <int I> static int launch_h(HParams p, int slices) {
-    constexpr g9::hgl::HgCfg G = g9::hgl::CFG[I];
+template <g9::hgl::HgCfg G> static int launch_h(HParams p, int slices) {
     constexpr int KB = g9::hgl::KB;
     p.tiles_m = (int)cdiv(p.M, G.BM), p.tiles_n = (int)cdiv(p.N, G.BN);
     const long long tiles = (long long)p.tiles_m * p.tiles_n;
@@ -74,18 +76,17 @@ static int tiles_product(HParams &p) {
     p.P = (float *)work;
     const Choice c = choose({p.M, p.N, p.K, 1, p.ldc, 0, 1}, SPLIT_BYTES, num_cus);
     switch (c.cfg) {
-    case 0: return launch_h<0>(p, c.slices);
-    case 1: return launch_h<1>(p, c.slices);
-    case 3: return launch_h<3>(p, c.slices);
-    case 4: return launch_h<4>(p, c.slices);
-    case 5: return launch_h<5>(p, c.slices);
-    case 6: return launch_h<6>(p, c.slices);
+    case 0: return launch_h<CFG[0]>(p, c.slices);
+    case 1: return launch_h<CFG[1]>(p, c.slices);
+    case 3: return launch_h<CFG[3]>(p, c.slices);
+    case 4: return launch_h<CFG[4]>(p, c.slices);
+    case 5: return launch_h<CFG[5]>(p, c.slices);
+    case 6: return launch_h<CFG[6]>(p, c.slices);
     }
-    return launch_h<2>(p, c.slices);
+    return launch_h<CFG[2]>(p, c.slices);
 }
 
-template <int I> static int launch_s(SParams p, int slices) {
-    constexpr g9::sgl::SgCfg G = g9::sgl::CFG[I];
+template <g9::sgl::SgCfg G> static int launch_s(SParams p, int slices) {
     p.tiles_m = (int)cdiv(p.M, G.BM), p.tiles_n = (int)cdiv(p.N, G.BN);
     const long long tiles = (long long)p.tiles_m * p.tiles_n;
     const dim3 block(G.WM * G.WN * 64);
@@ -109,11 +110,11 @@ static int tiles_product(SParams &p) {
     p.P = (float *)work;
     const Choice c = choose({p.M, p.N, p.K, 1}, SPLIT_BYTES, false, false, num_cus);
     switch (c.cfg) {
-    case 1: return launch_s<1>(p, c.slices);
-    case 3: return launch_s<3>(p, c.slices);
-    case 4: return launch_s<4>(p, c.slices);
+    case 1: return launch_s<CFG[1]>(p, c.slices);
+    case 3: return launch_s<CFG[3]>(p, c.slices);
+    case 4: return launch_s<CFG[4]>(p, c.slices);
     }
-    return launch_s<2>(p, c.slices);
+    return launch_s<CFG[2]>(p, c.slices);
 }
 
 // Up to 16 rows: the weights streamed once, as gen9blas_gemm's few rows are (skinny.hip has what chose the shapes).
@@ -142,26 +143,61 @@ template <class T> static int few_rows(const FewParams<T> &p, bool vec) {
 #undef G9_FEW
 }
 
+template <class T, int MT, int NS> static int some_rows(RowsArgs<T> a) {
+    const long long tiles = cdiv(a.N, 64);
+    const int pieces = (int)cdiv(a.K, 512 / sizeof(T));
+    a.per = (int)cdiv(pieces, std::max(1LL, std::min<long long>(pieces, num_cus / tiles)));
+    a.slices = (int)cdiv(pieces, a.per);
+    if (a.slices > 1) G9_TRY(scratch(SLOT_PART, (size_t)a.slices * tiles * 4 * MT * 1024, (void **)&a.parts));
+    G9_TRY(check_grid(tiles * a.slices, 512));
+    hipLaunchKernelGGL((linear_rows_kernel<T, MT, NS>), dim3((unsigned)(tiles * a.slices)), dim3(512), 0, stream, a);
+    G9_HIP(hipGetLastError());
+    if (a.slices > 1) hipLaunchKernelGGL((linear_rows_sum_kernel<T, MT>), dim3((unsigned)(tiles * MT)), dim3(256), 0, stream, a, (int)tiles);
+    G9_HIP(hipGetLastError());
+    return 0;
+}
+
+// Whether linear_rows_kernel takes M rows, by what it and the others measure (µs, it / others).
+// - FP32 up to 64 rows, of 8 M weights: 32 × 4096 × 2048 (at 4 M alike) and 16 × 8192 × 1024 13 / 19, 32 × 4096 × 11008 45 / 65, 64 of them
+//   60 / 67, 5 to 8 rows from 32 M on, 8 × 11008 × 4096 33 / 41. Not 4 × 4096 × 11008 41 / 34, nor more than 48 rows where the columns
+//   alone make as many workgroups as there can be, and leave CUs without one: 64 × 11008 × 4096 78 / 67.
+// - FP16 up to 32 rows, of 32 M weights: 32 × 4096 × 11008 23 / 25, 32 × 11008 × 4096 20.6 / 24.1 (32 × 4096 × 4096 13 / 13); up to 16, which
+//   the streaming kernel takes without a second one, only where no slices of k are needed: 16 × 11008 × 4096 18.5 / 22.7, but 16 × 4096 ×
+//   11008 21.7 / 19.2.
+template <class T> static bool takes_rows(int M, int N, int K) {
+    const long long weights = (long long)N * K;
+    const bool alone = cdiv(N, 64) * 2 > num_cus;   // one slice of k
+    if (sizeof(T) == 4) return weights >= (M > 8 ? 8 << 20 : 32 << 20) && M > 4 && M <= (alone ? 48 : 64);
+    return weights >= 32 << 20 && M <= 32 && (M > 16 || (alone && M > 2));
+}
+
 template <class T>
 static int linear(int M, int N, int K, const T *X, long long ldx, const T *W, long long ldw, const Epilogue<T> &e, T *Y, long long ldy) {
-    if (M <= 16) {
+    constexpr int KB = sizeof(T) == 2 ? g9::hgl::KB : g9::sgl::KB;
+    // The kernels on direct copies take more than one k-step of k, FP16 operands at 4-byte alignment with even row strides, and rows
+    // of a tile within 4 GiB; for these, others are copied first, and a short k is filled up with zeros.
+    auto copied = [&](const T *p, long long ld) { return K < KB || ld * 256 * (long long)sizeof(T) >= 1LL << 32 || (sizeof(T) == 2 && ((uintptr_t)p % 4 || ld % 2)); };
+    const bool cx = copied(X, ldx), cw = copied(W, ldw), some = M <= 64 && takes_rows<T>(M, N, K);
+    if (M <= 16 && (!some || cx || cw)) {
         FewParams<T> p{};
         p.a = X, p.w = W, p.C = Y, p.sam = ldx, p.swn = ldw, p.scm = ldy, p.scn = 1, p.M = M, p.N = N, p.K = K, p.epilogue = e;
         constexpr int V = 16 / sizeof(T);
         return few_rows<T>(p, (uintptr_t)X % 16 == 0 && (uintptr_t)W % 16 == 0 && ldx % V == 0 && ldw % V == 0);
     }
-    // The tile kernels take more than one k-step of k, FP16 operands at 4-byte alignment with even row strides, and rows
-    // of a tile within 4 GiB; others are copied first, and a short k is filled up with zeros.
-    constexpr int KB = sizeof(T) == 2 ? g9::hgl::KB : g9::sgl::KB;
     const int Kp = K < KB ? KB : K, ldp = (int)cdiv(Kp, 8) * 8;
-    auto copied = [&](const T *p, long long ld) { return K < KB || ld * 256 * (long long)sizeof(T) >= 1LL << 32 || (sizeof(T) == 2 && ((uintptr_t)p % 4 || ld % 2)); };
-    if (copied(X, ldx)) {
+    if (cx) {
         G9_TRY(pad_rows(X, ldx, M, K, ldp, SLOT_X, &X));
         ldx = ldp;
     }
-    if (copied(W, ldw)) {
+    if (cw) {
         G9_TRY(pad_rows(W, ldw, N, K, ldp, SLOT_W, &W));
         ldw = ldp;
+    }
+    if (some) {
+        const RowsArgs<T> a = {X, W, Y, ldx, ldw, ldy, M, N, Kp, 1, 0, nullptr, e};
+        if (M <= 16) return some_rows<T, 1, 3>(a);
+        if (M <= 32) return some_rows<T, 2, 3>(a);
+        if constexpr (sizeof(T) == 4) return M <= 48 ? some_rows<T, 3, 2>(a) : some_rows<T, 4, 2>(a);
     }
     std::conditional_t<sizeof(T) == 2, HParams, SParams> p{};
     p.A = X, p.B = W, p.C = Y, p.lda = ldx, p.ldb = ldw, p.ldc = ldy, p.M = M, p.N = N, p.K = Kp, p.alpha = 1.f, p.epilogue = e;
@@ -169,37 +205,51 @@ static int linear(int M, int N, int K, const T *X, long long ldx, const T *W, lo
 }
 
 // dZ = act'(Z) · dropout(dY) and, for each block of `rows` rows, the sums of its columns (before they are rounded). A workgroup
-// has 2^cols threads side by side, eight columns each, and the others below them. dZ and Z may be null (no activation:
-// dZ = dropout(dY)).
+// has 2^cols threads side by side, eight columns each, and the others below them, each with every (256 >> cols)th row of the
+// block, four of them on their way at once. dZ and Z may be null (no activation: dZ = dropout(dY)).
 template <class T, int KIND>
 __global__ void __launch_bounds__(256) linear_back_kernel(const T *__restrict__ dY, long long lddy, const T *__restrict__ Z, long long ldz, Activation act, Dropout d,
                                                           int M, int N, int rows, int cols, T *__restrict__ dZ, long long lddz, float *__restrict__ sums) {
-    constexpr int V = 8;
+    constexpr int V = 8, U = 4;
     __shared__ float part[256][V + 1];
-    const int ct = 1 << cols, c = threadIdx.x & (ct - 1), r = threadIdx.x >> cols, n = ((blockIdx.x << cols) + c) * V, valid = N - n;
+    const int ct = 1 << cols, c = threadIdx.x & (ct - 1), r = threadIdx.x >> cols, step = 256 >> cols, n = ((blockIdx.x << cols) + c) * V, valid = N - n;
     const long long block = blockIdx.y, m0 = block * rows, m1 = min(m0 + rows, (long long)M);
     float sum[V] = {};
-    if (valid > 0)
-        for (long long m = m0 + r; m < m1; m += 256 >> cols) {
-            float v[V];
-            load_some<V>(dY + m * lddy + n, valid, v);
-            if (d.limit) drop<V>(d, (unsigned)m, n, v);
-            if (Z) {
-                float z[V];
-                load_some<V>(Z + m * ldz + n, valid, z);
+    auto row = [&](long long m, float *v, const float *z) {
+        if (d.limit) drop<V>(d, (unsigned)m, n, v);
+        if (Z)
 #pragma unroll
-                for (int e = 0; e < V; e++) v[e] *= slope<T, KIND>(act, z[e]);
+            for (int e = 0; e < V; e++) v[e] *= slope<T, KIND>(act, z[e]);
+        if (dZ) store_some<V>(dZ + m * lddz + n, valid, v);
+#pragma unroll
+        for (int e = 0; e < V; e++) sum[e] += v[e];
+    };
+    long long m = m0 + r;
+    if (valid >= V) {
+        for (; m + (U - 1) * step < m1; m += U * step) {
+            float v[U][V], z[U][V];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                load_some<V>(dY + (m + u * step) * lddy + n, V, v[u]);
+                if (Z) load_some<V>(Z + (m + u * step) * ldz + n, V, z[u]);
             }
-            if (dZ) store_some<V>(dZ + m * lddz + n, valid, v);
 #pragma unroll
-            for (int e = 0; e < V; e++) sum[e] += v[e];
+            for (int u = 0; u < U; u++) row(m + u * step, v[u], z[u]);
+        }
+    }
+    if (valid > 0)
+        for (; m < m1; m += step) {
+            float v[V], z[V];
+            load_some<V>(dY + m * lddy + n, valid, v);
+            if (Z) load_some<V>(Z + m * ldz + n, valid, z);
+            row(m, v, z);
         }
     if (!sums) return;
 #pragma unroll
     for (int e = 0; e < V; e++) part[threadIdx.x][e] = sum[e];
     __syncthreads();
     if (r || valid <= 0) return;
-    for (int i = 1; i < 256 >> cols; i++)
+    for (int i = 1; i < step; i++)
 #pragma unroll
         for (int e = 0; e < V; e++) sum[e] += part[(i << cols) + c][e];
     store_some<V>(sums + block * N + n, valid, sum);
@@ -218,7 +268,7 @@ static int backward(int type, int M, int N, int K, const T *dY, int lddy, const 
         dZ = (T *)p;
     }
     float *sums = nullptr;
-    const int rows = (int)std::max(32LL, cdiv(M, 512));
+    const int rows = (int)std::max(64LL, cdiv(M, 512));
     const long long blocks = cdiv(M, rows);
     if (db) {
         G9_TRY(scratch(SLOT_SUMS, (size_t)blocks * N * 4, &p));
@@ -227,7 +277,7 @@ static int backward(int type, int M, int N, int K, const T *dY, int lddy, const 
     if (dZ || db) {
         const Activation a = make_act(act);
         int cols = 0;
-        while (cols < 8 && (8 << cols) < N) cols++;
+        while (cols < 5 && (8 << cols) < N) cols++;
         const dim3 grid((unsigned)cdiv(N, 8 << cols), (unsigned)blocks);
         auto run = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, dY, lddy, act ? Z : nullptr, ldz, a, d, M, N, rows, cols, dZ, lddz, sums);

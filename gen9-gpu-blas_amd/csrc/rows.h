@@ -23,13 +23,15 @@ template <int V, class T> __device__ __forceinline__ void load_some(const T *p, 
 #pragma unroll
         for (int e = 0; e < V; e++) v[e] = e < valid ? (float)p[e] : 0.f;
 }
-template <int V, class T> __device__ __forceinline__ void store_some(T *p, int valid, const float *v) {
+// PAST: past the caches, for what nothing reads soon.
+template <int V, class T, bool PAST = false> __device__ __forceinline__ void store_some(T *p, int valid, const float *v) {
     typedef T TV __attribute__((ext_vector_type(V), aligned(sizeof(T))));
     if (valid >= V) {
         TV q;
 #pragma unroll
         for (int e = 0; e < V; e++) q[e] = (T)v[e];
-        *reinterpret_cast<TV *>(p) = q;
+        if constexpr (PAST) __builtin_nontemporal_store(q, reinterpret_cast<TV *>(p));
+        else *reinterpret_cast<TV *>(p) = q;
     } else
 #pragma unroll
         for (int e = 0; e < V; e++)

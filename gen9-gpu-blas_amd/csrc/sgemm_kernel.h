@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(WM *WN * 64) sgemm_kernel(Par p) {
                     for (int j = 0; j < TM; j++) {
                         const int m = m0 + wm * WTM + 32 * j + (lane & 31);
                         const f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                        if (m < p.M) p.epilogue.template row<float, 4>(kind, C, p.ldc, m, n, cols, p.N - n, v);
+                        if (m < p.M) p.epilogue.template row<float, 4>(kind, C, p.ldc, m, n, cols, p.epilogue.template residual<4>(m, p.M, n, p.N - n), p.N - n, v);
                     }
                 }
         });
@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(256) split_sum(Par p, int slices, int tiles) {
     f32x4 v = P[0];
     for (int s = 1; s < slices; s++) v += P[s * slice];
     if constexpr (requires { p.epilogue; })
-        p.epilogue.each([&](auto kind) { p.epilogue.template row<float, 4>(kind, p.C, p.ldc, m, n, p.epilogue.template columns<4>(n, p.N - n), p.N - n, v); });
+        p.epilogue.each([&](auto kind) { p.epilogue.template row<float, 4>(kind, p.C, p.ldc, m, n, p.epilogue.template columns<4>(n, p.N - n), p.epilogue.template residual<4>(m, p.M, n, p.N - n), p.N - n, v); });
     else store4<TRI>(p.C + (long long)m * p.ldc + n, v, p.alpha, p.beta, m, n, p.N, TRI != 0 && m0 == n0);
 }
 

@@ -129,6 +129,15 @@ def test_linear_tiles(g9, torch_dev, dtype, M, N, K):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K", [(3, 8300, 4090), (8, 8200, 4224), (12, 2100, 4100), (16, 8193, 4352), (17, 4100, 8320), (24, 5000, 8000), (32, 8256, 4100), (33, 3000, 2817),
+                                   (40, 9000, 3900), (47, 2100, 4096), (64, 2050, 4224), (64, 8300, 1100), (30, 34000, 1000)])
+@pytest.mark.parametrize("pad,shift", [(0, 0), (2, 2), (3, 1)])
+def test_linear_of_some_rows(g9, torch_dev, dtype, M, N, K, pad, shift):
+    """Large weights under few rows: whole and cut pieces of k, columns that end inside a workgroup's."""
+    check_linear(g9, torch_dev, dtype, M, N, K, "silu", residual=True, save=pad > 0, pad=pad, shift=shift)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("name", ACTS)
 def test_activations_over_their_range(g9, torch_dev, dtype, name):
     """Z straight from the bias: every size of argument, both zeros, infinities and NaN (which ReLU keeps, too)."""
