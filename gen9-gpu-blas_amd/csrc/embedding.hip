@@ -41,6 +41,25 @@ __global__ void __launch_bounds__(256) embedding_kernel(const T *__restrict__ ta
     }
 }
 
+// Rows without tokens are cleared in groups of CLEAR, whole rows, so that what is written at a time lies together.
+constexpr int CLEAR = 16;
+struct ClearArgs {
+    const uint8_t *has;   // of each row whether it has tokens
+    void *out;
+    long long ldo;
+    int V, D, groups, cols;   // 2^cols threads side by side
+};
+template <class O> __device__ __forceinline__ void clear_rows(const ClearArgs &a, long long group) {
+    constexpr int E = 8;
+    const float none[E] = {};
+    const long long v0 = group * CLEAR;
+    const int lane = threadIdx.x & 63, c = threadIdx.x & ((1 << a.cols) - 1);
+    const unsigned long long empty = __ballot(lane < CLEAR && v0 + lane < a.V && !a.has[min(v0 + lane, a.V - 1LL)]);
+    for (int r = threadIdx.x >> a.cols; r < CLEAR; r += (int)blockDim.x >> a.cols)
+        if (empty >> r & 1)
+            for (int x = c * E; x < a.D; x += E << a.cols) store_some<E, O, true>((O *)a.out + (v0 + r) * a.ldo + x, a.D - x, none);
+}
+
 // ---- the sort: least digits first, 8 bits a pass ----
 // A workgroup has `per` consecutive places (a multiple of 1024). The first pass reads the ids themselves; the last place of a list
 // of n is n − 1.
@@ -50,8 +69,14 @@ __device__ __forceinline__ void place(const Ids &ids, const Sorted &in, long lon
     if (in.key) key = in.key[i], at = in.at[i];
     else key = ids.key(i, V), at = (int)i;
 }
-// counts[workgroup][digit]; the first pass clears the marks of the rows that have tokens, too.
-__global__ void __launch_bounds__(256) sort_count_kernel(Ids ids, Sorted in, int n, int V, int shift, int per, int *__restrict__ counts, uint8_t *__restrict__ has) {
+// counts[workgroup][digit]; the first pass clears the marks of the rows that have tokens, too. From the second pass on the marks are
+// set, and workgroups behind the `groups` of the sort, which leave most CUs idle, clear rows from group `first` on.
+template <class O>
+__global__ void __launch_bounds__(256) sort_count_kernel(Ids ids, Sorted in, int n, int V, int shift, int per, int *__restrict__ counts, uint8_t *__restrict__ has, int groups, ClearArgs clear, int first) {
+    if ((int)blockIdx.x >= groups) {
+        clear_rows<O>(clear, first + blockIdx.x - groups);
+        return;
+    }
     __shared__ int count[256];
     count[threadIdx.x] = 0;
     if (has)
@@ -66,35 +91,44 @@ __global__ void __launch_bounds__(256) sort_count_kernel(Ids ids, Sorted in, int
     counts[blockIdx.x * 256 + threadIdx.x] = count[threadIdx.x];
 }
 // Where a workgroup's places of a digit begin: all places of smaller digits, and this digit's of the workgroups before.
-// Within 1024 places, a wave counts its lanes of a digit by ballots, and the waves' counts are added in their order.
-__global__ void __launch_bounds__(1024) sort_place_kernel(Ids ids, Sorted in, int n, int V, int shift, int per, const int *__restrict__ counts, Sorted out, uint8_t *__restrict__ has) {
-    __shared__ int base[256], all[256], wave_count[16][256];
+// Within 1024 places, a wave counts its lanes of a digit by ballots, and the waves' counts are added in their order. Latencies bound
+// it: 16384 tokens 6 µs a pass (9 with the sums over digits by barriers, and the waves' counts read one after the other).
+template <class O>
+__global__ void __launch_bounds__(1024) sort_place_kernel(Ids ids, Sorted in, int n, int V, int shift, int per, const int *__restrict__ counts, Sorted out, uint8_t *__restrict__ has, int groups, ClearArgs clear, int from) {
+    if ((int)blockIdx.x >= groups) {
+        clear_rows<O>(clear, from + blockIdx.x - groups);
+        return;
+    }
+    __shared__ int waves[4], wave_count[16][256];
     const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+    const long long begin = (long long)blockIdx.x * per, end = min((long long)n, begin + per);
+    int key = 0, at = 0;
+    if (begin + t < end) place(ids, in, begin + t, V, key, at);   // on its way while the places are found
+    for (int i = t; i < 16 * 256; i += 1024) (&wave_count[0][0])[i] = 0;
+    int base = 0;   // threads 0..255: of the digit with this number
     if (t < 256) {
         int before = 0, total = 0;
-        for (int b = 0; b < (int)gridDim.x; b++) {
+#pragma unroll 8
+        for (int b = 0; b < groups; b++) {
             const int c = counts[b * 256 + t];
-            if (b < (int)blockIdx.x) before += c;
+            before += b < (int)blockIdx.x ? c : 0;
             total += c;
         }
-        base[t] = before, all[t] = total;
+        int sum = total;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int v = __shfl_up(sum, d);
+            if (lane >= d) sum += v;
+        }
+        if (lane == 63) waves[wv] = sum;
+        base = before + sum - total;
     }
     __syncthreads();
-    for (int d = 1; d < 256; d <<= 1) {   // sums up to each digit
-        const int v = t < 256 && t >= d ? all[t - d] : 0;
-        __syncthreads();
-        if (t < 256) all[t] += v;
-        __syncthreads();
-    }
-    if (t > 0 && t < 256) base[t] += all[t - 1];
-    const long long end = min((long long)n, (blockIdx.x + 1LL) * per);
-    for (long long i0 = (long long)blockIdx.x * per; i0 < end; i0 += 1024) {
-        for (int i = t; i < 16 * 256; i += 1024) (&wave_count[0][0])[i] = 0;
-        __syncthreads();
+    if (t < 256)
+        for (int w = 0; w < wv; w++) base += waves[w];
+    for (long long i0 = begin; i0 < end; i0 += 1024) {
         const long long i = i0 + t;
         const bool mine = i < end;
-        int key = 0, at = 0;
-        if (mine) place(ids, in, i, V, key, at);
         const int digit = key >> shift & 255;
         unsigned long long same = __ballot(mine);
 #pragma unroll
@@ -107,13 +141,14 @@ __global__ void __launch_bounds__(1024) sort_place_kernel(Ids ids, Sorted in, in
         if (mine && rank == 0) wave_count[wv][digit] = __popcll(same);
         __syncthreads();
         if (t < 256) {
-            int at0 = base[t];
+            int c[16];
+#pragma unroll
+            for (int w = 0; w < 16; w++) c[w] = wave_count[w][t];
+#pragma unroll
             for (int w = 0; w < 16; w++) {
-                const int c = wave_count[w][t];
-                wave_count[w][t] = at0;
-                at0 += c;
+                wave_count[w][t] = base;
+                base += c[w];
             }
-            base[t] = at0;
         }
         __syncthreads();
         if (mine) {
@@ -121,8 +156,83 @@ __global__ void __launch_bounds__(1024) sort_place_kernel(Ids ids, Sorted in, in
             out.key[to] = key, out.at[to] = at;
             if (has && key < V) has[key] = 1;
         }
+        if (i0 + 1024 >= end) break;
+        if (i + 1024 < end) place(ids, in, i + 1024, V, key, at);
+        __syncthreads();
+        for (int j = t; j < 16 * 256; j += 1024) (&wave_count[0][0])[j] = 0;
         __syncthreads();
     }
+}
+
+// Up to 4096 tokens: the whole sort in one workgroup, in LDS.
+constexpr int SMALL = 4096;
+__global__ void __launch_bounds__(1024) sort_small_kernel(Ids ids, int n, int V, int bits, Sorted out, uint8_t *__restrict__ has) {
+    __shared__ int keys[2][SMALL], ats[2][SMALL], waves[4], wave_count[16][256], base[256];
+    const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+    if (has)
+        for (int v = t * 16; v < V; v += 1024 * 16) *reinterpret_cast<u32x4 *>(has + v) = u32x4{0, 0, 0, 0};   // rounded up to 16
+    __syncthreads();
+    for (int i = t; i < n; i += 1024) {
+        const int key = ids.key(i, V);
+        keys[0][i] = key, ats[0][i] = i;
+        if (has && key < V) has[key] = 1;
+    }
+    int from = 0;
+    for (int shift = 0; shift < bits; shift += 8, from ^= 1) {
+        if (t < 256) base[t] = 0;
+        __syncthreads();
+        for (int i = t; i < n; i += 1024) atomicAdd(&base[keys[from][i] >> shift & 255], 1);
+        __syncthreads();
+        int mine = 0, sum = 0;
+        if (t < 256) {
+            mine = sum = base[t];
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int v = __shfl_up(sum, d);
+                if (lane >= d) sum += v;
+            }
+            if (lane == 63) waves[wv] = sum;
+        }
+        __syncthreads();
+        if (t < 256) {
+            sum -= mine;
+            for (int w = 0; w < wv; w++) sum += waves[w];
+        }
+        for (int i0 = 0; i0 < n; i0 += 1024) {
+            for (int j = t; j < 16 * 256; j += 1024) (&wave_count[0][0])[j] = 0;
+            __syncthreads();
+            const int i = i0 + t;
+            const bool is = i < n;
+            const int key = is ? keys[from][i] : 0, digit = key >> shift & 255;
+            unsigned long long same = __ballot(is);
+#pragma unroll
+            for (int b = 0; b < 8; b++) {
+                const bool bit = digit >> b & 1;
+                const unsigned long long set = __ballot(bit);
+                same &= bit ? set : ~set;
+            }
+            const int rank = __popcll(same & ((1ULL << lane) - 1));
+            if (is && rank == 0) wave_count[wv][digit] = __popcll(same);
+            __syncthreads();
+            if (t < 256) {
+                int c[16];
+#pragma unroll
+                for (int w = 0; w < 16; w++) c[w] = wave_count[w][t];
+#pragma unroll
+                for (int w = 0; w < 16; w++) {
+                    wave_count[w][t] = sum;
+                    sum += c[w];
+                }
+            }
+            __syncthreads();
+            if (is) {
+                const int to = wave_count[wv][digit] + rank;
+                keys[from ^ 1][to] = key, ats[from ^ 1][to] = ats[from][i];
+            }
+            __syncthreads();
+        }
+    }
+    for (int i = t; i < n; i += 1024) out.key[i] = keys[from][i], out.at[i] = ats[from][i];
 }
 
 // ---- the sums ----
@@ -130,7 +240,6 @@ struct GradArgs {
     const void *dY;
     long long lddy;
     Sorted s;
-    const uint8_t *has;   // null: rows without tokens stay
     void *out;
     long long ldo;
     float *parts;         // two rows of ldp for each piece
@@ -144,63 +253,76 @@ template <class T, int E> __device__ __forceinline__ void put(const GradArgs &a,
     if (a.accumulate) load_some<E>(o, a.D - d, v);
 #pragma unroll
     for (int e = 0; e < E; e++) v[e] = a.accumulate ? __builtin_fmaf(sum[e], a.scale, v[e]) : sum[e] * a.scale;
-    store_some<E>(o, a.D - d, v);
+    store_some<E, T, true>(o, a.D - d, v);
 }
-// 2^cols threads side by side have 8 columns each; blockIdx.x: pieces, then groups of 64 rows to clear; blockIdx.y: columns.
+// 2^cols threads side by side have 8 columns each; blockIdx.x: pieces (blockIdx.y: their columns), then groups of rows to clear.
 template <class T, class O>
-__global__ void __launch_bounds__(256) embedding_grad_kernel(GradArgs a) {
-    constexpr int E = 8;
+__global__ void __launch_bounds__(256) embedding_grad_kernel(GradArgs a, ClearArgs clear, int cleared) {
+    constexpr int E = 8, U = 8;
     const int c = threadIdx.x & ((1 << a.cols) - 1), side = threadIdx.x >> a.cols, sides = 256 >> a.cols;
     const int d = ((blockIdx.y << a.cols) + c) * E;
-    if (d >= a.D) return;
     const int piece_groups = (a.pieces + sides - 1) / sides;
     if ((int)blockIdx.x >= piece_groups) {
-        const float none[E] = {};
-        const int v0 = (blockIdx.x - piece_groups) * 64;
-        for (int v = v0 + side; v < min(v0 + 64, a.V); v += sides)
-            if (!a.has[v]) store_some<E>((O *)a.out + v * a.ldo + d, a.D - d, none);
+        clear_rows<O>(clear, cleared + (long long)(blockIdx.x - piece_groups) * gridDim.y + blockIdx.y);
         return;
     }
+    if (d >= a.D) return;
     const int piece = blockIdx.x * sides + side;
     if (piece >= a.pieces) return;
     const int i0 = piece * a.per, i1 = (int)min((long long)i0 + a.per, (long long)a.n);
     const int before = i0 ? a.s.key[i0 - 1] : -1, behind = i1 < a.n ? a.s.key[i1] : -1;
     float sum[E] = {};
     int first = i0;
-    for (int i = i0; i < i1; i++) {
-        const int key = a.s.key[i];
-        if (key >= a.V) break;   // no row's: the end of the list
-        float v[E];
-        load_some<E>((const T *)a.dY + a.s.at[i] * a.lddy + d, a.D - d, v);
+    for (int i = i0; i < i1; i += U) {   // U rows on their way
+        int key[U + 1];
+        float v[U][E];
 #pragma unroll
-        for (int e = 0; e < E; e++) sum[e] += v[e];
-        const int next = i + 1 < i1 ? a.s.key[i + 1] : behind;
-        if (next == key && i + 1 < i1) continue;
-        if ((first == i0 && before == key) || next == key) store_some<E>(a.parts + (2LL * piece + (first > i0)) * a.ldp + d, a.D - d, sum);
-        else put<O, E>(a, key, d, sum);
+        for (int u = 0; u <= U; u++) key[u] = i + u < i1 ? a.s.key[i + u] : behind;
 #pragma unroll
-        for (int e = 0; e < E; e++) sum[e] = 0.f;
-        first = i + 1;
+        for (int u = 0; u < U; u++) load_some<E>((const T *)a.dY + a.s.at[min(i + u, i1 - 1)] * a.lddy + d, a.D - d, v[u]);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (i + u >= i1 || key[u] >= a.V) return;   // no row's: the end of the list
+#pragma unroll
+            for (int e = 0; e < E; e++) sum[e] += v[u][e];
+            if (key[u + 1] == key[u] && i + u + 1 < i1) continue;
+            if ((first == i0 && before == key[u]) || key[u + 1] == key[u]) store_some<E>(a.parts + (2LL * piece + (first > i0)) * a.ldp + d, a.D - d, sum);
+            else put<O, E>(a, key[u], d, sum);
+#pragma unroll
+            for (int e = 0; e < E; e++) sum[e] = 0.f;
+            first = i + u + 1;
+        }
     }
 }
 // Rows whose tokens begin in a piece and go on in others.
 template <class O>
 __global__ void __launch_bounds__(256) embedding_join_kernel(GradArgs a) {
-    constexpr int E = 8;
+    constexpr int E = 8, U = 8;
     const int c = threadIdx.x & ((1 << a.cols) - 1), side = threadIdx.x >> a.cols, sides = 256 >> a.cols;
     const int d = ((blockIdx.y << a.cols) + c) * E, piece = blockIdx.x * sides + side;
     if (d >= a.D || piece >= a.pieces - 1) return;
-    const int i0 = piece * a.per, i1 = i0 + a.per, key = a.s.key[i1 - 1];
-    if (key >= a.V || a.s.key[i1] != key) return;            // does not go on
-    const bool whole = a.s.key[i0] == key;
-    if (whole && i0 && a.s.key[i0 - 1] == key) return;       // begins in an earlier one
+    const int i0 = piece * a.per, i1 = i0 + a.per, key = a.s.key[i1 - 1], behind = a.s.key[i1], first = a.s.key[i0], before = i0 ? a.s.key[i0 - 1] : -1;
+    const bool whole = first == key;
+    if (key >= a.V || behind != key || (whole && before == key)) return;   // does not go on, or begins in an earlier one
     float sum[E];
     load_some<E>(a.parts + (2LL * piece + !whole) * a.ldp + d, a.D - d, sum);
-    for (int p = piece + 1; p < a.pieces && a.s.key[p * a.per] == key; p++) {
-        float v[E];
-        load_some<E>(a.parts + 2LL * p * a.ldp + d, a.D - d, v);
+    for (int p = piece + 1; p < a.pieces; p += U) {
+        int at[U];
+        float v[U][E];
 #pragma unroll
-        for (int e = 0; e < E; e++) sum[e] += v[e];
+        for (int u = 0; u < U; u++) at[u] = a.s.key[min(p + u, a.pieces - 1) * a.per];
+        int more = 0;   // pieces that go on with this row, of the next U
+#pragma unroll
+        for (int u = 0; u < U; u++) more += p + u < a.pieces && at[u] == key;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (u < more) load_some<E>(a.parts + 2LL * (p + u) * a.ldp + d, a.D - d, v[u]);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (u < more)
+#pragma unroll
+                for (int e = 0; e < E; e++) sum[e] += v[u][e];
+        if (more < U) break;
     }
     put<O, E>(a, key, d, sum);
 }
@@ -209,31 +331,47 @@ template <class T, class O>
 static int gradient(int n, int V, int D, const T *dY, int lddy, const Ids &ids, float scale, O *out, int ldo, int accumulate) {
     // places of a workgroup of the sort, and of a piece: few enough of both that what reads all of them stays short
     const int per = (int)(cdiv(cdiv(n, 256), 1024) * 1024), groups = (int)cdiv(n, per);
-    const int piece = (int)std::max(32LL, cdiv(n, 1024)), pieces = (int)cdiv(n, piece);
+    const int piece = (int)std::max(8LL, cdiv(n, 512)), pieces = (int)cdiv(n, piece);
     const long long ldp = cdiv(D, 8) * 8;
+    int cols = 0;
+    while (cols < 8 && (8 << cols) < D) cols++;
+    const unsigned slabs = (unsigned)cdiv(D, 8 << cols), piece_groups = (unsigned)cdiv(pieces, 256 >> cols);
+    if (slabs > 65535 || V > 1 << 27) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "embedding_backward: more rows or columns than one launch can index (V %d, D %d)", V, D);
     char *w;
-    const size_t lists = (size_t)n * 4, marks = ((size_t)V + 15) / 16 * 16;
+    const size_t lists = ((size_t)n * 4 + 15) / 16 * 16, marks = ((size_t)V + 15) / 16 * 16;
     G9_TRY(scratch(SLOT_SORT, 4 * lists + (size_t)groups * 1024 + marks, (void **)&w));
     Sorted s[2] = {{(int *)w, (int *)(w + lists)}, {(int *)(w + 2 * lists), (int *)(w + 3 * lists)}};
     int *counts = (int *)(w + 4 * lists);
     uint8_t *has = accumulate ? nullptr : (uint8_t *)(counts + groups * 256);
-    Sorted in = {nullptr, nullptr};
-    int bits = 1;
-    while (bits < 31 && V >> bits) bits++;   // of V, which stands for no row
-    for (int shift = 0, pass = 0; shift < bits; shift += 8, pass++) {
-        uint8_t *h = pass ? nullptr : has;
-        hipLaunchKernelGGL(sort_count_kernel, dim3(groups), dim3(256), 0, stream, ids, in, n, V, shift, per, counts, h);
-        hipLaunchKernelGGL(sort_place_kernel, dim3(groups), dim3(1024), 0, stream, ids, in, n, V, shift, per, (const int *)counts, s[pass & 1], h);
-        G9_HIP(hipGetLastError());
-        in = s[pass & 1];
-    }
     void *parts;
     G9_TRY(scratch(SLOT_SUMS, (size_t)pieces * 2 * ldp * 4, &parts));
-    GradArgs a = {dY, lddy, in, has, out, ldo, (float *)parts, ldp, scale, n, V, D, piece, pieces, 0, accumulate};
-    while (a.cols < 8 && (8 << a.cols) < D) a.cols++;
-    const unsigned slabs = (unsigned)cdiv(D, 8 << a.cols), piece_groups = (unsigned)cdiv(pieces, 256 >> a.cols);
-    if (slabs > 65535 || V > 1 << 29) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "embedding_backward: more rows or columns than one launch can index (V %d, D %d)", V, D);
-    hipLaunchKernelGGL((embedding_grad_kernel<T, O>), dim3(piece_groups + (has ? (unsigned)cdiv(V, 64) : 0), slabs), dim3(256), 0, stream, a);
+
+    const ClearArgs clear = {has, out, ldo, V, D, has ? (int)cdiv(V, CLEAR) : 0, cols};
+    int cleared = 0;   // groups of rows that the sort's launches have cleared
+    int bits = 1;
+    while (bits < 31 && V >> bits) bits++;   // of V, which stands for no row
+    Sorted in = {nullptr, nullptr};
+    // one workgroup clears a million marks in some 10 µs
+    if (n <= SMALL && (!has || V <= 1 << 20)) {
+        in = s[0];
+        hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(1024), 0, stream, ids, n, V, bits, in, has);
+    } else {
+        // what the idle CUs clear beside a launch of the sort: about 4 µs of writing, 24 MB
+        const int beside = (int)std::max<long long>(1, (24 << 20) / ((long long)CLEAR * D * (int)sizeof(O)));
+        for (int shift = 0, pass = 0; shift < bits; shift += 8, pass++) {
+            uint8_t *h = pass ? nullptr : has;
+            int more = pass ? std::min(beside, clear.groups - cleared) : 0;
+            hipLaunchKernelGGL((sort_count_kernel<O>), dim3(groups + more), dim3(256), 0, stream, ids, in, n, V, shift, per, counts, h, groups, clear, cleared);
+            cleared += more;
+            more = pass ? std::min(beside, clear.groups - cleared) : 0;
+            hipLaunchKernelGGL((sort_place_kernel<O>), dim3(groups + more), dim3(1024), 0, stream, ids, in, n, V, shift, per, (const int *)counts, s[pass & 1], h, groups, clear, cleared);
+            cleared += more;
+            in = s[pass & 1];
+        }
+    }
+    G9_HIP(hipGetLastError());
+    const GradArgs a = {dY, lddy, in, out, ldo, (float *)parts, ldp, scale, n, V, D, piece, pieces, cols, accumulate};
+    hipLaunchKernelGGL((embedding_grad_kernel<T, O>), dim3(piece_groups + (unsigned)cdiv(clear.groups - cleared, slabs), slabs), dim3(256), 0, stream, a, clear, cleared);
     G9_HIP(hipGetLastError());
     if (pieces > 1) hipLaunchKernelGGL((embedding_join_kernel<O>), dim3(piece_groups, slabs), dim3(256), 0, stream, a);
     G9_HIP(hipGetLastError());
