@@ -52,49 +52,62 @@ __global__ void __launch_bounds__(L > 256 ? L : 256) norm_kernel(const T *__rest
                                                                  int M, int N, T *__restrict__ Y, long long ldy, float *__restrict__ stats) {
     using P = Piece<T>;
     constexpr int V = P::V, ROWS = (L > 256 ? L : 256) / L;
-    __shared__ float part[L > 64 ? 3 * (L / 64) : 1];
+    constexpr bool KEEP = C * V <= 16;   // gamma and beta stay in registers from row to row
+    __shared__ float part[2][L > 64 ? 3 * (L / 64) : 1];
     const int t = threadIdx.x % L;
-    const long long m = (long long)blockIdx.x * ROWS + threadIdx.x / L;
-    if (L <= 64 && m >= M) return;   // whole rows of threads, and no barrier below
-    const T *x = X + m * ldx;
-    typename P::Vec v[C];
-#pragma unroll
-    for (int c = 0; c < C; c++) v[c] = P::template load<TAIL>(x, (c * L + t) * V, N);
-    float s[2] = {0.f, 0.f};
-#pragma unroll
-    for (int c = 0; c < C; c++)
-#pragma unroll
-        for (int e = 0; e < V; e++) s[0] += (float)v[c][e];
-    row_sum<L, 1>(s, part);
-    const float inv = 1.f / N, mean = s[0] * inv;
-    s[0] = 0.f;
-#pragma unroll
-    for (int c = 0; c < C; c++) {
-        const int valid = N - (c * L + t) * V;
-        if (valid <= 0) break;
-#pragma unroll
-        for (int e = 0; e < V; e++) {
-            const float d = !TAIL || e < valid ? (float)v[c][e] - mean : 0.f;
-            s[0] += d, s[1] = __builtin_fmaf(d, d, s[1]);
-        }
-    }
-    row_sum<L, 2>(s, part + (L > 64 ? L / 64 : 0));
-    const float left = s[0] * inv, rstd = 1.f / sqrtf(fmaxf(s[1] * inv - left * left, 0.f) + eps);
-    if (stats && t == 0) *reinterpret_cast<float2 *>(stats + 2 * m) = float2{mean + left, rstd};
-    T *y = Y + m * ldy;
-#pragma unroll
-    for (int c = 0; c < C; c++) {
+    const float inv = 1.f / N;
+    float g[KEEP ? C : 1][V], b[KEEP ? C : 1][V];
+    auto weights = [&](int c, float *gc, float *bc) {
         const int n = (c * L + t) * V, valid = some<TAIL, V>(N - n);
-        if (n >= N) break;
-        float g[V], b[V];
-        if (gamma) load_some<V>(gamma + n, valid, g);
-        if (beta) load_some<V>(beta + n, valid, b);
 #pragma unroll
-        for (int e = 0; e < V; e++) {
-            const float z = (((float)v[c][e] - mean) - left) * rstd;
-            b[e] = (gamma ? z * g[e] : z) + (beta ? b[e] : 0.f);
+        for (int e = 0; e < V; e++) gc[e] = 1.f, bc[e] = 0.f;
+        if (n >= N) return;
+        if (gamma) load_some<V>(gamma + n, valid, gc);
+        if (beta) load_some<V>(beta + n, valid, bc);
+    };
+    if constexpr (KEEP)
+#pragma unroll
+        for (int c = 0; c < C; c++) weights(c, g[c], b[c]);
+    int flip = 0;
+    for (long long m0 = (long long)blockIdx.x * ROWS; m0 < M; m0 += (long long)gridDim.x * ROWS, flip ^= 1) {
+        const long long m = m0 + threadIdx.x / L;
+        if (L <= 64 && m >= M) break;   // whole rows of threads, and no barrier below
+        const T *x = X + m * ldx;
+        typename P::Vec v[C];
+#pragma unroll
+        for (int c = 0; c < C; c++) v[c] = P::template load<TAIL>(x, (c * L + t) * V, N);
+        float s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+            for (int e = 0; e < V; e++) s[0] += (float)v[c][e];
+        row_sum<L, 1>(s, part[flip]);
+        const float mean = s[0] * inv;
+        s[0] = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const int valid = N - (c * L + t) * V;
+            if (valid <= 0) break;
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const float d = !TAIL || e < valid ? (float)v[c][e] - mean : 0.f;
+                s[0] += d, s[1] = __builtin_fmaf(d, d, s[1]);
+            }
         }
-        store_some<V>(y + n, valid, b);
+        row_sum<L, 2>(s, part[flip] + (L > 64 ? L / 64 : 0));
+        const float left = s[0] * inv, rstd = 1.f / sqrtf(fmaxf(s[1] * inv - left * left, 0.f) + eps);
+        if (stats && t == 0) *reinterpret_cast<float2 *>(stats + 2 * m) = float2{mean + left, rstd};
+        T *y = Y + m * ldy;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const int n = (c * L + t) * V, valid = some<TAIL, V>(N - n);
+            if (n >= N) break;
+            float gn[V], bn[V];
+            if constexpr (!KEEP) weights(c, gn, bn);
+#pragma unroll
+            for (int e = 0; e < V; e++) bn[e] = __builtin_fmaf((((float)v[c][e] - mean) - left) * rstd, KEEP ? g[KEEP ? c : 0][e] : gn[e], KEEP ? b[KEEP ? c : 0][e] : bn[e]);
+            store_some<V>(y + n, valid, bn);
+        }
     }
 }
 // Rows too long for the registers of a workgroup: three passes over memory.
@@ -159,12 +172,23 @@ template <class T, int L, int C, int B, bool TAIL>
 __global__ void __launch_bounds__(B) norm_back_kernel(BackArgs a) {
     using P = Piece<T>;
     constexpr int V = P::V, ROWS = B / L;
+    constexpr bool KEEP = C * V <= 16;   // gamma stays in registers from row to row
     __shared__ float part[2][L > 64 ? 2 * (B / 64) : 1];
-    __shared__ float join[ROWS > 1 ? L * V * 2 : 1];
+    __shared__ float join[ROWS > 1 ? 2 * V : 1][ROWS > 2 ? B + 64 / V : ROWS > 1 ? L : 1];   // reads of V by 64 / V lie in different banks
     const int t = threadIdx.x % L, group = threadIdx.x / L, N = a.N;
     const float inv = 1.f / N;
     float sg[C][V] = {}, sb[C][V] = {};
     int flip = 0;
+    float keep[KEEP ? C : 1][V];
+    auto weights = [&](int c, float *g) {
+        const int n = (c * L + t) * V;
+#pragma unroll
+        for (int e = 0; e < V; e++) g[e] = 1.f;
+        if (a.gamma && n < N) load_some<V>(a.gamma + n, some<TAIL, V>(N - n), g);
+    };
+    if constexpr (KEEP)
+#pragma unroll
+        for (int c = 0; c < C; c++) weights(c, keep[c]);
     for (long long m0 = (long long)blockIdx.x * ROWS; m0 < a.M; m0 += (long long)gridDim.x * ROWS, flip ^= 1) {
         const bool is = ROWS == 1 || m0 + group < a.M;   // a row group without a row goes along where the others wait for it
         if (L <= 64 && !is) break;
@@ -178,13 +202,12 @@ __global__ void __launch_bounds__(B) norm_back_kernel(BackArgs a) {
         float s[2] = {0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < C; c++) {
-            const int n = (c * L + t) * V, valid = some<TAIL, V>(N - n);
-            if (n >= N || (L > 64 && !is)) break;
+            if ((c * L + t) * V >= N || (L > 64 && !is)) break;
             float g[V];
-            if (a.gamma) load_some<V>(a.gamma + n, valid, g);
+            if constexpr (!KEEP) weights(c, g);
 #pragma unroll
             for (int e = 0; e < V; e++) {
-                const float d = (float)vd[c][e], xh = ((float)vx[c][e] - mean) * rstd, w = a.gamma ? d * g[e] : d;
+                const float d = (float)vd[c][e], xh = ((float)vx[c][e] - mean) * rstd, w = d * (KEEP ? keep[KEEP ? c : 0][e] : g[e]);
                 s[0] += w, s[1] = __builtin_fmaf(w, xh, s[1]);
                 sg[c][e] = __builtin_fmaf(d, xh, sg[c][e]), sb[c][e] += d;
             }
@@ -198,49 +221,65 @@ __global__ void __launch_bounds__(B) norm_back_kernel(BackArgs a) {
             const int n = (c * L + t) * V, valid = some<TAIL, V>(N - n);
             if (n >= N || (L > 64 && !is)) break;
             float g[V];
-            if (a.gamma) load_some<V>(a.gamma + n, valid, g);
+            if constexpr (!KEEP) weights(c, g);
 #pragma unroll
             for (int e = 0; e < V; e++) {
                 const float d = (float)vd[c][e], xh = ((float)vx[c][e] - mean) * rstd;
-                g[e] = rstd * ((a.gamma ? d * g[e] : d) - p - xh * q);
+                g[e] = rstd * (d * (KEEP ? keep[KEEP ? c : 0][e] : g[e]) - p - xh * q);
             }
             store_some<V>(dx + n, valid, g);
         }
     }
     if (!a.sums && !a.dgamma && !a.dbeta) return;
+    if constexpr (ROWS > 2) {
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < V; e++) join[e][threadIdx.x] = sg[c][e], join[V + e][threadIdx.x] = sb[c][e];
+            __syncthreads();
+            for (int o = threadIdx.x; o < 2 * V * L; o += B) {
+                const int beta = o / (V * L), at = o % (V * L), n = c * V * L + at;
+                float sum = 0.f;
+#pragma unroll
+                for (int r = 0; r < ROWS; r++) sum += join[beta * V + at % V][r * L + at / V];
+                if (n >= N) continue;
+                float *out = a.sums ? a.sums + (2LL * blockIdx.x + beta) * N : beta ? a.dbeta : a.dgamma;
+                if (out) out[n] = !a.sums && a.accumulate ? out[n] + sum : sum;
+            }
+        }
+        return;
+    }
+    if constexpr (ROWS == 2) {
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            __syncthreads();
+            if (group)
+#pragma unroll
+                for (int e = 0; e < V; e++) join[e][t] = sg[c][e], join[V + e][t] = sb[c][e];
+            __syncthreads();
+            if (!group)
+#pragma unroll
+                for (int e = 0; e < V; e++) sg[c][e] += join[e][t], sb[c][e] += join[V + e][t];
+        }
+        if (group) return;
+    }
 #pragma unroll
     for (int c = 0; c < C; c++) {
         const int n = (c * L + t) * V, valid = some<TAIL, V>(N - n);
-        if constexpr (ROWS > 1) {
-            for (int r = 1; r < ROWS; r++) {
-                __syncthreads();
-                if (group == r)
-#pragma unroll
-                    for (int e = 0; e < V; e++) join[e * L + t] = sg[c][e], join[(V + e) * L + t] = sb[c][e];
-                __syncthreads();
-                if (group == 0)
-#pragma unroll
-                    for (int e = 0; e < V; e++) sg[c][e] += join[e * L + t], sb[c][e] += join[(V + e) * L + t];
-            }
-        }
-        if (group || n >= N) continue;
-        if (a.sums) {
-            store_some<V>(a.sums + 2LL * blockIdx.x * N + n, valid, sg[c]);
-            store_some<V>(a.sums + (2LL * blockIdx.x + 1) * N + n, valid, sb[c]);
-            continue;
-        }
+        if (n >= N) break;
         auto put = [&](float *out, float *v) {
             if (!out) return;
             float old[V];
-            if (a.accumulate) {
+            if (!a.sums && a.accumulate) {
                 load_some<V>(out + n, valid, old);
 #pragma unroll
                 for (int e = 0; e < V; e++) v[e] += old[e];
             }
             store_some<V>(out + n, valid, v);
         };
-        put(a.dgamma, sg[c]);
-        put(a.dbeta, sb[c]);
+        put(a.sums ? a.sums + 2LL * blockIdx.x * N : a.dgamma, sg[c]);
+        put(a.sums ? a.sums + (2LL * blockIdx.x + 1) * N : a.dbeta, sb[c]);
     }
 }
 
@@ -308,14 +347,12 @@ template <class T>
 static int norm(int M, int N, const T *X, int ldx, const float *gamma, const float *beta, float eps, T *Y, int ldy, float *stats) {
     int rc = 0;
     const bool fits = by_length<T>(N, [&](auto shape, auto tail) {
-        constexpr int L = shape.L, C = shape.C, ROWS = 256 / L;
-        rc = by_rows(cdiv(M, ROWS), 256, [&](long long b0, unsigned blocks) -> int {
-            const long long m0 = b0 * ROWS;
-            hipLaunchKernelGGL((norm_kernel<T, L, C, tail()>), dim3(blocks), dim3(256), 0, stream, X + m0 * ldx, ldx, gamma, beta, eps, (int)(M - m0), N, Y + m0 * ldy, ldy, stats ? stats + 2 * m0 : nullptr);
-            G9_HIP(hipGetLastError());
-            return 0;
-        });
-    }, Shape<16, 1>(), Shape<16, 2>(), Shape<64, 1>(), Shape<64, 2>(), Shape<64, 4>(), Shape<64, 8>(), Shape<256, 4>(), Shape<256, 8>());
+        constexpr int L = shape.L, C = shape.C, B = L > 256 ? L : 256, ROWS = B / L;
+        const long long blocks = std::min(cdiv(M, ROWS), 1536LL / B * num_cus);   // as many as run at once
+        hipLaunchKernelGGL((norm_kernel<T, L, C, tail()>), dim3((unsigned)blocks), dim3(B), 0, stream, X, ldx, gamma, beta, eps, M, N, Y, ldy, stats);
+        const hipError_t e = hipGetLastError();
+        rc = e == hipSuccess ? 0 : hip_fail(e, "norm_kernel", __FILE__, __LINE__);
+    }, Shape<16, 1>(), Shape<16, 2>(), Shape<64, 1>(), Shape<64, 2>(), Shape<64, 4>(), Shape<256, 2>(), Shape<256, 4>(), Shape<256, 8>(), Shape<1024, 4>());
     if (fits) return rc;
     return by_rows(M, 1024, [&](long long m0, unsigned rows) -> int {
         hipLaunchKernelGGL((norm_long_kernel<T>), dim3(rows), dim3(1024), 0, stream, X + m0 * ldx, ldx, gamma, beta, eps, N, Y + m0 * ldy, ldy, stats ? stats + 2 * m0 : nullptr);
@@ -341,7 +378,7 @@ template <class T> static int norm_back(BackArgs a) {
             return a.sums ? column_sums((float *)sums, blocks, a.N, 2LL * a.N, dgamma, dbeta, a.accumulate) : 0;
         };
         rc = run();
-    }, Shape<16, 1>(), Shape<16, 2>(), Shape<64, 1>(), Shape<64, 2>(), Shape<64, 4>(), Shape<256, 2>(), Shape<256, 4>(), Shape<1024, 2>());
+    }, Shape<16, 1>(), Shape<16, 2>(), Shape<64, 1>(), Shape<64, 2>(), Shape<256, 1>(), Shape<256, 2>(), Shape<512, 2>(), Shape<1024, 2>());
     if (fits) return rc;
     if (a.dX)
         G9_TRY(by_rows(a.M, 1024, [&](long long m0, unsigned rows) -> int {
