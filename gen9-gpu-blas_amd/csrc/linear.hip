@@ -258,8 +258,12 @@ __global__ void __launch_bounds__(256) linear_back_kernel(const T *__restrict__ 
 template <class T>
 static int backward(int type, int M, int N, int K, const T *dY, int lddy, const T *Z, int ldz, int act, const Dropout &d, const T *X, int ldx, const T *W, int ldw,
                     T *dX, int lddx, T *dW, int lddw, float *db, int accumulate) {
+    // gen9blas_gemm has its slower kernel for FP16 operands with odd row strides or addresses: where the product is long enough
+    // to pay for it, they are copied (gradients of 2685 × 4952 × 1081 230 µs without, 117 with)
+    constexpr int LONG = 128;
+    auto odd = [&](const T *p, int ld) { return sizeof(T) == 2 && (ld % 2 || (uintptr_t)p % 4); };
     // without an activation or dropout dZ is dY itself
-    const bool own = act || d.limit;
+    const bool own = act || d.limit || (odd(dY, lddy) && M >= LONG && K >= LONG && (dX || dW));
     const int lddz = own ? (int)cdiv(N, 8) * 8 : lddy;
     T *dZ = nullptr;
     void *p;
@@ -289,6 +293,16 @@ static int backward(int type, int M, int N, int K, const T *dY, int lddy, const 
         if (db) G9_TRY(column_sums(sums, blocks, N, N, db, nullptr, accumulate));
     }
     const T *g = own ? dZ : dY;
+    if (dX && odd(W, ldw) && M >= LONG) {
+        const int ldp = (int)cdiv(K, 8) * 8;
+        G9_TRY(pad_rows(W, ldw, N, K, ldp, SLOT_W, &W));
+        ldw = ldp;
+    }
+    if (dW && odd(X, ldx) && N >= LONG) {
+        const int ldp = (int)cdiv(K, 8) * 8;
+        G9_TRY(pad_rows(X, ldx, M, K, ldp, SLOT_X, &X));
+        ldx = ldp;
+    }
     auto product = [&](int tA, int m, int n, int k, const void *A, int lda, const void *B, int ldb, double beta, void *C, int ldc) -> int {
         if (int r = gen9blas_gemm(type, tA, 0, m, n, k, 1.0, A, lda, B, ldb, beta, C, ldc)) return fail(r, "%s", gen9blas_error());
         return 0;

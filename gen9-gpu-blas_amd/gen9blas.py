@@ -1203,7 +1203,8 @@ def _floats(v, n, what):
     """A vector of n float32 on the GPU, or None."""
     if v is None:
         return None
-    v = _device_rows(v, (1,))[0].float().contiguous()
+    if not (isinstance(v, _torch.Tensor) and v.is_cuda and v.dtype is _torch.float32 and v.dim() == 1 and v.is_contiguous()):
+        v = _device_rows(v, (1,))[0].float().contiguous()
     if v.shape[0] != n:
         raise ValueError(f"{what} has {v.shape[0]} elements, expected {n}")
     return v
