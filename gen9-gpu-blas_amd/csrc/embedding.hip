@@ -50,14 +50,19 @@ struct ClearArgs {
     int V, D, groups, cols;   // 2^cols threads side by side
 };
 template <class O> __device__ __forceinline__ void clear_rows(const ClearArgs &a, long long group) {
-    constexpr int E = 8;
-    const float none[E] = {};
+    constexpr int V = 16 / sizeof(O);
+    typedef O Vec __attribute__((ext_vector_type(V)));
     const long long v0 = group * CLEAR;
     const int lane = threadIdx.x & 63, c = threadIdx.x & ((1 << a.cols) - 1);
     const unsigned long long empty = __ballot(lane < CLEAR && v0 + lane < a.V && !a.has[min(v0 + lane, a.V - 1LL)]);
-    for (int r = threadIdx.x >> a.cols; r < CLEAR; r += (int)blockDim.x >> a.cols)
-        if (empty >> r & 1)
-            for (int x = c * E; x < a.D; x += E << a.cols) store_some<E, O, true>((O *)a.out + (v0 + r) * a.ldo + x, a.D - x, none);
+    for (int r = threadIdx.x >> a.cols; r < CLEAR; r += (int)blockDim.x >> a.cols) {
+        if (!(empty >> r & 1)) continue;
+        // whole 16 bytes at 16-byte addresses, past the caches, and single elements before and behind
+        O *row = (O *)a.out + (v0 + r) * a.ldo;
+        const int head = min((int)(-(uintptr_t)row & 15) / (int)sizeof(O), a.D), body = (a.D - head) / V * V;
+        for (int x = c; x < a.D - body; x += 1 << a.cols) row[x < head ? x : x + body] = O(0);
+        for (int x = c * V; x < body; x += V << a.cols) __builtin_nontemporal_store(Vec{}, reinterpret_cast<Vec *>(row + head + x));
+    }
 }
 
 // ---- the sort: least digits first, 8 bits a pass ----
@@ -246,6 +251,7 @@ struct GradArgs {
     long long ldp;
     float scale;
     int n, V, D, per, pieces, cols, accumulate;
+    int past;             // results go out past the caches: FP16 rows of whole 128-byte lines
 };
 template <class T, int E> __device__ __forceinline__ void put(const GradArgs &a, int key, int d, const float *sum) {
     T *o = (T *)a.out + key * a.ldo + d;
@@ -253,7 +259,8 @@ template <class T, int E> __device__ __forceinline__ void put(const GradArgs &a,
     if (a.accumulate) load_some<E>(o, a.D - d, v);
 #pragma unroll
     for (int e = 0; e < E; e++) v[e] = a.accumulate ? __builtin_fmaf(sum[e], a.scale, v[e]) : sum[e] * a.scale;
-    store_some<E, T, true>(o, a.D - d, v);
+    if (a.past) store_some<E, T, true>(o, a.D - d, v);
+    else store_some<E>(o, a.D - d, v);
 }
 // 2^cols threads side by side have 8 columns each; blockIdx.x: pieces (blockIdx.y: their columns), then groups of rows to clear.
 template <class T, class O>
@@ -370,7 +377,8 @@ static int gradient(int n, int V, int D, const T *dY, int lddy, const Ids &ids, 
         }
     }
     G9_HIP(hipGetLastError());
-    const GradArgs a = {dY, lddy, in, out, ldo, (float *)parts, ldp, scale, n, V, D, piece, pieces, cols, accumulate};
+    const GradArgs a = {dY, lddy, in, out, ldo, (float *)parts, ldp, scale, n, V, D, piece, pieces, cols, accumulate,
+                        sizeof(O) == 2 && (uintptr_t)out % 128 == 0 && ldo % 64 == 0};
     hipLaunchKernelGGL((embedding_grad_kernel<T, O>), dim3(piece_groups + (unsigned)cdiv(clear.groups - cleared, slabs), slabs), dim3(256), 0, stream, a, clear, cleared);
     G9_HIP(hipGetLastError());
     if (pieces > 1) hipLaunchKernelGGL((embedding_join_kernel<O>), dim3(piece_groups, slabs), dim3(256), 0, stream, a);

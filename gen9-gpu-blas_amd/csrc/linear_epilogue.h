@@ -84,6 +84,7 @@ template <class T> struct Epilogue {
     long long ldz, ldr;
     Activation act;
     Dropout dropout;
+    int past = 0;        // results go out past the caches
 
     template <int V> struct Cols { float bias[V]; };
     template <int V> struct Res {
@@ -94,7 +95,7 @@ template <class T> struct Epilogue {
     // Keeps the loads of these kernel arguments before this place.
     __device__ __forceinline__ void pin() {
         asm volatile("" : "+s"(bias), "+s"(Z), "+s"(R), "+s"(ldz), "+s"(ldr), "+s"(act.kind), "+s"(act.low), "+s"(act.a), "+s"(act.b));
-        asm volatile("" : "+s"(dropout.limit), "+s"(dropout.scale), "+s"(dropout.seed[0]), "+s"(dropout.seed[1]), "+s"(dropout.offset[0]), "+s"(dropout.offset[1]));
+        asm volatile("" : "+s"(dropout.limit), "+s"(dropout.scale), "+s"(dropout.seed[0]), "+s"(dropout.seed[1]), "+s"(dropout.offset[0]), "+s"(dropout.offset[1]), "+s"(past));
     }
     template <class F> __device__ __forceinline__ void each(F f) const {
         if (act.kind == KIND_CLIP) f(std::integral_constant<int, KIND_CLIP>{});
@@ -122,22 +123,24 @@ template <class T> struct Epilogue {
                 if (e < valid) r.v[e] = p[e];
         return r;
     }
-    // Row m, columns n .. n + V − 1 (n a multiple of V) from their sums: four, or eight in `v` and `hi`. FP16 results go out past
-    // the caches, as those of the products without an epilogue do.
+    // Row m, columns n .. n + V − 1 (n a multiple of V) from their sums: four, or eight in `v` and `hi`.
     template <class O, int V, class K> __device__ __forceinline__ void row(K, O *Y, long long ldy, int m, int n, const Cols<V> &cols, const Res<V> &res, int valid, f32x4 v, f32x4 hi = {}) const {
         if (valid <= 0) return;
-        constexpr bool PAST = sizeof(T) == 2;
         float x[V];
 #pragma unroll
         for (int e = 0; e < V; e++) x[e] = (e < 4 ? v[e & 3] : hi[e & 3]) + cols.bias[e];
-        if (Z) store_some<V, T, PAST>(Z + m * ldz + n, valid, x);
+        auto store = [&](T *p) {
+            if (past) store_some<V, T, true>(p, valid, x);
+            else store_some<V>(p, valid, x);
+        };
+        if (Z) store(Z + m * ldz + n);
 #pragma unroll
         for (int e = 0; e < V; e++) x[e] = activate<T, K::value>(act, x[e]);
         if (dropout.limit) drop<V>(dropout, m, n, x);
         if (R)
 #pragma unroll
             for (int e = 0; e < V; e++) x[e] += (float)res.v[e];
-        store_some<V, T, PAST>(Y + m * ldy + n, valid, x);
+        store(Y + m * ldy + n);
     }
     // One element.
     template <class O> __device__ __forceinline__ void one(O *Y, long long ldy, int m, int n, float sum) const {
