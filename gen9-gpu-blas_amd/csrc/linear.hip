@@ -263,7 +263,8 @@ template <class T>
 static int backward(int type, int M, int N, int K, const T *dY, int lddy, const T *Z, int ldz, int act, const Dropout &d, const T *X, int ldx, const T *W, int ldw,
                     T *dX, int lddx, T *dW, int lddw, float *db, int accumulate) {
     // gen9blas_gemm has its slower kernel for FP16 operands with odd row strides or addresses: where the product is long enough
-    // to pay for it, they are copied (gradients of 2685 × 4952 × 1081 230 µs without, 117 with)
+    // to pay for it, they are copied (gradients of 2685 × 4952 × 1081 132 µs, as they lie 230; 128 × 4096 × 4097 68 and 80, 64 rows 75
+    // and 72)
     constexpr int LONG = 128;
     auto odd = [&](const T *p, int ld) { return sizeof(T) == 2 && (ld % 2 || (uintptr_t)p % 4); };
     // without an activation or dropout dZ is dY itself
@@ -322,6 +323,11 @@ using namespace g9llm;
 
 static bool known(int type) { return type == GEN9BLAS_H || type == GEN9BLAS_S; }
 constexpr int LONGEST_K = 1 << 22;   // 256 rows of FP16 or FP32 within 4 GiB
+// Kernels count rows and columns in an int, up to the end of the last tile.
+static int countable(int M, int N, const char *who) {
+    if (M > 0x7ffff000 || N > 0x7ffff000) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "%s: more rows or columns than kernels count (M %d, N %d)", who, M, N);
+    return 0;
+}
 
 extern "C" {
 
@@ -334,6 +340,7 @@ int gen9blas_linear(int type, int M, int N, int K, const void *X, int ldx, const
     if (M <= 0 || N <= 0) return 0;
     if (K < 1 || ldx < K || ldw < K || ldy < N || (Z && ldz < N) || (R && ldr < N))
         G9_FAIL(GEN9BLAS_ERR_INVALID_ARG, "linear: M %d, N %d, K %d, ldx %d, ldw %d, ldz %d, ldr %d, ldy %d", M, N, K, ldx, ldw, ldz, ldr, ldy);
+    G9_TRY(countable(M, N, "linear"));
     if (K >= LONGEST_K) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "linear: rows of %d values; the longest have %d", K, LONGEST_K - 1);
     const size_t es = elem_size(type);
     G9_TRY(need_device(X, ((size_t)(M - 1) * ldx + K) * es, "linear: X"));
@@ -359,6 +366,7 @@ int gen9blas_linear_backward(int type, int M, int N, int K, const void *dY, int 
     M = std::max(M, 0);
     if (K < 1 || lddy < N || (act && ldz < N) || (dW && (ldx < K || lddw < K)) || (dX && (ldw < K || lddx < K)))
         G9_FAIL(GEN9BLAS_ERR_INVALID_ARG, "linear_backward: M %d, N %d, K %d, lddy %d, ldz %d, ldx %d, ldw %d, lddx %d, lddw %d", M, N, K, lddy, ldz, ldx, ldw, lddx, lddw);
+    G9_TRY(countable(M, N, "linear_backward"));
     const size_t es = elem_size(type);
     if (M) {
         G9_TRY(need_device(dY, ((size_t)(M - 1) * lddy + N) * es, "linear_backward: dY"));

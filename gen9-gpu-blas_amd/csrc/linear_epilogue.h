@@ -20,10 +20,10 @@ struct Activation {
 };
 inline Activation make_act(int act) {
     switch (act) {
-    case 1: return {KIND_CLIP, 0.f, 0.f, 0.f};
-    case 2: return {KIND_ERF, 0.f, 0.f, 0.f};
-    case 3: return {KIND_SIGMOID, 0.f, 1.5957691216057308f, 0.0713548162726009f};
-    case 4: return {KIND_SIGMOID, 0.f, 1.f, 0.f};
+    case GEN9BLAS_ACT_RELU: return {KIND_CLIP, 0.f, 0.f, 0.f};
+    case GEN9BLAS_ACT_GELU: return {KIND_ERF, 0.f, 0.f, 0.f};
+    case GEN9BLAS_ACT_GELU_TANH: return {KIND_SIGMOID, 0.f, 1.5957691216057308f, 0.0713548162726009f};
+    case GEN9BLAS_ACT_SILU: return {KIND_SIGMOID, 0.f, 1.f, 0.f};
     }
     return {KIND_CLIP, -INFINITY, 0.f, 0.f};
 }
@@ -35,7 +35,7 @@ template <class T> __device__ __forceinline__ float sigmoid(float x) {
 }
 // The normal distribution function, and its density. For FP16: with t = |z|, Φ(−t) = e^(−t²/2)·h(t), h(t) = erfcx(t/√2)/2 a
 // polynomial without constant term in 1 / (1 + 0.26 t), fitted here to 2^-25 of h over t = 0..14 (least squares, reweighted by the
-// error); the exponential's argument adds t² units of 2^-24. erfcf and expf take 102 of the 2048 × 11008 gradient's µs, this 36.
+// error); the exponential's argument adds t² units of 2^-24. erfcf and expf take 102 of the 2048 × 11008 gradient's µs, this 31.
 template <class T> __device__ __forceinline__ float phi(float z, float *density = nullptr) {
     if constexpr (sizeof(T) == 2) {
         const float e = __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z), u = __builtin_amdgcn_rcpf(__builtin_fmaf(0.26f, fabsf(z), 1.f));

@@ -14,7 +14,7 @@ template <class T> struct Piece {
     typedef T Vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
     // Elements n .. n + V − 1 of a row of N, zeros past its end. TAIL: the row may end inside a piece.
     template <bool TAIL = true> static __device__ __forceinline__ Vec load(const T *row, int n, int N) {
-        if (n + V <= N) return *reinterpret_cast<const Vec *>(row + n);
+        if (n <= N - V) return *reinterpret_cast<const Vec *>(row + n);
         Vec v = {};
         if constexpr (TAIL)
 #pragma unroll

@@ -911,16 +911,18 @@ _LLM_SIGNATURES = """
 """
 _llm = None
 _llm_device = 0        # torch's index of the library's device
+_llm_gpu = None        # the same as a torch.device
 _raw_stream = None     # torch's current stream on it as an int: the public torch.cuda.current_stream() takes 2.7 us
 
 
 def _llm_library():
     """libgen9blas_llm.so, loaded at first use from the directory of libgen9blas.so."""
-    global _llm, _llm_device, _raw_stream
+    global _llm, _llm_device, _llm_gpu, _raw_stream
     if _llm is None:
         torch = _torch_module()
         _init()
         _llm_device = torch.cuda.current_device()
+        _llm_gpu = torch.device("cuda", _llm_device)
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
         lib = ctypes.CDLL(os.path.join(os.path.dirname(_library_path()), "libgen9blas_llm.so"))
         for item in _LLM_SIGNATURES.split():
@@ -940,7 +942,7 @@ def _llm_call(fn, *args):
         if fn(*args) != 0:
             raise RuntimeError(_llm.gen9blas_llm_error().decode())
     else:
-        current, ours = _torch.cuda.current_stream(), _torch.cuda.ExternalStream(hip_stream())
+        current, ours = _torch.cuda.current_stream(_llm_device), _torch.cuda.ExternalStream(hip_stream(), device=_llm_gpu)
         ours.wait_stream(current)
         rc = fn(*args)
         current.wait_stream(ours)
@@ -957,7 +959,7 @@ def _on_gpu(X):
         if isinstance(X, np.ndarray) and any(step < 0 for step in X.strides):
             X = X.copy()                                    # torch takes no negative strides
         X = torch.as_tensor(X)
-    return X if X.is_cuda else X.cuda()
+    return X if X.is_cuda else X.to(_llm_gpu)
 
 
 def _device_rows(X, dims, shared=False):
@@ -996,7 +998,7 @@ def _host_like(X, result):
 def _llm_out(C, shape, dtype, what="C"):
     """The given result, or a new one: a GPU tensor of this shape and type with contiguous rows."""
     if C is None:
-        return _torch.empty(shape, dtype=dtype, device="cuda")
+        return _torch.empty(shape, dtype=dtype, device=_llm_gpu)
     if not (isinstance(C, _torch.Tensor) and C.is_cuda and C.shape == shape and C.dtype is dtype and (C.stride(-1) == 1 or shape[-1] <= 1)):
         raise ValueError(f"{what} must be a GPU tensor of shape {tuple(shape)} and type {dtype} with contiguous rows")
     return C
@@ -1189,9 +1191,24 @@ def _act_code(act):
     return _ACT_CODE[act]
 
 
-def _matrix_like(X, shape, t, what):
-    """X as _device_rows gives it, of this shape and type."""
+def _rows(X, what):
+    """A matrix as _device_rows gives it, on the library's device."""
     x, ld = _device_rows(X, (2,))
+    if x.get_device() != _llm_device:
+        raise ValueError(f"{what} is on {x.device}; the library runs on {_llm_gpu}")
+    return x, ld
+
+
+def _result(C, shape, dtype, what):
+    C = _llm_out(C, shape, dtype, what)
+    if C.get_device() != _llm_device:
+        raise ValueError(f"{what} is on {C.device}; the library runs on {_llm_gpu}")
+    return C
+
+
+def _matrix_like(X, shape, t, what):
+    """X as _rows gives it, of this shape and type."""
+    x, ld = _rows(X, what)
     if tuple(x.shape) != tuple(shape):
         raise ValueError(f"{what} has shape {tuple(x.shape)}, expected {tuple(shape)}")
     if x.dtype is not t:
@@ -1207,6 +1224,8 @@ def _floats(v, n, what):
         v = _device_rows(v, (1,))[0].float().contiguous()
     if v.shape[0] != n:
         raise ValueError(f"{what} has {v.shape[0]} elements, expected {n}")
+    if v.get_device() != _llm_device:
+        raise ValueError(f"{what} is on {v.device}; the library runs on {_llm_gpu}")
     return v
 
 
@@ -1216,7 +1235,7 @@ def _float_sums(v, n, wanted, accumulate, what):
         return None
     if v is None and accumulate:
         raise ValueError(f"accumulate needs {what}")
-    return _llm_out(v, (n,), _torch.float32, what)
+    return _result(v, (n,), _torch.float32, what)
 
 
 def _ptr(X):
@@ -1229,9 +1248,9 @@ def linear(X, W, bias=None, act=None, dropout=0.0, seed=0, offset=0, residual=No
     pre-activations X·Wᵀ + bias, which linear_backward needs for an activation."""
     lib = _llm_library()
     a = _act_code(act)
-    x, ldx = _device_rows(X, (2,))
+    x, ldx = _rows(X, "X")
     (M, K), t = x.shape, x.dtype
-    w, ldw = _device_rows(W, (2,))
+    w, ldw = _rows(W, "W")
     N = w.shape[0]
     if w.shape[1] != K:
         raise ValueError(f"incompatible dimensions: {tuple(x.shape)} · {tuple(w.shape)}ᵀ")
@@ -1239,8 +1258,8 @@ def linear(X, W, bias=None, act=None, dropout=0.0, seed=0, offset=0, residual=No
         raise TypeError(f"W is of {w.dtype}, X of {t}")
     b = _floats(bias, N, "bias")
     r, ldr = (None, 0) if residual is None else _matrix_like(residual, (M, N), t, "residual")
-    z = None if Z is None else _llm_out(Z, (M, N), t, "Z")
-    out = _llm_out(C, (M, N), t)
+    z = None if Z is None else _result(Z, (M, N), t, "Z")
+    out = _result(C, (M, N), t, "C")
     _llm_call(lib.gen9blas_linear, 1 if t is _torch.float32 else 0, M, N, K, x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(b), a,
               _ptr(z), 0 if z is None else _out_step(z, "Z"), dropout, seed & _U64, offset & _U64, _ptr(r), ldr,
               out.data_ptr(), N if C is None else _out_step(out))
@@ -1253,9 +1272,9 @@ def linear_backward(dY, X, W, Z=None, act=None, dropout=0.0, seed=0, offset=0, d
     grads: those wanted ("x", "w", "b"); the others are None."""
     lib = _llm_library()
     a = _act_code(act)
-    dy, lddy = _device_rows(dY, (2,))
+    dy, lddy = _rows(dY, "dY")
     (M, N), t = dy.shape, dy.dtype
-    w, ldw = _device_rows(W, (2,))
+    w, ldw = _rows(W, "W")
     K = w.shape[1]
     w, ldw = _matrix_like(w, (N, K), t, "W")
     x, ldx = _matrix_like(X, (M, K), t, "X")
@@ -1264,10 +1283,10 @@ def linear_backward(dY, X, W, Z=None, act=None, dropout=0.0, seed=0, offset=0, d
     z, ldz = _matrix_like(Z, (M, N), t, "Z") if a else (None, 0)
     if not set(grads) <= set("xwb"):
         raise ValueError(f"grads {grads!r}: of 'x', 'w' and 'b'")
-    gx = _llm_out(dX, (M, K), t, "dX") if "x" in grads else None
+    gx = _result(dX, (M, K), t, "dX") if "x" in grads else None
     if "w" in grads and dW is None and accumulate:
         raise ValueError("accumulate needs dW")
-    gw = _llm_out(dW, (N, K), t, "dW") if "w" in grads else None
+    gw = _result(dW, (N, K), t, "dW") if "w" in grads else None
     gb = _float_sums(db, N, "b" in grads, accumulate, "db")
     _llm_call(lib.gen9blas_linear_backward, 1 if t is _torch.float32 else 0, M, N, K, dy.data_ptr(), lddy, _ptr(z), ldz, a, dropout,
               seed & _U64, offset & _U64, x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(gx), 0 if gx is None else _out_step(gx, "dX"),
@@ -1279,11 +1298,11 @@ def layer_norm(X, gamma=None, beta=None, eps=1e-5, out=None, stats=None):
     """(X - mean)·rstd·gamma + beta over each row of X (M, N), rstd = 1 / sqrt(variance + eps); gamma and beta (N,) float32.
     stats, a GPU tensor (M, 2) of float32 if given, takes each row's mean and rstd, for layer_norm_backward."""
     lib = _llm_library()
-    x, ldx = _device_rows(X, (2,))
+    x, ldx = _rows(X, "X")
     M, N = x.shape
     g, b = _floats(gamma, N, "gamma"), _floats(beta, N, "beta")
-    y = _llm_out(out, (M, N), x.dtype, "out")
-    if stats is not None and not _llm_out(stats, (M, 2), _torch.float32, "stats").is_contiguous():
+    y = _result(out, (M, N), x.dtype, "out")
+    if stats is not None and not _result(stats, (M, 2), _torch.float32, "stats").is_contiguous():
         raise ValueError("stats must be contiguous")
     _llm_call(lib.gen9blas_layer_norm, 1 if x.dtype is _torch.float32 else 0, M, N, x.data_ptr(), ldx, _ptr(g), _ptr(b), eps,
               y.data_ptr(), N if out is None else _out_step(y, "out"), _ptr(stats))
@@ -1294,14 +1313,14 @@ def layer_norm_backward(dY, X, stats, gamma=None, dX=None, dgamma=None, dbeta=No
     """The gradients of layer_norm() from dY and its X, stats and gamma: (dX, dgamma, dbeta), the sums in float32. accumulate:
     dgamma and dbeta are added to the given ones. grads: those wanted ("x", "g", "b"); the others are None."""
     lib = _llm_library()
-    dy, lddy = _device_rows(dY, (2,))
+    dy, lddy = _rows(dY, "dY")
     (M, N), t = dy.shape, dy.dtype
     x, ldx = _matrix_like(X, (M, N), t, "X")
     stats = _matrix_like(stats, (M, 2), _torch.float32, "stats")[0].contiguous()
     g = _floats(gamma, N, "gamma")
     if not set(grads) <= set("xgb"):
         raise ValueError(f"grads {grads!r}: of 'x', 'g' and 'b'")
-    gx = _llm_out(dX, (M, N), t, "dX") if "x" in grads else None
+    gx = _result(dX, (M, N), t, "dX") if "x" in grads else None
     gg, gb = _float_sums(dgamma, N, "g" in grads, accumulate, "dgamma"), _float_sums(dbeta, N, "b" in grads, accumulate, "dbeta")
     _llm_call(lib.gen9blas_layer_norm_backward, 1 if t is _torch.float32 else 0, M, N, dy.data_ptr(), lddy, x.data_ptr(), ldx,
               stats.data_ptr(), _ptr(g), _ptr(gx), 0 if gx is None else _out_step(gx, "dX"), _ptr(gg), _ptr(gb), bool(accumulate))
@@ -1313,10 +1332,10 @@ def dropout(X, p, seed=0, offset=0, residual=None, out=None):
     is a function of place, seed and offset (Philox4x32-10, include/gen9blas_llm.h): the same call on the gradient of the
     result gives X's. Take another offset for each layer and step."""
     lib = _llm_library()
-    x, ldx = _device_rows(X, (2,))
+    x, ldx = _rows(X, "X")
     M, N = x.shape
     r, ldr = (None, 0) if residual is None else _matrix_like(residual, (M, N), x.dtype, "residual")
-    y = _llm_out(out, (M, N), x.dtype, "out")
+    y = _result(out, (M, N), x.dtype, "out")
     _llm_call(lib.gen9blas_dropout, 1 if x.dtype is _torch.float32 else 0, M, N, x.data_ptr(), ldx, p, seed & _U64, offset & _U64,
               _ptr(r), ldr, y.data_ptr(), N if out is None else _out_step(y, "out"))
     return _host_like(X, y) if out is None else y
@@ -1333,17 +1352,19 @@ def _token_ids(ids):
         raise ValueError(f"{i.shape[0]} ids; the most are {_LONGEST}")
     if i.dtype is not _torch.int64 and i.dtype is not _torch.int32:
         i = i.to(_torch.int64)
+    if i.get_device() != _llm_device:
+        raise ValueError(f"ids are on {i.device}; the library runs on {_llm_gpu}")
     return i.contiguous()
 
 
 def embedding(table, ids, scale=1.0, out=None):
     """scale · table[ids]: table (V, D), ids (T,) integers; one outside 0..V-1 (-1) has a row of zeros."""
     lib = _llm_library()
-    x, ldt = _device_rows(table, (2,))
+    x, ldt = _rows(table, "table")
     V, D = x.shape
     i = _token_ids(ids)
     T = i.shape[0]
-    y = _llm_out(out, (T, D), x.dtype, "out")
+    y = _result(out, (T, D), x.dtype, "out")
     _llm_call(lib.gen9blas_embedding, 1 if x.dtype is _torch.float32 else 0, T, V, D, x.data_ptr(), ldt, i.data_ptr(), i.element_size(),
               scale, y.data_ptr(), D if out is None else _out_step(y, "out"))
     return _host_like(table, y) if out is None else y
@@ -1354,7 +1375,7 @@ def embedding_backward(dY, ids, rows, scale=1.0, out=None, accumulate=False):
     tokens that are v, in their order; rows without tokens are zeros. out may be float32 for float16 dY. accumulate: added
     to the given out, where rows without tokens stay as they are."""
     lib = _llm_library()
-    dy, lddy = _device_rows(dY, (2,))
+    dy, lddy = _rows(dY, "dY")
     (T, D), t = dy.shape, dy.dtype
     i = _token_ids(ids)
     if i.shape[0] != T:
@@ -1364,7 +1385,7 @@ def embedding_backward(dY, ids, rows, scale=1.0, out=None, accumulate=False):
     if out is None and accumulate:
         raise ValueError("accumulate needs out")
     f32 = _torch.float32
-    g = _llm_out(out, (rows, D), f32 if out is not None and out.dtype is f32 else t, "out")
+    g = _result(out, (rows, D), f32 if out is not None and out.dtype is f32 else t, "out")
     _llm_call(lib.gen9blas_embedding_backward, 1 if t is f32 else 0, T, rows, D, dy.data_ptr(), lddy, i.data_ptr(), i.element_size(), scale,
               1 if g.dtype is f32 else 0, g.data_ptr(), D if out is None else _out_step(g, "out"), bool(accumulate))
     return _host_like(dY, g) if out is None else g

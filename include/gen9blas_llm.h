@@ -85,7 +85,8 @@ GEN9BLAS_API int gen9blas_moe_gemm(int type, int T, int S, const int *ids, const
 // ---- Linear layers ----
 // Weights are N×K (a row for each output); biases, norms' weights and their gradients are FP32 whatever the type is.
 enum { GEN9BLAS_ACT_NONE = 0, GEN9BLAS_ACT_RELU = 1, GEN9BLAS_ACT_GELU = 2, GEN9BLAS_ACT_GELU_TANH = 3, GEN9BLAS_ACT_SILU = 4 };
-// Y (M×N) = R + dropout(act(Z)), Z = X·Wᵀ + bias (X M×K, W N×K, 1 <= K < 2^22), in FP32, rounded once.
+// Y (M×N) = R + dropout(act(Z)), Z = X·Wᵀ + bias (X M×K, W N×K, 1 <= K < 2^22, M and N up to 2^31 − 4096), in
+// FP32, rounded once.
 // - bias (N floats), R (M×N) and Z may be NULL; Z: where the pre-activations go, which the gradients need if there is an activation.
 // - act: max(z, 0); z·Φ(z); its tanh form 0.5·z·(1 + tanh(√(2/π)·(z + 0.044715·z³))); z / (1 + e^−z).
 // - p, seed, offset: as in gen9blas_dropout (p = 0: none).

@@ -548,6 +548,19 @@ def test_refusals(g9, torch_dev):
             call()
 
 
+def test_another_device_is_refused(g9, torch_dev, monkeypatch):
+    """Operands on another GPU than the library's, as if it had opened the second one."""
+    torch = torch_dev
+    f = lambda *s: torch.ones(s, device="cuda")  # noqa: E731
+    g9.linear(f(2, 8), f(3, 8))
+    monkeypatch.setattr(g9, "_llm_device", g9._llm_device + 1)
+    for call in (lambda: g9.linear(f(2, 8), f(3, 8)), lambda: g9.linear_backward(f(2, 3), f(2, 8), f(3, 8)), lambda: g9.layer_norm(f(2, 8)), lambda: g9.layer_norm_backward(f(2, 8), f(2, 8), f(2, 2)),
+                 lambda: g9.dropout(f(2, 8), 0.5), lambda: g9.embedding(f(4, 8), torch.zeros(2, dtype=torch.int64, device="cuda")),
+                 lambda: g9.embedding_backward(f(2, 8), torch.zeros(2, dtype=torch.int64, device="cuda"), 4)):
+        with pytest.raises(ValueError, match="library runs on"):
+            call()
+
+
 def test_c_refusals(g9, torch_dev):
     """The C entry points: host memory, NULL and operands that run past their allocation, wrong sizes, unknown types."""
     torch = torch_dev
@@ -562,7 +575,7 @@ def test_c_refusals(g9, torch_dev):
     for k in (dict(X=host), dict(W=None), dict(Y=host), dict(R=host, ldr=64), dict(Z=host, ldz=64), dict(bias=host), dict(ldx=3), dict(ldw=3), dict(ldy=3), dict(R=d, ldr=3), dict(Z=d, ldz=3), dict(K=0),
               dict(p=2.0), dict(M=big, ldx=4, ldy=4)):
         assert linear(**k) == BAD and L.gen9blas_llm_error() and L.gen9blas_llm_last_status() == BAD, k
-    for k in (dict(type=2), dict(type=3), dict(act=5), dict(act=-1), dict(K=1 << 22, ldx=1 << 22, ldw=1 << 22)):
+    for k in (dict(type=2), dict(type=3), dict(act=5), dict(act=-1), dict(K=1 << 22, ldx=1 << 22, ldw=1 << 22), dict(M=0x7fffffff), dict(N=0x7ffffff0, ldy=0x7fffffff)):
         assert linear(**k) == NOT, k
     back = lambda **k: L.gen9blas_linear_backward(*{**dict(type=1, M=4, N=4, K=4, dY=d, lddy=64, Z=d, ldz=64, act=2, p=0.0, seed=0, offset=0, X=d, ldx=64, W=d, ldw=64, dX=None, lddx=0, dW=None, lddw=0, db=None, acc=0), **k}.values())  # noqa: E731
     assert back() == 0 and back(dX=e, lddx=64, X=None) == 0 and back(dW=e, lddw=64, W=None) == 0 and back(db=e, X=None, W=None) == 0
