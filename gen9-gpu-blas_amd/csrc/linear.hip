@@ -208,7 +208,7 @@ static int linear(int M, int N, int K, const T *X, long long ldx, const T *W, lo
     return tiles_product(p);
 }
 
-// dZ = act'(Z) · dropout(dY) and, for each block of `rows` rows, the sums of its columns (before they are rounded). A workgroup
+// dZ = dropout(act'(Z) · dY) and, for each block of `rows` rows, the sums of its columns (before they are rounded). A workgroup
 // has 2^cols threads side by side, eight columns each, and the others below them, each with every (256 >> cols)th row of the
 // block, four of them on their way at once. dZ and Z may be null (no activation: dZ = dropout(dY)).
 template <class T, int KIND>
@@ -220,10 +220,10 @@ __global__ void __launch_bounds__(256) linear_back_kernel(const T *__restrict__ 
     const long long block = blockIdx.y, m0 = block * rows, m1 = min(m0 + rows, (long long)M);
     float sum[V] = {};
     auto row = [&](long long m, float *v, const float *z) {
-        if (d.limit) drop<V>(d, (unsigned)m, n, v);
         if (Z)
 #pragma unroll
             for (int e = 0; e < V; e++) v[e] *= slope<T, KIND>(act, z[e]);
+        if (d.limit) drop<V>(d, (unsigned)m, n, v);   // last: what is dropped is zero, whatever Z is there
         if (dZ) store_some<V>(dZ + m * lddz + n, valid, v);
 #pragma unroll
         for (int e = 0; e < V; e++) sum[e] += v[e];

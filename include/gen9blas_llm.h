@@ -92,7 +92,7 @@ enum { GEN9BLAS_ACT_NONE = 0, GEN9BLAS_ACT_RELU = 1, GEN9BLAS_ACT_GELU = 2, GEN9
 // - p, seed, offset: as in gen9blas_dropout (p = 0: none).
 GEN9BLAS_API int gen9blas_linear(int type, int M, int N, int K, const void *X, int ldx, const void *W, int ldw, const float *bias, int act,
                                  void *Z, int ldz, double p, uint64_t seed, uint64_t offset, const void *R, int ldr, void *Y, int ldy);
-// Its gradients: dZ = act'(Z)·dropout(dY), rounded to the type for the products; dX (M×K) = dZ·W; dW (N×K) = dZᵀ·X; db (N floats) =
+// Its gradients: dZ = dropout(act'(Z)·dY), rounded to the type for the products; dX (M×K) = dZ·W; dW (N×K) = dZᵀ·X; db (N floats) =
 // the column sums of dZ before that rounding. Each may be NULL, and what only it needs is not read then (Z: without an activation).
 // R's gradient is dY. accumulate: dW and db are added to what is there. M = 0: dW and db are zeros, or stay. The products are
 // gen9blas_gemm's, which wait unless gen9blas_set_nowait is on.

@@ -130,7 +130,7 @@ def test_linear_tiles(g9, torch_dev, dtype, M, N, K):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("M,N,K", [(3, 8300, 4090), (8, 8200, 4224), (12, 2100, 4100), (16, 8193, 4352), (17, 4100, 8320), (24, 5000, 8000), (32, 8256, 4100), (33, 3000, 2817),
-                                   (40, 9000, 3900), (47, 2100, 4096), (64, 2050, 4224), (64, 8300, 1100), (30, 34000, 1000)])
+                                   (40, 9000, 3900), (47, 2100, 4096), (64, 2050, 4224), (64, 8300, 1100), (30, 34000, 1000), (20, 90000, 100), (20, 170000, 200)])
 @pytest.mark.parametrize("pad,shift", [(0, 0), (2, 2), (3, 1)])
 def test_linear_of_some_rows(g9, torch_dev, dtype, M, N, K, pad, shift):
     """Large weights under few rows: whole and cut pieces of k, columns that end inside a workgroup's."""
@@ -188,6 +188,29 @@ def test_linear_backward(g9, torch_dev, dtype, name, M, N, K, p):
     near(db2, 1 + g.sum(0), eg.sum(0) + (M + 2) * U * (1 + np.abs(g).sum(0)), np.float32)
     only = g9.linear_backward(gpu(torch, dy), gpu(torch, x), gpu(torch, w), Z=Z, act=name, dropout=p, seed=seed, offset=offset, grads="x")
     assert only[1] is None and only[2] is None and torch.equal(only[0], dX)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("name", ACTS)
+def test_what_is_dropped_is_zero(g9, torch_dev, dtype, name):
+    """Infinities and NaN in places that dropout takes, forward and backward: zeros are left of them, in the gradients too."""
+    torch = torch_dev
+    M, N, K, p, seed, offset = 40, 72, 64, 0.5, 3, 9
+    t = torch.float16 if dtype is np.float16 else torch.float32
+    lost = torch.from_numpy(dropout_factor(M, N, p, seed, offset) == 0).cuda()
+    bad = torch.tensor([float("nan"), float("inf"), -float("inf")], dtype=t, device="cuda").repeat(M * N // 3).view(M, N)
+    x, w = torch.eye(K, dtype=t, device="cuda")[:M], torch.ones(N, K, dtype=t, device="cuda")
+    good = torch.ones(M, N, dtype=t, device="cuda")
+    z = torch.where(lost, bad, good)
+    for rows in (1, 3, 12, M):                     # a bias that is bad where the first row is dropped
+        b = torch.where(lost[0], bad[0], good[0]).float()
+        y = g9.linear(torch.zeros(rows, K, dtype=t, device="cuda"), w, b, name, p, seed, offset)[0]
+        assert torch.isfinite(y).all() and (y[lost[0]] == 0).all()
+    for dy in (torch.where(lost, bad, good), good):
+        got = g9.linear_backward(dy, x, w, Z=z if name != "none" else None, act=name, dropout=p, seed=seed, offset=offset)
+        want = g9.linear_backward(good, x, w, Z=good if name != "none" else None, act=name, dropout=p, seed=seed, offset=offset)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
 
 
 @pytest.mark.parametrize("name", ACTS[1:])
@@ -401,7 +424,7 @@ def embedding_grad(dy, ids, V):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,V,D", [(1, 1, 1), (3, 1, 5), (31, 40, 8), (32, 2, 100), (33, 1, 64), (64, 3, 2049), (100, 255, 33), (1000, 256, 16), (1023, 257, 24), (1025, 65535, 9), (5000, 65536, 4),
-                                   (5000, 70, 130), (40000, 300, 20), (3000, 1 << 17, 12)])
+                                   (5000, 70, 130), (40000, 300, 20), (3000, 1 << 17, 12), (9, (1 << 20) + 100, 4), (5000, 1 << 18, 8)])
 def test_embedding_backward(g9, torch_dev, dtype, T, V, D):
     torch = torch_dev
     r = np.random.default_rng(T + V)
