@@ -5,7 +5,7 @@
 // has, stores the rows whose tokens all lie in it, and leaves the sums of the first and the last row, where their tokens go on in
 // the pieces before or behind, to a second kernel. So a token as frequent as all others together costs no more than they do,
 // no sum depends on the order in which workgroups run, and no atomics are needed. Rows without tokens are cleared by other
-// workgroups of the same launch.
+// workgroups of these launches, beside the sort as well, which leaves most CUs idle.
 #include "llm.h"
 #include "rows.h"
 #include <algorithm>
@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(256) embedding_kernel(const T *__restrict__ ta
 // Rows without tokens are cleared in groups of CLEAR, whole rows, so that what is written at a time lies together.
 constexpr int CLEAR = 16;
 struct ClearArgs {
-    const uint8_t *has;   // of each row whether it has tokens
+    const uint8_t *has;   // of each row whether it has tokens; null: clear all
     void *out;
     long long ldo;
     int V, D, groups, cols;   // 2^cols threads side by side
@@ -54,7 +54,7 @@ template <class O> __device__ __forceinline__ void clear_rows(const ClearArgs &a
     typedef O Vec __attribute__((ext_vector_type(V)));
     const long long v0 = group * CLEAR;
     const int lane = threadIdx.x & 63, c = threadIdx.x & ((1 << a.cols) - 1);
-    const unsigned long long empty = __ballot(lane < CLEAR && v0 + lane < a.V && !a.has[min(v0 + lane, a.V - 1LL)]);
+    const unsigned long long empty = __ballot(lane < CLEAR && v0 + lane < a.V && !(a.has && a.has[min(v0 + lane, a.V - 1LL)]));
     for (int r = threadIdx.x >> a.cols; r < CLEAR; r += (int)blockDim.x >> a.cols) {
         if (!(empty >> r & 1)) continue;
         // whole 16 bytes at 16-byte addresses, past the caches, and single elements before and behind
@@ -74,8 +74,9 @@ __device__ __forceinline__ void place(const Ids &ids, const Sorted &in, long lon
     if (in.key) key = in.key[i], at = in.at[i];
     else key = ids.key(i, V), at = (int)i;
 }
-// counts[workgroup][digit]; the first pass clears the marks of the rows that have tokens, too. From the second pass on the marks are
-// set, and workgroups behind the `groups` of the sort, which leave most CUs idle, clear rows from group `first` on.
+// counts[workgroup][digit]; the first pass clears the marks of the rows that have tokens, too. Workgroups behind the `groups` of the
+// sort, which leave most CUs idle, clear rows from group `first` on: in the first pass, whose marks are not set yet, all of them (the
+// sums come later), then those without tokens.
 template <class O>
 __global__ void __launch_bounds__(256) sort_count_kernel(Ids ids, Sorted in, int n, int V, int shift, int per, int *__restrict__ counts, uint8_t *__restrict__ has, int groups, ClearArgs clear, int first) {
     if ((int)blockIdx.x >= groups) {
@@ -85,7 +86,7 @@ __global__ void __launch_bounds__(256) sort_count_kernel(Ids ids, Sorted in, int
     __shared__ int count[256];
     count[threadIdx.x] = 0;
     if (has)
-        for (long long v = (long long)blockIdx.x * 256 + threadIdx.x; v < V; v += (long long)gridDim.x * 256) has[v] = 0;
+        for (long long v = (long long)blockIdx.x * 256 + threadIdx.x; v < V; v += (long long)groups * 256) has[v] = 0;
     __syncthreads();
     const long long end = min((long long)n, (blockIdx.x + 1LL) * per);
     for (long long i = (long long)blockIdx.x * per + threadIdx.x; i < end; i += 256) {
@@ -353,7 +354,7 @@ static int gradient(int n, int V, int D, const T *dY, int lddy, const Ids &ids, 
     void *parts;
     G9_TRY(scratch(SLOT_SUMS, (size_t)pieces * 2 * ldp * 4, &parts));
 
-    const ClearArgs clear = {has, out, ldo, V, D, has ? (int)cdiv(V, CLEAR) : 0, cols};
+    const ClearArgs all = {has, out, ldo, V, D, has ? (int)cdiv(V, CLEAR) : 0, cols};
     int cleared = 0;   // groups of rows that the sort's launches have cleared
     int bits = 1;
     while (bits < 31 && V >> bits) bits++;   // of V, which stands for no row
@@ -367,10 +368,12 @@ static int gradient(int n, int V, int D, const T *dY, int lddy, const Ids &ids, 
         const int beside = (int)std::max<long long>(1, (24 << 20) / ((long long)CLEAR * D * (int)sizeof(O)));
         for (int shift = 0, pass = 0; shift < bits; shift += 8, pass++) {
             uint8_t *h = pass ? nullptr : has;
-            int more = pass ? std::min(beside, clear.groups - cleared) : 0;
+            ClearArgs clear = all;
+            if (!pass) clear.has = nullptr;
+            int more = std::min(beside, clear.groups - cleared);
             hipLaunchKernelGGL((sort_count_kernel<O>), dim3(groups + more), dim3(256), 0, stream, ids, in, n, V, shift, per, counts, h, groups, clear, cleared);
             cleared += more;
-            more = pass ? std::min(beside, clear.groups - cleared) : 0;
+            more = std::min(beside, clear.groups - cleared);
             hipLaunchKernelGGL((sort_place_kernel<O>), dim3(groups + more), dim3(1024), 0, stream, ids, in, n, V, shift, per, (const int *)counts, s[pass & 1], h, groups, clear, cleared);
             cleared += more;
             in = s[pass & 1];
@@ -379,7 +382,7 @@ static int gradient(int n, int V, int D, const T *dY, int lddy, const Ids &ids, 
     G9_HIP(hipGetLastError());
     const GradArgs a = {dY, lddy, in, out, ldo, (float *)parts, ldp, scale, n, V, D, piece, pieces, cols, accumulate,
                         sizeof(O) == 2 && (uintptr_t)out % 128 == 0 && ldo % 64 == 0};
-    hipLaunchKernelGGL((embedding_grad_kernel<T, O>), dim3(piece_groups + (unsigned)cdiv(clear.groups - cleared, slabs), slabs), dim3(256), 0, stream, a, clear, cleared);
+    hipLaunchKernelGGL((embedding_grad_kernel<T, O>), dim3(piece_groups + (unsigned)cdiv(all.groups - cleared, slabs), slabs), dim3(256), 0, stream, a, all, cleared);
     G9_HIP(hipGetLastError());
     if (pieces > 1) hipLaunchKernelGGL((embedding_join_kernel<O>), dim3(piece_groups, slabs), dim3(256), 0, stream, a);
     G9_HIP(hipGetLastError());

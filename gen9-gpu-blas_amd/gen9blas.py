@@ -1193,6 +1193,10 @@ def _act_code(act):
 
 def _rows(X, what):
     """A matrix as _device_rows gives it, on the library's device."""
+    if type(X) is _torch.Tensor and X.get_device() == _llm_device and X.is_contiguous():   # what most calls have
+        shape, t = X.shape, X.dtype
+        if len(shape) == 2 and (t is _torch.float16 or t is _torch.float32) and 0 < shape[1] <= _LONGEST and shape[0] <= _LONGEST:
+            return X, shape[1]
     x, ld = _device_rows(X, (2,))
     if x.get_device() != _llm_device:
         raise ValueError(f"{what} is on {x.device}; the library runs on {_llm_gpu}")
@@ -1200,10 +1204,18 @@ def _rows(X, what):
 
 
 def _result(C, shape, dtype, what):
-    C = _llm_out(C, shape, dtype, what)
+    """The given result, or a new one, as _llm_out has it, on the library's device; and its row stride."""
+    if C is None:
+        return _torch.empty(shape, dtype=dtype, device=_llm_gpu), shape[-1]
+    if not (type(C) is _torch.Tensor and C.dtype is dtype and C.is_contiguous() and C.shape == shape and 0 < shape[-1] <= _LONGEST):
+        _llm_out(C, shape, dtype, what)
+        if len(shape) > 1:
+            step = _out_step(C, what)
+            if C.get_device() == _llm_device:
+                return C, step
     if C.get_device() != _llm_device:
         raise ValueError(f"{what} is on {C.device}; the library runs on {_llm_gpu}")
-    return C
+    return C, shape[-1]
 
 
 def _matrix_like(X, shape, t, what):
@@ -1235,7 +1247,7 @@ def _float_sums(v, n, wanted, accumulate, what):
         return None
     if v is None and accumulate:
         raise ValueError(f"accumulate needs {what}")
-    return _result(v, (n,), _torch.float32, what)
+    return _result(v, (n,), _torch.float32, what)[0]
 
 
 def _ptr(X):
@@ -1258,11 +1270,10 @@ def linear(X, W, bias=None, act=None, dropout=0.0, seed=0, offset=0, residual=No
         raise TypeError(f"W is of {w.dtype}, X of {t}")
     b = _floats(bias, N, "bias")
     r, ldr = (None, 0) if residual is None else _matrix_like(residual, (M, N), t, "residual")
-    z = None if Z is None else _result(Z, (M, N), t, "Z")
-    out = _result(C, (M, N), t, "C")
+    z, ldz = (None, 0) if Z is None else _result(Z, (M, N), t, "Z")
+    out, ldc = _result(C, (M, N), t, "C")
     _llm_call(lib.gen9blas_linear, 1 if t is _torch.float32 else 0, M, N, K, x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(b), a,
-              _ptr(z), 0 if z is None else _out_step(z, "Z"), dropout, seed & _U64, offset & _U64, _ptr(r), ldr,
-              out.data_ptr(), N if C is None else _out_step(out))
+              _ptr(z), ldz, dropout, seed & _U64, offset & _U64, _ptr(r), ldr, out.data_ptr(), ldc)
     return _host_like(X, out) if C is None else out
 
 
@@ -1283,14 +1294,13 @@ def linear_backward(dY, X, W, Z=None, act=None, dropout=0.0, seed=0, offset=0, d
     z, ldz = _matrix_like(Z, (M, N), t, "Z") if a else (None, 0)
     if not set(grads) <= set("xwb"):
         raise ValueError(f"grads {grads!r}: of 'x', 'w' and 'b'")
-    gx = _result(dX, (M, K), t, "dX") if "x" in grads else None
+    gx, lddx = _result(dX, (M, K), t, "dX") if "x" in grads else (None, 0)
     if "w" in grads and dW is None and accumulate:
         raise ValueError("accumulate needs dW")
-    gw = _result(dW, (N, K), t, "dW") if "w" in grads else None
+    gw, lddw = _result(dW, (N, K), t, "dW") if "w" in grads else (None, 0)
     gb = _float_sums(db, N, "b" in grads, accumulate, "db")
     _llm_call(lib.gen9blas_linear_backward, 1 if t is _torch.float32 else 0, M, N, K, dy.data_ptr(), lddy, _ptr(z), ldz, a, dropout,
-              seed & _U64, offset & _U64, x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(gx), 0 if gx is None else _out_step(gx, "dX"),
-              _ptr(gw), 0 if gw is None else _out_step(gw, "dW"), _ptr(gb), bool(accumulate))
+              seed & _U64, offset & _U64, x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(gx), lddx, _ptr(gw), lddw, _ptr(gb), bool(accumulate))
     return tuple(g if g is None or given is not None else _host_like(dY, g) for g, given in ((gx, dX), (gw, dW), (gb, db)))
 
 
@@ -1301,11 +1311,11 @@ def layer_norm(X, gamma=None, beta=None, eps=1e-5, out=None, stats=None):
     x, ldx = _rows(X, "X")
     M, N = x.shape
     g, b = _floats(gamma, N, "gamma"), _floats(beta, N, "beta")
-    y = _result(out, (M, N), x.dtype, "out")
-    if stats is not None and not _result(stats, (M, 2), _torch.float32, "stats").is_contiguous():
+    y, ldy = _result(out, (M, N), x.dtype, "out")
+    if stats is not None and not _result(stats, (M, 2), _torch.float32, "stats")[0].is_contiguous():
         raise ValueError("stats must be contiguous")
     _llm_call(lib.gen9blas_layer_norm, 1 if x.dtype is _torch.float32 else 0, M, N, x.data_ptr(), ldx, _ptr(g), _ptr(b), eps,
-              y.data_ptr(), N if out is None else _out_step(y, "out"), _ptr(stats))
+              y.data_ptr(), ldy, _ptr(stats))
     return _host_like(X, y) if out is None else y
 
 
@@ -1320,10 +1330,10 @@ def layer_norm_backward(dY, X, stats, gamma=None, dX=None, dgamma=None, dbeta=No
     g = _floats(gamma, N, "gamma")
     if not set(grads) <= set("xgb"):
         raise ValueError(f"grads {grads!r}: of 'x', 'g' and 'b'")
-    gx = _result(dX, (M, N), t, "dX") if "x" in grads else None
+    gx, lddx = _result(dX, (M, N), t, "dX") if "x" in grads else (None, 0)
     gg, gb = _float_sums(dgamma, N, "g" in grads, accumulate, "dgamma"), _float_sums(dbeta, N, "b" in grads, accumulate, "dbeta")
     _llm_call(lib.gen9blas_layer_norm_backward, 1 if t is _torch.float32 else 0, M, N, dy.data_ptr(), lddy, x.data_ptr(), ldx,
-              stats.data_ptr(), _ptr(g), _ptr(gx), 0 if gx is None else _out_step(gx, "dX"), _ptr(gg), _ptr(gb), bool(accumulate))
+              stats.data_ptr(), _ptr(g), _ptr(gx), lddx, _ptr(gg), _ptr(gb), bool(accumulate))
     return tuple(v if v is None or given is not None else _host_like(dY, v) for v, given in ((gx, dX), (gg, dgamma), (gb, dbeta)))
 
 
@@ -1335,26 +1345,31 @@ def dropout(X, p, seed=0, offset=0, residual=None, out=None):
     x, ldx = _rows(X, "X")
     M, N = x.shape
     r, ldr = (None, 0) if residual is None else _matrix_like(residual, (M, N), x.dtype, "residual")
-    y = _result(out, (M, N), x.dtype, "out")
+    y, ldy = _result(out, (M, N), x.dtype, "out")
     _llm_call(lib.gen9blas_dropout, 1 if x.dtype is _torch.float32 else 0, M, N, x.data_ptr(), ldx, p, seed & _U64, offset & _U64,
-              _ptr(r), ldr, y.data_ptr(), N if out is None else _out_step(y, "out"))
+              _ptr(r), ldr, y.data_ptr(), ldy)
     return _host_like(X, y) if out is None else y
 
 
 def _token_ids(ids):
     """Tokens as a dense GPU vector of int32 or int64."""
-    i = ids if isinstance(ids, _torch.Tensor) and ids.is_cuda else _on_gpu(ids)
-    if i.is_floating_point() or i.is_complex() or i.dtype is _torch.bool:
-        raise TypeError(f"ids are integers, not {i.dtype}")
-    if i.dim() != 1:
-        raise ValueError(f"ids of {i.dim()} dimensions, expected 1")
+    i = ids
+    if not (type(i) is _torch.Tensor and (i.dtype is _torch.int64 or i.dtype is _torch.int32) and i.is_contiguous() and i.dim() == 1):
+        i = _on_gpu(ids)
+        if i.is_floating_point() or i.is_complex() or i.dtype is _torch.bool:
+            raise TypeError(f"ids are integers, not {i.dtype}")
+        if i.dim() != 1:
+            raise ValueError(f"ids of {i.dim()} dimensions, expected 1")
+        if i.dtype is not _torch.int64 and i.dtype is not _torch.int32:
+            i = i.to(_torch.int64)
+        i = i.contiguous()
+    if not i.is_cuda:
+        i = i.to(_llm_gpu)
     if i.shape[0] > _LONGEST:
         raise ValueError(f"{i.shape[0]} ids; the most are {_LONGEST}")
-    if i.dtype is not _torch.int64 and i.dtype is not _torch.int32:
-        i = i.to(_torch.int64)
     if i.get_device() != _llm_device:
         raise ValueError(f"ids are on {i.device}; the library runs on {_llm_gpu}")
-    return i.contiguous()
+    return i
 
 
 def embedding(table, ids, scale=1.0, out=None):
@@ -1364,9 +1379,9 @@ def embedding(table, ids, scale=1.0, out=None):
     V, D = x.shape
     i = _token_ids(ids)
     T = i.shape[0]
-    y = _result(out, (T, D), x.dtype, "out")
+    y, ldy = _result(out, (T, D), x.dtype, "out")
     _llm_call(lib.gen9blas_embedding, 1 if x.dtype is _torch.float32 else 0, T, V, D, x.data_ptr(), ldt, i.data_ptr(), i.element_size(),
-              scale, y.data_ptr(), D if out is None else _out_step(y, "out"))
+              scale, y.data_ptr(), ldy)
     return _host_like(table, y) if out is None else y
 
 
@@ -1385,7 +1400,7 @@ def embedding_backward(dY, ids, rows, scale=1.0, out=None, accumulate=False):
     if out is None and accumulate:
         raise ValueError("accumulate needs out")
     f32 = _torch.float32
-    g = _result(out, (rows, D), f32 if out is not None and out.dtype is f32 else t, "out")
+    g, ldg = _result(out, (rows, D), f32 if out is not None and out.dtype is f32 else t, "out")
     _llm_call(lib.gen9blas_embedding_backward, 1 if t is f32 else 0, T, rows, D, dy.data_ptr(), lddy, i.data_ptr(), i.element_size(), scale,
-              1 if g.dtype is f32 else 0, g.data_ptr(), D if out is None else _out_step(g, "out"), bool(accumulate))
+              1 if g.dtype is f32 else 0, g.data_ptr(), ldg, bool(accumulate))
     return _host_like(dY, g) if out is None else g
