@@ -5,7 +5,8 @@
 
 namespace g9llm {
 
-// A thread has the eight columns of a Philox counter.
+// A thread has the eight columns of a Philox counter. The mask is made where it is used and never stored. HBM bounds it: 8192 × 11008
+// FP16 with R 96 µs, 541 MB at 5.6 TB/s (Philox's 20 products of 32 bits for 8 elements run beside the loads).
 template <class T>
 __global__ void __launch_bounds__(256) dropout_kernel(const T *__restrict__ X, long long ldx, Dropout d, const T *__restrict__ R, long long ldr, int M, int N, int groups,
                                                       T *__restrict__ Y, long long ldy) {

@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const T *__restrict__ X, 
 template <class T> static int pad_rows(const void *X, long long ldx, long long rows, int K, int ldd, int slot, const T **D) {
     void *d;
     const long long total = rows * (ldd / 8);
-    G9_TRY(scratch(slot, (size_t)total * 8 * sizeof(T), &d));
+    G9_TRY(work_buffer("linear", slot, (size_t)total * 8 * sizeof(T), &d));
     hipLaunchKernelGGL((pad_rows_kernel<T>), dim3((unsigned)std::min(cdiv(total, 256), 32LL * num_cus)), dim3(256), 0, stream, (const T *)X, ldx, K, (T *)d, ldd / 8, total);
     G9_HIP(hipGetLastError());
     *D = (const T *)d;
@@ -71,10 +71,8 @@ template <g9::hgl::HgCfg G> static int launch_h(HParams p, int slices) {
 }
 static int tiles_product(HParams &p) {
     using namespace g9::hgl;
-    void *work;
-    G9_TRY(scratch(SLOT_PART, SPLIT_BYTES, &work));
-    p.P = (float *)work;
     const Choice c = choose({p.M, p.N, p.K, 1, p.ldc, 0, 1}, SPLIT_BYTES, num_cus);
+    if (c.slices > 1) G9_TRY(work_buffer("linear", SLOT_PART, SPLIT_BYTES, (void **)&p.P));
     switch (c.cfg) {
     case 0: return launch_h<CFG[0]>(p, c.slices);
     case 1: return launch_h<CFG[1]>(p, c.slices);
@@ -105,10 +103,8 @@ template <g9::sgl::SgCfg G> static int launch_s(SParams p, int slices) {
 }
 static int tiles_product(SParams &p) {
     using namespace g9::sgl;
-    void *work;
-    G9_TRY(scratch(SLOT_PART, SPLIT_BYTES, &work));
-    p.P = (float *)work;
     const Choice c = choose({p.M, p.N, p.K, 1}, SPLIT_BYTES, false, false, num_cus);
+    if (c.slices > 1) G9_TRY(work_buffer("linear", SLOT_PART, SPLIT_BYTES, (void **)&p.P));
     switch (c.cfg) {
     case 1: return launch_s<CFG[1]>(p, c.slices);
     case 3: return launch_s<CFG[3]>(p, c.slices);
@@ -148,7 +144,7 @@ template <class T, int MT, int NS> static int some_rows(RowsArgs<T> a) {
     const int pieces = (int)cdiv(a.K, 512 / sizeof(T));
     a.per = (int)cdiv(pieces, std::max(1LL, std::min<long long>(pieces, num_cus / tiles)));
     a.slices = (int)cdiv(pieces, a.per);
-    if (a.slices > 1) G9_TRY(scratch(SLOT_PART, (size_t)a.slices * tiles * 4 * MT * 1024, (void **)&a.parts));
+    if (a.slices > 1) G9_TRY(work_buffer("linear", SLOT_PART, (size_t)a.slices * tiles * 4 * MT * 1024, (void **)&a.parts));
     G9_TRY(check_grid(tiles * a.slices, 512));
     hipLaunchKernelGGL((linear_rows_kernel<T, MT, NS>), dim3((unsigned)(tiles * a.slices)), dim3(512), 0, stream, a);
     G9_HIP(hipGetLastError());
@@ -273,14 +269,14 @@ static int backward(int type, int M, int N, int K, const T *dY, int lddy, const 
     T *dZ = nullptr;
     void *p;
     if (own && (dX || dW)) {
-        G9_TRY(scratch(SLOT_DZ, (size_t)M * lddz * sizeof(T), &p));
+        G9_TRY(work_buffer("linear_backward", SLOT_DZ, (size_t)M * lddz * sizeof(T), &p));
         dZ = (T *)p;
     }
     float *sums = nullptr;
     const int rows = (int)std::max(64LL, cdiv(M, 512));
     const long long blocks = cdiv(M, rows);
     if (db) {
-        G9_TRY(scratch(SLOT_SUMS, (size_t)blocks * N * 4, &p));
+        G9_TRY(work_buffer("linear_backward", SLOT_SUMS, (size_t)blocks * N * 4, &p));
         sums = (float *)p;
     }
     if (dZ || db) {
@@ -382,6 +378,7 @@ int gen9blas_linear_backward(int type, int M, int N, int K, const void *dY, int 
         if (dW) G9_TRY(zero_rows(dW, (long long)lddw * es, N, (long long)K * es));
         return db ? zero_rows(db, 4LL * N, 1, 4LL * N) : 0;
     }
+    G9_TRY(not_captured("linear_backward"));   // the products' library has buffers of its own
     const Dropout d = make_dropout(p, seed, offset);
     typedef _Float16 H;
     if (type == GEN9BLAS_H)

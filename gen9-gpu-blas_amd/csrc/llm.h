@@ -47,6 +47,13 @@ G9_HIDDEN int need_device(const void *p, size_t bytes, const char *what);
 // Device scratch, grown on demand and kept; growing waits for queued work.
 enum Slot { SLOT_A = 0, SLOT_PART, SLOT_PLAN, SLOT_SLOTS, SLOT_X, SLOT_W, SLOT_DZ, SLOT_SUMS, SLOT_SORT, NSLOTS };
 G9_HIDDEN int scratch(int slot, size_t bytes, void **p);
+// 0, or UNSUPPORTED while the stream is being captured into a graph: for calls that queue more than kernels on their operands.
+G9_HIDDEN int not_captured(const char *who);
+// scratch(), refused while captured: a graph would go on using a buffer that later calls write, and free as they outgrow it.
+inline int work_buffer(const char *who, int slot, size_t bytes, void **p) {
+    G9_TRY(not_captured(who));
+    return scratch(slot, bytes, p);
+}
 // Clears `rows` rows of `bytes` bytes (a multiple of 2), `ld` bytes apart.
 G9_HIDDEN int zero_rows(void *p, long long ld, long long rows, long long bytes);
 // The longest rows: kernels count k in an int, up to the end of the last 128-k chunk.

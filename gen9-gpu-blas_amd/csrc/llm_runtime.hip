@@ -48,6 +48,12 @@ int need_device(const void *p, size_t bytes, const char *what) {
     return 0;
 }
 
+int not_captured(const char *who) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    G9_HIP(hipStreamIsCapturing(stream, &status));
+    if (status != hipStreamCaptureStatusNone) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "%s: needs work buffers, which a captured graph cannot keep", who);
+    return 0;
+}
 int scratch(int slot, size_t bytes, void **p) {
     static struct { void *p; size_t size; } buf[NSLOTS];
     if (buf[slot].size < bytes) {

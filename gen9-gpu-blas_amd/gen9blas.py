@@ -28,6 +28,7 @@ import ctypes
 import importlib.util
 import os
 import sys
+from operator import index as _index
 from typing import NamedTuple
 
 import numpy as np
@@ -1273,7 +1274,7 @@ def linear(X, W, bias=None, act=None, dropout=0.0, seed=0, offset=0, residual=No
     z, ldz = (None, 0) if Z is None else _result(Z, (M, N), t, "Z")
     out, ldc = _result(C, (M, N), t, "C")
     _llm_call(lib.gen9blas_linear, 1 if t is _torch.float32 else 0, M, N, K, x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(b), a,
-              _ptr(z), ldz, dropout, seed & _U64, offset & _U64, _ptr(r), ldr, out.data_ptr(), ldc)
+              _ptr(z), ldz, dropout, _index(seed) & _U64, _index(offset) & _U64, _ptr(r), ldr, out.data_ptr(), ldc)
     return _host_like(X, out) if C is None else out
 
 
@@ -1300,7 +1301,7 @@ def linear_backward(dY, X, W, Z=None, act=None, dropout=0.0, seed=0, offset=0, d
     gw, lddw = _result(dW, (N, K), t, "dW") if "w" in grads else (None, 0)
     gb = _float_sums(db, N, "b" in grads, accumulate, "db")
     _llm_call(lib.gen9blas_linear_backward, 1 if t is _torch.float32 else 0, M, N, K, dy.data_ptr(), lddy, _ptr(z), ldz, a, dropout,
-              seed & _U64, offset & _U64, x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(gx), lddx, _ptr(gw), lddw, _ptr(gb), bool(accumulate))
+              _index(seed) & _U64, _index(offset) & _U64, x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(gx), lddx, _ptr(gw), lddw, _ptr(gb), bool(accumulate))
     return tuple(g if g is None or given is not None else _host_like(dY, g) for g, given in ((gx, dX), (gw, dW), (gb, db)))
 
 
@@ -1346,7 +1347,7 @@ def dropout(X, p, seed=0, offset=0, residual=None, out=None):
     M, N = x.shape
     r, ldr = (None, 0) if residual is None else _matrix_like(residual, (M, N), x.dtype, "residual")
     y, ldy = _result(out, (M, N), x.dtype, "out")
-    _llm_call(lib.gen9blas_dropout, 1 if x.dtype is _torch.float32 else 0, M, N, x.data_ptr(), ldx, p, seed & _U64, offset & _U64,
+    _llm_call(lib.gen9blas_dropout, 1 if x.dtype is _torch.float32 else 0, M, N, x.data_ptr(), ldx, p, _index(seed) & _U64, _index(offset) & _U64,
               _ptr(r), ldr, y.data_ptr(), ldy)
     return _host_like(X, y) if out is None else y
 

@@ -511,6 +511,57 @@ def test_a_training_step(g9, torch_dev, M):
         assert (got.cpu().double() - want).abs().max() <= 8 * 2 * 5 * 260 * U * max(1, float(want.abs().max()))
 
 
+def test_captured_and_replayed(g9, torch_dev):
+    """A graph of the operators that need no work buffers (a token through embedding, norm, linear layers and dropout), replayed on
+    new tokens with other work between; those that need some are refused, and the capture can be left."""
+    torch = torch_dev
+    V, D, F = 300, 512, 2048
+    gen = torch.Generator().manual_seed(5)
+    table, w1, w2 = (torch.randn(s, generator=gen).half().cuda() / 8 for s in ((V, D), (F, D), (D, F)))
+    gamma, bias = torch.rand(D, generator=gen).cuda(), torch.randn(F, generator=gen).cuda()
+    ids = torch.tensor([7], device="cuda")
+
+    def step():
+        e = g9.embedding(table, ids, scale=2.0)
+        h = g9.linear(g9.layer_norm(e, gamma), w1, bias, act="silu")
+        return g9.dropout(g9.linear(h, w2, residual=e), 0.25, seed=3, offset=4)
+
+    big = torch.randn(4096, D, generator=gen).half().cuda()
+    before = g9.linear(big, w1, bias)
+    g9.set_nowait(True)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = step()
+        for token in (7, 0, 299, -1, 8):
+            ids.fill_(token)
+            graph.replay()
+            got = y.clone()
+            g9.linear(big, w1, bias)                                       # other work, and another residual stream's buffers
+            g9.embedding_backward(big, torch.arange(4096, device="cuda") % V, V)
+            assert torch.equal(got, step()), token
+            torch.cuda.synchronize()
+        dy, tokens = torch.randn(4096, F, generator=gen).half().cuda(), torch.arange(4096, device="cuda") % V
+        for call in (lambda: g9.linear_backward(dy, big, w1), lambda: g9.embedding_backward(big, tokens, V),
+                     lambda: g9.layer_norm_backward(big, big, torch.ones(4096, 2, device="cuda"))):
+            refused = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(refused):
+                with pytest.raises(RuntimeError, match="captured"):
+                    call()
+    finally:
+        g9.set_nowait(False)
+    assert torch.equal(g9.linear(big, w1, bias), before)
+
+
+def test_counters_of_other_integer_types(g9, torch_dev):
+    torch = torch_dev
+    x = torch.ones(5, 40, device="cuda")
+    want = g9.dropout(x, 0.5, seed=-1, offset=1 << 40)
+    assert torch.equal(g9.dropout(x, 0.5, seed=np.int64(-1), offset=np.int64(1 << 40)), want)
+    with pytest.raises(TypeError):
+        g9.dropout(x, 0.5, seed=1.5)
+
+
 def test_streams(g9, torch_dev):
     """Calls from another torch stream are ordered with it on both sides; in no-wait mode too."""
     torch = torch_dev
