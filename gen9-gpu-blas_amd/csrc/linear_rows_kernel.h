@@ -8,7 +8,7 @@
 // v_mfma_f32_16x16x4_f32 (a sum over k in any order). FP32 sums of a stage begin at zero and are added to the running ones, whose
 // rounding grows with the stages then (24 × 4096 × 11008: 1.3e-7 of the result, one running sum 8e-7).
 // One barrier a stage: behind it stage j is there, and stage j − 1 has been read and is filled again.
-// 24 × 4096 × 11008 FP32 48 µs, 40 of them this kernel: 180 MB at 4.5 TB/s, what its 1.4 µs a stage leave of HBM's 6. The 64 × 64 tiles of
+// 24 × 4096 × 11008 FP32 44 µs, 39 of them this kernel: 180 MB at 4.6 TB/s, what its 1.4 µs a stage leave of HBM's 6. The 64 × 64 tiles of
 // the large products take 77, with 32 × 128 tiles 50. Operands straight from memory into registers 84 (a load of 16 bytes from each of 16 rows
 // takes 80 clocks); four waves 55; pieces of k dealt out evenly over the CUs whatever the shape, with cut tiles, 53.
 #pragma once
