@@ -347,7 +347,7 @@ static int gradient(int n, int V, int D, const T *dY, int lddy, const Ids &ids, 
     int cols = 0;
     while (cols < 8 && (8 << cols) < D) cols++;
     const unsigned slabs = (unsigned)cdiv(D, 8 << cols), piece_groups = (unsigned)cdiv(pieces, 256 >> cols);
-    if (slabs > 65535 || V > 1 << 27) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "embedding_backward: more rows or columns than one launch can index (V %d, D %d)", V, D);
+    if (slabs > 65535 || V > 1 << 27 || n > 0x7ffff000) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "embedding_backward: more than kernels can index (%d tokens, V %d, D %d)", n, V, D);
     char *w;
     const size_t lists = ((size_t)n * 4 + 15) / 16 * 16, marks = ((size_t)V + 15) / 16 * 16;
     G9_TRY(work_buffer("embedding_backward", SLOT_SORT, 4 * lists + (size_t)groups * 1024 + marks, (void **)&w));

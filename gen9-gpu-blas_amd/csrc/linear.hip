@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(256) linear_back_kernel(const T *__restrict__ 
     auto row = [&](long long m, float *v, const float *z) {
         if (Z)
 #pragma unroll
-            for (int e = 0; e < V; e++) v[e] *= slope<T, KIND>(act, z[e]);
+            for (int e = 0; e < V; e++) v[e] = gradient<T, KIND>(act, v[e], z[e]);
         if (d.limit) drop<V>(d, (unsigned)m, n, v);   // last: what is dropped is zero, whatever Z is there
         if (dZ) store_some<V>(dZ + m * lddz + n, valid, v);
 #pragma unroll

@@ -65,16 +65,16 @@ template <class T, int KIND> __device__ __forceinline__ float activate(const Act
     if constexpr (KIND == KIND_SIGMOID) return z * sigmoid<T>(z * (act.a + act.b * square(z)));
     return z * phi<T>(z);
 }
-// d activate / dz
-template <class T, int KIND> __device__ __forceinline__ float slope(const Activation &act, float z) {
-    if constexpr (KIND == KIND_CLIP) return z > act.low || z != z ? 1.f : 0.f;
+// dy times d activate / dz; what ReLU clips is zero, whatever dy is.
+template <class T, int KIND> __device__ __forceinline__ float gradient(const Activation &act, float dy, float z) {
+    if constexpr (KIND == KIND_CLIP) return z > act.low || z != z ? dy : 0.f;
     if constexpr (KIND == KIND_SIGMOID) {
         const float q = square(z), s = sigmoid<T>(z * (act.a + act.b * q));
-        return s + z * s * (1.f - s) * (act.a + 3.f * act.b * q);
+        return dy * (s + z * s * (1.f - s) * (act.a + 3.f * act.b * q));
     }
     float density;
     const float p = phi<T>(z, &density);
-    return __builtin_fmaf(z, density, p);
+    return dy * __builtin_fmaf(z, density, p);
 }
 
 template <class T> struct Epilogue {

@@ -95,7 +95,7 @@ enum { GEN9BLAS_ACT_NONE = 0, GEN9BLAS_ACT_RELU = 1, GEN9BLAS_ACT_GELU = 2, GEN9
 // - p, seed, offset: as in gen9blas_dropout (p = 0: none).
 GEN9BLAS_API int gen9blas_linear(int type, int M, int N, int K, const void *X, int ldx, const void *W, int ldw, const float *bias, int act,
                                  void *Z, int ldz, double p, uint64_t seed, uint64_t offset, const void *R, int ldr, void *Y, int ldy);
-// Its gradients: dZ = dropout(act'(Z)·dY), rounded to the type for the products; dX (M×K) = dZ·W; dW (N×K) = dZᵀ·X; db (N floats) =
+// Its gradients: dZ = dropout(act'(Z)·dY) (what ReLU clips or dropout takes is 0 whatever dY is), rounded to the type for the products; dX (M×K) = dZ·W; dW (N×K) = dZᵀ·X; db (N floats) =
 // the column sums of dZ before that rounding. Each may be NULL, and what only it needs is not read then (Z: without an activation).
 // R's gradient is dY. accumulate: dW and db are added to what is there. M = 0: dW and db are zeros, or stay. The products are
 // gen9blas_gemm's, which wait unless gen9blas_set_nowait is on.
@@ -126,7 +126,7 @@ GEN9BLAS_API int gen9blas_dropout(int type, int M, int N, const void *X, int ldx
 GEN9BLAS_API int gen9blas_embedding(int type, int T, int V, int D, const void *table, int ldt, const void *ids, int id_bytes, float scale,
                                     void *Y, int ldy);
 // The table's gradient: dT(v) = scale · Σ dY(t) over the tokens t with ids[t] = v, in their order, summed in FP32; rows without tokens
-// are zeros. accumulate: added to what is there, rows without tokens stay. out_type, dT's: type, or GEN9BLAS_S.
+// are zeros. accumulate: added to what is there, rows without tokens stay. out_type, dT's: type, or GEN9BLAS_S. V up to 2^27, D up to 2^26.
 GEN9BLAS_API int gen9blas_embedding_backward(int type, int T, int V, int D, const void *dY, int lddy, const void *ids, int id_bytes, float scale,
                                              int out_type, void *dT, int lddt, int accumulate);
 

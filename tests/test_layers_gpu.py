@@ -213,6 +213,23 @@ def test_what_is_dropped_is_zero(g9, torch_dev, dtype, name):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_what_relu_clips_has_no_gradient(g9, torch_dev, dtype):
+    """Infinities and NaN of dY where Z is not above zero; a NaN of Z passes dY on."""
+    torch = torch_dev
+    M, N, K = 33, 70, 64
+    t = torch.float16 if dtype is np.float16 else torch.float32
+    z = torch.tensor([1.0, -1.0, 0.0, -float("inf"), float("inf")], dtype=t, device="cuda").repeat(M * N // 5).view(M, N)
+    bad = torch.tensor([float("nan"), float("inf"), -float("inf")], dtype=t, device="cuda").repeat(M * N // 3).view(M, N)
+    x, w = torch.eye(K, dtype=t, device="cuda")[:M], torch.ones(N, K, dtype=t, device="cuda")
+    got = g9.linear_backward(torch.where(z > 0, torch.ones_like(z), bad), x, w, Z=z, act="relu")
+    want = g9.linear_backward((z > 0).to(t), x, w)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    _, _, db = g9.linear_backward(torch.ones_like(z), x, w, Z=torch.full_like(z, float("nan")), act="relu")
+    assert (db == M).all()
+
+
 @pytest.mark.parametrize("name", ACTS[1:])
 def test_linear_gradients_against_differences(g9, torch_dev, name):
     """Central differences of the framework's own forward pass in FP32: a step h = 2^-6 leaves h²/6 of the third derivative (at most 4
