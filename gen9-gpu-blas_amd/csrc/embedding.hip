@@ -52,19 +52,21 @@ struct ClearArgs {
     long long ldo;
     int V, D, groups, cols;   // 2^cols threads side by side
 };
-template <class O> __device__ __forceinline__ void clear_rows(const ClearArgs &a, long long group) {
+// Thread c of `threads`: whole 16 bytes at 16-byte addresses, past the caches, and single elements before and behind.
+template <class O> __device__ __forceinline__ void clear_row(O *row, int D, int c, int threads) {
     constexpr int V = 16 / sizeof(O);
     typedef O Vec __attribute__((ext_vector_type(V)));
+    const int head = min((int)(-(uintptr_t)row & 15) / (int)sizeof(O), D), body = (D - head) / V * V;
+    for (int x = c; x < D - body; x += threads) row[x < head ? x : x + body] = O(0);
+    for (int x = c * V; x < body; x += V * threads) __builtin_nontemporal_store(Vec{}, reinterpret_cast<Vec *>(row + head + x));
+}
+template <class O> __device__ __forceinline__ void clear_rows(const ClearArgs &a, long long group) {
     const long long v0 = group * CLEAR;
     const int lane = threadIdx.x & 63, c = threadIdx.x & ((1 << a.cols) - 1);
     const unsigned long long empty = __ballot(lane < CLEAR && v0 + lane < a.V && !(a.has && a.has[min(v0 + lane, a.V - 1LL)]));
     for (int r = threadIdx.x >> a.cols; r < CLEAR; r += (int)blockDim.x >> a.cols) {
         if (!(empty >> r & 1)) continue;
-        // whole 16 bytes at 16-byte addresses, past the caches, and single elements before and behind
-        O *row = (O *)a.out + (v0 + r) * a.ldo;
-        const int head = min((int)(-(uintptr_t)row & 15) / (int)sizeof(O), a.D), body = (a.D - head) / V * V;
-        for (int x = c; x < a.D - body; x += 1 << a.cols) row[x < head ? x : x + body] = O(0);
-        for (int x = c * V; x < body; x += V << a.cols) __builtin_nontemporal_store(Vec{}, reinterpret_cast<Vec *>(row + head + x));
+        clear_row((O *)a.out + (v0 + r) * a.ldo, a.D, c, 1 << a.cols);
     }
 }
 
@@ -173,7 +175,7 @@ __global__ void __launch_bounds__(1024) sort_place_kernel(Ids ids, Sorted in, in
     }
 }
 
-// Up to 4096 tokens: the whole sort in one workgroup, in LDS.
+// Up to 4096 tokens: the whole sort in one workgroup, in LDS (2000 tokens 9 µs, 4000 16).
 constexpr int SMALL = 4096;
 __global__ void __launch_bounds__(1024) sort_small_kernel(Ids ids, int n, int V, int bits, Sorted out, uint8_t *__restrict__ has) {
     __shared__ int keys[2][SMALL], ats[2][SMALL], waves[4], wave_count[16][256], base[256];
@@ -338,14 +340,142 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(GradArgs a) {
     put<O, E>(a, key, d, sum);
 }
 
+// Up to 1024 tokens in one launch, without work buffers: a workgroup has `rows` rows and 8 << cols columns. It sorts the tokens of
+// its rows by row in LDS, each wave a quarter of them in their order, cuts that list into a piece for each of its 256 >> cols rows
+// of threads, and joins the pieces' ends through LDS: as the kernels above do through memory. The rows without tokens are
+// dealt out among the workgroups of the same rows. The read of the tokens' first rows bounds it (1976 × 152 FP32, 64 tokens 6 µs), or
+// the clearing does (32000 × 4096 FP16 56).
+constexpr int FEW = 1024;
+template <class T, class O>
+__global__ void __launch_bounds__(256) embedding_few_kernel(GradArgs a, Ids ids, int rows, int clear_cols) {
+    constexpr int E = 8, U = 8;
+    __shared__ int list[FEW], base[4][64], total;   // list: row << 16 | token
+    __shared__ unsigned long long none;
+    __shared__ float part[256][2][E];
+    const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+    const int v0 = blockIdx.x * rows, mine = min(rows, a.V - v0);
+    const int quarter = (a.n + 3) / 4, t0 = wv * quarter, t1 = min(t0 + quarter, a.n);
+    base[wv][lane] = 0;
+    __syncthreads();
+    for (int i = t0 + lane; i < t1; i += 64) {
+        const int r = ids.key(i, a.V) - v0;   // no row's: V − v0 >= mine
+        if (r >= 0 && r < mine) atomicAdd(&base[wv][r], 1);
+    }
+    __syncthreads();
+    if (wv == 0) {   // a lane a row: where each wave's tokens of it begin
+        int c[4], sum = 0;
+#pragma unroll
+        for (int w = 0; w < 4; w++) c[w] = base[w][lane], sum += c[w];
+        int end = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int v = __shfl_up(end, d);
+            if (lane >= d) end += v;
+        }
+        int at = end - sum;
+#pragma unroll
+        for (int w = 0; w < 4; w++) base[w][lane] = at, at += c[w];
+        const unsigned long long empty = __ballot(sum == 0 && lane < mine);
+        if (lane == 63) total = end, none = empty;
+    }
+    __syncthreads();
+    const int m = total;
+    if (!a.accumulate) {
+        const unsigned long long empty = none;
+        const int c = t & ((1 << clear_cols) - 1);
+        for (int r = blockIdx.y + (t >> clear_cols) * gridDim.y; r < mine; r += (256 >> clear_cols) * gridDim.y)
+            if (empty >> r & 1) clear_row((O *)a.out + (long long)(v0 + r) * a.ldo, a.D, c, 1 << clear_cols);
+    }
+    if (!m) return;
+    for (int i0 = t0; i0 < t1; i0 += 64) {
+        const int i = i0 + lane, r = i < t1 ? ids.key(i, a.V) - v0 : -1;
+        const bool is = r >= 0 && r < mine;
+        unsigned long long same = __ballot(is);
+        if (!same) continue;
+#pragma unroll
+        for (int b = 0; b < 6; b++) {
+            const bool bit = r >> b & 1;
+            const unsigned long long set = __ballot(bit);
+            same &= bit ? set : ~set;
+        }
+        const int rank = __popcll(same & ((1ULL << lane) - 1)), at = is ? base[wv][r] : 0;
+        __builtin_amdgcn_wave_barrier();
+        if (is) {
+            list[at + rank] = r << 16 | i;
+            if (rank == 0) base[wv][r] = at + __popcll(same);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    const int c = t & ((1 << a.cols) - 1), side = t >> a.cols, d = ((blockIdx.y << a.cols) + c) * E;
+    const int per = (m + (256 >> a.cols) - 1) / (256 >> a.cols), i0 = min(side * per, m), i1 = d < a.D ? min(i0 + per, m) : i0;
+    auto row = [&](int i) { return list[i] >> 16; };
+    float sum[E] = {};
+    if (i0 < i1) {
+        const int before = i0 ? row(i0 - 1) : -1, behind = i1 < m ? row(i1) : -1;
+        int first = i0;
+        for (int i = i0; i < i1; i += U) {   // U rows on their way
+            float v[U][E];
+#pragma unroll
+            for (int u = 0; u < U; u++) load_some<E>((const T *)a.dY + (list[min(i + u, i1 - 1)] & 0xffff) * a.lddy + d, a.D - d, v[u]);
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (i + u >= i1) break;
+                const int key = row(i + u), next = i + u + 1 < i1 ? row(i + u + 1) : behind;
+#pragma unroll
+                for (int e = 0; e < E; e++) sum[e] += v[u][e];
+                if (next == key && i + u + 1 < i1) continue;
+                if ((first == i0 && before == key) || next == key) {
+#pragma unroll
+                    for (int e = 0; e < E; e++) part[t][first > i0][e] = sum[e];
+                } else put<O, E>(a, v0 + key, d, sum);
+#pragma unroll
+                for (int e = 0; e < E; e++) sum[e] = 0.f;
+                first = i + u + 1;
+            }
+        }
+    }
+    __syncthreads();
+    if (i0 >= i1 || i1 == m) return;
+    const int key = row(i1 - 1);
+    const bool whole = row(i0) == key;
+    if (row(i1) != key || (whole && i0 && row(i0 - 1) == key)) return;   // does not go on, or begins in an earlier one
+#pragma unroll
+    for (int e = 0; e < E; e++) sum[e] = part[t][!whole][e];
+    for (int p = 1; i0 + p * per < m && row(i0 + p * per) == key; p++)
+#pragma unroll
+        for (int e = 0; e < E; e++) sum[e] += part[t + (p << a.cols)][0][e];
+    put<O, E>(a, v0 + key, d, sum);
+}
+
+// The exponent of 2 of how many threads side by side, of 8 columns each, D columns take.
+static int widths(int D, int most) {
+    int cols = 0;
+    while (cols < most && (8 << cols) < D) cols++;
+    return cols;
+}
 template <class T, class O>
 static int gradient(int n, int V, int D, const T *dY, int lddy, const Ids &ids, float scale, O *out, int ldo, int accumulate) {
+    const int past = sizeof(O) == 2 && (uintptr_t)out % 128 == 0 && ldo % 64 == 0;
+    const int cols = widths(D, 8);
+    // Few tokens: every workgroup reads all of them, so the columns of one, which narrow leave more threads for a token's sum, are as wide
+    // as 10 workgroups a CU ask for; and with nothing to clear, 20 a CU are the most (µs, here / sorted by a launch of its own: 816 tokens,
+    // 1976 × 152 FP32 7.6 / 15.6, one token in all places 15 / 30; 32000 × 1024 FP16 20 / 23, one token 45 / 39; 32000 × 4096 FP32 101 /
+    // 111; 256 tokens accumulated, 32000 × 4096 19 / 15, 64 tokens 14 / 16).
+    int few_cols = std::min(cols, 3);
+    auto workgroups = [&](int rows) { return cdiv(V, rows) * cdiv(D, 8 << few_cols); };
+    while (few_cols < std::min(cols, 5) && workgroups(64) > 10 * num_cus) few_cols++;
+    if (n <= FEW && D <= 1 << 21 && V <= 1 << 27 && (!accumulate || n <= 64 || workgroups(64) <= 20 * num_cus)) {
+        const int rows = workgroups(64) >= 2 * num_cus ? 64 : 16;
+        const GradArgs a = {dY, lddy, {}, out, ldo, nullptr, 0, scale, n, V, D, 0, 0, few_cols, accumulate, past};
+        hipLaunchKernelGGL((embedding_few_kernel<T, O>), dim3((unsigned)cdiv(V, rows), (unsigned)cdiv(D, 8 << few_cols)), dim3(256), 0, stream, a, ids, rows, cols);
+        G9_HIP(hipGetLastError());
+        return 0;
+    }
     // places of a workgroup of the sort, and of a piece: few enough of both that what reads all of them stays short
     const int per = (int)(cdiv(cdiv(n, 256), 1024) * 1024), groups = (int)cdiv(n, per);
     const int piece = (int)std::max(8LL, cdiv(n, 512)), pieces = (int)cdiv(n, piece);
     const long long ldp = cdiv(D, 8) * 8;
-    int cols = 0;
-    while (cols < 8 && (8 << cols) < D) cols++;
     const unsigned slabs = (unsigned)cdiv(D, 8 << cols), piece_groups = (unsigned)cdiv(pieces, 256 >> cols);
     if (slabs > 65535 || V > 1 << 27 || n > 0x7ffff000) G9_FAIL(GEN9BLAS_ERR_UNSUPPORTED, "embedding_backward: more than kernels can index (%d tokens, V %d, D %d)", n, V, D);
     char *w;
@@ -384,7 +514,7 @@ static int gradient(int n, int V, int D, const T *dY, int lddy, const Ids &ids, 
     }
     G9_HIP(hipGetLastError());
     const GradArgs a = {dY, lddy, in, out, ldo, (float *)parts, ldp, scale, n, V, D, piece, pieces, cols, accumulate,
-                        sizeof(O) == 2 && (uintptr_t)out % 128 == 0 && ldo % 64 == 0};
+                        past};
     hipLaunchKernelGGL((embedding_grad_kernel<T, O>), dim3(piece_groups + (unsigned)cdiv(all.groups - cleared, slabs), slabs), dim3(256), 0, stream, a, all, cleared);
     G9_HIP(hipGetLastError());
     if (pieces > 1) hipLaunchKernelGGL((embedding_join_kernel<O>), dim3(piece_groups, slabs), dim3(256), 0, stream, a);

@@ -15,8 +15,8 @@
 //   return NULL on error and set gen9blas_llm_last_status(). Non-positive M, T or rows make a call a no-op.
 // - Work buffers belong to the process and grow on demand (growing waits for queued work): callers serialize calls.
 // - HIP graphs: gen9blas_layer_norm, _dropout, _embedding, and gen9blas_linear where it splits no k and copies no operand, queue kernels
-//   on their operands only and can be captured. The backward calls (but layer_norm's of few rows) and other linear calls are
-//   UNSUPPORTED then; those of MX4 matrices and experts are not meant for it.
+//   on their operands only and can be captured, and the backward calls of layer_norm with few rows and of embedding with few tokens.
+//   The others around them are UNSUPPORTED then; those of MX4 matrices and experts are not meant for it.
 // - type is GEN9BLAS_H (FP16) or GEN9BLAS_S (FP32); sums are FP32, each result is rounded once.
 #pragma once
 #include <stddef.h>

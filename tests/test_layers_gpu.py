@@ -441,7 +441,7 @@ def embedding_grad(dy, ids, V):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,V,D", [(1, 1, 1), (3, 1, 5), (31, 40, 8), (32, 2, 100), (33, 1, 64), (64, 3, 2049), (100, 255, 33), (1000, 256, 16), (1023, 257, 24), (1025, 65535, 9), (5000, 65536, 4),
-                                   (5000, 70, 130), (40000, 300, 20), (3000, 1 << 17, 12), (9, (1 << 20) + 100, 4), (5000, 1 << 18, 8)])
+                                   (5000, 70, 130), (40000, 300, 20), (3000, 1 << 17, 12), (9, (1 << 20) + 100, 4), (5000, 1 << 18, 8), (1100, 200, 1500), (4096, 40, 257)])
 def test_embedding_backward(g9, torch_dev, dtype, T, V, D):
     torch = torch_dev
     r = np.random.default_rng(T + V)
@@ -473,6 +473,28 @@ def test_embedding_backward_is_exact_on_integers(g9, torch_dev, dtype):
     dy = r.integers(-1, 2, (len(ids), 72)).astype(dtype)
     want, _ = embedding_grad(dy, ids, 700)
     assert np.array_equal(g9.embedding_backward(gpu(torch, dy), gpu(torch, ids), 700).cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V,D", [(1, 1), (15, 8), (17, 70), (64, 72), (65, 300), (2000, 33), (10000, 900)])
+@pytest.mark.parametrize("T", [1, 2, 63, 64, 257, 1023, 1024])
+def test_embedding_backward_of_few_tokens(g9, torch_dev, dtype, T, V, D):
+    """Small integers, whose sums are exact: one token in all places, tokens in turn, and a few places of others among one's."""
+    torch = torch_dev
+    r = np.random.default_rng(T)
+    one = np.full(T, V // 2)
+    some = one.copy()
+    some[r.integers(0, T, 1 + T // 10)] = r.integers(-2, V + 2, 1 + T // 10)
+    for ids in (one, np.arange(T) * 7 % V, some):
+        dy = r.integers(-1, 2, (T, D)).astype(dtype)
+        want, _ = embedding_grad(dy, ids, V)
+        i = gpu(torch, ids)
+        out, buf = laid(torch, np.full((V, D), 7, dtype), 3, 1)
+        g9.embedding_backward(gpu(torch, dy), i, V, out=out)
+        assert np.array_equal(out.cpu().numpy(), want)
+        beside = buf[1:1 + V * (D + 3)].view(V, D + 3)[:, D:]
+        assert torch.isnan(beside).all() and torch.isnan(buf[:1]).all() and torch.isnan(buf[1 + V * (D + 3):]).all()
+        assert np.array_equal(g9.embedding_backward(gpu(torch, dy), i, V, out=torch.ones(V, D, device="cuda"), accumulate=True).cpu().numpy(), 1 + want)
 
 
 def test_embedding_empty(g9, torch_dev):
@@ -568,6 +590,39 @@ def test_captured_and_replayed(g9, torch_dev):
     finally:
         g9.set_nowait(False)
     assert torch.equal(g9.linear(big, w1, bias), before)
+
+
+def test_gradients_captured_and_replayed(g9, torch_dev):
+    """A graph of the gradients that need no work buffers: few tokens' tables, few rows' norms."""
+    torch = torch_dev
+    V, D, T = 500, 320, 600
+    gen = torch.Generator().manual_seed(6)
+    dy, x = (torch.randn(T, D, generator=gen).cuda() for _ in range(2))
+    ids, stats = torch.zeros(T, dtype=torch.int64, device="cuda"), torch.empty(4, 2, device="cuda")
+    table, total = torch.empty(V, D, device="cuda"), torch.zeros(V, D, device="cuda")
+
+    def step(table, total):
+        g9.embedding_backward(dy, ids, V, out=table)
+        g9.embedding_backward(dy, ids, V, out=total, accumulate=True)
+        g9.layer_norm(x[:4], stats=stats)
+        return g9.layer_norm_backward(dy[:4], x[:4], stats)
+
+    g9.set_nowait(True)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step(table, total)
+        for seed in range(4):
+            ids.copy_(torch.randint(-1, V if seed % 2 else 2, (T,), generator=gen))
+            x.mul_(-1.5)
+            want = torch.empty_like(table), total.clone()
+            graph.replay()
+            norm = step(*want)
+            for a, b in zip((table, total, *got), (*want, *norm)):
+                assert torch.equal(a, b), seed
+            torch.cuda.synchronize()
+    finally:
+        g9.set_nowait(False)
 
 
 def test_counters_of_other_integer_types(g9, torch_dev):
