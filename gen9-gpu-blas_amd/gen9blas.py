@@ -943,6 +943,8 @@ def _llm_call(fn, *args):
         if fn(*args) != 0:
             raise RuntimeError(_llm.gen9blas_llm_error().decode())
     else:
+        if not _nowait and _torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a call that waits cannot be captured: set_nowait(True) before the capture")
         current, ours = _torch.cuda.current_stream(_llm_device), _torch.cuda.ExternalStream(hip_stream(), device=_llm_gpu)
         ours.wait_stream(current)
         rc = fn(*args)

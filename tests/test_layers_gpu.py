@@ -625,6 +625,20 @@ def test_gradients_captured_and_replayed(g9, torch_dev):
         g9.set_nowait(False)
 
 
+def test_calls_that_wait_are_not_captured(g9, torch_dev):
+    torch = torch_dev
+    x = torch.randn(3, 40, device="cuda")
+    want = g9.layer_norm(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = x + 1
+        with pytest.raises(RuntimeError, match="set_nowait"):
+            g9.layer_norm(x)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, x + 1) and torch.equal(g9.layer_norm(x), want)
+
+
 def test_counters_of_other_integer_types(g9, torch_dev):
     torch = torch_dev
     x = torch.ones(5, 40, device="cuda")
