@@ -382,6 +382,12 @@ template <class T> static int norm_back(BackArgs a) {
         rc = run();
     }, Shape<16, 1>(), Shape<16, 2>(), Shape<64, 1>(), Shape<64, 2>(), Shape<256, 1>(), Shape<256, 2>(), Shape<512, 2>(), Shape<1024, 2>());
     if (fits) return rc;
+    const int rows = (int)std::max(32LL, cdiv(a.M, 512));
+    const long long blocks = cdiv(a.M, rows);
+    if (both) {   // before the first launch: what is refused has written nothing
+        G9_TRY(work_buffer("layer_norm_backward", SLOT_SUMS, (size_t)blocks * 2 * a.N * 4, &sums));
+        a.sums = (float *)sums;
+    }
     if (a.dX)
         G9_TRY(by_rows(a.M, 1024, [&](long long m0, unsigned rows) -> int {
             BackArgs b = a;
@@ -391,10 +397,6 @@ template <class T> static int norm_back(BackArgs a) {
             return 0;
         }));
     if (both) {
-        const int rows = (int)std::max(32LL, cdiv(a.M, 512));
-        const long long blocks = cdiv(a.M, rows);
-        G9_TRY(work_buffer("layer_norm_backward", SLOT_SUMS, (size_t)blocks * 2 * a.N * 4, &sums));
-        a.sums = (float *)sums;
         hipLaunchKernelGGL((norm_sums_long_kernel<T>), dim3((unsigned)cdiv(a.N, 256), (unsigned)blocks), dim3(256), 0, stream, a, rows);
         G9_HIP(hipGetLastError());
         G9_TRY(column_sums((float *)sums, blocks, a.N, 2LL * a.N, dgamma, dbeta, a.accumulate));

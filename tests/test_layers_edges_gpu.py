@@ -160,6 +160,31 @@ def test_layer_norm_of_many_rows(g9, torch_dev, dtype, M, N):
     check_norm(g9, torch_dev, x, (1 + r.normal(0, 0.3, N)).astype(np.float32), r.normal(0, 0.3, N).astype(np.float32))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N", [(70, 512), (3, 40000)])
+def test_a_refused_capture_leaves_no_kernels(g9, torch_dev, dtype, M, N):
+    """A backward norm that is refused in a capture, as its sums need a work buffer, has put nothing into the graph."""
+    torch = torch_dev
+    t = tensor_type(torch, dtype)
+    x = torch.randn(M, N, device="cuda").to(t)
+    stats, dX = torch.empty(M, 2, device="cuda"), torch.full((M, N), 5.0, dtype=t, device="cuda")
+    g9.layer_norm(x, stats=stats)
+    g9.set_nowait(True)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = x + 1
+            with pytest.raises(RuntimeError, match="captured"):
+                g9.layer_norm_backward(x, x, stats, dX=dX)
+        for i in range(3):
+            x.mul_(-1)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, x + 1) and (dX == 5).all(), i
+    finally:
+        g9.set_nowait(False)
+
+
 # ---- embeddings ----
 @pytest.mark.parametrize("T", [262144, 300001])
 @pytest.mark.parametrize("V", [500, 70000])
