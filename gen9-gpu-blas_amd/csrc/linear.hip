@@ -279,6 +279,17 @@ static int backward(int type, int M, int N, int K, const T *dY, int lddy, const 
         G9_TRY(work_buffer("linear_backward", SLOT_SUMS, (size_t)blocks * N * 4, &p));
         sums = (float *)p;
     }
+    // copies and their buffers come before a result is written: a call that lacks the memory leaves a db that it would be added to
+    if (dX && odd(W, ldw) && M >= LONG) {
+        const int ldp = (int)cdiv(K, 8) * 8;
+        G9_TRY(pad_rows(W, ldw, N, K, ldp, SLOT_W, &W));
+        ldw = ldp;
+    }
+    if (dW && odd(X, ldx) && N >= LONG) {
+        const int ldp = (int)cdiv(K, 8) * 8;
+        G9_TRY(pad_rows(X, ldx, M, K, ldp, SLOT_X, &X));
+        ldx = ldp;
+    }
     if (dZ || db) {
         const Activation a = make_act(act);
         int cols = 0;
@@ -294,16 +305,6 @@ static int backward(int type, int M, int N, int K, const T *dY, int lddy, const 
         if (db) G9_TRY(column_sums(sums, blocks, N, N, db, nullptr, accumulate));
     }
     const T *g = own ? dZ : dY;
-    if (dX && odd(W, ldw) && M >= LONG) {
-        const int ldp = (int)cdiv(K, 8) * 8;
-        G9_TRY(pad_rows(W, ldw, N, K, ldp, SLOT_W, &W));
-        ldw = ldp;
-    }
-    if (dW && odd(X, ldx) && N >= LONG) {
-        const int ldp = (int)cdiv(K, 8) * 8;
-        G9_TRY(pad_rows(X, ldx, M, K, ldp, SLOT_X, &X));
-        ldx = ldp;
-    }
     auto product = [&](int tA, int m, int n, int k, const void *A, int lda, const void *B, int ldb, double beta, void *C, int ldc) -> int {
         if (int r = gen9blas_gemm(type, tA, 0, m, n, k, 1.0, A, lda, B, ldb, beta, C, ldc)) return fail(r, "%s", gen9blas_error());
         return 0;
