@@ -41,7 +41,7 @@ template <int L, int K> __device__ __forceinline__ void row_sum(float *v, float 
 #pragma unroll
         for (int k = 0; k < K; k++) {
             v[k] = 0.f;
-#pragma unroll
+#pragma unroll 8   // all of 16 waves' at once cost 1024 threads 40 registers each
             for (int i = 0; i < L / 64; i++) v[k] += part[i * K + k];
         }
     }
@@ -167,15 +167,23 @@ struct BackArgs {
     float *dgamma, *dbeta; // where one workgroup has all rows: the results (each may be null), and no sums
     int accumulate;
 };
+// What the rounding of a row's mean to one FP32 number has left in z = (x − mean)·rstd, from the sum of z: at most a step of the mean.
+// More than that is not the mean's, but z's own roundings, which lie on one side where x has fewer bits than the mean.
+__device__ __forceinline__ float mean_left(float z, float inv, float mean, float rstd) {
+    const float most = fabsf(mean) * rstd * 0x1p-23f;
+    return fminf(fmaxf(z * inv, -most), most);
+}
 // dx = rstd·(g − mean(g) − x̂·mean(g·x̂)), g = dy·gamma, x̂ = (x − mean)·rstd, and the sums over the rows that dgamma and dbeta
-// need, from one read of x and dy. The workgroups go through the rows with a stride; a thread adds up its own columns, and the
-// row groups of a workgroup are added in their order.
+// need, from one read of x and dy. stats hold the mean as one FP32 number, whose rounding is all of x̂'s error in a row far from zero
+// (mean 2^18 times the spread: 2^-7); so what it leaves is added up with the others, and taken off: x̂ = z − off, z = (x − mean)·rstd,
+// off = mean(z), mean(g·x̂) = mean(g·z) − off·mean(g). The workgroups go through the rows with a stride; a thread adds up its own
+// columns, and the row groups of a workgroup are added in their order.
 template <class T, int L, int C, int B, bool TAIL>
 __global__ void __launch_bounds__(B) norm_back_kernel(BackArgs a) {
     using P = Piece<T>;
     constexpr int V = P::V, ROWS = B / L;
     constexpr bool KEEP = C * V <= 16;   // gamma stays in registers from row to row
-    __shared__ float part[2][L > 64 ? 2 * (B / 64) : 1];
+    __shared__ float part[2][L > 64 ? 3 * (B / 64) : 1];
     __shared__ float join[ROWS > 1 ? 2 * V : 1][ROWS > 2 ? B + 64 / V : ROWS > 1 ? L : 1];   // reads of V by 64 / V lie in different banks
     const int t = threadIdx.x % L, group = threadIdx.x / L, N = a.N;
     const float inv = 1.f / N;
@@ -201,22 +209,25 @@ __global__ void __launch_bounds__(B) norm_back_kernel(BackArgs a) {
         typename P::Vec vx[C], vd[C];
 #pragma unroll
         for (int c = 0; c < C; c++) vx[c] = P::template load<TAIL>(x, (c * L + t) * V, N), vd[c] = P::template load<TAIL>(dy, (c * L + t) * V, N);
-        float s[2] = {0.f, 0.f};
+        float s[3] = {0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < C; c++) {
-            if ((c * L + t) * V >= N || (L > 64 && !is)) break;
+            const int n = (c * L + t) * V;
+            if (n >= N || (L > 64 && !is)) break;
             float g[V];
             if constexpr (!KEEP) weights(c, g);
 #pragma unroll
             for (int e = 0; e < V; e++) {
-                const float d = (float)vd[c][e], xh = ((float)vx[c][e] - mean) * rstd, w = d * (KEEP ? keep[KEEP ? c : 0][e] : g[e]);
-                s[0] += w, s[1] = __builtin_fmaf(w, xh, s[1]);
-                sg[c][e] = __builtin_fmaf(d, xh, sg[c][e]), sb[c][e] += d;
+                const float d = (float)vd[c][e], z = ((float)vx[c][e] - mean) * rstd, w = d * (KEEP ? keep[KEEP ? c : 0][e] : g[e]);
+                sb[c][e] += d, s[0] += w, s[1] = __builtin_fmaf(w, z, s[1]), s[2] += !TAIL || n + e < N ? z : 0.f;
             }
         }
-        if (!a.dX) continue;
-        row_sum<L, 2>(s, part[flip] + (L > 64 ? group * (L / 64) * 2 : 0));
-        const float p = s[0] * inv, q = s[1] * inv;
+        if (!a.dX && !a.dgamma) continue;
+        row_sum<L, 3>(s, part[flip] + (L > 64 ? group * (L / 64) * 3 : 0));
+        // z and dy's FP32 values are made again from here: kept over the sum they cost FP16 rows 24 registers of each thread's 128, and spills
+#pragma unroll
+        for (int c = 0; c < C; c++) asm volatile("" : "+v"(vx[c]), "+v"(vd[c]));
+        const float off = mean_left(s[2], inv, mean, rstd), p = s[0] * inv, q = (s[1] - off * s[0]) * inv;
         T *dx = (T *)a.dX + m * a.lddx;
 #pragma unroll
         for (int c = 0; c < C; c++) {
@@ -226,10 +237,11 @@ __global__ void __launch_bounds__(B) norm_back_kernel(BackArgs a) {
             if constexpr (!KEEP) weights(c, g);
 #pragma unroll
             for (int e = 0; e < V; e++) {
-                const float d = (float)vd[c][e], xh = ((float)vx[c][e] - mean) * rstd;
+                const float d = (float)vd[c][e], xh = __builtin_fmaf((float)vx[c][e] - mean, rstd, -off);
                 g[e] = rstd * (d * (KEEP ? keep[KEEP ? c : 0][e] : g[e]) - p - xh * q);
+                sg[c][e] = __builtin_fmaf(d, xh, sg[c][e]);
             }
-            store_some<V>(dx + n, valid, g);
+            if (a.dX) store_some<V>(dx + n, valid, g);
         }
     }
     if (!a.sums && !a.dgamma && !a.dbeta) return;
@@ -285,49 +297,56 @@ __global__ void __launch_bounds__(B) norm_back_kernel(BackArgs a) {
     }
 }
 
-// Rows too long for that: dx alone, from two passes over x and dy, and the sums by themselves.
+// Rows too long for that: dx and off of each row (each may be null), from two passes over x and dy, and the sums by themselves.
 template <class T>
-__global__ void __launch_bounds__(1024) norm_back_long_kernel(BackArgs a) {
+__global__ void __launch_bounds__(1024) norm_back_long_kernel(BackArgs a, float *__restrict__ offs) {
     using P = Piece<T>;
     constexpr int V = P::V;
-    __shared__ float part[32];
+    __shared__ float part[48];
     const T *x = (const T *)a.X + blockIdx.x * a.ldx, *dy = (const T *)a.dY + blockIdx.x * a.lddy;
     T *dx = (T *)a.dX + blockIdx.x * a.lddx;
     const float mean = a.stats[2LL * blockIdx.x], rstd = a.stats[2LL * blockIdx.x + 1], inv = 1.f / a.N;
-    float s[2] = {0.f, 0.f};
+    float s[3] = {0.f, 0.f, 0.f};
     auto each = [&](auto use) {
         for (long long n = threadIdx.x * V; n < a.N; n += 1024 * V) {
             const typename P::Vec vx = P::load(x, (int)n, a.N), vd = P::load(dy, (int)n, a.N);
             const int valid = (int)(a.N - n);
-            float g[V], xh[V];
+            float g[V], z[V];
             if (a.gamma) load_some<V>(a.gamma + n, valid, g);
 #pragma unroll
-            for (int e = 0; e < V; e++) g[e] = a.gamma ? (float)vd[e] * g[e] : (float)vd[e], xh[e] = ((float)vx[e] - mean) * rstd;
-            use(n, valid, g, xh);
+            for (int e = 0; e < V; e++) g[e] = a.gamma ? (float)vd[e] * g[e] : (float)vd[e], z[e] = ((float)vx[e] - mean) * rstd;
+            use(n, valid, g, z);
         }
     };
-    each([&](long long, int valid, const float *g, const float *xh) {
+    each([&](long long, int valid, const float *g, const float *z) {
 #pragma unroll
-        for (int e = 0; e < V; e++) s[0] += g[e], s[1] += e < valid ? g[e] * xh[e] : 0.f;
+        for (int e = 0; e < V; e++) s[0] += g[e], s[1] += e < valid ? g[e] * z[e] : 0.f, s[2] += e < valid ? z[e] : 0.f;
     });
-    row_sum<1024, 2>(s, part);
-    const float p = s[0] * inv, q = s[1] * inv;
-    each([&](long long n, int valid, float *g, const float *xh) {
+    row_sum<1024, 3>(s, part);
+    const float off = mean_left(s[2], inv, mean, rstd), p = s[0] * inv, q = (s[1] - off * s[0]) * inv;
+    if (offs && threadIdx.x == 0) offs[blockIdx.x] = off;
+    if (!a.dX) return;
+    each([&](long long n, int valid, float *g, const float *z) {
 #pragma unroll
-        for (int e = 0; e < V; e++) g[e] = rstd * (g[e] - p - xh[e] * q);
+        for (int e = 0; e < V; e++) g[e] = rstd * (g[e] - p - (z[e] - off) * q);
         store_some<V>(dx + n, valid, g);
     });
 }
+// offs: null where dbeta alone is wanted
 template <class T>
-__global__ void __launch_bounds__(256) norm_sums_long_kernel(BackArgs a, int rows) {
+__global__ void __launch_bounds__(256) norm_sums_long_kernel(BackArgs a, const float *__restrict__ offs, int rows) {
     const int n = blockIdx.x * 256 + threadIdx.x;
     if (n >= a.N) return;
     const long long m0 = (long long)blockIdx.y * rows, m1 = min(m0 + rows, (long long)a.M);
     float g = 0.f, b = 0.f;
-    for (long long m = m0; m < m1; m++) {
-        const float d = (float)((const T *)a.dY)[m * a.lddy + n];
-        g = __builtin_fmaf(d, ((float)((const T *)a.X)[m * a.ldx + n] - a.stats[2 * m]) * a.stats[2 * m + 1], g), b += d;
-    }
+    const T *dy = (const T *)a.dY + n, *x = (const T *)a.X + n;
+    if (offs)
+        for (long long m = m0; m < m1; m++) {
+            const float d = (float)dy[m * a.lddy];
+            g = __builtin_fmaf(d, ((float)x[m * a.ldx] - a.stats[2 * m]) * a.stats[2 * m + 1] - offs[m], g), b += d;
+        }
+    else
+        for (long long m = m0; m < m1; m++) b += (float)dy[m * a.lddy];
     a.sums[2LL * blockIdx.y * a.N + n] = g;
     a.sums[(2LL * blockIdx.y + 1) * a.N + n] = b;
 }
@@ -384,20 +403,24 @@ template <class T> static int norm_back(BackArgs a) {
     if (fits) return rc;
     const int rows = (int)std::max(32LL, cdiv(a.M, 512));
     const long long blocks = cdiv(a.M, rows);
+    float *offs = nullptr;
     if (both) {   // before the first launch: what is refused has written nothing
-        G9_TRY(work_buffer("layer_norm_backward", SLOT_SUMS, (size_t)blocks * 2 * a.N * 4, &sums));
+        const long long planes = blocks * 2 * a.N;
+        G9_TRY(work_buffer("layer_norm_backward", SLOT_SUMS, (size_t)(planes + a.M) * 4, &sums));
         a.sums = (float *)sums;
+        if (dgamma) offs = a.sums + planes;
     }
-    if (a.dX)
+    if (a.dX || offs)
         G9_TRY(by_rows(a.M, 1024, [&](long long m0, unsigned rows) -> int {
             BackArgs b = a;
-            b.dY = (const T *)a.dY + m0 * a.lddy, b.X = (const T *)a.X + m0 * a.ldx, b.stats = a.stats + 2 * m0, b.dX = (T *)a.dX + m0 * a.lddx;
-            hipLaunchKernelGGL((norm_back_long_kernel<T>), dim3(rows), dim3(1024), 0, stream, b);
+            b.dY = (const T *)a.dY + m0 * a.lddy, b.X = (const T *)a.X + m0 * a.ldx, b.stats = a.stats + 2 * m0;
+            if (a.dX) b.dX = (T *)a.dX + m0 * a.lddx;
+            hipLaunchKernelGGL((norm_back_long_kernel<T>), dim3(rows), dim3(1024), 0, stream, b, offs ? offs + m0 : nullptr);
             G9_HIP(hipGetLastError());
             return 0;
         }));
     if (both) {
-        hipLaunchKernelGGL((norm_sums_long_kernel<T>), dim3((unsigned)cdiv(a.N, 256), (unsigned)blocks), dim3(256), 0, stream, a, rows);
+        hipLaunchKernelGGL((norm_sums_long_kernel<T>), dim3((unsigned)cdiv(a.N, 256), (unsigned)blocks), dim3(256), 0, stream, a, (const float *)offs, rows);
         G9_HIP(hipGetLastError());
         G9_TRY(column_sums((float *)sums, blocks, a.N, 2LL * a.N, dgamma, dbeta, a.accumulate));
     }

@@ -108,8 +108,9 @@ GEN9BLAS_API int gen9blas_linear_backward(int type, int M, int N, int K, const v
 // (N floats) may be NULL: ones and zeros. stats (M×2 floats, or NULL): mean and rstd of each row, for the gradients.
 GEN9BLAS_API int gen9blas_layer_norm(int type, int M, int N, const void *X, int ldx, const float *gamma, const float *beta, float eps, void *Y,
                                      int ldy, float *stats);
-// Its gradients from dY, X and stats: dX, and sums over the rows in dgamma and dbeta (N floats); each may be NULL. accumulate: dgamma and
-// dbeta are added to what is there. M = 0: they are zeros, or stay.
+// Its gradients from dY, X and stats: dX, and sums over the rows in dgamma and dbeta (N floats); each may be NULL. What the rounding of
+// a mean in stats leaves of it (up to one step) is found from X again. accumulate: dgamma and dbeta are added to what is there. M = 0:
+// they are zeros, or stay.
 GEN9BLAS_API int gen9blas_layer_norm_backward(int type, int M, int N, const void *dY, int lddy, const void *X, int ldx, const float *stats,
                                               const float *gamma, void *dX, int lddx, float *dgamma, float *dbeta, int accumulate);
 

@@ -4,7 +4,7 @@ that file's bounds: n units of 2^-24 for a sum of n products in any order, half 
 import numpy as np
 import pytest
 
-from layers_util import HALF, TINY, dropout_factor, slope
+from layers_util import HALF, TINY, dropout_factor, layer_norm, layer_norm_back, slope
 from test_layers_gpu import U, check_norm, embedding_grad, gpu, laid, near, untouched
 
 pytestmark = pytest.mark.gpu
@@ -151,6 +151,43 @@ def test_overflows_of_sums_and_scales(g9, torch_dev):
 
 
 # ---- layer norm ----
+@pytest.mark.parametrize("M,N", [(1, 100), (40, 100), (5, 4096), (600, 300), (37, 999), (3, 20000), (70, 9001)])
+def test_layer_norm_gradients_of_rows_far_from_zero(g9, torch_dev, M, N):
+    """Means of up to 2^18 times the spread (FP32), whose rounding in stats is 2^-7 of the spread: the gradients are those of the exact
+    mean and rstd.
+
+    x - mean is exact where the mean is that large (the two are within a factor of 2); a product and the mean's correction, a sum of
+    n = N terms, remain of x̂'s error. A thread sums up to 64 terms and the threads' sums go up a tree, so the forward pass' first
+    mean is within 64 units of it, 1; the variance, E(d²) - E(d)² with |E(d)| <= 1 around it, is off by 6 n units and rstd by half."""
+    torch = torch_dev
+    r = np.random.default_rng(N)
+    means = np.resize([2.0 ** 18, -1e5, 7.0 * 2 ** 10, 3.0, 2.0 ** 17 + 0.3], M)[:, None]
+    x = (means + r.normal(0, 1, (M, N))).astype(np.float32)
+    dy, gamma = r.normal(0, 1, (M, N)).astype(np.float32), (1 + r.normal(0, 0.3, N)).astype(np.float32)
+    stats = torch.empty(M, 2, device="cuda")
+    g9.layer_norm(gpu(torch, x), gpu(torch, gamma), None, stats=stats)
+    x64, dy64 = x.astype(np.float64), dy.astype(np.float64)
+    _, mean, rstd = layer_norm(x64, gamma.astype(np.float64), 0.0, 1e-5)
+    dx, dg, db = layer_norm_back(dy64, x64, mean, rstd, gamma.astype(np.float64))
+    n = N + 8
+    er = (3 * n + 4) * U
+    xh, gy, rs = np.abs((x64 - mean[:, None]) * rstd[:, None]), np.abs(dy64 * gamma), rstd[:, None]
+    off = np.abs(mean[:, None]) * U * rs                     # what the mean's rounding leaves to take off
+    exh = 4 * U * (xh + off) + n * U * (xh.mean(1, keepdims=True) + off) + xh * er
+    a, c = gy.mean(1, keepdims=True), (gy * (xh + off)).mean(1, keepdims=True)
+    q = n * U * c + off * n * U * a + (gy * exh).mean(1, keepdims=True) + exh * a    # the error of mean(g·x̂)
+    bound = rs * (n * U * a + xh * q + exh * c + 8 * U * (gy + a + xh * c) + er * (gy + a + xh * c))
+    bg, bb = (M + 4) * U * (np.abs(dy64) * xh).sum(0) + (np.abs(dy64) * exh).sum(0), (M + 4) * U * np.abs(dy64).sum(0)
+    got = g9.layer_norm_backward(gpu(torch, dy), gpu(torch, x), stats, gpu(torch, gamma))
+    near(got[0], dx, bound, np.float32)
+    near(got[1], dg, bg, np.float32)
+    near(got[2], db, bb, np.float32)
+    for grads in ("x", "g", "b", "xb", "gb"):
+        some = g9.layer_norm_backward(gpu(torch, dy), gpu(torch, x), stats, gpu(torch, gamma), grads=grads)
+        for v, w, key in zip(some, got, "xgb"):
+            assert v is None if key not in grads else torch.equal(v, w), (grads, key)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("M,N", [(30000, 40), (7000, 500), (7001, 1001), (2000, 3001), (700, 9001), (600, 16001), (1000, 20001)])
 def test_layer_norm_of_many_rows(g9, torch_dev, dtype, M, N):
