@@ -65,16 +65,17 @@ template <class T, int KIND> __device__ __forceinline__ float activate(const Act
     if constexpr (KIND == KIND_SIGMOID) return z * sigmoid<T>(z * (act.a + act.b * square(z)));
     return z * phi<T>(z);
 }
-// dy times d activate / dz; what ReLU clips is zero, whatever dy is.
+// dy times d activate / dz; what ReLU clips is zero, whatever dy is. An infinite z, as FP16's stored ones past 65504 are, has the slope
+// that they have, 0 or 1: a factor that is zero there takes a z with an end (a NaN stays in s and p).
 template <class T, int KIND> __device__ __forceinline__ float gradient(const Activation &act, float dy, float z) {
     if constexpr (KIND == KIND_CLIP) return z > act.low || z != z ? dy : 0.f;
     if constexpr (KIND == KIND_SIGMOID) {
         const float q = square(z), s = sigmoid<T>(z * (act.a + act.b * q));
-        return dy * (s + z * s * (1.f - s) * (act.a + 3.f * act.b * q));
+        return dy * (s + __builtin_amdgcn_fmed3f(z, -3e38f, 3e38f) * s * (1.f - s) * (act.a + 3.f * act.b * q));
     }
     float density;
     const float p = phi<T>(z, &density);
-    return dy * __builtin_fmaf(z, density, p);
+    return dy * __builtin_fmaf(__builtin_amdgcn_fmed3f(z, -3e38f, 3e38f), density, p);
 }
 
 template <class T> struct Epilogue {

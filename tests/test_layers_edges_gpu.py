@@ -99,6 +99,38 @@ def test_linear_backward_of_many_rows(g9, torch_dev, dtype, M, N, K):
     near(got[2], *want[2], np.float32)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("name", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_slopes_at_infinity(g9, torch_dev, dtype, name):
+    """Pre-activations past FP16's range are stored as infinities: the slope there is that of the end, 0 or 1, as it is next to
+    them; a NaN stays one."""
+    torch = torch_dev
+    t = tensor_type(torch, dtype)
+    ends = [-np.inf, np.inf, -60000.0, 60000.0] + ([] if dtype is np.float16 else [-3e38, 3e38, -1e20, 1e20])
+    z = torch.tensor(ends, dtype=t, device="cuda").repeat(40, 16)
+    M, N = z.shape
+    dy = torch.arange(-M * N // 2, M * N // 2, device="cuda").view(M, N).remainder(17).to(t) + 1
+    x, w = torch.ones(M, 64, dtype=t, device="cuda"), torch.eye(N, 64, dtype=t, device="cuda")
+    dX, dW, db = g9.linear_backward(dy, x, w, Z=z, act=name)
+    want = torch.where(z > 0, dy, torch.zeros_like(dy))
+    assert torch.equal(dX, (want.double() @ w.double()).to(t)) and torch.equal(db, want.float().sum(0)) and torch.equal(dW, want.double().sum(0).to(t)[:, None].expand(N, 64))
+    z[3, 5] = float("nan")
+    assert torch.isnan(g9.linear_backward(dy, x, w, Z=z, act=name, grads="b")[2][5]) == (name != "relu")   # ReLU's passes dY on
+
+
+@pytest.mark.parametrize("name", ["gelu", "gelu_tanh", "silu"])
+def test_pre_activations_past_fp16_train(g9, torch_dev, name):
+    """A forward pass that is finite though Z is not has finite gradients."""
+    torch = torch_dev
+    x, w = torch.ones(40, 64, device="cuda").half(), torch.ones(70, 64, device="cuda").half()
+    bias = torch.full((70,), -1e5, device="cuda")
+    Z = torch.empty(40, 70, device="cuda", dtype=torch.float16)
+    y = g9.linear(x, w, bias, name, Z=Z)
+    assert torch.isneginf(Z).all() and (y == 0).all()
+    for g in g9.linear_backward(torch.ones_like(y), x, w, Z=Z, act=name):
+        assert (g == 0).all()
+
+
 # ---- results past FP16's range ----
 def same(torch, got, want):
     """Equal in every element, infinities with their signs."""
