@@ -131,6 +131,19 @@ def test_pre_activations_past_fp16_train(g9, torch_dev, name):
         assert (g == 0).all()
 
 
+def test_columns_past_one_launch(g9, torch_dev):
+    """More columns than a launch of 1024 threads for 64 of them can have."""
+    torch = torch_dev
+    N = (1 << 28) + 77
+    dy = torch.randint(-9, 10, (2, N), dtype=torch.int8, device="cuda").half()
+    w, x = torch.zeros(N, 1, dtype=torch.float16, device="cuda"), torch.zeros(2, 1, dtype=torch.float16, device="cuda")
+    db = torch.full((N,), float("nan"), device="cuda")
+    g9.linear_backward(dy, x, w, db=db, grads="b")
+    assert torch.equal(db, dy[0].float() + dy[1].float())
+    del dy, w, x, db
+    torch.cuda.empty_cache()
+
+
 # ---- results past FP16's range ----
 def same(torch, got, want):
     """Equal in every element, infinities with their signs."""
