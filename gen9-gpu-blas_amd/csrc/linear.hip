@@ -1,8 +1,8 @@
 // Linear layers: Y = R + dropout(act(X·Wᵀ + b)) in one product (gen9blas_linear) and its gradients (gen9blas_linear_backward).
 //
 // The forward product runs on the library's own FP16 and FP32 kernels for direct global→LDS loads (hgemm_kernel.h,
-// sgemm_kernel.h), up to 16 rows on the ones that stream the weights (skinny_kernel.h), with linear_epilogue.h in the place
-// of alpha and beta: a product that is stored first, and read again for its bias, activation and residual, costs 2 passes more
+// sgemm_kernel.h), a few rows on the ones that stream the weights (skinny_kernel.h) or share them (linear_rows_kernel.h: some dozens of
+// rows, and 3 to 16 on large weights, takes_rows), with linear_epilogue.h in the place of alpha and beta: a product that is stored first, and read again for its bias, activation and residual, costs 2 passes more
 // over M·N values. The gradients' two products are gen9blas_gemm's.
 #include "llm.h"
 #include "linear_epilogue.h"
@@ -170,7 +170,7 @@ template <class T> static bool takes_rows(int M, int N, int K) {
 template <class T>
 static int linear(int M, int N, int K, const T *X, long long ldx, const T *W, long long ldw, const Epilogue<T> &e, T *Y, long long ldy) {
     constexpr int KB = sizeof(T) == 2 ? g9::hgl::KB : g9::sgl::KB;
-    // The kernels on direct copies take more than one k-step of k, FP16 operands at 4-byte alignment with even row strides, and rows
+    // The kernels on direct copies take one k-step of k or more, FP16 operands at 4-byte alignment with even row strides, and rows
     // of a tile within 4 GiB; for these, others are copied first, and a short k is filled up with zeros.
     auto copied = [&](const T *p, long long ld) { return K < KB || ld * 256 * (long long)sizeof(T) >= 1LL << 32 || (sizeof(T) == 2 && ((uintptr_t)p % 4 || ld % 2)); };
     const bool cx = copied(X, ldx), cw = copied(W, ldw), some = M <= 64 && takes_rows<T>(M, N, K);
@@ -263,7 +263,10 @@ static int backward(int type, int M, int N, int K, const T *dY, int lddy, const 
     // and 72)
     constexpr int LONG = 128;
     auto odd = [&](const T *p, int ld) { return sizeof(T) == 2 && (ld % 2 || (uintptr_t)p % 4); };
-    // without an activation or dropout dZ is dY itself
+    // without an activation or dropout dZ is dY itself. Otherwise it is rounded to the type, once, for the two products (db adds it up
+    // before): FP16 2^-11 of a value, so that dX and dW are off by 2.9e-4 of their size instead of 2.1e-4, their own rounding's (2048 × 11008 ×
+    // 4096, GELU). Products of FP32 dZ run on the FP32 matrix cores, at a ninth of the rate; dZ as the sum of two FP16 numbers takes
+    // twice the products.
     const bool own = act || d.limit || (odd(dY, lddy) && M >= LONG && K >= LONG && (dX || dW));
     const int lddz = own ? (int)cdiv(N, 8) * 8 : lddy;
     T *dZ = nullptr;

@@ -28,7 +28,8 @@ inline Activation make_act(int act) {
     return {KIND_CLIP, -INFINITY, 0.f, 0.f};
 }
 
-// T: the type of the result. For FP16 the hardware's exponential and reciprocal are enough (2^-21 of the value and less).
+// T: the type of the result. For FP16 the hardware's exponential and reciprocal are enough: a step of 2^-23 of the value each, and the
+// rounding of the exponential's argument adds |x| units of 2^-24 where x < 0 (2^-20 at −16, where z·sigmoid is a subnormal FP16 number).
 template <class T> __device__ __forceinline__ float sigmoid(float x) {
     if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
     else return 1.f / (1.f + expf(-x));

@@ -10,7 +10,7 @@ namespace g9llm {
 // A row is in the registers of L threads, C pieces of 16 bytes each, so that it is read once: its mean, the squares around it (the
 // second pass that a variance needs, without a second read) and its result come from there. L is 16, a wave, 256, 512 or 1024.
 // HBM bounds it where there are rows enough. 8192 × 4096 FP16: forward 29 µs, 134 MB at 4.6 TB/s (a copy of 1 GiB: 5.2); backward
-// 38, 201 MB at 5.3, and 4.5 for the sums of its blocks. 2047 × 2501 FP32 12, 17 and 4.
+// 39, 201 MB at 5.2, and 4.8 for the sums of its blocks. 2047 × 2501 FP32 12, 18 and 4.
 template <class T> struct Piece {
     static constexpr int V = 16 / sizeof(T);
     typedef T Vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));

@@ -93,19 +93,22 @@ enum { GEN9BLAS_ACT_NONE = 0, GEN9BLAS_ACT_RELU = 1, GEN9BLAS_ACT_GELU = 2, GEN9
 // - bias (N floats), R (M×N) and Z may be NULL; Z: where the pre-activations go, which the gradients need if there is an activation.
 // - act: max(z, 0); z·Φ(z); its tanh form 0.5·z·(1 + tanh(√(2/π)·(z + 0.044715·z³))); z / (1 + e^−z).
 // - p, seed, offset: as in gen9blas_dropout (p = 0: none).
+// - z = −∞ keeps what IEEE arithmetic has for these forms: 0 with ReLU, NaN with the three others.
 GEN9BLAS_API int gen9blas_linear(int type, int M, int N, int K, const void *X, int ldx, const void *W, int ldw, const float *bias, int act,
                                  void *Z, int ldz, double p, uint64_t seed, uint64_t offset, const void *R, int ldr, void *Y, int ldy);
-// Its gradients: dZ = dropout(act'(Z)·dY) (what ReLU clips or dropout takes is 0 whatever dY is), rounded to the type for the products; dX (M×K) = dZ·W; dW (N×K) = dZᵀ·X; db (N floats) =
-// the column sums of dZ before that rounding. Each may be NULL, and what only it needs is not read then (Z: without an activation).
-// R's gradient is dY. accumulate: dW and db are added to what is there. M = 0: dW and db are zeros, or stay. The products are
-// gen9blas_gemm's, which wait unless gen9blas_set_nowait is on.
+// Its gradients: dZ = dropout(act'(Z)·dY) (what ReLU clips or dropout takes is 0 whatever dY is; an infinite Z has the slope 0 or 1 of its
+// end), rounded to the type for the products (FP16: 2^-11 of a value, past 65504 an infinity; who needs more takes FP32 operands);
+// dX (M×K) = dZ·W; dW (N×K) = dZᵀ·X; db (N floats) = the column sums of dZ before that rounding. Each may be NULL, and what only it
+// needs is not read then (Z: without an activation). R's gradient is dY. accumulate: dW and db are added to what is there. M = 0: dW
+// and db are zeros, or stay. The products are gen9blas_gemm's, which wait unless gen9blas_set_nowait is on.
 GEN9BLAS_API int gen9blas_linear_backward(int type, int M, int N, int K, const void *dY, int lddy, const void *Z, int ldz, int act, double p,
                                           uint64_t seed, uint64_t offset, const void *X, int ldx, const void *W, int ldw, void *dX, int lddx,
                                           void *dW, int lddw, float *db, int accumulate);
 
 // ---- Layer norm ----
 // Y = (X − mean)·rstd·gamma + beta for each of M rows of N values, rstd = 1 / √(variance + eps) (of the population). gamma and beta
-// (N floats) may be NULL: ones and zeros. stats (M×2 floats, or NULL): mean and rstd of each row, for the gradients.
+// (N floats) may be NULL: ones and zeros. stats (M×2 floats, or NULL): mean and rstd of each row, for the gradients. Squares are added
+// in FP32: past about 2^63 / √N from the mean they overflow, and rstd is 0.
 GEN9BLAS_API int gen9blas_layer_norm(int type, int M, int N, const void *X, int ldx, const float *gamma, const float *beta, float eps, void *Y,
                                      int ldy, float *stats);
 // Its gradients from dY, X and stats: dX, and sums over the rows in dgamma and dbeta (N floats); each may be NULL. What the rounding of
@@ -119,6 +122,7 @@ GEN9BLAS_API int gen9blas_layer_norm_backward(int type, int M, int N, const void
 // be NULL. The mask is a function of place, seed and offset, so that the same call on the gradient is the backward pass: columns 8c ..
 // 8c+7 of row m take the 16-bit parts, low ones first, of Philox4x32-10 with the counter (c, m, offset, offset >> 32) and the
 // key (seed, seed >> 32); parts below limit = round(65536 p) are lost, the others scaled by 65536 / (65536 − limit).
+// A captured call keeps its seed and offset: every replay has the same mask.
 GEN9BLAS_API int gen9blas_dropout(int type, int M, int N, const void *X, int ldx, double p, uint64_t seed, uint64_t offset, const void *R,
                                   int ldr, void *Y, int ldy);
 
